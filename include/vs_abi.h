@@ -446,6 +446,135 @@ int32_t vs_search_sharded_device(vs_group* g, vs_store* s, const void* d_queries
                                  uint32_t flags, uint32_t* d_out_ids, float* d_out_dist,
                                  uint32_t* d_out_n, void* hip_stream);
 
+/* ---- learning from clicks (device buffers, asynchronous) --------------------- */
+
+/* The reference trains nothing: its embedders hand vectors over (src/vector/mod.rs:
+ * 210-311) and a `DistributionShift` moves the scores afterwards (:317-373). These
+ * entry points have no counterpart there. They stand beside the searches: the same
+ * rows, the same candidate words, the same products of queries and rows, reduced
+ * to what fits queries, document vectors and weights to the documents that
+ * visitors clicked. A table is either a caller's own device memory (vs_lookup*,
+ * vs_xent*: rows that change with every step) or a sealed store
+ * (vs_store_lookup*, vs_store_xent*: the rows of the last seal, under the same
+ * snapshot rule as the searches).
+ *
+ * Common to all of them:
+ *   - asynchronous on `hip_stream`, of the context's GPU; nothing is allocated and
+ *     nothing is kept between calls, so a call may be recorded into a graph (the
+ *     vs_store_* calls may not: they record an event for the snapshot rule);
+ *   - d_workspace: at least the bytes that the matching *_workspace_bytes call
+ *     says, private to the call until the stream has passed it (two graphs that may
+ *     run at once need one each); VS_E_CAPACITY if workspace_bytes is less;
+ *   - types are VS_F32 or VS_BF16; a stride counts elements from one row to the
+ *     next, at least `dim`; rows of 16-byte aligned length and address run fastest,
+ *     any other length and alignment (of one element) is served;
+ *   - an id that names no row (VS_ROW_NONE, any id from n_rows on, in a store any
+ *     document that is not in it) adds nothing and gets no gradient;
+ *   - sums are f32 or wider, in an order that depends on the sizes alone: a call
+ *     gives the same bits every time. */
+#define VS_ROW_NONE 0xFFFFFFFFu
+/* Dimensions of a table, at most; queries of one loss call; ids of one gradient call. */
+#define VS_LEARN_MAX_DIM 8192u
+#define VS_XENT_MAX_QUERIES 65536u
+#define VS_LOOKUP_MAX_IDS (1u << 24)
+
+/* Pooled lookup: d_out[b] = scale * sum of d_weights[i] * row[d_ids[i]] over the
+ * positions i of bag b (a query from documents a visitor liked; the embedding of a
+ * history). Bag b holds the positions [d_offsets[b], d_offsets[b + 1]); n_bags + 1
+ * ascending offsets into the n_ids <= VS_LOOKUP_MAX_IDS ids; positions in no bag are
+ * not used; d_offsets NULL: bag b is position b alone (a plain lookup). d_weights
+ * NULL: all 1. An empty bag gives zeros. Device counterpart of
+ * vs_store_item_vector. */
+int32_t vs_lookup_device(vs_ctx* ctx, const void* d_rows, int32_t dtype, uint64_t n_rows,
+                         uint64_t row_stride, uint32_t dim, const uint32_t* d_ids, uint64_t n_ids,
+                         const uint32_t* d_offsets, uint64_t n_bags, const float* d_weights,
+                         float scale, void* d_out, int32_t out_dtype, uint64_t out_stride,
+                         void* hip_stream);
+/* The same from the rows of a sealed store (VS_F32 or VS_BF16); ids are docids. */
+int32_t vs_store_lookup_device(vs_store* s, const uint32_t* d_ids, uint64_t n_ids,
+                               const uint32_t* d_offsets, uint64_t n_bags, const float* d_weights,
+                               float scale, void* d_out, int32_t out_dtype, uint64_t out_stride,
+                               void* hip_stream);
+
+/* Gradient of a pooled lookup's rows from that of its output (d_grad_out, n_bags rows
+ * of `dtype`): row r gets scale * sum of d_weights[i] * d_grad_out[bag of i] over the
+ * positions with d_ids[i] == r. Ids are sorted on the device; there are no atomics.
+ *   d_unique_ids and d_n_unique given: *d_n_unique distinct ids go out ascending in
+ *     d_unique_ids, their sums in the first rows of d_grad_rows (room for n_ids of
+ *     both); what lies behind them is left as it was;
+ *   both NULL: row r of d_grad_rows (n_rows of them) has its sum ADDED; rows that no
+ *     id names are left as they were (the gradient of a table that has others too).
+ * d_grad_rows is of grad_rows_dtype; each sum is rounded to it once. */
+int32_t vs_lookup_grad_workspace_bytes(vs_ctx* ctx, uint64_t n_ids, uint64_t n_rows, uint32_t dim,
+                                       uint64_t* bytes);
+int32_t vs_lookup_grad_device(vs_ctx* ctx, const void* d_grad_out, int32_t dtype,
+                              uint64_t grad_out_stride, uint32_t dim, const uint32_t* d_ids,
+                              uint64_t n_ids, const uint32_t* d_offsets, uint64_t n_bags,
+                              const float* d_weights, float scale, uint64_t n_rows,
+                              void* d_workspace, uint64_t workspace_bytes, void* d_grad_rows,
+                              int32_t grad_rows_dtype, uint64_t grad_rows_stride,
+                              uint32_t* d_unique_ids, uint32_t* d_n_unique, void* hip_stream);
+/* Gradient of its weights: d_grad_weights[i] = scale * <row[d_ids[i]], d_grad_out[bag of
+ * i]> (f32, n_ids of them; 0 for a position without row or bag). */
+int32_t vs_lookup_grad_weights_device(vs_ctx* ctx, const void* d_rows, int32_t dtype,
+                                      uint64_t n_rows, uint64_t row_stride, uint32_t dim,
+                                      const uint32_t* d_ids, uint64_t n_ids,
+                                      const uint32_t* d_offsets, uint64_t n_bags, float scale,
+                                      const void* d_grad_out, int32_t grad_dtype,
+                                      uint64_t grad_out_stride, float* d_grad_weights,
+                                      void* hip_stream);
+
+/* Softmax cross entropy of queries over a corpus: with z[j] = scale * <query, row j>
+ * for every candidate j,  d_lse[q] = log(sum of exp(z[j])),
+ * d_loss[q] = d_lse[q] - z[d_targets[q]]. The logits are never stored; a loss near
+ * zero keeps its relative precision.
+ *   d_queries:    n_q <= VS_XENT_MAX_QUERIES rows of `dtype`
+ *   d_targets:    the clicked row of each query. A query whose click is no candidate
+ *                 (VS_ROW_NONE; outside the filter) has loss 0 and gradients 0; its
+ *                 lse is that of the candidates (-inf if there are none)
+ *   d_mask_words: candidate words as in the searches, bit r & 63 of word r >> 6,
+ *                 ceil(n_rows / 64) words; NULL = every row. Rows that are no
+ *                 candidates are not read. */
+int32_t vs_xent_workspace_bytes(vs_ctx* ctx, uint32_t n_q, uint64_t n_rows, uint32_t dim,
+                                int32_t dtype, uint64_t* bytes);
+int32_t vs_xent_device(vs_ctx* ctx, const void* d_queries, uint32_t n_q, uint64_t query_stride,
+                       const void* d_rows, uint64_t n_rows, uint64_t row_stride, int32_t dtype,
+                       uint32_t dim, const uint32_t* d_targets, const uint64_t* d_mask_words,
+                       float scale, void* d_workspace, uint64_t workspace_bytes, float* d_loss,
+                       float* d_lse, void* hip_stream);
+/* Its gradients, from the d_loss and d_lse of the same arguments and the gradient of
+ * each query's loss (d_grad_loss; NULL: all 1):
+ *   d_grad_queries: laid out as d_queries (same type and stride), or NULL
+ *   d_grad_rows:    laid out as d_rows, every row written (zeros for a row that is no
+ *                   candidate; between rows nothing is written), or NULL
+ * The products are recomputed, a piece of the rows at a time. With VS_BF16 the
+ * weights exp(z - lse) are rounded to bf16 before they multiply queries and rows, as
+ * those are; sums stay f32 and each gradient is rounded once. */
+int32_t vs_xent_grad_device(vs_ctx* ctx, const void* d_queries, uint32_t n_q, uint64_t query_stride,
+                            const void* d_rows, uint64_t n_rows, uint64_t row_stride, int32_t dtype,
+                            uint32_t dim, const uint32_t* d_targets, const uint64_t* d_mask_words,
+                            float scale, const float* d_loss, const float* d_lse,
+                            const float* d_grad_loss, void* d_workspace, uint64_t workspace_bytes,
+                            void* d_grad_queries, void* d_grad_rows, void* hip_stream);
+
+/* The same over a sealed store (VS_ANGULAR: logits are scale * cosine, VS_DOT: scale *
+ * product; other metrics VS_E_INVALID_ARG), whose rows stay as they are: the loss and
+ * the gradient of the queries, f32 [n_q][dim] in device memory as in
+ * vs_search_batch_device (rounded to bf16 for a VS_BF16 store). Targets are docids;
+ * d_mask_words as in vs_search_device (aligned to the store). The two calls of a step
+ * see the same rows if no seal comes between them. */
+int32_t vs_store_xent_workspace_bytes(vs_store* s, uint32_t n_q, uint64_t* bytes);
+int32_t vs_store_xent_device(vs_store* s, const float* d_queries, uint32_t n_q, uint32_t dim,
+                             const uint32_t* d_targets, const uint64_t* d_mask_words, float scale,
+                             void* d_workspace, uint64_t workspace_bytes, float* d_loss,
+                             float* d_lse, void* hip_stream);
+int32_t vs_store_xent_grad_device(vs_store* s, const float* d_queries, uint32_t n_q, uint32_t dim,
+                                  const uint32_t* d_targets, const uint64_t* d_mask_words,
+                                  float scale, const float* d_loss, const float* d_lse,
+                                  const float* d_grad_loss, void* d_workspace,
+                                  uint64_t workspace_bytes, float* d_grad_queries,
+                                  void* hip_stream);
+
 /* ---- candidate bitmaps ---------------------------------------------------- */
 
 /* Host-side expansion of a serialised RoaringBitmap into a dense mask of

@@ -18,6 +18,8 @@ VS_KEY_NONE = 0xFFFFFFFFFFFFFFFF
 VS_MAX_K = 1024
 VS_GROUP_ID_BYTES = 128
 VS_SHARDED_SHARE_PASSES, VS_SHARDED_ALWAYS_GATHER = 1, 2
+VS_ROW_NONE = 0xFFFFFFFF
+VS_LEARN_MAX_DIM, VS_XENT_MAX_QUERIES, VS_LOOKUP_MAX_IDS = 8192, 65536, 1 << 24
 
 # VS_AMD_LIB names another build of the same library (measurement variants of the tools)
 LIB_PATH = os.environ.get("VS_AMD_LIB") or os.path.join(os.path.dirname(os.path.abspath(__file__)), "libvs_amd.so")
@@ -31,6 +33,7 @@ _f32p = ctypes.POINTER(ctypes.c_float)
 _szp = ctypes.POINTER(ctypes.c_size_t)
 _u16, _u32, _i32, _u64, _sz = (ctypes.c_uint16, ctypes.c_uint32, ctypes.c_int32, ctypes.c_uint64,
                                ctypes.c_size_t)
+_f32 = ctypes.c_float
 
 # name -> argtypes; every entry point returns int32_t
 SIGNATURES = {
@@ -79,6 +82,20 @@ SIGNATURES = {
     "vs_group_create": [_vp, _i32, _i32, _u8p, ctypes.POINTER(_vp)],
     "vs_group_destroy": [_vp],
     "vs_search_sharded_device": [_vp, _vp, _vp, _u32, _u32, _u32, _vp, _u32, _vp, _vp, _vp, _vp],
+    "vs_lookup_device": [_vp, _vp, _i32, _u64, _u64, _u32, _vp, _u64, _vp, _u64, _vp, _f32, _vp, _i32, _u64, _vp],
+    "vs_store_lookup_device": [_vp, _vp, _u64, _vp, _u64, _vp, _f32, _vp, _i32, _u64, _vp],
+    "vs_lookup_grad_workspace_bytes": [_vp, _u64, _u64, _u32, _u64p],
+    "vs_lookup_grad_device": [_vp, _vp, _i32, _u64, _u32, _vp, _u64, _vp, _u64, _vp, _f32, _u64, _vp, _u64, _vp, _i32,
+                              _u64, _vp, _vp, _vp],
+    "vs_lookup_grad_weights_device": [_vp, _vp, _i32, _u64, _u64, _u32, _vp, _u64, _vp, _u64, _f32, _vp, _i32, _u64,
+                                      _vp, _vp],
+    "vs_xent_workspace_bytes": [_vp, _u32, _u64, _u32, _i32, _u64p],
+    "vs_xent_device": [_vp, _vp, _u32, _u64, _vp, _u64, _u64, _i32, _u32, _vp, _vp, _f32, _vp, _u64, _vp, _vp, _vp],
+    "vs_xent_grad_device": [_vp, _vp, _u32, _u64, _vp, _u64, _u64, _i32, _u32, _vp, _vp, _f32, _vp, _vp, _vp, _vp, _u64,
+                            _vp, _vp, _vp],
+    "vs_store_xent_workspace_bytes": [_vp, _u32, _u64p],
+    "vs_store_xent_device": [_vp, _vp, _u32, _u32, _vp, _vp, _f32, _vp, _u64, _vp, _vp, _vp],
+    "vs_store_xent_grad_device": [_vp, _vp, _u32, _u32, _vp, _vp, _f32, _vp, _vp, _vp, _vp, _u64, _vp, _vp],
     "vs_roaring_to_mask": [_u8p, _sz, _u64p, _u64, _u64p],
     "vs_mask_to_roaring": [_u64p, _u64, _u8p, _sz, _szp],
     "vs_cbo_roaring_to_mask": [_u8p, _sz, _u64p, _u64, _u64p],
@@ -225,6 +242,55 @@ class Context:
         _check(lib.vs_merge_topk_batch_device(self.handle, d_keys, n_lists, list_stride, n_queries,
                                               query_stride, k, metric, d_ids, d_dist, d_n, stream),
                self.handle)
+
+    # ---- learning from clicks: raw device addresses (ints, None = NULL), asynchronous on `stream` ----
+
+    def lookup_device(self, d_rows, dtype, n_rows, row_stride, dim, d_ids, n_ids, d_offsets, n_bags, d_weights, scale,
+                      d_out, out_dtype, out_stride, stream=0):
+        """vs_lookup_device: pooled, weighted lookup of rows by id."""
+        _check(lib.vs_lookup_device(self.handle, d_rows, dtype, n_rows, row_stride, dim, d_ids, n_ids, d_offsets, n_bags,
+                                    d_weights, scale, d_out, out_dtype, out_stride, stream), self.handle)
+
+    def lookup_grad_workspace_bytes(self, n_ids, n_rows, dim):
+        b = ctypes.c_uint64(0)
+        _check(lib.vs_lookup_grad_workspace_bytes(self.handle, n_ids, n_rows, dim, ctypes.byref(b)), self.handle)
+        return b.value
+
+    def lookup_grad_device(self, d_grad_out, dtype, grad_out_stride, dim, d_ids, n_ids, d_offsets, n_bags, d_weights,
+                           scale, n_rows, d_workspace, workspace_bytes, d_grad_rows, grad_rows_dtype, grad_rows_stride,
+                           d_unique_ids=None, d_n_unique=None, stream=0):
+        """vs_lookup_grad_device: the rows' gradient, compact (with d_unique_ids and d_n_unique) or added to a table."""
+        _check(lib.vs_lookup_grad_device(self.handle, d_grad_out, dtype, grad_out_stride, dim, d_ids, n_ids, d_offsets,
+                                         n_bags, d_weights, scale, n_rows, d_workspace, workspace_bytes, d_grad_rows,
+                                         grad_rows_dtype, grad_rows_stride, d_unique_ids, d_n_unique, stream),
+               self.handle)
+
+    def lookup_grad_weights_device(self, d_rows, dtype, n_rows, row_stride, dim, d_ids, n_ids, d_offsets, n_bags, scale,
+                                   d_grad_out, grad_dtype, grad_out_stride, d_grad_weights, stream=0):
+        """vs_lookup_grad_weights_device: the weights' gradient, f32 [n_ids]."""
+        _check(lib.vs_lookup_grad_weights_device(self.handle, d_rows, dtype, n_rows, row_stride, dim, d_ids, n_ids,
+                                                 d_offsets, n_bags, scale, d_grad_out, grad_dtype, grad_out_stride,
+                                                 d_grad_weights, stream), self.handle)
+
+    def xent_workspace_bytes(self, n_q, n_rows, dim, dtype):
+        b = ctypes.c_uint64(0)
+        _check(lib.vs_xent_workspace_bytes(self.handle, n_q, n_rows, dim, dtype, ctypes.byref(b)), self.handle)
+        return b.value
+
+    def xent_device(self, d_queries, n_q, query_stride, d_rows, n_rows, row_stride, dtype, dim, d_targets, d_mask, scale,
+                    d_workspace, workspace_bytes, d_loss, d_lse, stream=0):
+        """vs_xent_device: cross entropy of each query's click over the candidate rows, and its log-sum-exp."""
+        _check(lib.vs_xent_device(self.handle, d_queries, n_q, query_stride, d_rows, n_rows, row_stride, dtype, dim,
+                                  d_targets, d_mask, scale, d_workspace, workspace_bytes, d_loss, d_lse, stream),
+               self.handle)
+
+    def xent_grad_device(self, d_queries, n_q, query_stride, d_rows, n_rows, row_stride, dtype, dim, d_targets, d_mask,
+                         scale, d_loss, d_lse, d_grad_loss, d_workspace, workspace_bytes, d_grad_queries, d_grad_rows,
+                         stream=0):
+        """vs_xent_grad_device: gradients of queries and rows (either None: not wanted)."""
+        _check(lib.vs_xent_grad_device(self.handle, d_queries, n_q, query_stride, d_rows, n_rows, row_stride, dtype, dim,
+                                       d_targets, d_mask, scale, d_loss, d_lse, d_grad_loss, d_workspace,
+                                       workspace_bytes, d_grad_queries, d_grad_rows, stream), self.handle)
 
 
 def group_unique_id():
@@ -443,6 +509,30 @@ class Store:
     def search_device_noalloc(self, d_query, dim, k, d_mask, d_out_keys, stream=0):
         """vs_search_device on the library's static scratch: no workspace, no allocation."""
         self._ck(lib.vs_search_device_noalloc(self.handle, d_query, dim, k, d_mask, d_out_keys, stream))
+
+    # ---- learning from clicks over the sealed rows (raw device addresses, asynchronous on `stream`) ----
+
+    def lookup_device(self, d_ids, n_ids, d_offsets, n_bags, d_weights, scale, d_out, out_dtype, out_stride, stream=0):
+        """vs_store_lookup_device: pooled, weighted lookup of documents by docid."""
+        self._ck(lib.vs_store_lookup_device(self.handle, d_ids, n_ids, d_offsets, n_bags, d_weights, scale, d_out,
+                                            out_dtype, out_stride, stream))
+
+    def xent_workspace_bytes(self, n_q):
+        b = ctypes.c_uint64(0)
+        self._ck(lib.vs_store_xent_workspace_bytes(self.handle, n_q, ctypes.byref(b)))
+        return b.value
+
+    def xent_device(self, d_queries, n_q, dim, d_targets, d_mask, scale, d_workspace, workspace_bytes, d_loss, d_lse,
+                    stream=0):
+        """vs_store_xent_device: cross entropy of f32 queries over the store's documents under its metric."""
+        self._ck(lib.vs_store_xent_device(self.handle, d_queries, n_q, dim, d_targets, d_mask, scale, d_workspace,
+                                          workspace_bytes, d_loss, d_lse, stream))
+
+    def xent_grad_device(self, d_queries, n_q, dim, d_targets, d_mask, scale, d_loss, d_lse, d_grad_loss, d_workspace,
+                         workspace_bytes, d_grad_queries, stream=0):
+        """vs_store_xent_grad_device: the gradient of the queries."""
+        self._ck(lib.vs_store_xent_grad_device(self.handle, d_queries, n_q, dim, d_targets, d_mask, scale, d_loss, d_lse,
+                                               d_grad_loss, d_workspace, workspace_bytes, d_grad_queries, stream))
 
 
 # ---- arroy's on-disk item layout (host only) ---------------------------------------------

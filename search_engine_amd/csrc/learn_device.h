@@ -1,0 +1,103 @@
+// Helpers of the learning kernels: element types, packs of elements, sums over a wave and a workgroup, and the
+// carving of a caller's workspace.
+#pragma once
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include <algorithm>
+
+#include "vs_device.h"
+
+namespace vs {
+namespace learn {
+
+struct bf16 {
+    uint16_t bits;
+};
+
+__device__ __forceinline__ float to_f32(float x) { return x; }
+__device__ __forceinline__ float to_f32(bf16 x) { return __builtin_bit_cast(float, (uint32_t)x.bits << 16); }
+
+// Round to nearest even; a NaN stays one.
+__device__ __forceinline__ uint32_t bf16_bits(float x) {
+    return __builtin_bit_cast(uint16_t, (__bf16)x);
+}
+template <typename O>
+__device__ __forceinline__ O from_f32(float x) {
+    if constexpr (sizeof(O) == 4)
+        return x;
+    else
+        return O{(uint16_t)bf16_bits(x)};
+}
+
+// V elements that are loaded and stored at once.
+template <typename E, int V>
+struct alignas(sizeof(E) * V < 16 ? sizeof(E) * V : 16) Pack {
+    E e[V];
+};
+template <typename E, int V>
+__device__ __forceinline__ Pack<E, V> load_pack(const E* p) {
+    return *reinterpret_cast<const Pack<E, V>*>(p);
+}
+template <typename E, int V>
+__device__ __forceinline__ void store_pack(E* p, const Pack<E, V>& x) {
+    *reinterpret_cast<Pack<E, V>*>(p) = x;
+}
+// Whether every row of a table starts where a Pack<E, V> may.
+template <typename E, int V>
+inline bool aligned_rows(const void* base, uint64_t stride) {
+    return (uintptr_t)base % alignof(Pack<E, V>) == 0 && stride * sizeof(E) % alignof(Pack<E, V>) == 0;
+}
+
+__device__ __forceinline__ float wave_sum(float v) { return wave_sum_f32(v); }
+
+// Sum of x over the threads before this one, and over all, in a workgroup of 256.
+__device__ __forceinline__ uint32_t block_exclusive(uint32_t x, uint32_t* wave_sums /* 4, LDS */, uint32_t* total) {
+    const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    uint32_t in = x;
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) {
+        const uint32_t y = __shfl_up(in, d);
+        if (lane >= (uint32_t)d) in += y;
+    }
+    __syncthreads();  // the sums of a call before this one have been read
+    if (lane == 63) wave_sums[wave] = in;
+    __syncthreads();
+    uint32_t before = 0, all = 0;
+#pragma unroll
+    for (uint32_t w = 0; w < 4; ++w) {
+        if (w < wave) before += wave_sums[w];
+        all += wave_sums[w];
+    }
+    *total = all;
+    return before + in - x;
+}
+
+inline uint64_t round_up(uint64_t x, uint64_t to) { return (x + to - 1) / to * to; }
+
+// Hands out pieces of a workspace, each at a multiple of 256 bytes.
+class Carver {
+  public:
+    explicit Carver(void* base) : at_((char*)round_up((uintptr_t)base, 256)) {}
+    template <typename T>
+    T* take(uint64_t n) {
+        T* p = reinterpret_cast<T*>(at_);
+        at_ += round_up(n * sizeof(T), 256);
+        return p;
+    }
+    const char* at() const { return at_; }
+
+  private:
+    char* at_;
+};
+
+static __global__ __launch_bounds__(256) void fill_u32_kernel(uint32_t* p, uint64_t n, uint32_t value) {
+    for (uint64_t i = (uint64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (uint64_t)gridDim.x * 256) p[i] = value;
+}
+// (a kernel and not hipMemsetAsync: the call may be recorded into a graph, whose memset nodes this library keeps out)
+inline void fill_u32(uint32_t* p, uint64_t n, uint32_t value, hipStream_t stream) {
+    if (n) fill_u32_kernel<<<(uint32_t)std::min<uint64_t>((n + 255) / 256, 4096), 256, 0, stream>>>(p, n, value);
+}
+
+}  // namespace learn
+}  // namespace vs
