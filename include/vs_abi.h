@@ -473,8 +473,9 @@ int32_t vs_search_sharded_device(vs_group* g, vs_store* s, const void* d_queries
  *   - sums are f32 or wider, in an order that depends on the sizes alone: a call
  *     gives the same bits every time. */
 #define VS_ROW_NONE 0xFFFFFFFFu
-/* Dimensions of a table, at most; queries of one loss call; ids of one gradient call. */
+/* Dimensions and rows of a table, at most; queries of one loss call; ids of one lookup call. */
 #define VS_LEARN_MAX_DIM 8192u
+#define VS_LEARN_MAX_ROWS (1u << 31)
 #define VS_XENT_MAX_QUERIES 65536u
 #define VS_LOOKUP_MAX_IDS (1u << 24)
 

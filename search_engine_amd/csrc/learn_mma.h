@@ -1,0 +1,189 @@
+// Products of tiles on the bf16 matrix cores: the loop that the cross entropy's four products share.
+//
+// A workgroup of eight waves makes a tile of M x N sums over k, 64 k at a time. Both operands' pieces of a step go from
+// memory straight into LDS (16 bytes a lane, no registers), into the half that the step before last has left, while the
+// matrix cores work on the other half: one barrier a step, at which the loads that were issued a whole step ago are
+// waited for. 256 x 256 tiles read each byte of LDS for 128 x 64 products per wave, which leaves the LDS port at three
+// quarters of the matrix time; 64 KiB a step, twice, are 128 of the 160 KiB of a CU.
+//
+// Operands come in two shapes:
+//   Rows<R>  [R rows][64 k], k contiguous: read as one ds_read_b128 a fragment;
+//   Cols<C>  [64 k][C columns], columns contiguous (the sum runs over memory rows): read with the transposing
+//            ds_read_b64_tr_b16, four k x 16 columns per 16 lanes.
+// Both keep their 16-byte chunks rotated by XOR with the row, so that the lanes of a read fall on different banks.
+//
+// f32 operands are three bf16 planes: x = h + m + l exactly (8 + 8 + 8 bits), and a product takes the six steps hh, hm, mh,
+// mm, hl, lh; what is left out (ml, lm, ll) is below 2^-23 of hh. Six steps on the bf16 cores are 2.7 times as fast as the
+// f32 matrix instruction, whose rate is a sixteenth.
+#pragma once
+#include "learn_device.h"
+
+namespace vs {
+namespace learn {
+
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) void* lds_void;
+typedef __attribute__((address_space(1))) const void* global_void;
+typedef __attribute__((address_space(3))) s16x4* lds_s16x4;
+
+constexpr uint32_t THREADS = 512;
+constexpr uint32_t STEP = 64;  // k of a step
+
+// A matrix of bf16 planes in memory; every row starts at a multiple of 16 bytes.
+struct Planes {
+    const char* base;
+    uint64_t plane;        // bytes from one plane to the next
+    uint32_t stride;       // bytes from one row to the next
+    const uint32_t* list;  // row i is list[i]; null: i
+    uint32_t rows;         // valid rows; those behind are zeros
+    uint32_t chunks;       // 16-byte chunks of a row; those behind are zeros
+};
+
+__device__ __forceinline__ void load_to_lds(const char* from, char* to) {
+    __builtin_amdgcn_global_load_lds((global_void)from, (lds_void)to, 16, 0, 0);
+}
+
+// The same where transposing reads follow. Behind the builtin the compiler waits for every load under way before each
+// transposing read (it takes them to read what the loads write), and a step's loads would no longer pass under the step
+// before it. The instruction has no result: it writes LDS, and what it read is waited for at the step's barrier, by hand.
+__device__ __forceinline__ void load_to_lds_unseen(const char* from, char* to) {
+    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off"
+                 :
+                 : "v"((global_void)from), "s"(uniform_u32((uint32_t)(uintptr_t)(lds_void)to))
+                 : "memory", "m0");
+}
+__device__ __forceinline__ void step_barrier() {
+    __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0): my loads are in LDS
+    __syncthreads();
+}
+
+// [R][64 k]: 128 bytes a row, chunk c of row r at place c ^ (r & 7).
+template <int R>
+struct Rows {
+    static constexpr int BYTES = R * 128;
+    static constexpr int LOADS = R >= 64 ? R / 64 : 1;
+    const char* row[LOADS];
+    uint32_t index[LOADS];  // of the rows of the next aim, as listed
+    uint32_t chunk;
+    __device__ __forceinline__ void init() { chunk = (threadIdx.x & 7) ^ (threadIdx.x >> 3 & 7); }
+    // The rows of the tile that starts at row `first`: reads the list, ahead of its use (nothing looks at what was read
+    // until then, so nothing waits for it).
+    __device__ __forceinline__ void peek(const Planes& p, uint32_t first) {
+        if (!p.list) return;
+#pragma unroll
+        for (int i = 0; i < LOADS; ++i) index[i] = p.list[min(first + i * 64 + (threadIdx.x >> 3), p.rows - 1)];
+    }
+    __device__ __forceinline__ void aim(const Planes& p, uint32_t first) {
+#pragma unroll
+        for (int i = 0; i < LOADS; ++i) {
+            const uint32_t r = first + i * 64 + (threadIdx.x >> 3);
+            row[i] = r < p.rows ? p.base + (uint64_t)(p.list ? index[i] : r) * p.stride + chunk * 16 : nullptr;
+        }
+    }
+    __device__ __forceinline__ void load(const Planes& p, uint32_t kstep, uint32_t plane, const char* zeros, char* lds) const {
+        if (R < 64 && threadIdx.x >= R * 8) return;
+        const uint64_t off = (uint64_t)kstep * 128 + plane * p.plane;
+        const bool in = kstep * 8 + chunk < p.chunks;
+        char* to = lds + uniform_u32(threadIdx.x >> 6) * 1024;  // the wave's first lane; the others follow by 16 bytes
+#pragma unroll
+        for (int i = 0; i < LOADS; ++i) load_to_lds(in && row[i] ? row[i] + off : zeros, to + i * 8192);
+    }
+    // Lane's 8 k of fragment `t` (16 rows) in half `kk` of the step.
+    __device__ __forceinline__ static bf16x8 read(const char* lds, uint32_t tile, int kk) {
+        const uint32_t l = threadIdx.x & 63;
+        return *reinterpret_cast<const bf16x8*>(lds + (tile * 16 + (l & 15)) * 128 + (((kk * 4 + (l >> 4)) ^ (l & 7)) * 16));
+    }
+};
+
+// [64 k][C]: C * 2 bytes a k, chunk c of k at place c ^ turn(k).
+template <int C>
+struct Cols {
+    static constexpr int BYTES = C * 128;
+    static constexpr int CHUNKS = C / 8;
+    static constexpr int LOADS = CHUNKS / 8;
+    static constexpr int APART = 512 / CHUNKS;  // k between two loads of a thread
+    uint32_t index[LOADS];
+    uint32_t k0, chunk;
+    __device__ __forceinline__ static uint32_t turn(uint32_t k) {
+        return CHUNKS >= 16 ? (2 * (k & 3)) ^ (8 * (k >> 3 & 1)) : 2 * (k & 3);
+    }
+    __device__ __forceinline__ void init() {
+        k0 = threadIdx.x / CHUNKS;
+        chunk = (threadIdx.x % CHUNKS) ^ turn(k0);  // (the k of further loads are APART = 16, 32 apart: the same turn)
+    }
+    // The memory rows of the step whose first k is row `first` of `end`: reads the list, ahead of its use.
+    __device__ __forceinline__ void peek(const Planes& p, uint32_t first, uint32_t end) {
+        if (!p.list) return;
+#pragma unroll
+        for (int i = 0; i < LOADS; ++i) index[i] = p.list[min(first + k0 + i * APART, end - 1)];
+    }
+    __device__ __forceinline__ void load(const Planes& p, uint32_t first, uint32_t end, uint32_t first_chunk, uint32_t plane,
+                                         const char* zeros, char* lds) const {
+        const uint32_t c = first_chunk + chunk;
+        const char* base = p.base + plane * p.plane + c * 16ull;
+        char* to = lds + uniform_u32(threadIdx.x >> 6) * 1024;
+#pragma unroll
+        for (int i = 0; i < LOADS; ++i) {
+            const uint32_t r = first + k0 + i * APART;
+            load_to_lds_unseen(r < end && c < p.chunks ? base + (uint64_t)(p.list ? index[i] : r) * p.stride : zeros, to + i * 8192);
+        }
+    }
+    __device__ __forceinline__ static bf16x8 read(char* lds, uint32_t tile, int kk) {
+        const uint32_t l = threadIdx.x & 63, k = kk * 32 + (l >> 4) * 8 + (l >> 2 & 3);
+        char* at = lds + k * (C * 2) + (((tile * 2 + (l >> 1 & 1)) ^ turn((l >> 4) * 8 + (l >> 2 & 3))) * 16) + (l & 1) * 8;
+        union {
+            s16x4 half[2];
+            bf16x8 all;
+        } x;
+        x.half[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)at);
+        x.half[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)(at + 4 * (C * 2)));
+        return x.all;
+    }
+};
+
+// The products of a step: TM x TN fragments of 16 x 16 per wave, which start at fragments m0 and n0. Lane l holds rows
+// (of A) 4 (l >> 4) + 0..3 and column (of B) l & 15 of each.
+template <typename A, typename B, int TM, int TN>
+__device__ __forceinline__ void multiply(char* a, char* b, uint32_t m0, uint32_t n0, f32x4 (&acc)[TM][TN]) {
+#pragma unroll
+    for (int kk = 0; kk < 2; ++kk) {
+        bf16x8 fa[TM], fb[TN];
+#pragma unroll
+        for (int n = 0; n < TN; ++n) fb[n] = B::read(b, n0 + n, kk);
+#pragma unroll
+        for (int m = 0; m < TM; ++m) fa[m] = A::read(a, m0 + m, kk);
+#pragma unroll
+        for (int m = 0; m < TM; ++m)
+#pragma unroll
+            for (int n = 0; n < TN; ++n) acc[m][n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fa[m], fb[n], acc[m][n], 0, 0, 0);
+    }
+}
+
+// The steps of a product of planes: (plane of A, plane of B) of step c.
+struct Steps {
+    uint32_t n;
+    uint32_t a, b;  // two bits a step
+    __device__ __forceinline__ uint32_t plane_a(uint32_t c) const { return a >> (2 * c) & 3; }
+    __device__ __forceinline__ uint32_t plane_b(uint32_t c) const { return b >> (2 * c) & 3; }
+};
+
+// x = planes[0] + .. exactly, three bf16.
+struct Split {
+    uint16_t h, m, l;
+};
+__device__ __forceinline__ Split split(float x) {
+    Split s;
+    s.h = (uint16_t)bf16_bits(x);
+    const float hv = __builtin_bit_cast(float, (uint32_t)s.h << 16);
+    // beyond bf16's largest number the rounding gives an infinity; of an infinity, or a NaN, nothing is left to split
+    const bool whole = !(__builtin_fabsf(hv) < __builtin_inff());
+    if (whole && __builtin_fabsf(x) < __builtin_inff()) s.h = (uint16_t)(__builtin_bit_cast(uint32_t, x) >> 16);
+    const float r = whole && !(__builtin_fabsf(x) < __builtin_inff()) ? 0.0f : x - __builtin_bit_cast(float, (uint32_t)s.h << 16);
+    s.m = (uint16_t)bf16_bits(r);
+    s.l = (uint16_t)bf16_bits(r - __builtin_bit_cast(float, (uint32_t)s.m << 16));
+    return s;
+}
+
+}  // namespace learn
+}  // namespace vs

@@ -32,7 +32,7 @@ int32_t use_ctx(vs_ctx* ctx) {
 }
 
 int32_t check_table(const void* rows, int32_t dtype, uint64_t n_rows, uint64_t stride, uint32_t dim) {
-    if (n_rows == 0 || n_rows >= VS_ROW_NONE) return fail(VS_E_INVALID_ARG, "rows: a table of %llu rows", (unsigned long long)n_rows);
+    if (n_rows == 0 || n_rows > VS_LEARN_MAX_ROWS) return fail(VS_E_INVALID_ARG, "rows: a table of %llu rows", (unsigned long long)n_rows);
     return check_matrix("rows", rows, dtype, n_rows, stride, dim);
 }
 
@@ -71,6 +71,7 @@ int32_t check_sealed(vs_store* s) {
     if (int32_t rc = vsrt::check_store(s)) return rc;
     if (!s->sealed.load()) return fail(VS_E_NOT_SEALED, "store %u was never sealed", s->index);
     if (!is_float(s->dtype)) return fail(VS_E_INVALID_ARG, "store %u holds no f32 or bf16 rows", s->index);
+    if (s->capacity > VS_LEARN_MAX_ROWS) return fail(VS_E_INVALID_ARG, "store %u has more than %u slots", s->index, VS_LEARN_MAX_ROWS);
     return VS_OK;
 }
 
@@ -169,7 +170,7 @@ extern "C" int32_t vs_store_lookup_device(vs_store* s, const uint32_t* d_ids, ui
 extern "C" int32_t vs_lookup_grad_workspace_bytes(vs_ctx* ctx, uint64_t n_ids, uint64_t n_rows, uint32_t dim, uint64_t* bytes) {
     if (!bytes) return fail(VS_E_INVALID_ARG, "null argument");
     if (n_ids > VS_LOOKUP_MAX_IDS) return fail(VS_E_INVALID_ARG, "%llu ids are more than %u", (unsigned long long)n_ids, VS_LOOKUP_MAX_IDS);
-    if (n_rows == 0 || n_rows >= VS_ROW_NONE) return fail(VS_E_INVALID_ARG, "rows: a table of %llu rows", (unsigned long long)n_rows);
+    if (n_rows == 0 || n_rows > VS_LEARN_MAX_ROWS) return fail(VS_E_INVALID_ARG, "rows: a table of %llu rows", (unsigned long long)n_rows);
     if (dim == 0 || dim > VS_LEARN_MAX_DIM) return fail(VS_E_INVALID_ARG, "dimension %u out of range", dim);
     if (!ctx) return fail(VS_E_INVALID_ARG, "null context");
     *bytes = learn::lookup_grad_workspace_bytes(n_ids, n_rows, dim);
@@ -185,7 +186,7 @@ extern "C" int32_t vs_lookup_grad_device(vs_ctx* ctx, const void* d_grad_out, in
     if (int32_t rc = check_bags(d_ids, n_ids, n_bags)) return rc;
     if (int32_t rc = check_matrix("grad_out", d_grad_out, dtype, n_bags, grad_out_stride, dim)) return rc;
     if (!d_unique_ids != !d_n_unique) return fail(VS_E_INVALID_ARG, "unique_ids and n_unique: one without the other");
-    if (n_rows == 0 || n_rows >= VS_ROW_NONE) return fail(VS_E_INVALID_ARG, "rows: a table of %llu rows", (unsigned long long)n_rows);
+    if (n_rows == 0 || n_rows > VS_LEARN_MAX_ROWS) return fail(VS_E_INVALID_ARG, "rows: a table of %llu rows", (unsigned long long)n_rows);
     if (int32_t rc = check_matrix("grad_rows", d_grad_rows, grad_rows_dtype, d_unique_ids ? n_ids : n_rows, grad_rows_stride, dim)) return rc;
     if (int32_t rc = check_workspace(d_workspace, workspace_bytes, learn::lookup_grad_workspace_bytes(n_ids, n_rows, dim),
                                      "vs_lookup_grad_workspace_bytes"))
@@ -216,7 +217,7 @@ extern "C" int32_t vs_lookup_grad_weights_device(vs_ctx* ctx, const void* d_rows
 extern "C" int32_t vs_xent_workspace_bytes(vs_ctx* ctx, uint32_t n_q, uint64_t n_rows, uint32_t dim, int32_t dtype, uint64_t* bytes) {
     if (!bytes) return fail(VS_E_INVALID_ARG, "null argument");
     if (int32_t rc = check_queries(n_q)) return rc;
-    if (n_rows == 0 || n_rows >= VS_ROW_NONE) return fail(VS_E_INVALID_ARG, "rows: a table of %llu rows", (unsigned long long)n_rows);
+    if (n_rows == 0 || n_rows > VS_LEARN_MAX_ROWS) return fail(VS_E_INVALID_ARG, "rows: a table of %llu rows", (unsigned long long)n_rows);
     if (dim == 0 || dim > VS_LEARN_MAX_DIM) return fail(VS_E_INVALID_ARG, "dimension %u out of range", dim);
     if (!is_float(dtype)) return fail(VS_E_INVALID_ARG, "element type %d is not VS_F32 or VS_BF16", dtype);
     if (!ctx) return fail(VS_E_INVALID_ARG, "null context");

@@ -11,44 +11,65 @@
 //
 // Under a filter the candidates are listed first, and everything reads through the list: a row that is no candidate is
 // never read (whatever it holds), and costs nothing.
+//
+// Four products on the bf16 matrix cores (learn_mma.h) carry it: rows x queries for the loss, the same again for the
+// weights G, and G with the queries and with the rows for the gradients. G is made for a piece of the rows at a time and
+// read twice before the next piece takes its place. f32 tables, and bf16 ones whose rows are not 16-byte aligned, are
+// copied piece by piece into planes first.
 #include "../../include/vs_abi.h"
 #include "learn_kernels.h"
-#include "learn_device.h"
+#include "learn_mma.h"
 
 namespace vs {
 namespace learn {
 namespace {
 
 constexpr uint32_t NONE = 0xFFFFFFFFu;
+constexpr float LOG2E = 1.44269504088896340736f;
+constexpr int TILE = 256;  // candidates of a tile
 
 struct XentArgs {
-    Table t;
+    Planes rows;            // of the candidates, or of the whole table with the list of candidates
+    uint32_t place0;        // the candidate that is row 0 of `rows`
+    uint64_t n_rows;        // candidates where there is no list
     const uint32_t* list;   // candidate rows, ascending; null = every row
     const uint32_t* count;  // of the list
     const float* norms;
-    const void* q;          // [n_q][kp] of the table's type, zero from `dim` on
-    uint32_t kp, n_q;
+    Planes q;               // queries, with the sign of the scale
+    Planes qt;              // queries transposed
+    uint32_t n_q, gq, dim;  // gq: n_q rounded up to 64
     const uint32_t* click;  // [n_q] place of the clicked row among the candidates, or NONE
-    const float* qscale;    // [n_q] factor of a query's products
-    // loss
-    float* part_m;          // [splits][n_q]
-    float* part_l;
-    float* click_z;         // [n_q]
-    // gradients
-    const float* lse;
-    const float* loss;
-    const float* grad_loss;
-    float* g;               // [piece][n_q]
+    const float* qscale;    // [n_q] factor of a query's products, without its sign
+    float sign;
+    Steps score_steps, grad_steps;
+    const char* zeros;
     uint32_t piece_begin, piece_rows;
+    bool first_piece;
+    uint32_t across, splits;  // workgroups side by side (query or column tiles), and along the rows
+    // loss, base 2
+    float *part_m, *part_l;   // [splits][n_q]
+    float* click_z;           // [n_q]
+    // gradients
+    const float *lse, *loss, *grad_loss;
+    char* g;                  // [planes][piece][gq] bf16
+    uint64_t g_plane;
+    uint32_t g_planes;
     void* grad_rows;
     uint64_t grad_row_stride;
-    float* part_q;          // [splits][n_q][dim]
-    uint32_t splits;
-    bool first_piece;
+    bool grad_rows_wide;      // four elements at a time
+    float* part_q;            // [splits][n_q][dim]
 };
 
-__device__ __forceinline__ uint32_t candidates(const XentArgs& a) { return a.list ? *a.count : (uint32_t)a.t.n_rows; }
+__device__ __forceinline__ uint32_t candidates(const XentArgs& a) { return a.list ? *a.count : (uint32_t)a.n_rows; }
 __device__ __forceinline__ uint64_t row_at(const XentArgs& a, uint32_t place) { return a.list ? a.list[place] : place; }
+
+// Workgroups that share a tile of rows get numbers eight apart: the dispatcher deals numbers out to the eight XCDs in
+// turn, so they land on one XCD and its L2 holds the tile for all of them.
+__device__ __forceinline__ void place_of_workgroup(uint32_t across, uint32_t* a, uint32_t* along) {
+    const uint32_t local = blockIdx.x >> 3;
+    *a = local % across;
+    *along = local / across * 8 + (blockIdx.x & 7);
+}
 
 // ---- candidates and queries ------------------------------------------------------------------
 
@@ -82,27 +103,58 @@ __global__ __launch_bounds__(256) void list_candidates_kernel(const uint64_t* ma
     if (blockIdx.x == gridDim.x - 1 && !threadIdx.x) *count = before + total;
 }
 
-// A query in the table's type, its factor, and the place of its click; one workgroup per query.
-template <typename E, typename Q>
+// Queries as planes, [n_q][k] and transposed [dim][gq], by tiles of 64 x 64; the workgroups behind the tiles take four
+// queries each: length, factor, and the place of the click.
+template <typename Q, int P>
 __global__ __launch_bounds__(256) void pack_queries_kernel(XentArgs a, const Q* queries, uint64_t stride, const uint32_t* targets,
-                                                           float scale, uint32_t* click, float* qscale) {
-    __shared__ float sums[4];
-    const uint32_t q = blockIdx.x;
-    E* out = static_cast<E*>(const_cast<void*>(a.q)) + (uint64_t)q * a.kp;
-    float sq = 0;
-    for (uint32_t k = threadIdx.x; k < a.kp; k += 256) {
-        const E e = from_f32<E>(k < a.t.dim ? to_f32(queries[q * stride + k]) : 0.0f);
-        sq = __builtin_fmaf(to_f32(e), to_f32(e), sq);
-        out[k] = e;
+                                                           uint32_t first_id, uint64_t n_rows, float scale, uint32_t* click,
+                                                           float* qscale, uint32_t* zeros, bool transposed) {
+    __shared__ uint16_t t[P][64][66];
+    const uint32_t n_tiles = a.gq / 64 * (a.q.chunks / 8);
+    if (!blockIdx.x && threadIdx.x < 64) zeros[threadIdx.x] = 0;
+    if (blockIdx.x < n_tiles) {
+        const uint32_t q0 = blockIdx.x % (a.gq / 64) * 64, d0 = blockIdx.x / (a.gq / 64) * 64;
+        for (uint32_t i = threadIdx.x; i < 4096; i += 256) {
+            const uint32_t q = q0 + i / 64, d = d0 + i % 64;
+            const float x = q < a.n_q && d < a.dim ? to_f32(queries[q * stride + d]) : 0.0f;
+            const Split s = split(x);
+            const uint16_t part[3] = {s.h, s.m, s.l};
+#pragma unroll
+            for (int p = 0; p < P; ++p) {
+                t[p][i / 64][i % 64] = part[p];
+                if (q < a.n_q)
+                    reinterpret_cast<uint16_t*>(const_cast<char*>(a.q.base) + p * a.q.plane + q * (uint64_t)a.q.stride)[d] =
+                        part[p] ^ (a.sign < 0 ? 0x8000 : 0);
+            }
+        }
+        if (!transposed) return;
+        __syncthreads();
+        for (uint32_t i = threadIdx.x; i < 4096; i += 256) {
+            const uint32_t d = d0 + i / 64, q = q0 + i % 64;
+            if (d >= a.dim) continue;
+#pragma unroll
+            for (int p = 0; p < P; ++p)
+                reinterpret_cast<uint16_t*>(const_cast<char*>(a.qt.base) + p * a.qt.plane + d * (uint64_t)a.qt.stride)[q] =
+                    t[p][i % 64][i / 64];
+        }
+        return;
     }
-    sq = wave_sum(sq);
-    if (!(threadIdx.x & 63)) sums[threadIdx.x >> 6] = sq;
-    __syncthreads();
-    if (threadIdx.x) return;
-    const float norm = __builtin_sqrtf(sums[0] + sums[1] + sums[2] + sums[3]);
-    qscale[q] = !a.norms ? scale : norm > 0 ? scale / norm : 0.0f;
-    const uint32_t id = targets[q], row = id - a.t.first_id;
-    uint32_t place = id >= a.t.first_id && row < a.t.n_rows ? row : NONE;
+    const uint32_t q = (blockIdx.x - n_tiles) * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
+    if (q >= a.n_q) return;
+    float sq = 0;
+    if (a.norms) {
+        for (uint32_t d = lane; d < a.dim; d += 64) {
+            float x = to_f32(queries[q * stride + d]);
+            if (P == 1) x = __builtin_bit_cast(float, bf16_bits(x) << 16);  // as it is multiplied
+            sq = __builtin_fmaf(x, x, sq);
+        }
+        sq = wave_sum(sq);
+    }
+    if (lane) return;
+    const float norm = __builtin_sqrtf(sq), size = __builtin_fabsf(scale);
+    qscale[q] = !a.norms ? size : norm > 0 ? size / norm : 0.0f;
+    const uint32_t id = targets[q], row = id - first_id;
+    uint32_t place = id >= first_id && row < n_rows ? row : NONE;
     if (a.list && place != NONE) {
         uint32_t lo = 0, hi = *a.count;  // the first candidate that is not before the row
         while (lo < hi) {
@@ -117,214 +169,478 @@ __global__ __launch_bounds__(256) void pack_queries_kernel(XentArgs a, const Q* 
     click[q] = place;
 }
 
+// A piece of the candidates as planes: eight elements a thread, zeros from `dim` on.
+template <typename E, int P, bool WIDE>
+__global__ __launch_bounds__(256) void pack_rows_kernel(XentArgs a, const E* table, uint64_t stride, char* out) {
+    const uint32_t end = min(candidates(a), a.piece_begin + a.piece_rows);
+    const uint64_t total = end > a.piece_begin ? (uint64_t)(end - a.piece_begin) * a.rows.chunks : 0;
+    for (uint64_t i = (uint64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (uint64_t)gridDim.x * 256) {
+        const uint32_t r = (uint32_t)(i / a.rows.chunks), d = (uint32_t)(i - (uint64_t)r * a.rows.chunks) * 8;
+        const E* from = table + row_at(a, a.piece_begin + r) * stride + d;
+        float x[8];
+        if (WIDE && d + 8 <= a.dim) {
+            constexpr int V = 16 / sizeof(E);
+#pragma unroll
+            for (int h = 0; h < 8 / V; ++h) {
+                const Pack<E, V> v = load_pack<E, V>(from + h * V);
+#pragma unroll
+                for (int j = 0; j < V; ++j) x[h * V + j] = to_f32(v.e[j]);
+            }
+        } else {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) x[j] = d + j < a.dim ? to_f32(from[j]) : 0.0f;
+        }
+        Pack<uint16_t, 8> plane[3];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const Split s = split(x[j]);
+            plane[0].e[j] = s.h;
+            plane[1].e[j] = s.m;
+            plane[2].e[j] = s.l;
+        }
+#pragma unroll
+        for (int p = 0; p < P; ++p)
+            store_pack<uint16_t, 8>(reinterpret_cast<uint16_t*>(out + p * a.rows.plane + r * (uint64_t)a.rows.stride) + d, plane[p]);
+    }
+}
+
 // ---- products -----------------------------------------------------------------------------
 
-// A tile of 64 x 64 f32 sums by 256 threads, 4 x 4 each: sum over k of a(k, m) b(k, n).
-template <typename A, typename B>
-__device__ __forceinline__ void tile_product(A&& a, B&& b, uint32_t depth, float (&acc)[4][4]) {
-    __shared__ float sa[16][64], sb[16][64];
-    const uint32_t t = threadIdx.x, tm = t >> 4, tn = t & 15;
-    for (uint32_t k0 = 0; k0 < depth; k0 += 16) {
-        __syncthreads();
-        for (uint32_t i = t; i < 1024; i += 256) {
-            const uint32_t m = i >> 4, k = i & 15;
-            sa[k][m] = k0 + k < depth ? a(k0 + k, m) : 0.0f;
-            sb[k][m] = k0 + k < depth ? b(k0 + k, m) : 0.0f;
-        }
-        __syncthreads();
-#pragma unroll
-        for (int k = 0; k < 16; ++k)
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-#pragma unroll
-                for (int j = 0; j < 4; ++j) acc[i][j] = __builtin_fmaf(sa[k][tm * 4 + i], sb[k][tn * 4 + j], acc[i][j]);
-    }
-}
+// Tiles of candidates with one tile of queries: BQ queries by TILE candidates, `along` of `splits` workgroups. `done` is
+// called with each tile's sums and its first place; the loads of the next tile's first step are under way meanwhile.
+// LANES_ARE_QUERIES: a lane holds four candidates (rows of the product) of one query, else four queries of one candidate.
+template <int BQ, bool LANES_ARE_QUERIES>
+struct Scores {
+    static constexpr int WAVES_Q = BQ >= 256 ? 4 : BQ >= 128 ? 2 : 1;  // waves side by side along the queries
+    static constexpr int WAVES_R = 8 / WAVES_Q;
+    static constexpr int WQ = BQ / WAVES_Q / 16, WR = TILE / WAVES_R / 16;  // fragments of a wave
+    static constexpr int TM = LANES_ARE_QUERIES ? WR : WQ, TN = LANES_ARE_QUERIES ? WQ : WR;
+    using R = Rows<TILE>;
+    using Q = Rows<BQ>;
+    static constexpr int LDS = 2 * (R::BYTES + Q::BYTES);
 
-// Logit of the candidate at `place` for query q from their product.
-__device__ __forceinline__ float logit(const XentArgs& a, uint32_t q, uint32_t place, float product) {
-    float z = product * a.qscale[q];
-    if (a.norms) {
-        const float n = a.norms[row_at(a, place)];
-        z = n > 0 ? z / n : 0.0f;
-    }
-    return z;
-}
+    __device__ __forceinline__ static uint32_t wave_q() { return (threadIdx.x >> 6) % WAVES_Q; }
+    __device__ __forceinline__ static uint32_t wave_r() { return (threadIdx.x >> 6) / WAVES_Q; }
 
-// Products of the 64 candidates from `first` (rows of the tile) with the 64 queries from q0 (columns).
-template <typename E>
-__device__ __forceinline__ void scores(const XentArgs& a, uint32_t first, uint32_t n, uint32_t q0, float (&acc)[4][4]) {
-    const E* rows = static_cast<const E*>(a.t.rows);
-    const E* q = static_cast<const E*>(a.q);
-    tile_product([&](uint32_t k, uint32_t m) { return first + m < n ? to_f32(rows[row_at(a, first + m) * a.t.stride + k]) : 0.0f; },
-                 [&](uint32_t k, uint32_t m) { return q0 + m < a.n_q ? to_f32(q[(uint64_t)(q0 + m) * a.kp + k]) : 0.0f; },
-                 a.t.dim, acc);
-}
-
-template <typename E>
-__global__ __launch_bounds__(256) void loss_kernel(XentArgs a) {
-    __shared__ float sm[16][64], sl[16][64];
-    const uint32_t t = threadIdx.x, tm = t >> 4, tn = t & 15, q0 = blockIdx.y * 64;
-    const uint32_t n = candidates(a);
-    float m[4], l[4] = {};
-#pragma unroll
-    for (int j = 0; j < 4; ++j) m[j] = -__builtin_inff();
-    for (uint32_t first = blockIdx.x * 64; first < n; first += gridDim.x * 64) {
-        float acc[4][4] = {};
-        scores<E>(a, first, n, q0, acc);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const uint32_t q = q0 + tn * 4 + j;
-            if (q >= a.n_q) continue;
-            const uint32_t click = a.click[q];
-            for (int i = 0; i < 4; ++i) {
-                const uint32_t place = first + tm * 4 + i;
-                if (place >= n) continue;
-                const float z = logit(a, q, place, acc[i][j]);
-                if (place == click) {
-                    a.click_z[q] = z;
-                    continue;
-                }
-                const float top = __builtin_fmaxf(m[j], z), ref = top == -__builtin_inff() ? 0.0f : top;
-                l[j] = l[j] * __expf(m[j] - ref) + __expf(z - ref);
-                m[j] = top;
+    template <typename F>
+    __device__ __forceinline__ static void run(const XentArgs& a, uint32_t end, uint32_t q0, uint32_t along, char* lds, F&& done) {
+        Planes rows = a.rows;
+        rows.rows = end - a.place0;
+        R r;
+        Q q;
+        r.init();
+        q.init();
+        q.aim(a.q, q0);
+        const uint32_t tiles = (end - a.piece_begin + TILE - 1) / TILE;
+        if (along >= tiles) return;
+        const uint32_t steps = (a.rows.chunks + 7) / 8 * a.score_steps.n;
+        const uint32_t base = a.piece_begin - a.place0;
+        r.peek(rows, base + along * TILE);
+        r.aim(rows, base + along * TILE);
+        auto half = [&](uint32_t i) { return lds + i * (R::BYTES + Q::BYTES); };
+        uint32_t at = 0, c = 0, k = 0;
+        auto issue = [&](uint32_t to) {
+            // (steps are counted as queries x rows; which of the two is A does not matter to six symmetric steps)
+            r.load(rows, k, a.score_steps.plane_b(c), a.zeros, half(to));
+            q.load(a.q, k, a.score_steps.plane_a(c), a.zeros, half(to) + R::BYTES);
+            if (++c == a.score_steps.n) {
+                c = 0;
+                ++k;
             }
+        };
+        issue(0);
+        for (uint32_t tile = along; tile < tiles; tile += a.splits) {
+            const bool more = tile + a.splits < tiles;
+            f32x4 acc[TM][TN] = {};
+            if (more) r.peek(rows, base + (tile + a.splits) * TILE);
+            for (uint32_t s = 0; s < steps; ++s) {
+                step_barrier();
+                if (s + 1 < steps) {
+                    issue(at ^ 1);
+                } else if (more) {
+                    c = k = 0;
+                    r.aim(rows, base + (tile + a.splits) * TILE);
+                    issue(at ^ 1);
+                }
+                char *lr = half(at), *lq = half(at) + R::BYTES;
+                if constexpr (LANES_ARE_QUERIES)
+                    multiply<R, Q, TM, TN>(lr, lq, wave_r() * WR, wave_q() * WQ, acc);
+                else
+                    multiply<Q, R, TM, TN>(lq, lr, wave_q() * WQ, wave_r() * WR, acc);
+                at ^= 1;
+            }
+            done(acc, a.piece_begin + tile * TILE);
         }
     }
-    for (int j = 0; j < 4; ++j) {
-        sm[tm][tn * 4 + j] = m[j];
-        sl[tm][tn * 4 + j] = l[j];
+};
+
+__device__ __forceinline__ float finite_or_zero(float m) { return m == -__builtin_inff() ? 0.0f : m; }
+
+// Per query the largest logit of a share of the candidates and the sum of the exponentials over it, the clicked row kept
+// out. Everything is in base 2 (logits times log2 e): an exponential is one instruction. A lane keeps the running largest
+// and sum of its own candidates, in registers, for each of its queries; lanes, waves and shares are joined at the end.
+template <int BQ, bool NORMS>
+__global__ __launch_bounds__(THREADS, 2) void loss_kernel(XentArgs a) {
+    using S = Scores<BQ, true>;
+    extern __shared__ __attribute__((aligned(128))) char lds[];
+    __shared__ float inverse[TILE], sm[S::WAVES_R][BQ], sl[S::WAVES_R][BQ];
+    const uint32_t lane = threadIdx.x & 63, group = lane >> 4;
+    uint32_t tile_q, along;
+    place_of_workgroup(a.across, &tile_q, &along);
+    const uint32_t end = min(candidates(a), a.piece_begin + a.piece_rows);
+    uint32_t click[S::TN];
+    float s2[S::TN], m[S::TN], l[S::TN];
+#pragma unroll
+    for (int n = 0; n < S::TN; ++n) {
+        const uint32_t q = tile_q * BQ + (S::wave_q() * S::WQ + n) * 16 + (lane & 15);
+        click[n] = q < a.n_q ? a.click[q] : NONE;
+        // (a factor of zero would make a number of the -inf that stands for what is left out: this one's logits are zero too)
+        s2[n] = __builtin_fmaxf(q < a.n_q ? a.qscale[q] * LOG2E : 0.0f, 1e-37f);
+        m[n] = -__builtin_inff();
+        l[n] = 0;
+    }
+    if (end > a.piece_begin)
+        S::run(a, end, tile_q * BQ, along, lds, [&](f32x4 (&acc)[S::TM][S::TN], uint32_t first) {
+            if constexpr (NORMS) {
+                if (threadIdx.x < TILE) {
+                    const float x = first + threadIdx.x < end ? a.norms[row_at(a, first + threadIdx.x)] : 0.0f;
+                    inverse[threadIdx.x] = x > 0 ? 1.0f / x : 0.0f;
+                }
+                __syncthreads();
+            }
+            const uint32_t local = S::wave_r() * S::WR * 16 + group * 4;  // of the lane's candidates t * 16 + r
+            if constexpr (NORMS) {
+#pragma unroll
+                for (int t = 0; t < S::TM; ++t) {
+                    const f32x4 inv = *reinterpret_cast<const f32x4*>(inverse + local + t * 16);
+#pragma unroll
+                    for (int n = 0; n < S::TN; ++n) acc[t][n] *= inv;
+                }
+                __syncthreads();  // (the next tile writes them)
+            }
+            bool special = end - first < TILE;
+#pragma unroll
+            for (int n = 0; n < S::TN; ++n) special |= click[n] - first < TILE;
+            if (__any(special)) {
+                // a tile with a clicked row, or the last one: what does not belong to the sum is taken out of it
+#pragma unroll
+                for (int n = 0; n < S::TN; ++n) {
+                    const uint32_t at = click[n] - first - local;
+                    const int left = (int)min(end - first, (uint32_t)TILE) - (int)local;
+                    float clicked = 0;
+#pragma unroll
+                    for (int t = 0; t < S::TM; ++t)
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) {
+                            const uint32_t i = t * 16 + r;
+                            clicked = at == i ? acc[t][n][r] : clicked;
+                            acc[t][n][r] = at == i || left <= (int)i ? -__builtin_inff() : acc[t][n][r];
+                        }
+                    // (the clicked row is one of the lane's if it is 0 .. 3 rows into one of its fragments)
+                    if (click[n] != NONE && at < S::TM * 16 && at % 16 < 4)
+                        a.click_z[tile_q * BQ + (S::wave_q() * S::WQ + n) * 16 + (lane & 15)] = clicked * s2[n];
+                }
+            }
+#pragma unroll
+            for (int n = 0; n < S::TN; ++n) {
+                float x = acc[0][n][0];
+#pragma unroll
+                for (int t = 0; t < S::TM; ++t)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) x = __builtin_fmaxf(x, acc[t][n][r]);
+                const float top = __builtin_fmaxf(m[n], x * s2[n]);  // (the factor is not negative)
+                const float ref = finite_or_zero(top);
+                float sum[4] = {l[n] * __builtin_amdgcn_exp2f(m[n] - ref), 0, 0, 0};
+#pragma unroll
+                for (int t = 0; t < S::TM; ++t)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) sum[r] += __builtin_amdgcn_exp2f(__builtin_fmaf(acc[t][n][r], s2[n], -ref));
+                l[n] = (sum[0] + sum[1]) + (sum[2] + sum[3]);
+                m[n] = top;
+            }
+        });
+    // lanes that hold other candidates of the same query, then waves, then what the pieces before this one left
+#pragma unroll
+    for (int n = 0; n < S::TN; ++n) {
+#pragma unroll
+        for (int d = 16; d < 64; d *= 2) {
+            const float om = __shfl_xor(m[n], d), ol = __shfl_xor(l[n], d), top = __builtin_fmaxf(m[n], om), ref = finite_or_zero(top);
+            l[n] = l[n] * __builtin_amdgcn_exp2f(m[n] - ref) + ol * __builtin_amdgcn_exp2f(om - ref);
+            m[n] = top;
+        }
+        if (lane < 16) {
+            sm[S::wave_r()][(S::wave_q() * S::WQ + n) * 16 + lane] = m[n];
+            sl[S::wave_r()][(S::wave_q() * S::WQ + n) * 16 + lane] = l[n];
+        }
     }
     __syncthreads();
-    if (t >= 64 || q0 + t >= a.n_q) return;
-    float top = -__builtin_inff(), sum = 0;
-    for (int i = 0; i < 16; ++i) top = __builtin_fmaxf(top, sm[i][t]);
-    for (int i = 0; i < 16; ++i) sum += sl[i][t] * __expf(sm[i][t] - (top == -__builtin_inff() ? 0.0f : top));
-    a.part_m[(uint64_t)blockIdx.x * a.n_q + q0 + t] = top;
-    a.part_l[(uint64_t)blockIdx.x * a.n_q + q0 + t] = sum;
+    const uint32_t q = tile_q * BQ + threadIdx.x;
+    if (threadIdx.x >= BQ || q >= a.n_q) return;
+    const uint64_t to = (uint64_t)along * a.n_q + q;
+    float top = a.first_piece ? -__builtin_inff() : a.part_m[to], sum = a.first_piece ? 0.0f : a.part_l[to];
+    const float before = top;
+    for (int w = 0; w < S::WAVES_R; ++w) top = __builtin_fmaxf(top, sm[w][threadIdx.x]);
+    const float ref = finite_or_zero(top);
+    sum *= __builtin_amdgcn_exp2f(before - ref);
+    for (int w = 0; w < S::WAVES_R; ++w) sum += sl[w][threadIdx.x] * __builtin_amdgcn_exp2f(sm[w][threadIdx.x] - ref);
+    a.part_m[to] = top;
+    a.part_l[to] = sum;
 }
 
-// A query's parts joined, in 64 bits (one thread's worth of work per query); one workgroup per query.
+// A query's shares joined, in 64 bits (one thread's worth of work per query); a wave per query.
 __global__ __launch_bounds__(256) void join_loss_kernel(XentArgs a, float* loss, float* lse) {
-    __shared__ float sm[256];
-    __shared__ double sl[256];
-    const uint32_t q = blockIdx.x, t = threadIdx.x;
+    const uint32_t q = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
+    if (q >= a.n_q) return;
     float top = -__builtin_inff();
-    for (uint32_t s = t; s < a.splits; s += 256) top = __builtin_fmaxf(top, a.part_m[(uint64_t)s * a.n_q + q]);
-    sm[t] = top;
-    __syncthreads();
-    for (int d = 128; d; d /= 2) {
-        if (t < d) sm[t] = __builtin_fmaxf(sm[t], sm[t + d]);
-        __syncthreads();
-    }
-    top = sm[0];
-    const float ref = top == -__builtin_inff() ? 0.0f : top;
+    for (uint32_t s = lane; s < a.splits; s += 64) top = __builtin_fmaxf(top, a.part_m[(uint64_t)s * a.n_q + q]);
+#pragma unroll
+    for (int d = 32; d; d /= 2) top = __builtin_fmaxf(top, __shfl_xor(top, d));
+    const float ref = finite_or_zero(top);
     double sum = 0;
-    for (uint32_t s = t; s < a.splits; s += 256) {
+    for (uint32_t s = lane; s < a.splits; s += 64) {
         const uint64_t at = (uint64_t)s * a.n_q + q;
-        sum += (double)a.part_l[at] * exp((double)a.part_m[at] - ref);
+        sum += (double)a.part_l[at] * (double)__builtin_amdgcn_exp2f(a.part_m[at] - ref);
     }
-    sl[t] = sum;
-    __syncthreads();
-    for (int d = 128; d; d /= 2) {
-        if (t < d) sl[t] += sl[t + d];
-        __syncthreads();
-    }
-    if (t) return;
-    const double rest = ref + log(sl[0]);  // -inf: no other candidate
+#pragma unroll
+    for (int d = 32; d; d /= 2) sum += __shfl_xor(sum, d);
+    if (lane) return;
+    constexpr double LN2 = 0.693147180559945309417;
+    const double rest = ref * LN2 + log(sum);  // -inf: no other candidate
     if (a.click[q] == NONE) {
         loss[q] = 0.0f;
         lse[q] = (float)rest;
         return;
     }
-    const double z = a.click_z[q], d = rest - z;
+    const double z = a.click_z[q] * LN2, d = rest - z;
     loss[q] = (float)(d > 0 ? d + log1p(exp(-d)) : log1p(exp(d)));
     lse[q] = (float)(d > 0 ? rest + log1p(exp(-d)) : z + log1p(exp(d)));
 }
 
 // ---- gradients ----------------------------------------------------------------------------
 
-template <typename E>
-__global__ __launch_bounds__(256) void weights_kernel(XentArgs a) {
-    const uint32_t t = threadIdx.x, tm = t >> 4, tn = t & 15, q0 = blockIdx.y * 64;
-    const uint32_t n = candidates(a), first = a.piece_begin + blockIdx.x * 64;
-    if (first >= n) return;
-    float acc[4][4] = {};
-    scores<E>(a, first, n, q0, acc);
-    for (int i = 0; i < 4; ++i) {
-        const uint32_t place = first + tm * 4 + i;
-        if (place >= n) continue;
-        for (int j = 0; j < 4; ++j) {
-            const uint32_t q = q0 + tn * 4 + j;
-            if (q >= a.n_q) continue;
-            const uint32_t click = a.click[q];
-            const float z = logit(a, q, place, acc[i][j]);
-            float g = place == click ? expm1f(-a.loss[q]) : __expf(z - a.lse[q]);
-            g *= (a.grad_loss ? a.grad_loss[q] : 1.0f) * a.qscale[q];
-            if (a.norms) {
-                const float norm = a.norms[row_at(a, place)];
-                g = norm > 0 ? g / norm : 0.0f;
+// The weights G of a piece, [candidate][query], rounded to bf16 (PG = 1), or kept to 16 bits (2) or all 24 (3) by as many
+// planes. A lane holds four neighbouring queries of a candidate: eight bytes a store.
+template <int BQ, bool NORMS, int PG>
+__global__ __launch_bounds__(THREADS, 2) void weights_kernel(XentArgs a) {
+    using S = Scores<BQ, false>;
+    extern __shared__ __attribute__((aligned(128))) char lds[];
+    __shared__ __attribute__((aligned(16))) float s2[BQ], lse2[BQ], factor[BQ], at_click[BQ];
+    __shared__ __attribute__((aligned(16))) uint32_t click[BQ];
+    const uint32_t lane = threadIdx.x & 63, group = lane >> 4;
+    uint32_t tile_q, along;
+    place_of_workgroup(a.across, &tile_q, &along);
+    const uint32_t q0 = tile_q * BQ;
+    const uint32_t end = min(candidates(a), a.piece_begin + a.piece_rows);
+    if (end <= a.piece_begin) return;
+    if (threadIdx.x < BQ) {
+        const uint32_t q = q0 + threadIdx.x;
+        const bool in = q < a.n_q;
+        click[threadIdx.x] = in ? a.click[q] : NONE;
+        s2[threadIdx.x] = in ? a.qscale[q] * LOG2E : 0.0f;
+        lse2[threadIdx.x] = in ? a.lse[q] * LOG2E : 0.0f;
+        const float f = in && a.click[q] != NONE ? (a.grad_loss ? a.grad_loss[q] : 1.0f) * a.qscale[q] * a.sign : 0.0f;
+        factor[threadIdx.x] = f;
+        at_click[threadIdx.x] = in ? f * expm1f(-a.loss[q]) : 0.0f;
+    }
+    // (the first barrier of the loop below orders these before they are read)
+    S::run(a, end, q0, along, lds, [&](f32x4 (&acc)[S::TM][S::TN], uint32_t first) {
+#pragma unroll
+        for (int n = 0; n < S::TN; ++n) {
+            const uint32_t place = first + (S::wave_r() * S::WR + n) * 16 + (lane & 15);
+            if (place >= end) continue;
+            float inverse = 1.0f;
+            if constexpr (NORMS) {
+                const float x = a.norms[row_at(a, place)];
+                inverse = x > 0 ? 1.0f / x : 0.0f;
             }
-            a.g[(uint64_t)(place - a.piece_begin) * a.n_q + q] = click == NONE ? 0.0f : g;
+            char* out = a.g + (uint64_t)(place - a.piece_begin) * a.gq * 2;
+#pragma unroll
+            for (int t = 0; t < S::TM; ++t) {
+                const uint32_t i = (S::wave_q() * S::WQ + t) * 16 + group * 4;
+                if (q0 + i >= a.gq) continue;
+                const f32x4 vs = *reinterpret_cast<const f32x4*>(s2 + i), vl = *reinterpret_cast<const f32x4*>(lse2 + i);
+                const f32x4 vf = *reinterpret_cast<const f32x4*>(factor + i), vc = *reinterpret_cast<const f32x4*>(at_click + i);
+                const u32x4 vp = *reinterpret_cast<const u32x4*>(click + i);
+                Pack<uint16_t, 4> p[3];
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    float z = acc[t][n][r];
+                    if constexpr (NORMS) z *= inverse;
+                    float g = vp[r] == place ? vc[r] : vf[r] * __builtin_amdgcn_exp2f(__builtin_fmaf(z, vs[r], -vl[r]));
+                    if (vf[r] == 0.0f) g = 0.0f;  // no click, no query (an exponential over a lse of -inf is none)
+                    if constexpr (NORMS) g *= inverse;
+                    if constexpr (PG == 1) {
+                        p[0].e[r] = (uint16_t)bf16_bits(g);
+                    } else {
+                        const Split x = split(g);
+                        p[0].e[r] = x.h;
+                        p[1].e[r] = x.m;
+                        p[2].e[r] = x.l;
+                    }
+                }
+#pragma unroll
+                for (int k = 0; k < PG; ++k)
+                    store_pack<uint16_t, 4>(reinterpret_cast<uint16_t*>(out + k * a.g_plane) + q0 + i, p[k]);
+            }
+        }
+    });
+}
+
+// drows of a piece: transposed queries (BD columns of the rows) by G. A lane holds four neighbouring columns of a row.
+template <int BD, typename E>
+__global__ __launch_bounds__(THREADS, 2) void row_grads_kernel(XentArgs a) {
+    using A = Rows<BD>;
+    using B = Rows<TILE>;
+    constexpr int WAVES_D = BD >= 256 ? 2 : 2, WAVES_R = 8 / WAVES_D;
+    constexpr int TM = BD / WAVES_D / 16, TN = TILE / WAVES_R / 16;
+    extern __shared__ __attribute__((aligned(128))) char lds[];
+    const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wd = wave % WAVES_D, wr = wave / WAVES_D;
+    uint32_t tile_d, along;
+    place_of_workgroup(a.across, &tile_d, &along);
+    const uint32_t end = min(candidates(a), a.piece_begin + a.piece_rows);
+    const uint32_t tiles = end > a.piece_begin ? (end - a.piece_begin + TILE - 1) / TILE : 0;
+    if (along >= tiles) return;
+    const Planes g{a.g, a.g_plane, a.gq * 2, nullptr, end - a.piece_begin, a.gq / 8};
+    A q;
+    B r;
+    q.init();
+    r.init();
+    q.aim(a.qt, tile_d * BD);
+    r.aim(g, along * TILE);
+    const uint32_t steps = a.gq / 64 * a.grad_steps.n;
+    auto half = [&](uint32_t i) { return lds + i * (A::BYTES + B::BYTES); };
+    uint32_t at = 0, c = 0, k = 0;
+    auto issue = [&](uint32_t to) {
+        q.load(a.qt, k, a.grad_steps.plane_b(c), a.zeros, half(to));
+        r.load(g, k, a.grad_steps.plane_a(c), a.zeros, half(to) + A::BYTES);
+        if (++c == a.grad_steps.n) {
+            c = 0;
+            ++k;
+        }
+    };
+    issue(0);
+    for (uint32_t tile = along; tile < tiles; tile += a.splits) {
+        const bool more = tile + a.splits < tiles;
+        f32x4 acc[TM][TN] = {};
+        for (uint32_t s = 0; s < steps; ++s) {
+            step_barrier();
+            if (s + 1 < steps) {
+                issue(at ^ 1);
+            } else if (more) {
+                c = k = 0;
+                r.aim(g, (tile + a.splits) * TILE);
+                issue(at ^ 1);
+            }
+            multiply<A, B, TM, TN>(half(at), half(at) + A::BYTES, wd * TM, wr * TN, acc);
+            at ^= 1;
+        }
+#pragma unroll
+        for (int n = 0; n < TN; ++n) {
+            const uint32_t place = a.piece_begin + tile * TILE + (wr * TN + n) * 16 + (lane & 15);
+            if (place >= end) continue;
+            E* out = static_cast<E*>(a.grad_rows) + row_at(a, place) * a.grad_row_stride;
+#pragma unroll
+            for (int m = 0; m < TM; ++m) {
+                const uint32_t d = tile_d * BD + (wd * TM + m) * 16 + (lane >> 4) * 4;
+                Pack<E, 4> p;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) p.e[i] = from_f32<E>(acc[m][n][i]);
+                if (a.grad_rows_wide && d + 4 <= a.dim)
+                    store_pack<E, 4>(out + d, p);
+                else
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        if (d + i < a.dim) out[d + i] = p.e[i];
+            }
         }
     }
 }
 
-template <typename E>
-__global__ __launch_bounds__(256) void row_grads_kernel(XentArgs a) {
-    const uint32_t t = threadIdx.x, tm = t >> 4, tn = t & 15, d0 = blockIdx.y * 64;
-    const uint32_t n = candidates(a), first = a.piece_begin + blockIdx.x * 64;
-    if (first >= n) return;
-    const E* q = static_cast<const E*>(a.q);
-    float acc[4][4] = {};
-    tile_product([&](uint32_t k, uint32_t m) { return first + m < n ? a.g[(uint64_t)(first + m - a.piece_begin) * a.n_q + k] : 0.0f; },
-                 [&](uint32_t k, uint32_t m) { return d0 + m < a.t.dim ? to_f32(q[(uint64_t)k * a.kp + d0 + m]) : 0.0f; }, a.n_q, acc);
-    E* out = static_cast<E*>(a.grad_rows);
-    for (int i = 0; i < 4; ++i)
-        for (int j = 0; j < 4; ++j) {
-            const uint32_t place = first + tm * 4 + i, d = d0 + tn * 4 + j;
-            if (place < n && d < a.t.dim) out[row_at(a, place) * a.grad_row_stride + d] = from_f32<E>(acc[i][j]);
+// dqueries over one share of a piece's candidates: G by rows, the sum running over the candidates.
+template <int BQ, int BD>
+__global__ __launch_bounds__(THREADS, 2) void query_grads_kernel(XentArgs a) {
+    using A = Cols<BQ>;
+    using B = Cols<BD>;
+    constexpr int WAVES_Q = BQ >= 128 ? 2 : 1, WAVES_D = 8 / WAVES_Q;
+    constexpr int TM = BQ / WAVES_Q / 16, TN = BD / WAVES_D / 16;
+    extern __shared__ __attribute__((aligned(128))) char lds[];
+    const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wq = wave % WAVES_Q, wd = wave / WAVES_Q;
+    const uint32_t d_tiles = (a.dim + BD - 1) / BD;
+    uint32_t tile, share;
+    place_of_workgroup(a.across, &tile, &share);
+    const uint32_t tile_d = tile % d_tiles, tile_q = tile / d_tiles;
+    const uint32_t end = min(candidates(a), a.piece_begin + a.piece_rows);
+    const uint32_t n = end > a.piece_begin ? end - a.piece_begin : 0;
+    // shares are whole steps of the rows that there are
+    const uint32_t per = ((n + STEP - 1) / STEP + a.splits - 1) / a.splits * STEP;
+    const uint32_t begin = (uint32_t)min((uint64_t)share * per, (uint64_t)n), stop = min(begin + per, n);
+    f32x4 acc[TM][TN] = {};
+    const uint32_t blocks = (stop - begin + STEP - 1) / STEP, steps = blocks * a.grad_steps.n;
+    if (steps) {
+        const Planes g{a.g, a.g_plane, a.gq * 2, nullptr, n, a.gq / 8};
+        Planes rows = a.rows;
+        rows.rows = end - a.place0;
+        const uint32_t base = a.piece_begin - a.place0;
+        A w;
+        B r;
+        w.init();
+        r.init();
+        auto half = [&](uint32_t i) { return lds + i * (A::BYTES + B::BYTES); };
+        uint32_t c = 0, k = 0, at = 0;
+        auto issue = [&](uint32_t to) {
+            const uint32_t from = begin + k * STEP;
+            w.load(g, from, stop, tile_q * (BQ / 8), a.grad_steps.plane_a(c), a.zeros, half(to));
+            r.load(rows, base + from, base + stop, tile_d * (BD / 8), a.grad_steps.plane_b(c), a.zeros, half(to) + A::BYTES);
+            if (++c == a.grad_steps.n) {
+                c = 0;
+                ++k;
+                if (k < blocks) r.peek(rows, base + from + STEP, base + stop);  // while this step multiplies
+            }
+        };
+        r.peek(rows, base + begin, base + stop);
+        issue(0);
+        for (uint32_t s = 0; s < steps; ++s) {
+            step_barrier();
+            if (s + 1 < steps) issue(at ^ 1);
+            multiply<A, B, TM, TN>(half(at), half(at) + A::BYTES, wq * TM, wd * TN, acc);
+            at ^= 1;
         }
-}
-
-// dqueries over one share of a piece's candidates.
-template <typename E>
-__global__ __launch_bounds__(256) void query_grads_kernel(XentArgs a) {
-    const uint32_t t = threadIdx.x, tm = t >> 4, tn = t & 15, d0 = blockIdx.y * 64, q0 = blockIdx.z * 64;
-    const uint32_t n = min(candidates(a), a.piece_begin + a.piece_rows);
-    const uint32_t share = (a.piece_rows + a.splits - 1) / a.splits;
-    const uint32_t begin = min(a.piece_begin + blockIdx.x * share, n), end = min(begin + share, n);
-    const E* rows = static_cast<const E*>(a.t.rows);
-    float acc[4][4] = {};
-    tile_product([&](uint32_t k, uint32_t m) { return q0 + m < a.n_q ? a.g[(uint64_t)(begin + k - a.piece_begin) * a.n_q + q0 + m] : 0.0f; },
-                 [&](uint32_t k, uint32_t m) { return d0 + m < a.t.dim ? to_f32(rows[row_at(a, begin + k) * a.t.stride + d0 + m]) : 0.0f; },
-                 end - begin, acc);
-    for (int i = 0; i < 4; ++i)
-        for (int j = 0; j < 4; ++j) {
-            const uint32_t q = q0 + tm * 4 + i, d = d0 + tn * 4 + j;
-            if (q >= a.n_q || d >= a.t.dim) continue;
-            float* p = a.part_q + ((uint64_t)blockIdx.x * a.n_q + q) * a.t.dim + d;
-            *p = a.first_piece ? acc[i][j] : *p + acc[i][j];
+    }
+#pragma unroll
+    for (int m = 0; m < TM; ++m)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const uint32_t q = tile_q * BQ + (wq * TM + m) * 16 + (lane >> 4) * 4 + i;
+            if (q >= a.n_q) continue;
+#pragma unroll
+            for (int t = 0; t < TN; ++t) {
+                const uint32_t d = tile_d * BD + (wd * TN + t) * 16 + (lane & 15);
+                if (d >= a.dim) continue;
+                float* p = a.part_q + ((uint64_t)share * a.n_q + q) * a.dim + d;
+                *p = a.first_piece ? acc[m][t][i] : *p + acc[m][t][i];
+            }
         }
 }
 
 // The shares of a query's gradient joined, and taken through the query's length where logits are cosines; one
-// workgroup per query.
-template <typename E, typename O>
-__global__ __launch_bounds__(256) void join_query_grads_kernel(XentArgs a, O* out, uint64_t out_stride) {
+// workgroup per (query, 256 columns), or per query where its length is needed.
+template <typename Q, typename O>
+__global__ __launch_bounds__(256) void join_query_grads_kernel(XentArgs a, const Q* queries, uint64_t stride, bool round, O* out,
+                                                               uint64_t out_stride) {
     __shared__ float sums[8];
     const uint32_t q = blockIdx.x;
-    const E* query = static_cast<const E*>(a.q) + (uint64_t)q * a.kp;
-    float* sum0 = a.part_q + (uint64_t)q * a.t.dim;
+    float* sum0 = a.part_q + (uint64_t)q * a.dim;
     float dot = 0, sq = 0;
-    for (uint32_t d = threadIdx.x; d < a.t.dim; d += 256) {
+    for (uint32_t d = blockIdx.y * 256 + threadIdx.x; d < a.dim; d += gridDim.y * 256) {
         float sum = 0;
-        for (uint32_t s = 0; s < a.splits; ++s) sum += a.part_q[((uint64_t)s * a.n_q + q) * a.t.dim + d];
+#pragma unroll 8
+        for (uint32_t s = 0; s < a.splits; ++s) sum += a.part_q[((uint64_t)s * a.n_q + q) * a.dim + d];
         if (!a.norms) {
             out[q * out_stride + d] = from_f32<O>(sum);
             continue;
         }
-        const float x = to_f32(query[d]);
+        float x = to_f32(queries[q * stride + d]);
+        if (round) x = __builtin_bit_cast(float, bf16_bits(x) << 16);
         dot = __builtin_fmaf(sum, x, dot);
         sq = __builtin_fmaf(x, x, sq);
         sum0[d] = sum;
@@ -340,7 +656,11 @@ __global__ __launch_bounds__(256) void join_query_grads_kernel(XentArgs a, O* ou
     dot = sums[0] + sums[1] + sums[2] + sums[3];
     sq = sums[4] + sums[5] + sums[6] + sums[7];
     const float along = sq > 0 ? dot / sq : 0.0f;
-    for (uint32_t d = threadIdx.x; d < a.t.dim; d += 256) out[q * out_stride + d] = from_f32<O>(sum0[d] - along * to_f32(query[d]));
+    for (uint32_t d = threadIdx.x; d < a.dim; d += 256) {
+        float x = to_f32(queries[q * stride + d]);
+        if (round) x = __builtin_bit_cast(float, bf16_bits(x) << 16);
+        out[q * out_stride + d] = from_f32<O>(sum0[d] - along * x);
+    }
 }
 
 // Rows that are no candidates have gradient zero (`all`: every row, where there is no query).
@@ -355,87 +675,217 @@ __global__ __launch_bounds__(256) void clear_rows_kernel(const uint64_t* mask, c
 
 // ---- host side ----------------------------------------------------------------------------
 
-constexpr uint64_t PIECE_BYTES = 256u << 20;  // of the gradient weights that are held at a time
+constexpr uint64_t PIECE_BYTES = 256u << 20;  // of weights, and of planes, that are held at a time: the size of the
+                                              // memory-side cache, from which the products read them again
+constexpr uint32_t WORKGROUPS = 256;          // of a product: one per CU (the LDS of a tile fills one)
+
+// hh, hm, mh, mm, hl, lh | plane 0 alone | planes 0 and 1 of A
+constexpr Steps SIX{6, 0u | 0u << 2 | 1u << 4 | 1u << 6 | 0u << 8 | 2u << 10, 0u | 1u << 2 | 0u << 4 | 1u << 6 | 2u << 8 | 0u << 10};
+constexpr Steps ONE{1, 0, 0}, TWO{2, 0u | 1u << 2, 0};
 
 struct Plan {
-    uint32_t kp, loss_splits, grad_splits;
-    uint64_t piece_rows;
+    uint32_t planes, g_planes, kp, gq, loss_bq, bq, bd, q_tiles, loss_q_tiles, d_tiles;
+    uint32_t loss_splits, weight_splits, row_splits, grad_splits;
+    uint64_t piece_rows, packed_rows;
 };
+
+// Workgroups along the rows for `across` side by side: a multiple of eight (the XCDs), enough for every CU.
+uint32_t splits_for(uint32_t across, uint64_t tiles) {
+    const uint64_t want = std::max<uint64_t>(WORKGROUPS / across, 1);
+    return (uint32_t)round_up(std::min(want, tiles), 8);
+}
 
 Plan plan_for(uint32_t n_q, uint64_t n_rows, uint32_t dim, int32_t dtype) {
     Plan p;
-    p.kp = (dim + 63) / 64 * 64;
-    p.loss_splits = (uint32_t)std::min<uint64_t>((n_rows + 63) / 64, 1024);
-    p.piece_rows = std::min<uint64_t>(std::max<uint64_t>(PIECE_BYTES / 4 / n_q / 64 * 64, 64), (n_rows + 63) / 64 * 64);
-    p.grad_splits = (uint32_t)std::min<uint64_t>((p.piece_rows + 63) / 64, 16);
+    p.planes = dtype == VS_F32 ? 3 : 1;
+    // One rounding of a weight is of the size of the rounding of a gradient. Where few queries, or few large weights, make
+    // up a gradient it shows, and where queries are few the second plane costs nothing: the rows' bytes bound the products.
+    p.g_planes = dtype == VS_F32 ? 3 : n_q <= 64 ? 2 : 1;
+    p.kp = (uint32_t)round_up(dim, 64);
+    p.gq = (uint32_t)round_up(n_q, 64);
+    p.loss_bq = n_q <= 16 ? 16 : n_q <= 64 ? 64 : n_q <= 128 ? 128 : 256;
+    p.bq = n_q <= 64 ? 64 : n_q <= 128 ? 128 : 256;
+    p.bd = (dim + 127) / 128 % 2 ? 128 : 256;
+    p.loss_q_tiles = (n_q + p.loss_bq - 1) / p.loss_bq;
+    p.q_tiles = (n_q + p.bq - 1) / p.bq;
+    p.d_tiles = (dim + p.bd - 1) / p.bd;
+    const uint64_t rows = round_up(n_rows, TILE), per = TILE * (uint64_t)WORKGROUPS;
+    auto piece = [&](uint64_t row_bytes) {
+        uint64_t r = std::max<uint64_t>(PIECE_BYTES / row_bytes / TILE * TILE, TILE);
+        if (r > per) r = r / per * per;  // whole rounds of the workgroups
+        return std::min(r, rows);
+    };
+    p.piece_rows = piece((uint64_t)p.gq * 2 * p.g_planes);
+    p.packed_rows = std::min(p.piece_rows, piece((uint64_t)p.kp * 2 * p.planes));
+    const uint64_t tiles = rows / TILE;
+    p.loss_splits = splits_for(p.loss_q_tiles, tiles);
+    p.weight_splits = splits_for(p.q_tiles, tiles);
+    p.row_splits = splits_for(p.d_tiles, tiles);
+    p.grad_splits = splits_for(p.q_tiles * p.d_tiles, tiles * (TILE / STEP));
     return p;
 }
 
 struct Buffers {
-    uint32_t *list, *count, *click;
-    float *qscale, *part_m, *part_l, *click_z, *g, *part_q;
-    void* q;
+    uint32_t *zeros, *list, *count, *click;
+    float *qscale, *part_m, *part_l, *click_z, *part_q;
+    char *q, *qt, *g, *packed;
     uint64_t bytes;
 };
-Buffers carve(void* workspace, const Plan& p, uint32_t n_q, uint64_t n_rows, uint32_t dim, int32_t dtype) {
+Buffers carve(void* workspace, const Plan& p, uint32_t n_q, uint64_t n_rows, uint32_t dim) {
     Carver w(workspace);
     Buffers b;
+    b.zeros = w.take<uint32_t>(64);
     b.list = w.take<uint32_t>(n_rows);
     b.count = w.take<uint32_t>(1);
     b.click = w.take<uint32_t>(n_q);
     b.qscale = w.take<float>(n_q);
     b.click_z = w.take<float>(n_q);
-    b.q = w.take<char>((uint64_t)n_q * p.kp * (dtype == VS_F32 ? 4 : 2));
+    b.q = w.take<char>((uint64_t)n_q * p.kp * 2 * p.planes);
+    b.qt = w.take<char>((uint64_t)dim * p.gq * 2 * p.planes);
     b.part_m = w.take<float>((uint64_t)p.loss_splits * n_q);
     b.part_l = w.take<float>((uint64_t)p.loss_splits * n_q);
-    b.g = w.take<float>(p.piece_rows * n_q);
+    b.g = w.take<char>(p.piece_rows * p.gq * 2 * p.g_planes);
     b.part_q = w.take<float>((uint64_t)p.grad_splits * n_q * dim);
+    b.packed = w.take<char>(p.packed_rows * p.kp * 2 * p.planes);
     b.bytes = w.at() - (char*)workspace;
     return b;
 }
 
-XentArgs prepare(const Xent& x, const Plan& p, const Buffers& b, hipStream_t stream) {
+// A call's plan, buffers and arguments.
+struct Call {
+    const Xent& x;
+    Plan p;
+    Buffers b;
     XentArgs a{};
-    a.t = x.t;
-    a.norms = x.norms;
-    a.q = b.q;
-    a.kp = p.kp;
-    a.n_q = x.n_q;
-    a.click = b.click;
-    a.qscale = b.qscale;
-    a.part_m = b.part_m;
-    a.part_l = b.part_l;
-    a.click_z = b.click_z;
-    a.g = b.g;
-    a.part_q = b.part_q;
-    if (x.mask || x.t.present) {
-        a.list = b.list;
-        a.count = b.count;
-        const uint64_t n_words = (x.t.n_rows + 63) / 64;
-        list_candidates_kernel<<<(uint32_t)((n_words + 1023) / 1024), 256, 0, stream>>>(x.mask, x.t.present, x.t.n_rows, b.list, b.count);
-    }
-    if (x.t.dtype == VS_F32)
-        pack_queries_kernel<float, float><<<x.n_q, 256, 0, stream>>>(a, (const float*)x.queries, x.query_stride, x.targets, x.scale, b.click, b.qscale);
-    else if (x.queries_f32)
-        pack_queries_kernel<bf16, float><<<x.n_q, 256, 0, stream>>>(a, (const float*)x.queries, x.query_stride, x.targets, x.scale, b.click, b.qscale);
-    else
-        pack_queries_kernel<bf16, bf16><<<x.n_q, 256, 0, stream>>>(a, (const bf16*)x.queries, x.query_stride, x.targets, x.scale, b.click, b.qscale);
-    return a;
-}
+    bool packed;
+    hipStream_t stream;
+    hipError_t error = hipSuccess;
 
-template <typename E>
-void run_grads(XentArgs a, const Plan& p, bool rows_too, hipStream_t stream) {
-    const uint32_t qb = (a.n_q + 63) / 64, db = (a.t.dim + 63) / 64;
-    for (uint64_t begin = 0; begin < a.t.n_rows; begin += p.piece_rows) {
-        a.piece_begin = (uint32_t)begin;
-        a.piece_rows = (uint32_t)std::min<uint64_t>(p.piece_rows, a.t.n_rows - begin);
-        a.first_piece = !begin;
-        const uint32_t tiles = (a.piece_rows + 63) / 64;
-        weights_kernel<E><<<dim3(tiles, qb), 256, 0, stream>>>(a);
-        if (rows_too) row_grads_kernel<E><<<dim3(tiles, db), 256, 0, stream>>>(a);
-        if (a.part_q) query_grads_kernel<E><<<dim3(a.splits, db, qb), 256, 0, stream>>>(a);
+    Call(const Xent& x_, void* workspace, bool gradients, hipStream_t stream_)
+        : x(x_), p(plan_for(x.n_q, x.t.n_rows, x.t.dim, x.t.dtype)), b(carve(workspace, p, x.n_q, x.t.n_rows, x.t.dim)), stream(stream_) {
+        const uint32_t dim = x.t.dim;
+        // straight from the table where a row is whole 16-byte chunks at multiples of 16 bytes
+        packed = x.t.dtype == VS_F32 || (uintptr_t)x.t.rows % 16 || x.t.stride % 8 || x.t.stride * 2 > 0xFFFFFFFFu || dim % 8;
+        a.n_rows = x.t.n_rows;
+        a.norms = x.norms;
+        a.q = Planes{b.q, (uint64_t)x.n_q * p.kp * 2, p.kp * 2, nullptr, x.n_q, p.kp / 8};
+        a.qt = Planes{b.qt, (uint64_t)dim * p.gq * 2, p.gq * 2, nullptr, dim, p.gq / 8};
+        a.n_q = x.n_q;
+        a.gq = p.gq;
+        a.dim = dim;
+        a.click = b.click;
+        a.qscale = b.qscale;
+        a.sign = x.scale < 0 ? -1.0f : 1.0f;
+        a.score_steps = p.planes == 3 ? SIX : ONE;
+        a.grad_steps = p.planes == 3 ? SIX : p.g_planes == 2 ? TWO : ONE;
+        a.zeros = (const char*)b.zeros;
+        a.part_m = b.part_m;
+        a.part_l = b.part_l;
+        a.click_z = b.click_z;
+        a.g = b.g;
+        a.g_planes = p.g_planes;
+        a.g_plane = p.piece_rows * p.gq * 2;
+        a.part_q = b.part_q;
+        if (x.mask || x.t.present) {
+            a.list = b.list;
+            a.count = b.count;
+            const uint64_t n_words = (x.t.n_rows + 63) / 64;
+            list_candidates_kernel<<<(uint32_t)((n_words + 1023) / 1024), 256, 0, stream>>>(x.mask, x.t.present, x.t.n_rows, b.list, b.count);
+        }
+        a.rows = packed ? Planes{b.packed, p.packed_rows * p.kp * 2, p.kp * 2, nullptr, 0, p.kp / 8}
+                        : Planes{(const char*)x.t.rows, 0, (uint32_t)x.t.stride * 2, a.list, 0, dim / 8};
+        const uint32_t grid = p.gq / 64 * (p.kp / 64) + (x.n_q + 3) / 4;
+        auto pack = [&](auto kernel, auto* q) {
+            kernel<<<grid, 256, 0, stream>>>(a, q, x.query_stride, x.targets, x.t.first_id, x.t.n_rows, x.scale, b.click, b.qscale, b.zeros, gradients);
+        };
+        if (x.t.dtype == VS_F32)
+            pack(pack_queries_kernel<float, 3>, (const float*)x.queries);
+        else if (x.queries_f32)
+            pack(pack_queries_kernel<float, 1>, (const float*)x.queries);
+        else
+            pack(pack_queries_kernel<bf16, 1>, (const bf16*)x.queries);
     }
-}
+
+    // `body` for every piece of the candidates, of at most `rows`, its planes ready.
+    template <typename F>
+    void for_pieces(uint64_t rows, F&& body) {
+        for (uint64_t begin = 0; begin < x.t.n_rows; begin += rows) {
+            a.piece_begin = (uint32_t)begin;
+            a.piece_rows = (uint32_t)std::min(rows, x.t.n_rows - begin);
+            a.first_piece = !begin;
+            a.place0 = packed ? a.piece_begin : 0;
+            if (packed) pack_rows();
+            body();
+        }
+    }
+
+    void pack_rows() {
+        const uint64_t threads = (uint64_t)a.piece_rows * a.rows.chunks;
+        const uint32_t grid = (uint32_t)std::min<uint64_t>((threads + 255) / 256, 1u << 16);
+        auto go = [&](auto wide, auto kernel, auto* t) { kernel<<<grid, 256, 0, stream>>>(a, t, x.t.stride, b.packed); };
+        if (x.t.dtype == VS_F32) {
+            const float* t = (const float*)x.t.rows;
+            aligned_rows<float, 4>(t, x.t.stride) ? go(0, pack_rows_kernel<float, 3, true>, t) : go(0, pack_rows_kernel<float, 3, false>, t);
+        } else {
+            const bf16* t = (const bf16*)x.t.rows;
+            aligned_rows<bf16, 8>(t, x.t.stride) ? go(0, pack_rows_kernel<bf16, 1, true>, t) : go(0, pack_rows_kernel<bf16, 1, false>, t);
+        }
+    }
+
+    // A product over the tiles of the piece.
+    template <typename K>
+    void product(K kernel, uint32_t lds, uint32_t across, uint32_t splits) {
+        a.across = across;
+        a.splits = splits;
+        if (error == hipSuccess) error = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+        if (error == hipSuccess) kernel<<<across * splits, THREADS, lds, stream>>>(a);
+    }
+
+    template <bool NORMS>
+    void loss() {
+        switch (p.loss_bq) {
+            case 16: return product(loss_kernel<16, NORMS>, Scores<16, true>::LDS, p.loss_q_tiles, p.loss_splits);
+            case 64: return product(loss_kernel<64, NORMS>, Scores<64, true>::LDS, p.loss_q_tiles, p.loss_splits);
+            case 128: return product(loss_kernel<128, NORMS>, Scores<128, true>::LDS, p.loss_q_tiles, p.loss_splits);
+            default: return product(loss_kernel<256, NORMS>, Scores<256, true>::LDS, p.loss_q_tiles, p.loss_splits);
+        }
+    }
+
+    template <bool NORMS, int PG>
+    void weights() {
+        switch (p.bq) {
+            case 64: return product(weights_kernel<64, NORMS, PG>, Scores<64, false>::LDS, p.q_tiles, p.weight_splits);
+            case 128: return product(weights_kernel<128, NORMS, PG>, Scores<128, false>::LDS, p.q_tiles, p.weight_splits);
+            default: return product(weights_kernel<256, NORMS, PG>, Scores<256, false>::LDS, p.q_tiles, p.weight_splits);
+        }
+    }
+    template <bool NORMS>
+    void weights() {
+        if (p.g_planes == 3) return weights<NORMS, 3>();
+        if (p.g_planes == 2) return product(weights_kernel<64, NORMS, 2>, Scores<64, false>::LDS, p.q_tiles, p.weight_splits);
+        weights<NORMS, 1>();
+    }
+
+    template <typename E>
+    void row_grads() {
+        p.bd == 256 ? product(row_grads_kernel<256, E>, 2 * (Rows<256>::BYTES + Rows<TILE>::BYTES), p.d_tiles, p.row_splits)
+                    : product(row_grads_kernel<128, E>, 2 * (Rows<128>::BYTES + Rows<TILE>::BYTES), p.d_tiles, p.row_splits);
+    }
+
+    template <int BQ>
+    void query_grads() {
+        const uint32_t across = p.q_tiles * p.d_tiles;
+        p.bd == 256 ? product(query_grads_kernel<BQ, 256>, 2 * (Cols<BQ>::BYTES + Cols<256>::BYTES), across, p.grad_splits)
+                    : product(query_grads_kernel<BQ, 128>, 2 * (Cols<BQ>::BYTES + Cols<128>::BYTES), across, p.grad_splits);
+    }
+
+    template <typename Q, typename O>
+    void join_query_grads(void* out, uint64_t out_stride) {
+        a.splits = p.grad_splits;
+        const dim3 grid(x.n_q, a.norms ? 1 : (a.dim + 255) / 256);
+        join_query_grads_kernel<Q, O><<<grid, 256, 0, stream>>>(a, (const Q*)x.queries, x.query_stride, x.t.dtype == VS_BF16, (O*)out, out_stride);
+    }
+};
 
 void clear_rows(const Xent& x, void* grad_rows, uint64_t stride, bool all, hipStream_t stream) {
     const uint32_t grid = (uint32_t)std::min<uint64_t>((x.t.n_rows + 3) / 4, 1u << 16);
@@ -448,19 +898,15 @@ void clear_rows(const Xent& x, void* grad_rows, uint64_t stride, bool all, hipSt
 }  // namespace
 
 uint64_t xent_workspace_bytes(uint32_t n_q, uint64_t n_rows, uint32_t dim, int32_t dtype) {
-    return carve(nullptr, plan_for(n_q, n_rows, dim, dtype), n_q, n_rows, dim, dtype).bytes + 256;
+    return carve(nullptr, plan_for(n_q, n_rows, dim, dtype), n_q, n_rows, dim).bytes + 256;
 }
 
 hipError_t launch_xent(const Xent& x, void* workspace, float* loss, float* lse, hipStream_t stream) {
-    const Plan p = plan_for(x.n_q, x.t.n_rows, x.t.dim, x.t.dtype);
-    XentArgs a = prepare(x, p, carve(workspace, p, x.n_q, x.t.n_rows, x.t.dim, x.t.dtype), stream);
-    a.splits = p.loss_splits;
-    const dim3 grid(a.splits, (x.n_q + 63) / 64);
-    if (x.t.dtype == VS_F32)
-        loss_kernel<float><<<grid, 256, 0, stream>>>(a);
-    else
-        loss_kernel<bf16><<<grid, 256, 0, stream>>>(a);
-    join_loss_kernel<<<x.n_q, 256, 0, stream>>>(a, loss, lse);
+    Call c(x, workspace, false, stream);
+    c.for_pieces(c.packed ? c.p.packed_rows : x.t.n_rows, [&] { x.norms ? c.loss<true>() : c.loss<false>(); });
+    c.a.splits = c.p.loss_splits;
+    if (c.error != hipSuccess) return c.error;
+    join_loss_kernel<<<(x.n_q + 3) / 4, 256, 0, stream>>>(c.a, loss, lse);
     return hipGetLastError();
 }
 
@@ -471,27 +917,30 @@ hipError_t launch_xent_grad(const Xent& x, const float* loss, const float* lse, 
         if (grad_rows) clear_rows(x, grad_rows, grad_row_stride, true, stream);
         return hipGetLastError();
     }
-    const Plan p = plan_for(x.n_q, x.t.n_rows, x.t.dim, x.t.dtype);
-    XentArgs a = prepare(x, p, carve(workspace, p, x.n_q, x.t.n_rows, x.t.dim, x.t.dtype), stream);
-    a.splits = p.grad_splits;
-    a.loss = loss;
-    a.lse = lse;
-    a.grad_loss = grad_loss;
-    a.grad_rows = grad_rows;
-    a.grad_row_stride = grad_row_stride;
-    if (!grad_queries) a.part_q = nullptr;
-    if (grad_rows && a.list) clear_rows(x, grad_rows, grad_row_stride, false, stream);
-    if (x.t.dtype == VS_F32)
-        run_grads<float>(a, p, grad_rows != nullptr, stream);
-    else
-        run_grads<bf16>(a, p, grad_rows != nullptr, stream);
+    if (!grad_queries && !grad_rows) return hipSuccess;
+    Call c(x, workspace, true, stream);
+    c.a.loss = loss;
+    c.a.lse = lse;
+    c.a.grad_loss = grad_loss;
+    c.a.grad_rows = grad_rows;
+    c.a.grad_row_stride = grad_row_stride;
+    const bool f32 = x.t.dtype == VS_F32;
+    c.a.grad_rows_wide = f32 ? aligned_rows<float, 4>(grad_rows, grad_row_stride) : aligned_rows<bf16, 4>(grad_rows, grad_row_stride);
+    if (grad_rows && c.a.list) clear_rows(x, grad_rows, grad_row_stride, false, stream);
+    c.for_pieces(c.packed ? c.p.packed_rows : c.p.piece_rows, [&] {
+        x.norms ? c.weights<true>() : c.weights<false>();
+        if (grad_rows) f32 ? c.row_grads<float>() : c.row_grads<bf16>();
+        if (!grad_queries) return;
+        c.p.bq == 64 ? c.query_grads<64>() : c.p.bq == 128 ? c.query_grads<128>() : c.query_grads<256>();
+    });
+    if (c.error != hipSuccess) return c.error;
     if (grad_queries) {
-        if (x.t.dtype == VS_F32)
-            join_query_grads_kernel<float, float><<<x.n_q, 256, 0, stream>>>(a, (float*)grad_queries, grad_query_stride);
+        if (f32)
+            c.join_query_grads<float, float>(grad_queries, grad_query_stride);
         else if (grad_queries_f32)
-            join_query_grads_kernel<bf16, float><<<x.n_q, 256, 0, stream>>>(a, (float*)grad_queries, grad_query_stride);
+            c.join_query_grads<float, float>(grad_queries, grad_query_stride);
         else
-            join_query_grads_kernel<bf16, bf16><<<x.n_q, 256, 0, stream>>>(a, (bf16*)grad_queries, grad_query_stride);
+            c.join_query_grads<bf16, bf16>(grad_queries, grad_query_stride);
     }
     return hipGetLastError();
 }
