@@ -49,6 +49,20 @@ inline bool aligned_rows(const void* base, uint64_t stride) {
     return (uintptr_t)base % alignof(Pack<E, V>) == 0 && stride * sizeof(E) % alignof(Pack<E, V>) == 0;
 }
 
+// A value that the compiler takes for a new one: what is computed from it is not kept in registers across a loop.
+__device__ __forceinline__ uint32_t afresh(uint32_t x) {
+    asm volatile("" : "+v"(x));
+    return x;
+}
+
+// The same for a value that all lanes share (a flag of a loop: the compiler would make a copy of the loop's body for each
+// of its values, and run out of registers between them).
+__device__ __forceinline__ uint32_t afresh_uniform(uint32_t x) {
+    x = uniform_u32(x);
+    asm volatile("" : "+s"(x));
+    return x;
+}
+
 __device__ __forceinline__ float wave_sum(float v) { return wave_sum_f32(v); }
 
 // Sum of x over the threads before this one, and over all, in a workgroup of 256.

@@ -1,10 +1,8 @@
 // Products of tiles on the bf16 matrix cores: the loop that the cross entropy's four products share.
 //
 // A workgroup of eight waves makes a tile of M x N sums over k, 64 k at a time. Both operands' pieces of a step go from
-// memory straight into LDS (16 bytes a lane, no registers), into the half that the step before last has left, while the
-// matrix cores work on the other half: one barrier a step, at which the loads that were issued a whole step ago are
-// waited for. 256 x 256 tiles read each byte of LDS for 128 x 64 products per wave, which leaves the LDS port at three
-// quarters of the matrix time; 64 KiB a step, twice, are 128 of the 160 KiB of a CU.
+// memory straight into LDS (16 bytes a lane, no registers), into the half that the step before has left, while the matrix
+// cores work on the other half: one barrier a step. 64 KiB a step, twice, are 128 of the 160 KiB of a CU.
 //
 // Operands come in two shapes:
 //   Rows<R>  [R rows][64 k], k contiguous: read as one ds_read_b128 a fragment;
@@ -40,54 +38,57 @@ struct Planes {
     uint32_t chunks;       // 16-byte chunks of a row; those behind are zeros
 };
 
-__device__ __forceinline__ void load_to_lds(const char* from, char* to) {
-    __builtin_amdgcn_global_load_lds((global_void)from, (lds_void)to, 16, 0, 0);
-}
-
-// The same where transposing reads follow. Behind the builtin the compiler waits for every load under way before each
-// transposing read (it takes them to read what the loads write), and a step's loads would no longer pass under the step
-// before it. The instruction has no result: it writes LDS, and what it read is waited for at the step's barrier, by hand.
-__device__ __forceinline__ void load_to_lds_unseen(const char* from, char* to) {
+// 16 bytes of every lane from memory to LDS, to `to` + 16 * lane. In assembly, because behind the builtin the compiler
+// waits for every load under way before it reads LDS again (it takes the reads to need what the loads write), and a
+// step's loads would no longer pass under the step before it. The instruction has no result register; what it wrote is
+// waited for by hand, at step_barrier.
+__device__ __forceinline__ void load_to_lds(const char* from, const char* to) {
     asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off"
                  :
                  : "v"((global_void)from), "s"(uniform_u32((uint32_t)(uintptr_t)(lds_void)to))
                  : "memory", "m0");
 }
+// My loads have written LDS and my reads of it are done, and so are everybody's. STORES: so many stores of mine, at
+// least, were issued behind the last of those loads; they need not be done (the counter of loads and stores falls in the
+// order of their issue).
+template <int STORES = 0>
 __device__ __forceinline__ void step_barrier() {
-    __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0): my loads are in LDS
-    __syncthreads();
+    constexpr int N = STORES > 63 ? 63 : STORES;
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_waitcnt(0x0070 | (N & 15) | (N >> 4) << 14);  // vmcnt(N) lgkmcnt(0)
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_sched_barrier(0);
 }
 
 // [R][64 k]: 128 bytes a row, chunk c of row r at place c ^ (r & 7).
-template <int R>
+template <int R, bool LISTED = false>
 struct Rows {
     static constexpr int BYTES = R * 128;
     static constexpr int LOADS = R >= 64 ? R / 64 : 1;
-    const char* row[LOADS];
-    uint32_t index[LOADS];  // of the rows of the next aim, as listed
-    uint32_t chunk;
+    uint32_t index[LISTED ? LOADS : 1], next[LISTED ? LOADS : 1];  // rows in memory, of this tile and (as listed) the next
+    uint32_t first, chunk;
     __device__ __forceinline__ void init() { chunk = (threadIdx.x & 7) ^ (threadIdx.x >> 3 & 7); }
-    // The rows of the tile that starts at row `first`: reads the list, ahead of its use (nothing looks at what was read
+    // The rows of the tile that starts at row `at`: reads the list, ahead of its use (nothing looks at what was read
     // until then, so nothing waits for it).
-    __device__ __forceinline__ void peek(const Planes& p, uint32_t first) {
-        if (!p.list) return;
+    __device__ __forceinline__ void peek(const Planes& p, uint32_t at) {
+        if constexpr (LISTED)
 #pragma unroll
-        for (int i = 0; i < LOADS; ++i) index[i] = p.list[min(first + i * 64 + (threadIdx.x >> 3), p.rows - 1)];
+            for (int i = 0; i < LOADS; ++i) next[i] = p.list[min(at + i * 64 + (threadIdx.x >> 3), p.rows - 1)];
     }
-    __device__ __forceinline__ void aim(const Planes& p, uint32_t first) {
+    __device__ __forceinline__ void aim(uint32_t at) {
+        first = at;
+        if constexpr (LISTED)
 #pragma unroll
-        for (int i = 0; i < LOADS; ++i) {
-            const uint32_t r = first + i * 64 + (threadIdx.x >> 3);
-            row[i] = r < p.rows ? p.base + (uint64_t)(p.list ? index[i] : r) * p.stride + chunk * 16 : nullptr;
-        }
+            for (int i = 0; i < LOADS; ++i) index[i] = next[i];
     }
-    __device__ __forceinline__ void load(const Planes& p, uint32_t kstep, uint32_t plane, const char* zeros, char* lds) const {
+    // Piece i of the step's loads.
+    __device__ __forceinline__ void load(int i, const Planes& p, uint32_t kstep, uint32_t plane, const char* zeros, char* lds) const {
         if (R < 64 && threadIdx.x >= R * 8) return;
-        const uint64_t off = (uint64_t)kstep * 128 + plane * p.plane;
-        const bool in = kstep * 8 + chunk < p.chunks;
-        char* to = lds + uniform_u32(threadIdx.x >> 6) * 1024;  // the wave's first lane; the others follow by 16 bytes
-#pragma unroll
-        for (int i = 0; i < LOADS; ++i) load_to_lds(in && row[i] ? row[i] + off : zeros, to + i * 8192);
+        const uint32_t r = first + i * 64 + (threadIdx.x >> 3);
+        const bool in = kstep * 8 + chunk < p.chunks && r < p.rows;
+        const char* from = p.base + ((uint64_t)kstep * 128 + plane * p.plane) + ((uint64_t)(LISTED ? index[i] : r) * p.stride + chunk * 16);
+        load_to_lds(in ? from : zeros, lds + uniform_u32(threadIdx.x >> 6) * 1024 + i * 8192);
     }
     // Lane's 8 k of fragment `t` (16 rows) in half `kk` of the step.
     __device__ __forceinline__ static bf16x8 read(const char* lds, uint32_t tile, int kk) {
@@ -118,16 +119,11 @@ struct Cols {
 #pragma unroll
         for (int i = 0; i < LOADS; ++i) index[i] = p.list[min(first + k0 + i * APART, end - 1)];
     }
-    __device__ __forceinline__ void load(const Planes& p, uint32_t first, uint32_t end, uint32_t first_chunk, uint32_t plane,
+    __device__ __forceinline__ void load(int i, const Planes& p, uint32_t first, uint32_t end, uint32_t first_chunk, uint32_t plane,
                                          const char* zeros, char* lds) const {
-        const uint32_t c = first_chunk + chunk;
-        const char* base = p.base + plane * p.plane + c * 16ull;
-        char* to = lds + uniform_u32(threadIdx.x >> 6) * 1024;
-#pragma unroll
-        for (int i = 0; i < LOADS; ++i) {
-            const uint32_t r = first + k0 + i * APART;
-            load_to_lds_unseen(r < end && c < p.chunks ? base + (uint64_t)(p.list ? index[i] : r) * p.stride : zeros, to + i * 8192);
-        }
+        const uint32_t c = first_chunk + chunk, r = first + k0 + i * APART;
+        const char* from = p.base + (plane * p.plane + c * 16ull) + (uint64_t)(p.list ? index[i] : r) * p.stride;
+        load_to_lds(r < end && c < p.chunks ? from : zeros, lds + uniform_u32(threadIdx.x >> 6) * 1024 + i * 8192);
     }
     __device__ __forceinline__ static bf16x8 read(char* lds, uint32_t tile, int kk) {
         const uint32_t l = threadIdx.x & 63, k = kk * 32 + (l >> 4) * 8 + (l >> 2 & 3);
@@ -144,21 +140,69 @@ struct Cols {
 
 // The products of a step: TM x TN fragments of 16 x 16 per wave, which start at fragments m0 and n0. Lane l holds rows
 // (of A) 4 (l >> 4) + 0..3 and column (of B) l & 15 of each.
+//
+// A step is walked in phases of up to 16 matrix instructions, (half of k, half of A's fragments). Each phase first asks
+// for the fragments of the next one, and issues a few of the loads of later steps: issued all at once, behind the
+// barrier, they would queue up at the CU's one load path (16 cycles a piece) with the matrix cores idle. The step's one
+// barrier stands before its LAST phase, whose fragments are in registers by then: behind it the next step's half of LDS is
+// complete and this step's is free, and there is still a phase of products to issue while the first fragments of the
+// next step and the loads of the step after it are under way.
 template <typename A, typename B, int TM, int TN>
-__device__ __forceinline__ void multiply(char* a, char* b, uint32_t m0, uint32_t n0, f32x4 (&acc)[TM][TN]) {
+struct Engine {
+    static constexpr int HALVES = TM >= 8 ? 2 : 1, PHASES = 2 * HALVES, MH = TM / HALVES;
+    bf16x8 fa[2][MH], fb[2][TN];
+    uint32_t m0, n0;
+
+    __device__ __forceinline__ void ask(char* a, char* b, int phase) {
+        const int kk = phase / HALVES, h = phase % HALVES;
 #pragma unroll
-    for (int kk = 0; kk < 2; ++kk) {
-        bf16x8 fa[TM], fb[TN];
+        for (int m = 0; m < MH; ++m) fa[phase & 1][m] = A::read(a, m0 + h * MH + m, kk);
+        if (h == 0)
 #pragma unroll
-        for (int n = 0; n < TN; ++n) fb[n] = B::read(b, n0 + n, kk);
-#pragma unroll
-        for (int m = 0; m < TM; ++m) fa[m] = A::read(a, m0 + m, kk);
-#pragma unroll
-        for (int m = 0; m < TM; ++m)
-#pragma unroll
-            for (int n = 0; n < TN; ++n) acc[m][n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fa[m], fb[n], acc[m][n], 0, 0, 0);
+            for (int n = 0; n < TN; ++n) fb[kk][n] = B::read(b, n0 + n, kk);
+        __builtin_amdgcn_sched_barrier(0);
     }
-}
+    // (a, b): this step's operands in LDS; (next_a, next_b): the next one's. `under_way(phase)` issues loads: in phases
+    // before the last into the next step's half, in the last into this step's. `stored`: the next step's loads were all
+    // issued before the STORES of a tile's end.
+    template <int STORES, typename F>
+    __device__ __forceinline__ void step(char* a, char* b, char* next_a, char* next_b, f32x4 (&acc)[TM][TN], uint32_t stored, F&& under_way) {
+#pragma unroll
+        for (int p = 0; p < PHASES; ++p) {
+            const int kk = p / HALVES, h = p % HALVES;
+            if (p + 1 < PHASES) {
+                ask(a, b, p + 1);
+            } else {
+                if (STORES && stored)
+                    step_barrier<STORES>();
+                else
+                    step_barrier();
+                ask(next_a, next_b, 0);
+            }
+            under_way(p);
+#pragma unroll
+            for (int m = 0; m < MH; ++m)
+#pragma unroll
+                for (int n = 0; n < TN; ++n)
+                    acc[h * MH + m][n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fa[p & 1][m], fb[kk][n], acc[h * MH + m][n], 0, 0, 0);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+    }
+};
+
+// Which step of the products a side's loads have come to: plane pair c of 64 k block k of the workgroup's tile `tile`.
+struct Cursor {
+    uint32_t c, k, tile;
+    // Whether the tile ended.
+    __device__ __forceinline__ bool advance(uint32_t planes, uint32_t blocks, uint32_t stride) {
+        if (++c < planes) return false;
+        c = 0;
+        if (++k < blocks) return false;
+        k = 0;
+        tile += stride;
+        return true;
+    }
+};
 
 // The steps of a product of planes: (plane of A, plane of B) of step c.
 struct Steps {

@@ -20,6 +20,8 @@
 #include "learn_kernels.h"
 #include "learn_mma.h"
 
+#include <type_traits>
+
 namespace vs {
 namespace learn {
 namespace {
@@ -51,21 +53,29 @@ struct XentArgs {
     float* click_z;           // [n_q]
     // gradients
     const float *lse, *loss, *grad_loss;
-    char* g;                  // [planes][piece][gq] bf16
+    char* g;                  // [planes][piece][whole tiles of queries] bf16
     uint64_t g_plane;
-    uint32_t g_planes;
+    uint32_t g_stride;
+    char* spill;              // 16 bytes of every thread of a product, for what it has no place for
     void* grad_rows;
     uint64_t grad_row_stride;
-    bool grad_rows_wide;      // four elements at a time
     float* part_q;            // [splits][n_q][dim]
 };
 
-__device__ __forceinline__ uint32_t candidates(const XentArgs& a) { return a.list ? *a.count : (uint32_t)a.n_rows; }
+// (told to the compiler as one value for all lanes: the loops of the products run on it)
+__device__ __forceinline__ uint32_t candidates(const XentArgs& a) {
+    return uniform_u32(a.list ? *a.count : (uint32_t)a.n_rows);
+}
 __device__ __forceinline__ uint64_t row_at(const XentArgs& a, uint32_t place) { return a.list ? a.list[place] : place; }
 
 // Workgroups that share a tile of rows get numbers eight apart: the dispatcher deals numbers out to the eight XCDs in
 // turn, so they land on one XCD and its L2 holds the tile for all of them.
-__device__ __forceinline__ void place_of_workgroup(uint32_t across, uint32_t* a, uint32_t* along) {
+__device__ __forceinline__ void place_of_workgroup(uint32_t across, uint32_t splits, uint32_t* a, uint32_t* along) {
+    if (splits % 8) {  // (too few for that: see splits_for)
+        *a = blockIdx.x % across;
+        *along = blockIdx.x / across;
+        return;
+    }
     const uint32_t local = blockIdx.x >> 3;
     *a = local % across;
     *along = local / across * 8 + (blockIdx.x & 7);
@@ -209,20 +219,21 @@ __global__ __launch_bounds__(256) void pack_rows_kernel(XentArgs a, const E* tab
 // Tiles of candidates with one tile of queries: BQ queries by TILE candidates, `along` of `splits` workgroups. `done` is
 // called with each tile's sums and its first place; the loads of the next tile's first step are under way meanwhile.
 // LANES_ARE_QUERIES: a lane holds four candidates (rows of the product) of one query, else four queries of one candidate.
-template <int BQ, bool LANES_ARE_QUERIES>
+template <int BQ, bool LANES_ARE_QUERIES, bool LISTED>
 struct Scores {
     static constexpr int WAVES_Q = BQ >= 256 ? 4 : BQ >= 128 ? 2 : 1;  // waves side by side along the queries
     static constexpr int WAVES_R = 8 / WAVES_Q;
     static constexpr int WQ = BQ / WAVES_Q / 16, WR = TILE / WAVES_R / 16;  // fragments of a wave
     static constexpr int TM = LANES_ARE_QUERIES ? WR : WQ, TN = LANES_ARE_QUERIES ? WQ : WR;
-    using R = Rows<TILE>;
+    using R = Rows<TILE, LISTED>;
     using Q = Rows<BQ>;
     static constexpr int LDS = 2 * (R::BYTES + Q::BYTES);
 
-    __device__ __forceinline__ static uint32_t wave_q() { return (threadIdx.x >> 6) % WAVES_Q; }
-    __device__ __forceinline__ static uint32_t wave_r() { return (threadIdx.x >> 6) / WAVES_Q; }
+    __device__ __forceinline__ static uint32_t wave_q() { return uniform_u32(threadIdx.x >> 6) % WAVES_Q; }
+    __device__ __forceinline__ static uint32_t wave_r() { return uniform_u32(threadIdx.x >> 6) / WAVES_Q; }
 
-    template <typename F>
+    // STORES: done() returns whether it made at least so many stores.
+    template <int STORES, typename F>
     __device__ __forceinline__ static void run(const XentArgs& a, uint32_t end, uint32_t q0, uint32_t along, char* lds, F&& done) {
         Planes rows = a.rows;
         rows.rows = end - a.place0;
@@ -230,47 +241,75 @@ struct Scores {
         Q q;
         r.init();
         q.init();
-        q.aim(a.q, q0);
+        q.aim(q0);
         const uint32_t tiles = (end - a.piece_begin + TILE - 1) / TILE;
         if (along >= tiles) return;
-        const uint32_t steps = (a.rows.chunks + 7) / 8 * a.score_steps.n;
+        const uint32_t planes = a.score_steps.n, blocks = (a.rows.chunks + 7) / 8, steps = planes * blocks;
         const uint32_t base = a.piece_begin - a.place0;
+        auto half_r = [&](uint32_t i) { return lds + i * (R::BYTES + Q::BYTES); };
+        auto half_q = [&](uint32_t i) { return lds + i * (R::BYTES + Q::BYTES) + R::BYTES; };
+        // The rows have furthest to come: theirs go first, a step earlier than the queries'. (Steps are counted as
+        // queries x rows; which of the two is A does not matter to six symmetric steps.)
+        Cursor cr{0, 0, along}, cq{0, 0, along};
+        bool rows_left = true;
         r.peek(rows, base + along * TILE);
-        r.aim(rows, base + along * TILE);
-        auto half = [&](uint32_t i) { return lds + i * (R::BYTES + Q::BYTES); };
-        uint32_t at = 0, c = 0, k = 0;
-        auto issue = [&](uint32_t to) {
-            // (steps are counted as queries x rows; which of the two is A does not matter to six symmetric steps)
-            r.load(rows, k, a.score_steps.plane_b(c), a.zeros, half(to));
-            q.load(a.q, k, a.score_steps.plane_a(c), a.zeros, half(to) + R::BYTES);
-            if (++c == a.score_steps.n) {
-                c = 0;
-                ++k;
-            }
+        r.aim(base + along * TILE);
+        r.peek(rows, base + (along + a.splits) * TILE);
+        auto load_rows = [&](uint32_t to) {
+            if (!rows_left) return;
+#pragma unroll
+            for (int i = 0; i < R::LOADS; ++i) r.load(i, rows, cr.k, a.score_steps.plane_b(cr.c), a.zeros, half_r(to));
+            if (!cr.advance(planes, blocks, a.splits)) return;
+            rows_left = cr.tile < tiles;
+            r.aim(base + cr.tile * TILE);
+            r.peek(rows, base + (cr.tile + a.splits) * TILE);
         };
-        issue(0);
+        auto load_queries = [&](int i, uint32_t to) { q.load(i, a.q, cq.k, a.score_steps.plane_a(cq.c), a.zeros, half_q(to)); };
+        load_rows(0);
+#pragma unroll
+        for (int i = 0; i < Q::LOADS; ++i) load_queries(i, 0);
+        cq.advance(planes, blocks, a.splits);
+        step_barrier();
+        using E = Engine<std::conditional_t<LANES_ARE_QUERIES, R, Q>, std::conditional_t<LANES_ARE_QUERIES, Q, R>, TM, TN>;
+        E e;
+        e.m0 = LANES_ARE_QUERIES ? wave_r() * WR : wave_q() * WQ;
+        e.n0 = LANES_ARE_QUERIES ? wave_q() * WQ : wave_r() * WR;
+        e.ask(LANES_ARE_QUERIES ? half_r(0) : half_q(0), LANES_ARE_QUERIES ? half_q(0) : half_r(0), 0);
+        load_rows(1);
+        uint32_t at = 0;
+        uint32_t early = 0, stored = 0;  // the next step's queries are under way already; stores are
+#pragma nounroll
         for (uint32_t tile = along; tile < tiles; tile += a.splits) {
-            const bool more = tile + a.splits < tiles;
             f32x4 acc[TM][TN] = {};
-            if (more) r.peek(rows, base + (tile + a.splits) * TILE);
+#pragma nounroll
             for (uint32_t s = 0; s < steps; ++s) {
-                step_barrier();
-                if (s + 1 < steps) {
-                    issue(at ^ 1);
-                } else if (more) {
-                    c = k = 0;
-                    r.aim(rows, base + (tile + a.splits) * TILE);
-                    issue(at ^ 1);
-                }
-                char *lr = half(at), *lq = half(at) + R::BYTES;
-                if constexpr (LANES_ARE_QUERIES)
-                    multiply<R, Q, TM, TN>(lr, lq, wave_r() * WR, wave_q() * WQ, acc);
-                else
-                    multiply<Q, R, TM, TN>(lq, lr, wave_q() * WQ, wave_r() * WR, acc);
-                at ^= 1;
+                const uint32_t other = at ^ 1;
+                char *ar = half_r(at), *aq = half_q(at), *br = half_r(other), *bq = half_q(other);
+                e.template step<STORES>(LANES_ARE_QUERIES ? ar : aq, LANES_ARE_QUERIES ? aq : ar, LANES_ARE_QUERIES ? br : bq,
+                                        LANES_ARE_QUERIES ? bq : br, acc, stored, [&](int phase) {
+                    if (phase < E::PHASES - 1) {
+                        // the queries of the next step, over the phases before the barrier
+                        constexpr int EACH = (Q::LOADS + E::PHASES - 2) / (E::PHASES - 1);
+                        if (early || cq.tile >= tiles) return;
+#pragma unroll
+                        for (int i = phase * EACH; i < min((phase + 1) * EACH, Q::LOADS); ++i) load_queries(i, other);
+                        return;
+                    }
+                    load_rows(at);
+                    if (!early && cq.tile < tiles) cq.advance(planes, blocks, a.splits);
+                    early = afresh_uniform(STORES && s + 1 == steps && cq.tile < tiles);
+                    if (!early) return;
+                    // the end of a tile stores: what the step after next needs goes before that
+#pragma unroll
+                    for (int i = 0; i < Q::LOADS; ++i) load_queries(i, at);
+                    cq.advance(planes, blocks, a.splits);
+                });
+                stored = afresh_uniform(0);
+                at = other;
             }
-            done(acc, a.piece_begin + tile * TILE);
+            stored = afresh_uniform(done(acc, a.piece_begin + tile * TILE) && early);
         }
+        // (nothing is under way any more: the last step's barrier waited for all, and no load followed it)
     }
 };
 
@@ -279,14 +318,14 @@ __device__ __forceinline__ float finite_or_zero(float m) { return m == -__builti
 // Per query the largest logit of a share of the candidates and the sum of the exponentials over it, the clicked row kept
 // out. Everything is in base 2 (logits times log2 e): an exponential is one instruction. A lane keeps the running largest
 // and sum of its own candidates, in registers, for each of its queries; lanes, waves and shares are joined at the end.
-template <int BQ, bool NORMS>
+template <int BQ, bool NORMS, bool LISTED>
 __global__ __launch_bounds__(THREADS, 2) void loss_kernel(XentArgs a) {
-    using S = Scores<BQ, true>;
+    using S = Scores<BQ, true, LISTED>;
     extern __shared__ __attribute__((aligned(128))) char lds[];
     __shared__ float inverse[TILE], sm[S::WAVES_R][BQ], sl[S::WAVES_R][BQ];
     const uint32_t lane = threadIdx.x & 63, group = lane >> 4;
     uint32_t tile_q, along;
-    place_of_workgroup(a.across, &tile_q, &along);
+    place_of_workgroup(a.across, a.splits, &tile_q, &along);
     const uint32_t end = min(candidates(a), a.piece_begin + a.piece_rows);
     uint32_t click[S::TN];
     float s2[S::TN], m[S::TN], l[S::TN];
@@ -300,7 +339,7 @@ __global__ __launch_bounds__(THREADS, 2) void loss_kernel(XentArgs a) {
         l[n] = 0;
     }
     if (end > a.piece_begin)
-        S::run(a, end, tile_q * BQ, along, lds, [&](f32x4 (&acc)[S::TM][S::TN], uint32_t first) {
+        S::template run<0>(a, end, tile_q * BQ, along, lds, [&](f32x4 (&acc)[S::TM][S::TN], uint32_t first) {
             if constexpr (NORMS) {
                 if (threadIdx.x < TILE) {
                     const float x = first + threadIdx.x < end ? a.norms[row_at(a, first + threadIdx.x)] : 0.0f;
@@ -358,6 +397,7 @@ __global__ __launch_bounds__(THREADS, 2) void loss_kernel(XentArgs a) {
                 l[n] = (sum[0] + sum[1]) + (sum[2] + sum[3]);
                 m[n] = top;
             }
+            return false;
         });
     // lanes that hold other candidates of the same query, then waves, then what the pieces before this one left
 #pragma unroll
@@ -420,15 +460,14 @@ __global__ __launch_bounds__(256) void join_loss_kernel(XentArgs a, float* loss,
 
 // The weights G of a piece, [candidate][query], rounded to bf16 (PG = 1), or kept to 16 bits (2) or all 24 (3) by as many
 // planes. A lane holds four neighbouring queries of a candidate: eight bytes a store.
-template <int BQ, bool NORMS, int PG>
+template <int BQ, bool NORMS, bool LISTED, int PG>
 __global__ __launch_bounds__(THREADS, 2) void weights_kernel(XentArgs a) {
-    using S = Scores<BQ, false>;
+    using S = Scores<BQ, false, LISTED>;
     extern __shared__ __attribute__((aligned(128))) char lds[];
     __shared__ __attribute__((aligned(16))) float s2[BQ], lse2[BQ], factor[BQ], at_click[BQ];
     __shared__ __attribute__((aligned(16))) uint32_t click[BQ];
-    const uint32_t lane = threadIdx.x & 63, group = lane >> 4;
     uint32_t tile_q, along;
-    place_of_workgroup(a.across, &tile_q, &along);
+    place_of_workgroup(a.across, a.splits, &tile_q, &along);
     const uint32_t q0 = tile_q * BQ;
     const uint32_t end = min(candidates(a), a.piece_begin + a.piece_rows);
     if (end <= a.piece_begin) return;
@@ -443,32 +482,35 @@ __global__ __launch_bounds__(THREADS, 2) void weights_kernel(XentArgs a) {
         at_click[threadIdx.x] = in ? f * expm1f(-a.loss[q]) : 0.0f;
     }
     // (the first barrier of the loop below orders these before they are read)
-    S::run(a, end, q0, along, lds, [&](f32x4 (&acc)[S::TM][S::TN], uint32_t first) {
+    // Every lane stores every time (so that the number of stores is known to the next step's barrier): rows of G are whole
+    // tiles of queries, and G is whole tiles of candidates.
+    S::template run<S::TM * S::TN * PG>(a, end, q0, along, lds, [&](f32x4 (&acc)[S::TM][S::TN], uint32_t first) {
+        const uint32_t l = afresh(threadIdx.x) & 63, row0 = S::wave_r() * S::WR * 16 + (l & 15), i0 = S::wave_q() * S::WQ * 16 + (l >> 4) * 4;
+        char* out = a.g + (uint64_t)(first - a.piece_begin + row0) * a.g_stride + (q0 + i0) * 2;
+        float inverse[S::TN];
+        if constexpr (NORMS)
 #pragma unroll
-        for (int n = 0; n < S::TN; ++n) {
-            const uint32_t place = first + (S::wave_r() * S::WR + n) * 16 + (lane & 15);
-            if (place >= end) continue;
-            float inverse = 1.0f;
-            if constexpr (NORMS) {
-                const float x = a.norms[row_at(a, place)];
-                inverse = x > 0 ? 1.0f / x : 0.0f;
+            for (int n = 0; n < S::TN; ++n) {
+                const float x = a.norms[row_at(a, min(first + row0 + n * 16, end - 1))];
+                inverse[n] = x > 0 ? 1.0f / x : 0.0f;
             }
-            char* out = a.g + (uint64_t)(place - a.piece_begin) * a.gq * 2;
 #pragma unroll
-            for (int t = 0; t < S::TM; ++t) {
-                const uint32_t i = (S::wave_q() * S::WQ + t) * 16 + group * 4;
-                if (q0 + i >= a.gq) continue;
-                const f32x4 vs = *reinterpret_cast<const f32x4*>(s2 + i), vl = *reinterpret_cast<const f32x4*>(lse2 + i);
-                const f32x4 vf = *reinterpret_cast<const f32x4*>(factor + i), vc = *reinterpret_cast<const f32x4*>(at_click + i);
-                const u32x4 vp = *reinterpret_cast<const u32x4*>(click + i);
+        for (int t = 0; t < S::TM; ++t) {
+            const uint32_t i = i0 + t * 16;
+            const f32x4 vs = *reinterpret_cast<const f32x4*>(s2 + i), vl = *reinterpret_cast<const f32x4*>(lse2 + i);
+            const f32x4 vf = *reinterpret_cast<const f32x4*>(factor + i), vc = *reinterpret_cast<const f32x4*>(at_click + i);
+            const u32x4 vp = *reinterpret_cast<const u32x4*>(click + i);
+#pragma unroll
+            for (int n = 0; n < S::TN; ++n) {
+                const uint32_t place = first + row0 + n * 16;
                 Pack<uint16_t, 4> p[3];
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
                     float z = acc[t][n][r];
-                    if constexpr (NORMS) z *= inverse;
+                    if constexpr (NORMS) z *= inverse[n];
                     float g = vp[r] == place ? vc[r] : vf[r] * __builtin_amdgcn_exp2f(__builtin_fmaf(z, vs[r], -vl[r]));
                     if (vf[r] == 0.0f) g = 0.0f;  // no click, no query (an exponential over a lse of -inf is none)
-                    if constexpr (NORMS) g *= inverse;
+                    if constexpr (NORMS) g *= inverse[n];
                     if constexpr (PG == 1) {
                         p[0].e[r] = (uint16_t)bf16_bits(g);
                     } else {
@@ -480,79 +522,108 @@ __global__ __launch_bounds__(THREADS, 2) void weights_kernel(XentArgs a) {
                 }
 #pragma unroll
                 for (int k = 0; k < PG; ++k)
-                    store_pack<uint16_t, 4>(reinterpret_cast<uint16_t*>(out + k * a.g_plane) + q0 + i, p[k]);
+                    store_pack<uint16_t, 4>(reinterpret_cast<uint16_t*>(out + k * a.g_plane + n * 16ull * a.g_stride) + t * 16, p[k]);
+                if (PG == 3 || n + 1 == S::TN) __builtin_amdgcn_sched_barrier(0);  // (the registers hold no more at a time)
             }
         }
+        return true;
     });
 }
 
 // drows of a piece: transposed queries (BD columns of the rows) by G. A lane holds four neighbouring columns of a row.
-template <int BD, typename E>
+// WIDE: rows take four elements at a time; as in weights_kernel every lane stores every time, to its own 16 bytes of
+// a.spill where it has no row or column.
+template <int BD, typename E, bool WIDE>
 __global__ __launch_bounds__(THREADS, 2) void row_grads_kernel(XentArgs a) {
     using A = Rows<BD>;
     using B = Rows<TILE>;
     constexpr int WAVES_D = BD >= 256 ? 2 : 2, WAVES_R = 8 / WAVES_D;
     constexpr int TM = BD / WAVES_D / 16, TN = TILE / WAVES_R / 16;
     extern __shared__ __attribute__((aligned(128))) char lds[];
-    const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wd = wave % WAVES_D, wr = wave / WAVES_D;
+    const uint32_t wave = uniform_u32(threadIdx.x >> 6), wd = wave % WAVES_D, wr = wave / WAVES_D;
     uint32_t tile_d, along;
-    place_of_workgroup(a.across, &tile_d, &along);
+    place_of_workgroup(a.across, a.splits, &tile_d, &along);
     const uint32_t end = min(candidates(a), a.piece_begin + a.piece_rows);
     const uint32_t tiles = end > a.piece_begin ? (end - a.piece_begin + TILE - 1) / TILE : 0;
     if (along >= tiles) return;
-    const Planes g{a.g, a.g_plane, a.gq * 2, nullptr, end - a.piece_begin, a.gq / 8};
+    const Planes g{a.g, a.g_plane, a.g_stride, nullptr, end - a.piece_begin, a.gq / 8};
     A q;
     B r;
     q.init();
     r.init();
-    q.aim(a.qt, tile_d * BD);
-    r.aim(g, along * TILE);
-    const uint32_t steps = a.gq / 64 * a.grad_steps.n;
-    auto half = [&](uint32_t i) { return lds + i * (A::BYTES + B::BYTES); };
-    uint32_t at = 0, c = 0, k = 0;
-    auto issue = [&](uint32_t to) {
-        q.load(a.qt, k, a.grad_steps.plane_b(c), a.zeros, half(to));
-        r.load(g, k, a.grad_steps.plane_a(c), a.zeros, half(to) + A::BYTES);
-        if (++c == a.grad_steps.n) {
-            c = 0;
-            ++k;
-        }
+    q.aim(tile_d * BD);
+    r.aim(along * TILE);
+    const uint32_t planes = a.grad_steps.n, blocks = a.gq / 64, steps = planes * blocks;
+    auto half_q = [&](uint32_t i) { return lds + i * (A::BYTES + B::BYTES); };
+    auto half_g = [&](uint32_t i) { return lds + i * (A::BYTES + B::BYTES) + A::BYTES; };
+    Cursor cg{0, 0, along}, cq{0, 0, along};
+    auto load_weights = [&](uint32_t to) {
+        if (cg.tile >= tiles) return;
+#pragma unroll
+        for (int i = 0; i < B::LOADS; ++i) r.load(i, g, cg.k, a.grad_steps.plane_a(cg.c), a.zeros, half_g(to));
+        if (cg.advance(planes, blocks, a.splits)) r.aim(cg.tile * TILE);
     };
-    issue(0);
+    auto load_queries = [&](int i, uint32_t to) { q.load(i, a.qt, cq.k, a.grad_steps.plane_b(cq.c), a.zeros, half_q(to)); };
+    load_weights(0);
+#pragma unroll
+    for (int i = 0; i < A::LOADS; ++i) load_queries(i, 0);
+    cq.advance(planes, blocks, a.splits);
+    step_barrier();
+    using En = Engine<A, B, TM, TN>;
+    En e;
+    e.m0 = wd * TM;
+    e.n0 = wr * TN;
+    e.ask(half_q(0), half_g(0), 0);
+    load_weights(1);
+    uint32_t at = 0;
+    uint32_t early = 0, stored = 0;  // as in Scores::run
+#pragma nounroll
     for (uint32_t tile = along; tile < tiles; tile += a.splits) {
-        const bool more = tile + a.splits < tiles;
         f32x4 acc[TM][TN] = {};
+#pragma nounroll
         for (uint32_t s = 0; s < steps; ++s) {
-            step_barrier();
-            if (s + 1 < steps) {
-                issue(at ^ 1);
-            } else if (more) {
-                c = k = 0;
-                r.aim(g, (tile + a.splits) * TILE);
-                issue(at ^ 1);
-            }
-            multiply<A, B, TM, TN>(half(at), half(at) + A::BYTES, wd * TM, wr * TN, acc);
-            at ^= 1;
+            const uint32_t other = at ^ 1;
+            e.template step<WIDE ? TM * TN : 0>(half_q(at), half_g(at), half_q(other), half_g(other), acc, stored, [&](int phase) {
+                if (phase < En::PHASES - 1) {
+                    constexpr int EACH = (A::LOADS + En::PHASES - 2) / (En::PHASES - 1);
+                    if (early || cq.tile >= tiles) return;
+#pragma unroll
+                    for (int i = phase * EACH; i < min((phase + 1) * EACH, A::LOADS); ++i) load_queries(i, other);
+                    return;
+                }
+                load_weights(at);
+                if (!early && cq.tile < tiles) cq.advance(planes, blocks, a.splits);
+                early = afresh_uniform(WIDE && s + 1 == steps && cq.tile < tiles);
+                if (!early) return;
+#pragma unroll
+                for (int i = 0; i < A::LOADS; ++i) load_queries(i, at);
+                cq.advance(planes, blocks, a.splits);
+            });
+            stored = afresh_uniform(0);
+            at = other;
         }
+        const uint32_t l = afresh(threadIdx.x) & 63, d0 = tile_d * BD + wd * TM * 16 + (l >> 4) * 4;
 #pragma unroll
         for (int n = 0; n < TN; ++n) {
-            const uint32_t place = a.piece_begin + tile * TILE + (wr * TN + n) * 16 + (lane & 15);
-            if (place >= end) continue;
-            E* out = static_cast<E*>(a.grad_rows) + row_at(a, place) * a.grad_row_stride;
+            const uint32_t place = a.piece_begin + tile * TILE + (wr * TN + n) * 16 + (l & 15);
+            E* out = static_cast<E*>(a.grad_rows) + row_at(a, min(place, end - 1)) * a.grad_row_stride;
 #pragma unroll
             for (int m = 0; m < TM; ++m) {
-                const uint32_t d = tile_d * BD + (wd * TM + m) * 16 + (lane >> 4) * 4;
+                const uint32_t d = d0 + m * 16;
                 Pack<E, 4> p;
 #pragma unroll
                 for (int i = 0; i < 4; ++i) p.e[i] = from_f32<E>(acc[m][n][i]);
-                if (a.grad_rows_wide && d + 4 <= a.dim)
-                    store_pack<E, 4>(out + d, p);
-                else
+                if constexpr (WIDE) {
+                    E* const spill = reinterpret_cast<E*>(a.spill + (blockIdx.x * THREADS + threadIdx.x) * 16ull);
+                    store_pack<E, 4>(place < end && d < a.dim ? out + d : spill, p);
+                } else {
 #pragma unroll
                     for (int i = 0; i < 4; ++i)
-                        if (d + i < a.dim) out[d + i] = p.e[i];
+                        if (place < end && d + i < a.dim) out[d + i] = p.e[i];
+                }
             }
         }
+        stored = afresh_uniform(early);
     }
 }
 
@@ -564,10 +635,10 @@ __global__ __launch_bounds__(THREADS, 2) void query_grads_kernel(XentArgs a) {
     constexpr int WAVES_Q = BQ >= 128 ? 2 : 1, WAVES_D = 8 / WAVES_Q;
     constexpr int TM = BQ / WAVES_Q / 16, TN = BD / WAVES_D / 16;
     extern __shared__ __attribute__((aligned(128))) char lds[];
-    const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wq = wave % WAVES_Q, wd = wave / WAVES_Q;
+    const uint32_t lane = threadIdx.x & 63, wave = uniform_u32(threadIdx.x >> 6), wq = wave % WAVES_Q, wd = wave / WAVES_Q;
     const uint32_t d_tiles = (a.dim + BD - 1) / BD;
     uint32_t tile, share;
-    place_of_workgroup(a.across, &tile, &share);
+    place_of_workgroup(a.across, a.splits, &tile, &share);
     const uint32_t tile_d = tile % d_tiles, tile_q = tile / d_tiles;
     const uint32_t end = min(candidates(a), a.piece_begin + a.piece_rows);
     const uint32_t n = end > a.piece_begin ? end - a.piece_begin : 0;
@@ -577,7 +648,7 @@ __global__ __launch_bounds__(THREADS, 2) void query_grads_kernel(XentArgs a) {
     f32x4 acc[TM][TN] = {};
     const uint32_t blocks = (stop - begin + STEP - 1) / STEP, steps = blocks * a.grad_steps.n;
     if (steps) {
-        const Planes g{a.g, a.g_plane, a.gq * 2, nullptr, n, a.gq / 8};
+        const Planes g{a.g, a.g_plane, a.g_stride, nullptr, n, a.gq / 8};
         Planes rows = a.rows;
         rows.rows = end - a.place0;
         const uint32_t base = a.piece_begin - a.place0;
@@ -585,25 +656,46 @@ __global__ __launch_bounds__(THREADS, 2) void query_grads_kernel(XentArgs a) {
         B r;
         w.init();
         r.init();
-        auto half = [&](uint32_t i) { return lds + i * (A::BYTES + B::BYTES); };
-        uint32_t c = 0, k = 0, at = 0;
-        auto issue = [&](uint32_t to) {
-            const uint32_t from = begin + k * STEP;
-            w.load(g, from, stop, tile_q * (BQ / 8), a.grad_steps.plane_a(c), a.zeros, half(to));
-            r.load(rows, base + from, base + stop, tile_d * (BD / 8), a.grad_steps.plane_b(c), a.zeros, half(to) + A::BYTES);
-            if (++c == a.grad_steps.n) {
-                c = 0;
-                ++k;
-                if (k < blocks) r.peek(rows, base + from + STEP, base + stop);  // while this step multiplies
-            }
+        auto half_g = [&](uint32_t i) { return lds + i * (A::BYTES + B::BYTES); };
+        auto half_r = [&](uint32_t i) { return lds + i * (A::BYTES + B::BYTES) + A::BYTES; };
+        Cursor cr{0, 0, 0}, cg{0, 0, 0};
+        const uint32_t planes = a.grad_steps.n;
+        auto load_rows = [&](uint32_t to) {
+            if (cr.tile) return;
+            const uint32_t from = begin + cr.k * STEP;
+#pragma unroll
+            for (int i = 0; i < B::LOADS; ++i)
+                r.load(i, rows, base + from, base + stop, tile_d * (BD / 8), a.grad_steps.plane_b(cr.c), a.zeros, half_r(to));
+            if (!cr.advance(planes, blocks, 1) && !cr.c) r.peek(rows, base + from + STEP, base + stop);  // while this step multiplies
+        };
+        auto load_weights = [&](int i, uint32_t to) {
+            w.load(i, g, begin + cg.k * STEP, stop, tile_q * (BQ / 8), a.grad_steps.plane_a(cg.c), a.zeros, half_g(to));
         };
         r.peek(rows, base + begin, base + stop);
-        issue(0);
+        load_rows(0);
+#pragma unroll
+        for (int i = 0; i < A::LOADS; ++i) load_weights(i, 0);
+        cg.advance(planes, blocks, 1);
+        step_barrier();
+        using En = Engine<A, B, TM, TN>;
+        En e;
+        e.m0 = wq * TM;
+        e.n0 = wd * TN;
+        e.ask(half_g(0), half_r(0), 0);
+        load_rows(1);
+        uint32_t at = 0;
+#pragma nounroll
         for (uint32_t s = 0; s < steps; ++s) {
-            step_barrier();
-            if (s + 1 < steps) issue(at ^ 1);
-            multiply<A, B, TM, TN>(half(at), half(at) + A::BYTES, wq * TM, wd * TN, acc);
-            at ^= 1;
+            const uint32_t other = at ^ 1;
+            e.template step<0>(half_g(at), half_r(at), half_g(other), half_r(other), acc, false, [&](int phase) {
+                if (phase == En::PHASES - 1) return load_rows(at);
+                constexpr int EACH = (A::LOADS + En::PHASES - 2) / (En::PHASES - 1);
+                if (cg.tile) return;
+#pragma unroll
+                for (int i = phase * EACH; i < min((phase + 1) * EACH, A::LOADS); ++i) load_weights(i, other);
+            });
+            if (!cg.tile) cg.advance(planes, blocks, 1);
+            at = other;
         }
     }
 #pragma unroll
@@ -689,10 +781,13 @@ struct Plan {
     uint64_t piece_rows, packed_rows;
 };
 
-// Workgroups along the rows for `across` side by side: a multiple of eight (the XCDs), enough for every CU.
+// Workgroups along the rows for `across` side by side: one round of the CUs (a workgroup more would take a second one).
+// A multiple of eight keeps those that share rows on one XCD, unless more than a tenth of the CUs would go idle for it.
 uint32_t splits_for(uint32_t across, uint64_t tiles) {
     const uint64_t want = std::max<uint64_t>(WORKGROUPS / across, 1);
-    return (uint32_t)round_up(std::min(want, tiles), 8);
+    if (tiles <= want) return (uint32_t)tiles;
+    const uint64_t aligned = want / 8 * 8;
+    return (uint32_t)(aligned * across * 10 >= WORKGROUPS * 9 ? aligned : want);
 }
 
 Plan plan_for(uint32_t n_q, uint64_t n_rows, uint32_t dim, int32_t dtype) {
@@ -715,7 +810,7 @@ Plan plan_for(uint32_t n_q, uint64_t n_rows, uint32_t dim, int32_t dtype) {
         if (r > per) r = r / per * per;  // whole rounds of the workgroups
         return std::min(r, rows);
     };
-    p.piece_rows = piece((uint64_t)p.gq * 2 * p.g_planes);
+    p.piece_rows = piece((uint64_t)p.q_tiles * p.bq * 2 * p.g_planes);
     p.packed_rows = std::min(p.piece_rows, piece((uint64_t)p.kp * 2 * p.planes));
     const uint64_t tiles = rows / TILE;
     p.loss_splits = splits_for(p.loss_q_tiles, tiles);
@@ -728,7 +823,7 @@ Plan plan_for(uint32_t n_q, uint64_t n_rows, uint32_t dim, int32_t dtype) {
 struct Buffers {
     uint32_t *zeros, *list, *count, *click;
     float *qscale, *part_m, *part_l, *click_z, *part_q;
-    char *q, *qt, *g, *packed;
+    char *q, *qt, *g, *packed, *spill;
     uint64_t bytes;
 };
 Buffers carve(void* workspace, const Plan& p, uint32_t n_q, uint64_t n_rows, uint32_t dim) {
@@ -744,7 +839,8 @@ Buffers carve(void* workspace, const Plan& p, uint32_t n_q, uint64_t n_rows, uin
     b.qt = w.take<char>((uint64_t)dim * p.gq * 2 * p.planes);
     b.part_m = w.take<float>((uint64_t)p.loss_splits * n_q);
     b.part_l = w.take<float>((uint64_t)p.loss_splits * n_q);
-    b.g = w.take<char>(p.piece_rows * p.gq * 2 * p.g_planes);
+    b.g = w.take<char>(p.piece_rows * p.q_tiles * p.bq * 2 * p.g_planes);
+    b.spill = w.take<char>(16ull * THREADS * WORKGROUPS);
     b.part_q = w.take<float>((uint64_t)p.grad_splits * n_q * dim);
     b.packed = w.take<char>(p.packed_rows * p.kp * 2 * p.planes);
     b.bytes = w.at() - (char*)workspace;
@@ -783,8 +879,9 @@ struct Call {
         a.part_l = b.part_l;
         a.click_z = b.click_z;
         a.g = b.g;
-        a.g_planes = p.g_planes;
-        a.g_plane = p.piece_rows * p.gq * 2;
+        a.g_stride = p.q_tiles * p.bq * 2;
+        a.g_plane = p.piece_rows * a.g_stride;
+        a.spill = b.spill;
         a.part_q = b.part_q;
         if (x.mask || x.t.present) {
             a.list = b.list;
@@ -841,35 +938,56 @@ struct Call {
         if (error == hipSuccess) kernel<<<across * splits, THREADS, lds, stream>>>(a);
     }
 
-    template <bool NORMS>
+    // Calls `f` with whether logits are cosines and whether rows are read through the list, as constants.
+    template <typename F>
+    void by_kind(F&& f) {
+        const bool listed = a.rows.list;
+        if (a.norms)
+            listed ? f(std::true_type{}, std::true_type{}) : f(std::true_type{}, std::false_type{});
+        else
+            listed ? f(std::false_type{}, std::true_type{}) : f(std::false_type{}, std::false_type{});
+    }
+
+    template <int BQ>
     void loss() {
-        switch (p.loss_bq) {
-            case 16: return product(loss_kernel<16, NORMS>, Scores<16, true>::LDS, p.loss_q_tiles, p.loss_splits);
-            case 64: return product(loss_kernel<64, NORMS>, Scores<64, true>::LDS, p.loss_q_tiles, p.loss_splits);
-            case 128: return product(loss_kernel<128, NORMS>, Scores<128, true>::LDS, p.loss_q_tiles, p.loss_splits);
-            default: return product(loss_kernel<256, NORMS>, Scores<256, true>::LDS, p.loss_q_tiles, p.loss_splits);
-        }
+        by_kind([&](auto norms, auto listed) {
+            product(loss_kernel<BQ, norms, listed>, Scores<BQ, true, listed>::LDS, p.loss_q_tiles, p.loss_splits);
+        });
     }
 
-    template <bool NORMS, int PG>
+    template <int BQ, int PG>
     void weights() {
-        switch (p.bq) {
-            case 64: return product(weights_kernel<64, NORMS, PG>, Scores<64, false>::LDS, p.q_tiles, p.weight_splits);
-            case 128: return product(weights_kernel<128, NORMS, PG>, Scores<128, false>::LDS, p.q_tiles, p.weight_splits);
-            default: return product(weights_kernel<256, NORMS, PG>, Scores<256, false>::LDS, p.q_tiles, p.weight_splits);
-        }
+        by_kind([&](auto norms, auto listed) {
+            product(weights_kernel<BQ, norms, listed, PG>, Scores<BQ, false, listed>::LDS, p.q_tiles, p.weight_splits);
+        });
     }
-    template <bool NORMS>
+    template <int BQ>
     void weights() {
-        if (p.g_planes == 3) return weights<NORMS, 3>();
-        if (p.g_planes == 2) return product(weights_kernel<64, NORMS, 2>, Scores<64, false>::LDS, p.q_tiles, p.weight_splits);
-        weights<NORMS, 1>();
+        if (p.planes == 3) return product_f32_weights<BQ>();
+        if constexpr (BQ == 64)
+            weights<BQ, 2>();
+        else
+            weights<BQ, 1>();
+    }
+    template <int BQ>
+    void product_f32_weights() {  // (always from planes, never through the list)
+        if (a.norms)
+            product(weights_kernel<BQ, true, false, 3>, Scores<BQ, false, false>::LDS, p.q_tiles, p.weight_splits);
+        else
+            product(weights_kernel<BQ, false, false, 3>, Scores<BQ, false, false>::LDS, p.q_tiles, p.weight_splits);
     }
 
+    template <int BD, typename E>
+    void row_grads() {
+        constexpr uint32_t LDS = 2 * (Rows<BD>::BYTES + Rows<TILE>::BYTES);
+        if (aligned_rows<E, 4>(a.grad_rows, a.grad_row_stride) && a.dim % 4 == 0)
+            product(row_grads_kernel<BD, E, true>, LDS, p.d_tiles, p.row_splits);
+        else
+            product(row_grads_kernel<BD, E, false>, LDS, p.d_tiles, p.row_splits);
+    }
     template <typename E>
     void row_grads() {
-        p.bd == 256 ? product(row_grads_kernel<256, E>, 2 * (Rows<256>::BYTES + Rows<TILE>::BYTES), p.d_tiles, p.row_splits)
-                    : product(row_grads_kernel<128, E>, 2 * (Rows<128>::BYTES + Rows<TILE>::BYTES), p.d_tiles, p.row_splits);
+        p.bd == 256 ? row_grads<256, E>() : row_grads<128, E>();
     }
 
     template <int BQ>
@@ -903,7 +1021,14 @@ uint64_t xent_workspace_bytes(uint32_t n_q, uint64_t n_rows, uint32_t dim, int32
 
 hipError_t launch_xent(const Xent& x, void* workspace, float* loss, float* lse, hipStream_t stream) {
     Call c(x, workspace, false, stream);
-    c.for_pieces(c.packed ? c.p.packed_rows : x.t.n_rows, [&] { x.norms ? c.loss<true>() : c.loss<false>(); });
+    c.for_pieces(c.packed ? c.p.packed_rows : x.t.n_rows, [&] {
+        switch (c.p.loss_bq) {
+            case 16: return c.loss<16>();
+            case 64: return c.loss<64>();
+            case 128: return c.loss<128>();
+            default: return c.loss<256>();
+        }
+    });
     c.a.splits = c.p.loss_splits;
     if (c.error != hipSuccess) return c.error;
     join_loss_kernel<<<(x.n_q + 3) / 4, 256, 0, stream>>>(c.a, loss, lse);
@@ -925,10 +1050,9 @@ hipError_t launch_xent_grad(const Xent& x, const float* loss, const float* lse, 
     c.a.grad_rows = grad_rows;
     c.a.grad_row_stride = grad_row_stride;
     const bool f32 = x.t.dtype == VS_F32;
-    c.a.grad_rows_wide = f32 ? aligned_rows<float, 4>(grad_rows, grad_row_stride) : aligned_rows<bf16, 4>(grad_rows, grad_row_stride);
     if (grad_rows && c.a.list) clear_rows(x, grad_rows, grad_row_stride, false, stream);
     c.for_pieces(c.packed ? c.p.packed_rows : c.p.piece_rows, [&] {
-        x.norms ? c.weights<true>() : c.weights<false>();
+        c.p.bq == 64 ? c.weights<64>() : c.p.bq == 128 ? c.weights<128>() : c.weights<256>();
         if (grad_rows) f32 ? c.row_grads<float>() : c.row_grads<bf16>();
         if (!grad_queries) return;
         c.p.bq == 64 ? c.query_grads<64>() : c.p.bq == 128 ? c.query_grads<128>() : c.query_grads<256>();
