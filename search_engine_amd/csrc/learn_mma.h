@@ -190,6 +190,29 @@ struct Engine {
     }
 };
 
+// A wave's results on their way to memory. Lane l has, of row l & 15, the pieces m of PB bytes that lie at (4 m + (l >> 4))
+// PB: stored from there, an instruction would touch 16 rows for 4 PB bytes each. Taken through LDS it writes rows of
+// 4 M PB bytes (128 or 256) in whole. The 16-byte chunks of a row are rotated by XOR with it, as above.
+template <int PB, int M>
+struct Turn {
+    static constexpr int ROW = 4 * M * PB, CHUNKS = ROW / 16, BYTES = 16 * ROW, STORES = BYTES / 1024;
+    __device__ __forceinline__ static char* at(char* wave_lds, uint32_t row, uint32_t chunk) {
+        return wave_lds + row * ROW + (chunk ^ (row & (CHUNKS - 1))) * 16;
+    }
+    template <typename P>
+    __device__ __forceinline__ static void put(char* wave_lds, uint32_t lane, int m, const P& piece) {
+        static_assert(sizeof(P) == PB);
+        const uint32_t byte = (m * 4 + (lane >> 4)) * PB;
+        *reinterpret_cast<P*>(at(wave_lds, lane & 15, byte / 16) + byte % 16) = piece;
+    }
+    // The lane's part of store j: 16 bytes of row(), at 16 chunk().
+    __device__ __forceinline__ static uint32_t row(uint32_t lane, int j) { return (j * 64 + lane) / CHUNKS; }
+    __device__ __forceinline__ static uint32_t chunk(uint32_t lane) { return lane % CHUNKS; }
+    __device__ __forceinline__ static u32x4 get(char* wave_lds, uint32_t lane, int j) {
+        return *reinterpret_cast<const u32x4*>(at(wave_lds, row(lane, j), chunk(lane)));
+    }
+};
+
 // Which step of the products a side's loads have come to: plane pair c of 64 k block k of the workgroup's tile `tile`.
 struct Cursor {
     uint32_t c, k, tile;

@@ -484,55 +484,66 @@ __global__ __launch_bounds__(THREADS, 2) void weights_kernel(XentArgs a) {
     // (the first barrier of the loop below orders these before they are read)
     // Every lane stores every time (so that the number of stores is known to the next step's barrier): rows of G are whole
     // tiles of queries, and G is whole tiles of candidates.
-    S::template run<S::TM * S::TN * PG>(a, end, q0, along, lds, [&](f32x4 (&acc)[S::TM][S::TN], uint32_t first) {
-        const uint32_t l = afresh(threadIdx.x) & 63, row0 = S::wave_r() * S::WR * 16 + (l & 15), i0 = S::wave_q() * S::WQ * 16 + (l >> 4) * 4;
-        char* out = a.g + (uint64_t)(first - a.piece_begin + row0) * a.g_stride + (q0 + i0) * 2;
+    constexpr int UNIT = S::TM < 4 ? S::TM : 4;  // fragments that go through LDS at a time: 64 queries of 16 candidates
+    using T = Turn<8, UNIT>;
+    char* const wave_lds = lds + S::LDS + uniform_u32(threadIdx.x >> 6) * T::BYTES;
+    S::template run<S::TN * (S::TM / UNIT) * T::STORES * PG>(a, end, q0, along, lds, [&](f32x4 (&acc)[S::TM][S::TN], uint32_t first) {
+        const uint32_t l = afresh(threadIdx.x) & 63, row0 = S::wave_r() * S::WR * 16, i0 = S::wave_q() * S::WQ * 16 + (l >> 4) * 4;
+        char* out = a.g + (uint64_t)(first - a.piece_begin + row0) * a.g_stride + (q0 + S::wave_q() * S::WQ * 16) * 2;
         float inverse[S::TN];
         if constexpr (NORMS)
 #pragma unroll
             for (int n = 0; n < S::TN; ++n) {
-                const float x = a.norms[row_at(a, min(first + row0 + n * 16, end - 1))];
+                const float x = a.norms[row_at(a, min(first + row0 + (l & 15) + n * 16, end - 1))];
                 inverse[n] = x > 0 ? 1.0f / x : 0.0f;
             }
 #pragma unroll
-        for (int t = 0; t < S::TM; ++t) {
-            const uint32_t i = i0 + t * 16;
-            const f32x4 vs = *reinterpret_cast<const f32x4*>(s2 + i), vl = *reinterpret_cast<const f32x4*>(lse2 + i);
-            const f32x4 vf = *reinterpret_cast<const f32x4*>(factor + i), vc = *reinterpret_cast<const f32x4*>(at_click + i);
-            const u32x4 vp = *reinterpret_cast<const u32x4*>(click + i);
+        for (int u = 0; u < S::TM / UNIT; ++u)
 #pragma unroll
             for (int n = 0; n < S::TN; ++n) {
-                const uint32_t place = first + row0 + n * 16;
-                Pack<uint16_t, 4> p[3];
+                const uint32_t place = first + row0 + (l & 15) + n * 16;
+                Pack<uint16_t, 4> p[UNIT][3];
 #pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    float z = acc[t][n][r];
-                    if constexpr (NORMS) z *= inverse[n];
-                    float g = vp[r] == place ? vc[r] : vf[r] * __builtin_amdgcn_exp2f(__builtin_fmaf(z, vs[r], -vl[r]));
-                    if (vf[r] == 0.0f) g = 0.0f;  // no click, no query (an exponential over a lse of -inf is none)
-                    if constexpr (NORMS) g *= inverse[n];
-                    if constexpr (PG == 1) {
-                        p[0].e[r] = (uint16_t)bf16_bits(g);
-                    } else {
-                        const Split x = split(g);
-                        p[0].e[r] = x.h;
-                        p[1].e[r] = x.m;
-                        p[2].e[r] = x.l;
+                for (int t = 0; t < UNIT; ++t) {
+                    const uint32_t i = i0 + (u * UNIT + t) * 16;
+                    const f32x4 vs = *reinterpret_cast<const f32x4*>(s2 + i), vl = *reinterpret_cast<const f32x4*>(lse2 + i);
+                    const f32x4 vf = *reinterpret_cast<const f32x4*>(factor + i), vc = *reinterpret_cast<const f32x4*>(at_click + i);
+                    const u32x4 vp = *reinterpret_cast<const u32x4*>(click + i);
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        float z = acc[u * UNIT + t][n][r];
+                        if constexpr (NORMS) z *= inverse[n];
+                        // (a query without a click has factor 0 and a finite lse if there is any candidate)
+                        float g = vp[r] == place ? vc[r] : vf[r] * __builtin_amdgcn_exp2f(__builtin_fmaf(z, vs[r], -vl[r]));
+                        if constexpr (NORMS) g *= inverse[n];
+                        if constexpr (PG == 1) {
+                            p[t][0].e[r] = (uint16_t)bf16_bits(g);
+                        } else {
+                            const Split x = split(g);
+                            p[t][0].e[r] = x.h;
+                            p[t][1].e[r] = x.m;
+                            p[t][2].e[r] = x.l;
+                        }
                     }
                 }
 #pragma unroll
-                for (int k = 0; k < PG; ++k)
-                    store_pack<uint16_t, 4>(reinterpret_cast<uint16_t*>(out + k * a.g_plane + n * 16ull * a.g_stride) + t * 16, p[k]);
-                if (PG == 3 || n + 1 == S::TN) __builtin_amdgcn_sched_barrier(0);  // (the registers hold no more at a time)
+                for (int k = 0; k < PG; ++k) {
+#pragma unroll
+                    for (int t = 0; t < UNIT; ++t) T::put(wave_lds, l, t, p[t][k]);
+#pragma unroll
+                    for (int j = 0; j < T::STORES; ++j)
+                        *reinterpret_cast<u32x4*>(out + k * a.g_plane + (uint64_t)(n * 16 + T::row(l, j)) * a.g_stride + u * T::ROW +
+                                                  T::chunk(l) * 16) = T::get(wave_lds, l, j);
+                }
+                __builtin_amdgcn_sched_barrier(0);  // (the registers hold no more at a time)
             }
-        }
         return true;
     });
 }
 
 // drows of a piece: transposed queries (BD columns of the rows) by G. A lane holds four neighbouring columns of a row.
-// WIDE: rows take four elements at a time; as in weights_kernel every lane stores every time, to its own 16 bytes of
-// a.spill where it has no row or column.
+// WIDE: rows take 16 bytes at a time; as in weights_kernel every lane stores every time, to its own 16 bytes of a.spill
+// where it has no row or column.
 template <int BD, typename E, bool WIDE>
 __global__ __launch_bounds__(THREADS, 2) void row_grads_kernel(XentArgs a) {
     using A = Rows<BD>;
@@ -576,6 +587,9 @@ __global__ __launch_bounds__(THREADS, 2) void row_grads_kernel(XentArgs a) {
     e.ask(half_q(0), half_g(0), 0);
     load_weights(1);
     uint32_t at = 0;
+    constexpr int UNIT = sizeof(E) == 2 ? TM : 4;  // fragments that go through LDS at a time: 256 bytes of a row at most
+    using T = Turn<4 * sizeof(E), UNIT>;
+    char* const wave_lds = lds + 2 * (A::BYTES + B::BYTES) + wave * T::BYTES;
     uint32_t early = 0, stored = 0;  // as in Scores::run
 #pragma nounroll
     for (uint32_t tile = along; tile < tiles; tile += a.splits) {
@@ -583,7 +597,7 @@ __global__ __launch_bounds__(THREADS, 2) void row_grads_kernel(XentArgs a) {
 #pragma nounroll
         for (uint32_t s = 0; s < steps; ++s) {
             const uint32_t other = at ^ 1;
-            e.template step<WIDE ? TM * TN : 0>(half_q(at), half_g(at), half_q(other), half_g(other), acc, stored, [&](int phase) {
+            e.template step<WIDE ? TN * (TM / UNIT) * T::STORES : 0>(half_q(at), half_g(at), half_q(other), half_g(other), acc, stored, [&](int phase) {
                 if (phase < En::PHASES - 1) {
                     constexpr int EACH = (A::LOADS + En::PHASES - 2) / (En::PHASES - 1);
                     if (early || cq.tile >= tiles) return;
@@ -602,25 +616,40 @@ __global__ __launch_bounds__(THREADS, 2) void row_grads_kernel(XentArgs a) {
             stored = afresh_uniform(0);
             at = other;
         }
-        const uint32_t l = afresh(threadIdx.x) & 63, d0 = tile_d * BD + wd * TM * 16 + (l >> 4) * 4;
+        const uint32_t l = afresh(threadIdx.x) & 63, d0 = tile_d * BD + wd * TM * 16, place0 = a.piece_begin + tile * TILE + wr * TN * 16;
+        if constexpr (WIDE) {
+            char* const spill = a.spill + (blockIdx.x * THREADS + threadIdx.x) * 16ull;
 #pragma unroll
-        for (int n = 0; n < TN; ++n) {
-            const uint32_t place = a.piece_begin + tile * TILE + (wr * TN + n) * 16 + (l & 15);
-            E* out = static_cast<E*>(a.grad_rows) + row_at(a, min(place, end - 1)) * a.grad_row_stride;
+            for (int n = 0; n < TN; ++n)
 #pragma unroll
-            for (int m = 0; m < TM; ++m) {
-                const uint32_t d = d0 + m * 16;
-                Pack<E, 4> p;
+                for (int u = 0; u < TM / UNIT; ++u) {
 #pragma unroll
-                for (int i = 0; i < 4; ++i) p.e[i] = from_f32<E>(acc[m][n][i]);
-                if constexpr (WIDE) {
-                    E* const spill = reinterpret_cast<E*>(a.spill + (blockIdx.x * THREADS + threadIdx.x) * 16ull);
-                    store_pack<E, 4>(place < end && d < a.dim ? out + d : spill, p);
-                } else {
+                    for (int t = 0; t < UNIT; ++t) {
+                        Pack<E, 4> p;
 #pragma unroll
-                    for (int i = 0; i < 4; ++i)
-                        if (place < end && d + i < a.dim) out[d + i] = p.e[i];
+                        for (int i = 0; i < 4; ++i) p.e[i] = from_f32<E>(acc[u * UNIT + t][n][i]);
+                        T::put(wave_lds, l, t, p);
+                    }
+#pragma unroll
+                    for (int j = 0; j < T::STORES; ++j) {
+                        const uint32_t place = place0 + n * 16 + T::row(l, j), d = d0 + u * UNIT * 16 + T::chunk(l) * (16 / sizeof(E));
+                        E* out = static_cast<E*>(a.grad_rows) + row_at(a, min(place, end - 1)) * a.grad_row_stride + d;
+                        *reinterpret_cast<u32x4*>(place < end && d < a.dim ? (char*)out : spill) = T::get(wave_lds, l, j);
+                    }
+                    __builtin_amdgcn_sched_barrier(0);
                 }
+        } else {
+#pragma unroll
+            for (int n = 0; n < TN; ++n) {
+                const uint32_t place = place0 + n * 16 + (l & 15);
+                E* out = static_cast<E*>(a.grad_rows) + row_at(a, min(place, end - 1)) * a.grad_row_stride;
+#pragma unroll
+                for (int m = 0; m < TM; ++m)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const uint32_t d = d0 + m * 16 + (l >> 4) * 4 + i;
+                        if (place < end && d < a.dim) out[d] = from_f32<E>(acc[m][n][i]);
+                    }
             }
         }
         stored = afresh_uniform(early);
@@ -767,8 +796,8 @@ __global__ __launch_bounds__(256) void clear_rows_kernel(const uint64_t* mask, c
 
 // ---- host side ----------------------------------------------------------------------------
 
-constexpr uint64_t PIECE_BYTES = 256u << 20;  // of weights, and of planes, that are held at a time: the size of the
-                                              // memory-side cache, from which the products read them again
+constexpr uint64_t PIECE_BYTES = 512u << 20;  // of weights, and of planes, that are held at a time (half of it, a piece that
+                                              // the memory-side cache holds, costs more in launches than it saves)
 constexpr uint32_t WORKGROUPS = 256;          // of a product: one per CU (the LDS of a tile fills one)
 
 // hh, hm, mh, mm, hl, lh | plane 0 alone | planes 0 and 1 of A
@@ -958,7 +987,7 @@ struct Call {
     template <int BQ, int PG>
     void weights() {
         by_kind([&](auto norms, auto listed) {
-            product(weights_kernel<BQ, norms, listed, PG>, Scores<BQ, false, listed>::LDS, p.q_tiles, p.weight_splits);
+            product(weights_kernel<BQ, norms, listed, PG>, Scores<BQ, false, listed>::LDS + 8 * 2048, p.q_tiles, p.weight_splits);
         });
     }
     template <int BQ>
@@ -972,15 +1001,16 @@ struct Call {
     template <int BQ>
     void product_f32_weights() {  // (always from planes, never through the list)
         if (a.norms)
-            product(weights_kernel<BQ, true, false, 3>, Scores<BQ, false, false>::LDS, p.q_tiles, p.weight_splits);
+            product(weights_kernel<BQ, true, false, 3>, Scores<BQ, false, false>::LDS + 8 * 2048, p.q_tiles, p.weight_splits);
         else
-            product(weights_kernel<BQ, false, false, 3>, Scores<BQ, false, false>::LDS, p.q_tiles, p.weight_splits);
+            product(weights_kernel<BQ, false, false, 3>, Scores<BQ, false, false>::LDS + 8 * 2048, p.q_tiles, p.weight_splits);
     }
 
     template <int BD, typename E>
     void row_grads() {
-        constexpr uint32_t LDS = 2 * (Rows<BD>::BYTES + Rows<TILE>::BYTES);
-        if (aligned_rows<E, 4>(a.grad_rows, a.grad_row_stride) && a.dim % 4 == 0)
+        constexpr int V = 16 / sizeof(E);
+        constexpr uint32_t LDS = 2 * (Rows<BD>::BYTES + Rows<TILE>::BYTES) + 8 * 4096;  // and a Turn's rows for every wave
+        if (aligned_rows<E, V>(a.grad_rows, a.grad_row_stride) && a.dim % V == 0)
             product(row_grads_kernel<BD, E, true>, LDS, p.d_tiles, p.row_splits);
         else
             product(row_grads_kernel<BD, E, false>, LDS, p.d_tiles, p.row_splits);
