@@ -35,13 +35,33 @@ template <typename E, int V>
 struct alignas(sizeof(E) * V < 16 ? sizeof(E) * V : 16) Pack {
     E e[V];
 };
+// (as vectors: element by element the compiler would join a wide store with the narrow one of another branch, and
+// take the narrow)
 template <typename E, int V>
 __device__ __forceinline__ Pack<E, V> load_pack(const E* p) {
-    return *reinterpret_cast<const Pack<E, V>*>(p);
+    constexpr int N = sizeof(E) * V;
+    if constexpr (N % 16 == 0) {
+        Pack<E, V> x;
+#pragma unroll
+        for (int i = 0; i < N / 16; ++i) reinterpret_cast<u32x4*>(&x)[i] = reinterpret_cast<const u32x4*>(p)[i];
+        return x;
+    } else if constexpr (N == 8) {
+        return __builtin_bit_cast(Pack<E, V>, *reinterpret_cast<const u32x2*>(p));
+    } else {
+        return *reinterpret_cast<const Pack<E, V>*>(p);
+    }
 }
 template <typename E, int V>
 __device__ __forceinline__ void store_pack(E* p, const Pack<E, V>& x) {
-    *reinterpret_cast<Pack<E, V>*>(p) = x;
+    constexpr int N = sizeof(E) * V;
+    if constexpr (N % 16 == 0) {
+#pragma unroll
+        for (int i = 0; i < N / 16; ++i) reinterpret_cast<u32x4*>(p)[i] = reinterpret_cast<const u32x4*>(&x)[i];
+    } else if constexpr (N == 8) {
+        *reinterpret_cast<u32x2*>(p) = __builtin_bit_cast(u32x2, x);
+    } else {
+        *reinterpret_cast<Pack<E, V>*>(p) = x;
+    }
 }
 // Whether every row of a table starts where a Pack<E, V> may.
 template <typename E, int V>

@@ -171,7 +171,7 @@ namespace {
 // The n (row, position) pairs are sorted by row, positions ascending within a row, so that a row's sum is a run of
 // neighbours, taken in one order. Positions outside every bag and ids without a row get the row n_rows and come last.
 constexpr uint32_t SMALL = 2048;      // ids of the one-kernel sort
-constexpr uint32_t TILE = 4096;       // keys of a workgroup in a pass of the long sort
+constexpr uint32_t TILE = 1024;       // keys of a workgroup in a pass of the long sort
 constexpr uint32_t RUN = 64;          // sorted entries that one thread sums before it hands over
 
 struct GradArgs {
@@ -187,8 +187,11 @@ struct GradArgs {
     uint32_t* places[2];  // after the sort, behind its last pass' keys: bag (places) and weight (keys) of each entry
     uint32_t* hist;
     uint32_t* totals;
+    uint32_t* bag_at;  // [n] the bag of each position
     uint32_t* heads;   // first entries of runs, counted per TILE of sorted entries
+    uint32_t* handed;  // [n_runs] number of the run that each piece hands over at its end
     float* partial;    // [n_runs][2][chunks * V]
+    bool wide;         // rows of the result take V elements at a time
     RowGrads out;
 };
 
@@ -213,24 +216,34 @@ __device__ __forceinline__ uint32_t key_of(const GradArgs& a, uint32_t p) {
     return !a.b.offsets && p >= a.b.n_bags ? (uint32_t)a.n_rows : id;
 }
 
-// Up to SMALL ids: entry p's place is the number of entries that sort before it, counted against all of them in LDS
-// (four comparisons per 16-byte read that all lanes share). One launch of a few microseconds, where the passes below
-// are nine launches.
+// Up to SMALL ids: entry p's place is the number of entries that sort before it, counted against all of them in LDS,
+// four threads an entry and four comparisons a read. One launch, where the passes below are nine. The offsets are
+// searched in LDS too: from memory, each step of a search would wait for the one before it.
 __global__ __launch_bounds__(256) void rank_sort_kernel(GradArgs a) {
     __shared__ __align__(16) uint32_t keys[SMALL];
-    for (uint32_t i = threadIdx.x; i < SMALL; i += 256) keys[i] = i < a.n ? key_of(a, i) : NONE;
+    __shared__ uint32_t offsets[SMALL + 1];
+    const bool near = a.b.offsets && a.b.n_bags <= SMALL;
+    if (near)
+        for (uint32_t i = threadIdx.x; i <= a.b.n_bags; i += 256) offsets[i] = a.b.offsets[i];
+    const uint32_t padded = (a.n + 15) / 16 * 16;
+    for (uint32_t i = threadIdx.x; i < padded; i += 256) keys[i] = i < a.n ? key_of(a, i) : NONE;
     __syncthreads();
-    const uint32_t p = blockIdx.x * 256 + threadIdx.x;
+    const uint32_t p = blockIdx.x * 64 + (threadIdx.x >> 2), quarter = threadIdx.x & 3;
     const uint32_t key = p < a.n ? keys[p] : NONE;
     uint32_t place = 0;
-    for (uint32_t i = 0; i < a.n; i += 4) {
+#pragma unroll 4
+    for (uint32_t i = quarter * 4; i < padded; i += 16) {
         const u32x4 k = *reinterpret_cast<const u32x4*>(keys + i);
 #pragma unroll
         for (int j = 0; j < 4; ++j) place += k[j] < key || (k[j] == key && i + j < p);
     }
-    if (p >= a.n) return;
+    place += __shfl_xor(place, 1);
+    place += __shfl_xor(place, 2);
+    if (p >= a.n || quarter) return;
+    Bags b = a.b;
+    if (near) b.offsets = offsets;
     a.keys[0][place] = key;
-    a.places[1][place] = key < a.n_rows ? bag_of(a.b, p) : 0;
+    a.places[1][place] = key < a.n_rows ? bag_of(b, p) : 0;
     reinterpret_cast<float*>(a.keys[1])[place] = a.b.weights ? a.b.weights[p] : 1.0f;
 }
 
@@ -309,16 +322,26 @@ __device__ __forceinline__ bool is_head(const GradArgs& a, const uint32_t* keys,
     return keys[i] < a.n_rows && (!i || keys[i - 1] != keys[i]);
 }
 
+// The bag of every position (neighbours walk the same way through the offsets, so one line serves a wave at each step;
+// looked up after the sort, every lane would walk its own).
+__global__ __launch_bounds__(256) void map_bags_kernel(GradArgs a) {
+    const uint32_t p = blockIdx.x * 256 + threadIdx.x;
+    if (p < a.n) a.bag_at[p] = bag_of(a.b, p);
+}
+
 // After the last pass: each entry's bag and weight, so that the sums read them in order, and the heads of each tile.
 __global__ __launch_bounds__(256) void settle_kernel(GradArgs a, int side) {
     __shared__ uint32_t wave_sum[4];
     uint32_t n = 0;
     const uint32_t begin = blockIdx.x * TILE, end = min(begin + TILE, a.n);
     const uint32_t *keys = a.keys[side], *places = a.places[side];
-    for (uint32_t i = begin + threadIdx.x; i < end; i += 256) {
+#pragma unroll
+    for (uint32_t k = 0; k < TILE; k += 256) {
+        const uint32_t i = begin + k + threadIdx.x;
+        if (i >= end) break;
         n += is_head(a, keys, i);
         const uint32_t p = places[i];
-        a.places[!side][i] = keys[i] < a.n_rows ? bag_of(a.b, p) : 0;
+        a.places[!side][i] = keys[i] < a.n_rows ? a.bag_at[p] : 0;
         reinterpret_cast<float*>(a.keys[!side])[i] = a.b.weights ? a.b.weights[p] : 1.0f;
     }
     uint32_t total;
@@ -341,12 +364,24 @@ __device__ uint32_t heads_before(const GradArgs& a, const uint32_t* keys, uint32
 template <typename O, int V>
 __device__ __forceinline__ void store_row(const GradArgs& a, uint32_t row, uint32_t compact, uint32_t col, const float (&acc)[V]) {
     O* out = static_cast<O*>(a.out.rows) + (uint64_t)(a.out.unique ? compact : row) * a.out.stride + col;
+    Pack<O, V> p;
+    if (!a.out.unique) {  // a row belongs to one thread: a plain addition
+        if (a.wide)
+            p = load_pack<O, V>(out);
+        else
 #pragma unroll
-    for (int v = 0; v < V; ++v)
-        if (V == 1 || col + v < a.dim) {
-            const float x = acc[v] * a.b.scale;
-            out[v] = from_f32<O>(a.out.unique ? x : x + to_f32(out[v]));  // a row belongs to one thread: a plain addition
-        }
+            for (int v = 0; v < V; ++v) p.e[v] = out[v];
+    }
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+        const float x = acc[v] * a.b.scale;
+        p.e[v] = from_f32<O>(a.out.unique ? x : x + to_f32(p.e[v]));
+    }
+    if (a.wide)
+        store_pack<O, V>(out, p);
+    else
+#pragma unroll
+        for (int v = 0; v < V; ++v) out[v] = p.e[v];
 }
 
 // Up to SMALL ids: a workgroup per (sorted entry, 64 pieces). The ones at a run's head sum the run, a quarter in each
@@ -463,7 +498,9 @@ __global__ __launch_bounds__(256) void sum_runs_kernel(GradArgs a, int side) {
             for (int v = 0; v < V; ++v) acc[v] = __builtin_fmaf(w[u], to_f32(x[u].e[v]), acc[v]);
         }
     }
-    if (row < a.n_rows) hand_over(end < a.n && keys[end] == row);
+    if (row >= a.n_rows) return;
+    if (!chunk) a.handed[run] = compact;
+    hand_over(end < a.n && keys[end] == row);
 }
 
 // The runs that were handed over: a workgroup per (piece where one began, 64 pieces of columns); four waves take every
@@ -471,7 +508,6 @@ __global__ __launch_bounds__(256) void sum_runs_kernel(GradArgs a, int side) {
 template <typename O, int V>
 __global__ __launch_bounds__(256) void join_runs_kernel(GradArgs a, int side) {
     __shared__ float part[4][V][64];
-    __shared__ uint32_t wave_sum[4];
     const uint32_t* keys = a.keys[side];
     const uint32_t run = blockIdx.x, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const uint32_t begin = run * RUN, end = min(begin + RUN, a.n);
@@ -487,14 +523,7 @@ __global__ __launch_bounds__(256) void join_runs_kernel(GradArgs a, int side) {
         else
             hi = mid;
     }
-    const uint32_t last = lo;
-    uint32_t compact = 0;
-    if (a.out.unique) {
-        uint32_t mine = 0, length;  // of the run within this piece
-        for (uint32_t j = begin + threadIdx.x; j < end; j += 256) mine += keys[j] == row;
-        block_exclusive(mine, wave_sum, &length);
-        compact = heads_before(a, keys, end - length, wave_sum);
-    }
+    const uint32_t last = lo, compact = a.handed[run];
     const uint32_t chunk = blockIdx.y * 64 + lane;
     float acc[V] = {};
     if (chunk < a.chunks) {
@@ -519,8 +548,8 @@ __global__ __launch_bounds__(256) void join_runs_kernel(GradArgs a, int side) {
     store_row<O, V>(a, row, compact, chunk * V, acc);
 }
 
-// A wave takes `span` neighbouring positions, four at a time: the products of each one's row with its bag's gradient, in
-// pieces of V columns, joined over the lanes.
+// A wave takes `span` neighbouring positions (64 at most: a lane looks up the row and the bag of each), four at a time:
+// the products of each one's row with its bag's gradient, in pieces of V columns, joined over the lanes.
 struct WeightArgs {
     Table t;
     Bags b;
@@ -533,51 +562,56 @@ template <typename E, typename G, int V>
 __global__ __launch_bounds__(256) void weight_grads_kernel(WeightArgs a) {
     constexpr int U = 4;
     const uint32_t lane = threadIdx.x & 63, wave = uniform_u32(threadIdx.x >> 6);
-    const uint64_t begin = ((uint64_t)blockIdx.x * 4 + wave) * a.span, end = min(begin + a.span, a.b.n_ids);
-    if (begin >= end) return;
+    const uint64_t begin = ((uint64_t)blockIdx.x * 4 + wave) * a.span;
+    if (begin >= a.b.n_ids) return;
+    const uint32_t n = (uint32_t)min((uint64_t)a.span, a.b.n_ids - begin);
+    uint32_t row = NONE, bag = NONE;
+    if (lane < n) {
+        row = row_of(a.t, a.b.ids[begin + lane]);
+        bag = bag_of(a.b, (uint32_t)begin + lane);
+        if (bag == NONE) row = NONE;
+    }
+    float result = 0;
     const E* rows = static_cast<const E*>(a.t.rows);
     const G* grads = static_cast<const G*>(a.grad_out);
-    for (uint64_t i = begin; i < end; i += U) {
-        uint32_t r[U], bag[U];
+    for (uint32_t i = 0; i < n; i += U) {
+        uint32_t r[U], g[U];
         float sum[U] = {};
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            const uint64_t p = i + u;
-            r[u] = p < end ? row_of(a.t, a.b.ids[p]) : NONE;
-            bag[u] = r[u] != NONE ? bag_of(a.b, (uint32_t)p) : NONE;
-            if (bag[u] == NONE) r[u] = NONE;
+            r[u] = (uint32_t)__builtin_amdgcn_readlane((int)row, (int)min(i + u, 63u));
+            g[u] = (uint32_t)__builtin_amdgcn_readlane((int)bag, (int)min(i + u, 63u));
         }
         for (uint32_t c = lane; c < a.chunks; c += 64) {
             Pack<E, V> x[U];
-            Pack<G, V> g[U];
+            Pack<G, V> y[U];
 #pragma unroll
-            for (int u = 0; u < U; ++u) {
-                if (r[u] == NONE) continue;
-                x[u] = load_pack<E, V>(rows + (uint64_t)r[u] * a.t.stride + c * V);
-                g[u] = load_pack<G, V>(grads + (uint64_t)bag[u] * a.grad_stride + c * V);
+            for (int u = 0; u < U; ++u) {  // (a position without a row reads row 0 and bag 0, and is not used)
+                x[u] = load_pack<E, V>(rows + (uint64_t)(r[u] == NONE ? 0 : r[u]) * a.t.stride + c * V);
+                y[u] = load_pack<G, V>(grads + (uint64_t)(r[u] == NONE ? 0 : g[u]) * a.grad_stride + c * V);
             }
 #pragma unroll
-            for (int u = 0; u < U; ++u) {
-                if (r[u] == NONE) continue;
+            for (int u = 0; u < U; ++u)
 #pragma unroll
-                for (int v = 0; v < V; ++v) sum[u] = __builtin_fmaf(to_f32(x[u].e[v]), to_f32(g[u].e[v]), sum[u]);
-            }
+                for (int v = 0; v < V; ++v) sum[u] = __builtin_fmaf(to_f32(x[u].e[v]), to_f32(y[u].e[v]), sum[u]);
         }
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             const float total = wave_sum(sum[u]);
-            if (!lane && i + u < end) a.out[i + u] = total * a.b.scale;
+            if (lane == i + u) result = row == NONE ? 0.0f : total * a.b.scale;
         }
     }
+    if (lane < n) a.out[begin + lane] = result;
 }
 
 template <typename E, typename O, int V>
 hipError_t run_lookup_grad(GradArgs a, hipStream_t stream) {
-    a.chunks = (a.dim + V - 1) / V;
+    a.chunks = a.dim / V;
+    a.wide = aligned_rows<O, V>(a.out.rows, a.out.stride);
     const uint32_t col_blocks = (a.chunks + 63) / 64;
     if (a.n <= SMALL) {
         a.heads = nullptr;
-        rank_sort_kernel<<<(a.n + 255) / 256, 256, 0, stream>>>(a);
+        rank_sort_kernel<<<(a.n + 63) / 64, 256, 0, stream>>>(a);
         sum_small_kernel<E, O, V><<<dim3(a.n, col_blocks), 256, 0, stream>>>(a);
         return hipGetLastError();
     }
@@ -590,6 +624,7 @@ hipError_t run_lookup_grad(GradArgs a, hipStream_t stream) {
         sort_scatter_kernel<<<n_tiles, 256, 0, stream>>>(a, pass, n_tiles);
     }
     const int side = passes & 1;
+    map_bags_kernel<<<(a.n + 255) / 256, 256, 0, stream>>>(a);
     settle_kernel<<<n_tiles, 256, 0, stream>>>(a, side);
     const uint64_t threads = (uint64_t)a.n_runs * a.chunks;
     sum_runs_kernel<E, O, V><<<(uint32_t)((threads + 255) / 256), 256, 0, stream>>>(a, side);
@@ -603,7 +638,7 @@ uint64_t padded_dim(uint32_t dim) { return (dim + 7ull) / 8 * 8; }
 
 uint64_t lookup_grad_workspace_bytes(uint64_t n_ids, uint64_t n_rows, uint32_t dim) {
     const uint64_t n_tiles = (n_ids + TILE - 1) / TILE, n_runs = (n_ids + RUN - 1) / RUN;
-    return 4 * round_up(n_ids * 4, 256) + round_up(n_tiles * 1024, 256) + 1024 + round_up(n_tiles * 4, 256) +
+    return 5 * round_up(n_ids * 4, 256) + round_up(n_tiles * 1024, 256) + 1024 + round_up(n_tiles * 4, 256) + round_up(n_runs * 4, 256) +
            (n_ids <= SMALL ? 0 : round_up(n_runs * 2 * padded_dim(dim) * 4, 256)) + 256;
 }
 
@@ -628,7 +663,9 @@ hipError_t launch_lookup_grad(const void* grad_out, int32_t dtype, uint64_t grad
     const uint32_t n_tiles = (a.n + TILE - 1) / TILE;
     a.hist = w.take<uint32_t>(256ull * n_tiles);
     a.totals = w.take<uint32_t>(256);
+    a.bag_at = w.take<uint32_t>(a.n);
     a.heads = w.take<uint32_t>(n_tiles);
+    a.handed = w.take<uint32_t>(a.n_runs);
     a.partial = w.take<float>(a.n <= SMALL ? 0 : (uint64_t)a.n_runs * 2 * padded_dim(dim));
     auto pick = [&](auto e, auto o) {
         using E = decltype(e);
@@ -645,7 +682,12 @@ hipError_t launch_lookup_grad_weights(const Table& t, const Bags& b, const void*
                                       uint64_t grad_stride, float* out, hipStream_t stream) {
     WeightArgs a{t, b, grad_out, grad_stride, out, 0, 0};
     if (!b.n_ids) return hipSuccess;
-    a.span = (uint32_t)std::min<uint64_t>(std::max<uint64_t>(b.n_ids / 8192, 1), 16);  // enough waves for every SIMD first
+    if (!b.n_bags) {  // (nothing to multiply with)
+        fill_u32(reinterpret_cast<uint32_t*>(out), b.n_ids, 0u, stream);
+        return hipGetLastError();
+    }
+    // enough waves for every SIMD to hold eight first; then longer spans, which look more bags up at once
+    a.span = (uint32_t)std::min<uint64_t>((b.n_ids + 8191) / 8192, 64);
     const uint32_t grid = (uint32_t)((b.n_ids + 4 * a.span - 1) / (4 * a.span));
     auto pick = [&](auto e, auto g) {
         using E = decltype(e);

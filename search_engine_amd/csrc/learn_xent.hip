@@ -62,6 +62,17 @@ struct XentArgs {
     float* part_q;            // [splits][n_q][dim]
 };
 
+// What the loss of a few queries reads as the caller has it.
+struct Few {
+    const void *rows, *queries;
+    uint64_t stride, query_stride;
+    const uint32_t* targets;
+    const uint64_t *mask, *present;
+    uint32_t first_id;
+    float scale;
+    uint32_t parts;  // of a word that waves take: 1, 2, 4 or 8
+};
+
 // (told to the compiler as one value for all lanes: the loops of the products run on it)
 __device__ __forceinline__ uint32_t candidates(const XentArgs& a) {
     return uniform_u32(a.list ? *a.count : (uint32_t)a.n_rows);
@@ -90,26 +101,27 @@ __device__ __forceinline__ uint64_t word_at(const uint64_t* mask, const uint64_t
     return left < 64 ? w & ((1ull << left) - 1) : w;
 }
 
-// The candidate rows in ascending order: 1024 words of the masks per workgroup, which counts the words before its own
-// by itself (at ten million rows the last one reads 1.2 MB for that).
+// The candidate rows in ascending order: 256 words of the masks per workgroup, which counts the words before its own by
+// itself (at ten million rows the last one reads 1.2 MB for that). A wave writes a word's rows together, lane l the l-th
+// bit's: a lane writing its own word's rows would touch a line of its own with each.
+constexpr uint32_t LIST_WORDS = 256;
 __global__ __launch_bounds__(256) void list_candidates_kernel(const uint64_t* mask, const uint64_t* present, uint64_t n_rows,
                                                               uint32_t* list, uint32_t* count) {
     __shared__ uint32_t wave_sum[4];
-    const uint64_t n_words = (n_rows + 63) / 64, first = (uint64_t)blockIdx.x * 1024;
+    const uint64_t n_words = (n_rows + 63) / 64, first = (uint64_t)blockIdx.x * LIST_WORDS;
     uint32_t n = 0, before, total;
     for (uint64_t i = threadIdx.x; i < first; i += 256) n += __popcll(word_at(mask, present, i, n_rows));
     block_exclusive(n, wave_sum, &before);
-    uint64_t words[4];
-    n = 0;
-    for (int j = 0; j < 4; ++j) {
-        const uint64_t i = first + threadIdx.x * 4 + j;
-        words[j] = i < n_words ? word_at(mask, present, i, n_rows) : 0;
-        n += __popcll(words[j]);
+    const uint64_t i = first + threadIdx.x;
+    const uint64_t word = i < n_words ? word_at(mask, present, i, n_rows) : 0;
+    const uint32_t at = before + block_exclusive((uint32_t)__popcll(word), wave_sum, &total);
+    const uint32_t lane = threadIdx.x & 63;
+    const uint32_t row0 = (uint32_t)(first + (threadIdx.x & ~63u)) * 64;  // of the wave's first word
+    for (int k = 0; k < 64; ++k) {
+        const uint64_t w = readlane_u64(word, k);
+        const uint32_t to = (uint32_t)__builtin_amdgcn_readlane((int)at, k);
+        if (w >> lane & 1) list[to + __popcll(w & ((1ull << lane) - 1))] = row0 + k * 64 + lane;
     }
-    uint32_t at = before + block_exclusive(n, wave_sum, &total);
-    for (int j = 0; j < 4; ++j)
-        for (uint64_t w = words[j]; w; w &= w - 1)
-            list[at++] = (uint32_t)((first + threadIdx.x * 4 + j) * 64 + __builtin_ctzll(w));
     if (blockIdx.x == gridDim.x - 1 && !threadIdx.x) *count = before + total;
 }
 
@@ -119,33 +131,43 @@ template <typename Q, int P>
 __global__ __launch_bounds__(256) void pack_queries_kernel(XentArgs a, const Q* queries, uint64_t stride, const uint32_t* targets,
                                                            uint32_t first_id, uint64_t n_rows, float scale, uint32_t* click,
                                                            float* qscale, uint32_t* zeros, bool transposed) {
-    __shared__ uint16_t t[P][64][66];
+    __shared__ uint16_t t[P][64][72];  // [column][query], eight queries more than there are: rows stay 16-byte aligned
     const uint32_t n_tiles = a.gq / 64 * (a.q.chunks / 8);
     if (!blockIdx.x && threadIdx.x < 64) zeros[threadIdx.x] = 0;
     if (blockIdx.x < n_tiles) {
         const uint32_t q0 = blockIdx.x % (a.gq / 64) * 64, d0 = blockIdx.x / (a.gq / 64) * 64;
-        for (uint32_t i = threadIdx.x; i < 4096; i += 256) {
-            const uint32_t q = q0 + i / 64, d = d0 + i % 64;
-            const float x = q < a.n_q && d < a.dim ? to_f32(queries[q * stride + d]) : 0.0f;
-            const Split s = split(x);
-            const uint16_t part[3] = {s.h, s.m, s.l};
+#pragma unroll
+        for (uint32_t k = 0; k < 512; k += 256) {
+            const uint32_t i = k + threadIdx.x, q = q0 + i / 8, d = d0 + i % 8 * 8;
+            Pack<uint16_t, 8> part[3];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const Split s = split(q < a.n_q && d + j < a.dim ? to_f32(queries[q * stride + d + j]) : 0.0f);
+                part[0].e[j] = s.h;
+                part[1].e[j] = s.m;
+                part[2].e[j] = s.l;
+            }
 #pragma unroll
             for (int p = 0; p < P; ++p) {
-                t[p][i / 64][i % 64] = part[p];
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    t[p][i % 8 * 8 + j][i / 8] = part[p].e[j];
+                    part[p].e[j] ^= a.sign < 0 ? 0x8000 : 0;
+                }
                 if (q < a.n_q)
-                    reinterpret_cast<uint16_t*>(const_cast<char*>(a.q.base) + p * a.q.plane + q * (uint64_t)a.q.stride)[d] =
-                        part[p] ^ (a.sign < 0 ? 0x8000 : 0);
+                    store_pack<uint16_t, 8>(reinterpret_cast<uint16_t*>(const_cast<char*>(a.q.base) + p * a.q.plane + q * (uint64_t)a.q.stride) + d, part[p]);
             }
         }
         if (!transposed) return;
         __syncthreads();
-        for (uint32_t i = threadIdx.x; i < 4096; i += 256) {
-            const uint32_t d = d0 + i / 64, q = q0 + i % 64;
+#pragma unroll
+        for (uint32_t k = 0; k < 512; k += 256) {
+            const uint32_t i = k + threadIdx.x, d = d0 + i / 8, q = q0 + i % 8 * 8;
             if (d >= a.dim) continue;
 #pragma unroll
             for (int p = 0; p < P; ++p)
-                reinterpret_cast<uint16_t*>(const_cast<char*>(a.qt.base) + p * a.qt.plane + d * (uint64_t)a.qt.stride)[q] =
-                    t[p][i % 64][i / 64];
+                store_pack<uint16_t, 8>(reinterpret_cast<uint16_t*>(const_cast<char*>(a.qt.base) + p * a.qt.plane + d * (uint64_t)a.qt.stride) + q,
+                                        load_pack<uint16_t, 8>(&t[p][i / 8][i % 8 * 8]));
         }
         return;
     }
@@ -427,8 +449,118 @@ __global__ __launch_bounds__(THREADS, 2) void loss_kernel(XentArgs a) {
     a.part_l[to] = sum;
 }
 
+// Up to four queries: bound by the rows' bytes, so plain f32 products, straight from the table and under the masks
+// themselves, with nothing laid out before. A wave takes the words of the masks in turn, and of each word's candidates U at
+// a time: their loads are in flight together, and the U x NQ sums over the lanes leave each (candidate, query) to a lane
+// of its own, which keeps the running largest and sum of its logits.
+template <typename E, typename Q, int V, int NQ, bool NORMS>
+__global__ __launch_bounds__(256) void loss_few_kernel(XentArgs a, Few f) {
+    constexpr int U = NQ == 1 ? 8 : 4;
+    extern __shared__ __attribute__((aligned(128))) char lds[];
+    __shared__ float sm[4][64], sl[4][64], sums[4];
+    float* const query = reinterpret_cast<float*>(lds);  // [NQ][padded], as they are multiplied
+    const uint32_t lane = threadIdx.x & 63, wave = uniform_u32(threadIdx.x >> 6);
+    const uint32_t chunks = (a.dim + V - 1) / V, padded = chunks * V;
+    const Q* queries = static_cast<const Q*>(f.queries);
+    float factor = 0;  // of the lane's query, base 2
+    const uint32_t mine = lane % NQ;
+    for (int q = 0; q < NQ; ++q) {
+        float sq = 0;
+        for (uint32_t d = threadIdx.x; d < padded; d += 256) {
+            float x = d < a.dim ? to_f32(queries[q * f.query_stride + d]) : 0.0f;
+            if (sizeof(E) == 2) x = __builtin_bit_cast(float, bf16_bits(x) << 16);
+            query[q * padded + d] = x;
+            sq = __builtin_fmaf(x, x, sq);
+        }
+        float scale = f.scale * LOG2E;
+        if constexpr (NORMS) {
+            sq = wave_sum(sq);
+            __syncthreads();
+            if (!lane) sums[wave] = sq;
+            __syncthreads();
+            const float norm = __builtin_sqrtf(sums[0] + sums[1] + sums[2] + sums[3]);
+            scale = norm > 0 ? scale / norm : 0.0f;
+        }
+        if (mine == (uint32_t)q) factor = scale;
+    }
+    __syncthreads();
+    const uint32_t click = f.targets[mine] < f.first_id ? NONE : f.targets[mine] - f.first_id;
+    const E* const table = static_cast<const E*>(f.rows);
+    float m = -__builtin_inff(), l = 0;
+    const uint32_t n_units = (uint32_t)((a.n_rows + 63) / 64) * f.parts, size = 64 / f.parts;
+    for (uint32_t i = blockIdx.x * 4 + wave; i < n_units; i += gridDim.x * 4) {
+        const uint32_t w = i / f.parts, part = i % f.parts;
+        uint64_t bits = uniform_u64(word_at(f.mask, f.present, w, a.n_rows));
+        bits = bits >> (part * size) << (64 - size) >> (64 - size) << (part * size);
+        while (bits) {
+            uint32_t row[U];
+            uint32_t n = 0;
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                // (a place without a candidate repeats the last one's row, and its sum is not looked at)
+                row[u] = bits ? w * 64 + (uint32_t)__builtin_ctzll(bits) : row[u ? u - 1 : 0];
+                n += bits != 0;
+                bits &= bits - 1;
+            }
+            float acc[U][NQ] = {};
+            for (uint32_t c = lane; c < chunks; c += 64) {
+                Pack<E, V> x[U];
+#pragma unroll
+                for (int u = 0; u < U; ++u) x[u] = load_pack<E, V>(table + (uint64_t)row[u] * f.stride + c * V);
+#pragma unroll
+                for (int q = 0; q < NQ; ++q) {
+                    const Pack<float, V> y = load_pack<float, V>(query + q * padded + c * V);
+#pragma unroll
+                    for (int u = 0; u < U; ++u)
+#pragma unroll
+                        for (int v = 0; v < V; ++v) acc[u][q] = __builtin_fmaf(to_f32(x[u].e[v]), y.e[v], acc[u][q]);
+                }
+            }
+            // lane u NQ + q takes candidate u's product with query q
+            float z = 0;
+            uint32_t r = 0;
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+#pragma unroll
+                for (int q = 0; q < NQ; ++q) {
+                    const float sum = wave_sum(acc[u][q]);
+                    if (lane == (uint32_t)(u * NQ + q)) {
+                        z = sum;
+                        r = row[u];
+                    }
+                }
+            if (lane < n * NQ) {
+                z *= factor;
+                if constexpr (NORMS) {
+                    const float x = a.norms[r];
+                    z = x > 0 ? z / x : 0.0f;
+                }
+                if (r == click) {
+                    a.click_z[mine] = z;
+                } else {
+                    const float top = __builtin_fmaxf(m, z), ref = finite_or_zero(top);
+                    l = l * __builtin_amdgcn_exp2f(m - ref) + __builtin_amdgcn_exp2f(z - ref);
+                    m = top;
+                }
+            }
+        }
+    }
+    sm[wave][lane] = m;
+    sl[wave][lane] = l;
+    __syncthreads();
+    if (threadIdx.x >= NQ) return;
+    float top = -__builtin_inff(), sum = 0;
+    for (int w = 0; w < 4; ++w)
+        for (int u = 0; u < U; ++u) top = __builtin_fmaxf(top, sm[w][u * NQ + threadIdx.x]);
+    const float ref = finite_or_zero(top);
+    for (int w = 0; w < 4; ++w)
+        for (int u = 0; u < U; ++u) sum += sl[w][u * NQ + threadIdx.x] * __builtin_amdgcn_exp2f(sm[w][u * NQ + threadIdx.x] - ref);
+    a.part_m[(uint64_t)blockIdx.x * NQ + threadIdx.x] = top;
+    a.part_l[(uint64_t)blockIdx.x * NQ + threadIdx.x] = sum;
+}
+
 // A query's shares joined, in 64 bits (one thread's worth of work per query); a wave per query.
-__global__ __launch_bounds__(256) void join_loss_kernel(XentArgs a, float* loss, float* lse) {
+__global__ __launch_bounds__(256) void join_loss_kernel(XentArgs a, Few f, float* loss, float* lse) {
     const uint32_t q = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
     if (q >= a.n_q) return;
     float top = -__builtin_inff();
@@ -446,7 +578,14 @@ __global__ __launch_bounds__(256) void join_loss_kernel(XentArgs a, float* loss,
     if (lane) return;
     constexpr double LN2 = 0.693147180559945309417;
     const double rest = ref * LN2 + log(sum);  // -inf: no other candidate
-    if (a.click[q] == NONE) {
+    bool clicked;
+    if (a.click) {
+        clicked = a.click[q] != NONE;
+    } else {  // (few queries: whether the click is a candidate stands in the masks)
+        const uint32_t id = f.targets[q], row = id - f.first_id;
+        clicked = id >= f.first_id && row < a.n_rows && word_at(f.mask, f.present, row >> 6, a.n_rows) >> (row & 63) & 1;
+    }
+    if (!clicked) {
         loss[q] = 0.0f;
         lse[q] = (float)rest;
         return;
@@ -799,10 +938,15 @@ __global__ __launch_bounds__(256) void clear_rows_kernel(const uint64_t* mask, c
 constexpr uint64_t PIECE_BYTES = 512u << 20;  // of weights, and of planes, that are held at a time (half of it, a piece that
                                               // the memory-side cache holds, costs more in launches than it saves)
 constexpr uint32_t WORKGROUPS = 256;          // of a product: one per CU (the LDS of a tile fills one)
+constexpr uint32_t FEW_WORKGROUPS = 2048;     // of the loss of a few queries: eight per CU
 
 // hh, hm, mh, mm, hl, lh | plane 0 alone | planes 0 and 1 of A
 constexpr Steps SIX{6, 0u | 0u << 2 | 1u << 4 | 1u << 6 | 0u << 8 | 2u << 10, 0u | 1u << 2 | 0u << 4 | 1u << 6 | 2u << 8 | 0u << 10};
 constexpr Steps ONE{1, 0, 0}, TWO{2, 0u | 1u << 2, 0};
+
+// The matrix cores take sixteen queries at least, and rows through LDS; plain products of four queries or fewer take less
+// time than the rows' bytes do. (Queries of all lanes' columns have to fit LDS.)
+bool few_queries(uint32_t n_q, uint32_t dim) { return n_q <= 4 && n_q * (uint64_t)dim <= 12288; }
 
 struct Plan {
     uint32_t planes, g_planes, kp, gq, loss_bq, bq, bd, q_tiles, loss_q_tiles, d_tiles;
@@ -866,8 +1010,9 @@ Buffers carve(void* workspace, const Plan& p, uint32_t n_q, uint64_t n_rows, uin
     b.click_z = w.take<float>(n_q);
     b.q = w.take<char>((uint64_t)n_q * p.kp * 2 * p.planes);
     b.qt = w.take<char>((uint64_t)dim * p.gq * 2 * p.planes);
-    b.part_m = w.take<float>((uint64_t)p.loss_splits * n_q);
-    b.part_l = w.take<float>((uint64_t)p.loss_splits * n_q);
+    const uint64_t parts = n_q * (uint64_t)(few_queries(n_q, dim) ? FEW_WORKGROUPS : p.loss_splits);
+    b.part_m = w.take<float>(parts);
+    b.part_l = w.take<float>(parts);
     b.g = w.take<char>(p.piece_rows * p.q_tiles * p.bq * 2 * p.g_planes);
     b.spill = w.take<char>(16ull * THREADS * WORKGROUPS);
     b.part_q = w.take<float>((uint64_t)p.grad_splits * n_q * dim);
@@ -916,7 +1061,7 @@ struct Call {
             a.list = b.list;
             a.count = b.count;
             const uint64_t n_words = (x.t.n_rows + 63) / 64;
-            list_candidates_kernel<<<(uint32_t)((n_words + 1023) / 1024), 256, 0, stream>>>(x.mask, x.t.present, x.t.n_rows, b.list, b.count);
+            list_candidates_kernel<<<(uint32_t)((n_words + LIST_WORDS - 1) / LIST_WORDS), 256, 0, stream>>>(x.mask, x.t.present, x.t.n_rows, b.list, b.count);
         }
         a.rows = packed ? Planes{b.packed, p.packed_rows * p.kp * 2, p.kp * 2, nullptr, 0, p.kp / 8}
                         : Planes{(const char*)x.t.rows, 0, (uint32_t)x.t.stride * 2, a.list, 0, dim / 8};
@@ -1035,6 +1180,50 @@ struct Call {
     }
 };
 
+template <typename E, typename Q, int V, int NQ>
+hipError_t run_loss_few(const Xent& x, XentArgs a, const Few& f, float* loss, float* lse, hipStream_t stream) {
+    a.splits = (uint32_t)std::min<uint64_t>(((x.t.n_rows + 63) / 64 * f.parts + 3) / 4, FEW_WORKGROUPS);
+    const uint32_t lds = NQ * (uint32_t)round_up(a.dim, V) * 4;
+    if (a.norms)
+        loss_few_kernel<E, Q, V, NQ, true><<<a.splits, 256, lds, stream>>>(a, f);
+    else
+        loss_few_kernel<E, Q, V, NQ, false><<<a.splits, 256, lds, stream>>>(a, f);
+    join_loss_kernel<<<1, 256, 0, stream>>>(a, f, loss, lse);
+    return hipGetLastError();
+}
+template <typename E, typename Q, int V>
+hipError_t pick_loss_few(const Xent& x, const XentArgs& a, const Few& f, float* loss, float* lse, hipStream_t stream) {
+    switch (x.n_q) {
+        case 1: return run_loss_few<E, Q, V, 1>(x, a, f, loss, lse, stream);
+        case 2: return run_loss_few<E, Q, V, 2>(x, a, f, loss, lse, stream);
+        case 3: return run_loss_few<E, Q, V, 3>(x, a, f, loss, lse, stream);
+        default: return run_loss_few<E, Q, V, 4>(x, a, f, loss, lse, stream);
+    }
+}
+template <typename E, typename Q>
+hipError_t pick_loss_few(const Xent& x, const XentArgs& a, const Few& f, float* loss, float* lse, hipStream_t stream) {
+    constexpr int V = 16 / sizeof(E);
+    // (columns from dim on are read too where a slab has them, times zero: only if they are whole chunks of the row)
+    return aligned_rows<E, V>(x.t.rows, x.t.stride) && x.t.dim % V == 0 ? pick_loss_few<E, Q, V>(x, a, f, loss, lse, stream)
+                                                                        : pick_loss_few<E, Q, 1>(x, a, f, loss, lse, stream);
+}
+hipError_t launch_loss_few(const Xent& x, void* workspace, float* loss, float* lse, hipStream_t stream) {
+    const Buffers b = carve(workspace, plan_for(x.n_q, x.t.n_rows, x.t.dim, x.t.dtype), x.n_q, x.t.n_rows, x.t.dim);
+    XentArgs a{};
+    a.n_rows = x.t.n_rows;
+    a.dim = x.t.dim;
+    a.n_q = x.n_q;
+    a.norms = x.norms;
+    a.part_m = b.part_m;
+    a.part_l = b.part_l;
+    a.click_z = b.click_z;
+    Few f{x.t.rows, x.queries, x.t.stride, x.query_stride, x.targets, x.mask, x.t.present, x.t.first_id, x.scale, 1};
+    // small tables: parts of a word, down to eight rows, until there is one for every wave
+    while (f.parts < 8 && (x.t.n_rows + 63) / 64 * f.parts * 2 <= FEW_WORKGROUPS * 4) f.parts *= 2;
+    if (x.t.dtype == VS_F32) return pick_loss_few<float, float>(x, a, f, loss, lse, stream);
+    return x.queries_f32 ? pick_loss_few<bf16, float>(x, a, f, loss, lse, stream) : pick_loss_few<bf16, bf16>(x, a, f, loss, lse, stream);
+}
+
 void clear_rows(const Xent& x, void* grad_rows, uint64_t stride, bool all, hipStream_t stream) {
     const uint32_t grid = (uint32_t)std::min<uint64_t>((x.t.n_rows + 3) / 4, 1u << 16);
     if (x.t.dtype == VS_F32)
@@ -1050,6 +1239,7 @@ uint64_t xent_workspace_bytes(uint32_t n_q, uint64_t n_rows, uint32_t dim, int32
 }
 
 hipError_t launch_xent(const Xent& x, void* workspace, float* loss, float* lse, hipStream_t stream) {
+    if (few_queries(x.n_q, x.t.dim)) return launch_loss_few(x, workspace, loss, lse, stream);
     Call c(x, workspace, false, stream);
     c.for_pieces(c.packed ? c.p.packed_rows : x.t.n_rows, [&] {
         switch (c.p.loss_bq) {
@@ -1061,7 +1251,7 @@ hipError_t launch_xent(const Xent& x, void* workspace, float* loss, float* lse, 
     });
     c.a.splits = c.p.loss_splits;
     if (c.error != hipSuccess) return c.error;
-    join_loss_kernel<<<(x.n_q + 3) / 4, 256, 0, stream>>>(c.a, loss, lse);
+    join_loss_kernel<<<(x.n_q + 3) / 4, 256, 0, stream>>>(c.a, Few{}, loss, lse);
     return hipGetLastError();
 }
 
