@@ -63,6 +63,90 @@ __device__ __forceinline__ void store_pack(E* p, const Pack<E, V>& x) {
         *reinterpret_cast<Pack<E, V>*>(p) = x;
     }
 }
+// Four and two words at the address of an element of SIZE bytes.
+template <int SIZE>
+struct Words;
+template <>
+struct Words<4> {
+    typedef uint32_t four __attribute__((ext_vector_type(4), aligned(4)));
+    typedef uint32_t two __attribute__((ext_vector_type(2), aligned(4)));
+};
+template <>
+struct Words<2> {
+    typedef uint32_t four __attribute__((ext_vector_type(4), aligned(2)));
+    typedef uint32_t two __attribute__((ext_vector_type(2), aligned(2)));
+};
+
+// V elements from any place that an element may have (the memory path takes vectors at any address; what it costs is
+// a second line where one is crossed); from `limit` elements on, zeros, which are not read.
+template <typename E, int V>
+__device__ __forceinline__ Pack<E, V> load_any(const E* p, uint32_t limit) {
+    constexpr int N = 16 / sizeof(E);  // elements of a vector
+    using four = typename Words<sizeof(E)>::four;
+    Pack<E, V> x = {};
+    if (V % N == 0 && limit >= V) {
+#pragma unroll
+        for (int i = 0; i < V / N; ++i) reinterpret_cast<u32x4*>(&x)[i] = reinterpret_cast<const four*>(p)[i];
+    } else if (V * sizeof(E) == 8 && limit >= V) {
+        using two = typename Words<sizeof(E)>::two;
+        *reinterpret_cast<u32x2*>(&x) = *reinterpret_cast<const two*>(p);
+    } else {
+#pragma unroll
+        for (int v = 0; v < V; ++v)
+            if (v < (int)min(limit, (uint32_t)V)) x.e[v] = p[v];
+    }
+    return x;
+}
+// The same for a store; elements from `limit` on are left as they are.
+template <typename E, int V>
+__device__ __forceinline__ void store_any(E* p, const Pack<E, V>& x, uint32_t limit) {
+    constexpr int N = 16 / sizeof(E);
+    using four = typename Words<sizeof(E)>::four;
+    if (V % N == 0 && limit >= V) {
+#pragma unroll
+        for (int i = 0; i < V / N; ++i) reinterpret_cast<four*>(p)[i] = reinterpret_cast<const u32x4*>(&x)[i];
+    } else if (V * sizeof(E) == 8 && limit >= V) {
+        using two = typename Words<sizeof(E)>::two;
+        *reinterpret_cast<two*>(p) = *reinterpret_cast<const u32x2*>(&x);
+    } else {
+#pragma unroll
+        for (int v = 0; v < V; ++v)
+            if (v < (int)min(limit, (uint32_t)V)) p[v] = x.e[v];
+    }
+}
+
+// The c-th piece of V of a row's `dim` columns. The last one, where dim is no multiple of V, starts earlier and has its
+// first `skip` columns in common with the one before: so it is one load like the others. (A row of less than V columns:
+// one piece, column by column.)
+template <int V>
+struct Piece {
+    uint32_t col, skip;
+    __host__ __device__ __forceinline__ Piece(uint32_t c, uint32_t dim) {
+        const uint32_t first = c * V;
+        skip = first + V > dim && dim >= V ? first + V - dim : 0;
+        col = first - skip;
+    }
+};
+template <typename E, int V>
+__device__ __forceinline__ Pack<E, V> load_piece(const E* row, const Piece<V>& piece, uint32_t dim) {
+    if (dim >= V) return load_any<E, V>(row + piece.col, V);
+    return load_any<E, V>(row, dim);
+}
+// Stores a piece; the columns in common with the one before are left to that one if ONCE (an addition), or else get the
+// same value twice.
+template <typename E, int V>
+__device__ __forceinline__ void store_piece(E* row, const Piece<V>& piece, uint32_t dim, const Pack<E, V>& x, bool once) {
+    if (dim < V) {
+        store_any<E, V>(row, x, dim);
+    } else if (once && piece.skip) {
+#pragma unroll
+        for (int v = 0; v < V; ++v)
+            if (v >= (int)piece.skip) row[piece.col + v] = x.e[v];
+    } else {
+        store_any<E, V>(row + piece.col, x, V);
+    }
+}
+
 // Whether every row of a table starts where a Pack<E, V> may.
 template <typename E, int V>
 inline bool aligned_rows(const void* base, uint64_t stride) {

@@ -44,12 +44,12 @@ __device__ __forceinline__ void bag_range(const Bags& b, uint64_t bag, uint64_t*
     *begin = lo < *end ? lo : *end;
 }
 
-// acc += the weighted rows at positions begin, begin + step, .. < end of V columns from `col`.
+// acc += the weighted rows at positions begin, begin + step, .. < end, of a piece of V columns.
 // Four rows are in flight at a time; a position without a row adds nothing (its load goes to row 0, and what that
 // holds, not even a NaN, gets into the sum).
 template <typename E, int V>
-__device__ __forceinline__ void add_rows(const LookupArgs& a, uint64_t begin, uint64_t end, uint32_t step, uint32_t col,
-                                         float (&acc)[V]) {
+__device__ __forceinline__ void add_rows(const LookupArgs& a, uint64_t begin, uint64_t end, uint32_t step,
+                                         const Piece<V>& piece, float (&acc)[V]) {
     constexpr int U = 4;
     const E* rows = static_cast<const E*>(a.t.rows);
     for (uint64_t i = begin; i < end; i += (uint64_t)U * step) {
@@ -64,7 +64,7 @@ __device__ __forceinline__ void add_rows(const LookupArgs& a, uint64_t begin, ui
             w[u] = in && a.b.weights ? a.b.weights[p] : 1.0f;
         }
 #pragma unroll
-        for (int u = 0; u < U; ++u) x[u] = load_pack<E, V>(rows + (uint64_t)(r[u] == NONE ? 0 : r[u]) * a.t.stride + col);
+        for (int u = 0; u < U; ++u) x[u] = load_piece<E, V>(rows + (uint64_t)(r[u] == NONE ? 0 : r[u]) * a.t.stride, piece, a.t.dim);
 #pragma unroll
         for (int u = 0; u < U; ++u)
 #pragma unroll
@@ -73,16 +73,11 @@ __device__ __forceinline__ void add_rows(const LookupArgs& a, uint64_t begin, ui
 }
 
 template <typename O, int V>
-__device__ __forceinline__ void store_out(const LookupArgs& a, uint64_t bag, uint32_t col, const float (&acc)[V]) {
-    O* out = static_cast<O*>(a.out) + bag * a.out_stride + col;
+__device__ __forceinline__ void store_out(const LookupArgs& a, uint64_t bag, const Piece<V>& piece, const float (&acc)[V]) {
     Pack<O, V> p;
 #pragma unroll
     for (int v = 0; v < V; ++v) p.e[v] = from_f32<O>(acc[v] * a.b.scale);
-    if (col + V <= a.t.dim)
-        store_pack<O, V>(out, p);
-    else
-        for (int v = 0; v < V; ++v)
-            if (col + v < a.t.dim) out[v] = p.e[v];
+    store_piece<O, V>(static_cast<O*>(a.out) + bag * a.out_stride, piece, a.t.dim, p, false);
 }
 
 // One thread per (bag, V columns): a wave reads 64 neighbouring pieces of a row (1 KiB of 16-byte pieces), and no lane
@@ -95,12 +90,12 @@ __global__ __launch_bounds__(256) void lookup_kernel(LookupArgs a) {
         const uint64_t bag0 = base / a.chunks;
         const uint32_t local = (uint32_t)(base - bag0 * a.chunks) + threadIdx.x;
         const uint64_t bag = bag0 + local / a.chunks;
-        const uint32_t col = local % a.chunks * V;
+        const Piece<V> piece(local % a.chunks, a.t.dim);
         uint64_t begin, end;
         bag_range(a.b, bag, &begin, &end);
         float acc[V] = {};
-        add_rows<E, V>(a, begin, end, 1, col, acc);
-        store_out<O, V>(a, bag, col, acc);
+        add_rows<E, V>(a, begin, end, 1, piece, acc);
+        store_out<O, V>(a, bag, piece, acc);
     }
 }
 
@@ -116,7 +111,8 @@ __global__ __launch_bounds__(1024) void lookup_split_kernel(LookupArgs a) {
     uint64_t begin, end;
     bag_range(a.b, bag, &begin, &end);
     float acc[V] = {};
-    if (chunk < a.chunks) add_rows<E, V>(a, begin + wave, end, 16, chunk * V, acc);
+    const Piece<V> piece(min(chunk, a.chunks - 1), a.t.dim);
+    if (chunk < a.chunks) add_rows<E, V>(a, begin + wave, end, 16, piece, acc);
 #pragma unroll
     for (int v = 0; v < V; ++v) part[wave][v][lane] = acc[v];
     __syncthreads();
@@ -127,7 +123,7 @@ __global__ __launch_bounds__(1024) void lookup_split_kernel(LookupArgs a) {
         for (int w = 0; w < 16; ++w) sum += part[w][v][lane];
         acc[v] = sum;
     }
-    store_out<O, V>(a, bag, chunk * V, acc);
+    store_out<O, V>(a, bag, piece, acc);
 }
 
 template <typename E, typename O, int V>
@@ -144,15 +140,6 @@ hipError_t run_lookup(LookupArgs a, hipStream_t stream) {
     return hipGetLastError();
 }
 
-// 16-byte pieces where every row, in and out, starts at a multiple of what is loaded and stored at once.
-template <typename E, typename O>
-hipError_t pick_lookup(const LookupArgs& a, hipStream_t stream) {
-    constexpr int V = 16 / sizeof(E);
-    const bool wide = aligned_rows<E, V>(a.t.rows, a.t.stride) && aligned_rows<O, V>(a.out, a.out_stride) &&
-                      (a.t.dim + V - 1) / V * V <= a.t.dim_read;
-    return wide ? run_lookup<E, O, V>(a, stream) : run_lookup<E, O, 1>(a, stream);
-}
-
 }  // namespace
 
 hipError_t launch_lookup(const Table& t, const Bags& b, void* out, int32_t out_dtype, uint64_t out_stride,
@@ -160,8 +147,8 @@ hipError_t launch_lookup(const Table& t, const Bags& b, void* out, int32_t out_d
     LookupArgs a{t, b, out, out_stride, 0};
     if (!b.n_bags) return hipSuccess;
     if (t.dtype == VS_F32)
-        return out_dtype == VS_F32 ? pick_lookup<float, float>(a, stream) : pick_lookup<float, bf16>(a, stream);
-    return out_dtype == VS_F32 ? pick_lookup<bf16, float>(a, stream) : pick_lookup<bf16, bf16>(a, stream);
+        return out_dtype == VS_F32 ? run_lookup<float, float, 4>(a, stream) : run_lookup<float, bf16, 4>(a, stream);
+    return out_dtype == VS_F32 ? run_lookup<bf16, float, 8>(a, stream) : run_lookup<bf16, bf16, 8>(a, stream);
 }
 
 // ---- gradients -----------------------------------------------------------------------------
@@ -191,7 +178,6 @@ struct GradArgs {
     uint32_t* heads;   // first entries of runs, counted per TILE of sorted entries
     uint32_t* handed;  // [n_runs] number of the run that each piece hands over at its end
     float* partial;    // [n_runs][2][chunks * V]
-    bool wide;         // rows of the result take V elements at a time
     RowGrads out;
 };
 
@@ -362,26 +348,16 @@ __device__ uint32_t heads_before(const GradArgs& a, const uint32_t* keys, uint32
 }
 
 template <typename O, int V>
-__device__ __forceinline__ void store_row(const GradArgs& a, uint32_t row, uint32_t compact, uint32_t col, const float (&acc)[V]) {
-    O* out = static_cast<O*>(a.out.rows) + (uint64_t)(a.out.unique ? compact : row) * a.out.stride + col;
+__device__ __forceinline__ void store_row(const GradArgs& a, uint32_t row, uint32_t compact, const Piece<V>& piece, const float (&acc)[V]) {
+    O* out = static_cast<O*>(a.out.rows) + (uint64_t)(a.out.unique ? compact : row) * a.out.stride;
     Pack<O, V> p;
-    if (!a.out.unique) {  // a row belongs to one thread: a plain addition
-        if (a.wide)
-            p = load_pack<O, V>(out);
-        else
-#pragma unroll
-            for (int v = 0; v < V; ++v) p.e[v] = out[v];
-    }
+    if (!a.out.unique) p = load_piece<O, V>(out, piece, a.dim);  // a column of a row belongs to one thread: a plain addition
 #pragma unroll
     for (int v = 0; v < V; ++v) {
         const float x = acc[v] * a.b.scale;
         p.e[v] = from_f32<O>(a.out.unique ? x : x + to_f32(p.e[v]));
     }
-    if (a.wide)
-        store_pack<O, V>(out, p);
-    else
-#pragma unroll
-        for (int v = 0; v < V; ++v) out[v] = p.e[v];
+    store_piece<O, V>(out, piece, a.dim, p, !a.out.unique);
 }
 
 // Up to SMALL ids: a workgroup per (sorted entry, 64 pieces). The ones at a run's head sum the run, a quarter in each
@@ -408,10 +384,10 @@ __global__ __launch_bounds__(256) void sum_small_kernel(GradArgs a) {
     if (a.out.unique && !blockIdx.y && !threadIdx.x) a.out.unique[compact] = row;
     float acc[V] = {};
     if (chunk < a.chunks) {
-        const E* g = static_cast<const E*>(a.grad_out) + chunk * V;
+        const E* g = static_cast<const E*>(a.grad_out);
 #pragma unroll 4
         for (uint32_t j = i + wave; j < end; j += 4) {
-            const Pack<E, V> x = load_pack<E, V>(g + (uint64_t)bags[j] * a.grad_stride);
+            const Pack<E, V> x = load_piece<E, V>(g + (uint64_t)bags[j] * a.grad_stride, Piece<V>(chunk, a.dim), a.dim);
 #pragma unroll
             for (int v = 0; v < V; ++v) acc[v] = __builtin_fmaf(weights[j], to_f32(x.e[v]), acc[v]);
         }
@@ -422,7 +398,7 @@ __global__ __launch_bounds__(256) void sum_small_kernel(GradArgs a) {
     if (wave || chunk >= a.chunks) return;
 #pragma unroll
     for (int v = 0; v < V; ++v) acc[v] = part[0][v][lane] + part[1][v][lane] + part[2][v][lane] + part[3][v][lane];
-    store_row<O, V>(a, row, compact, chunk * V, acc);
+    store_row<O, V>(a, row, compact, Piece<V>(chunk, a.dim), acc);
 }
 
 // Many ids: one thread per (RUN sorted entries, V columns) walks its entries in order, eight gradients in flight. A
@@ -438,7 +414,7 @@ __global__ __launch_bounds__(256) void sum_runs_kernel(GradArgs a, int side) {
     const uint64_t first = (uint64_t)blockIdx.x * 256;
     const uint32_t run0 = (uint32_t)(first / a.chunks);
     const uint32_t local = (uint32_t)(first - (uint64_t)run0 * a.chunks) + threadIdx.x;
-    const uint32_t run = run0 + local / a.chunks, chunk = local % a.chunks, col = chunk * V;
+    const uint32_t run = run0 + local / a.chunks, chunk = local % a.chunks;
     uint32_t compact = 0;  // of the next head
     if (a.out.unique) {
         const uint32_t before = heads_before(a, keys, min(run0 * RUN, a.n), wave_sum);
@@ -457,7 +433,8 @@ __global__ __launch_bounds__(256) void sum_runs_kernel(GradArgs a, int side) {
     }
     if (run >= a.n_runs) return;
     const uint32_t begin = run * RUN, end = min(begin + RUN, a.n);
-    const E* g = static_cast<const E*>(a.grad_out) + col;
+    const E* g = static_cast<const E*>(a.grad_out);
+    const Piece<V> piece(chunk, a.dim);
     float* partial = a.partial + ((uint64_t)run * 2 * a.chunks + chunk) * V;
     uint32_t row = keys[begin];
     bool open = begin && keys[begin - 1] == row;  // the run began before
@@ -469,7 +446,7 @@ __global__ __launch_bounds__(256) void sum_runs_kernel(GradArgs a, int side) {
 #pragma unroll
             for (int v = 0; v < V; ++v) to[v] = acc[v];
         } else {
-            store_row<O, V>(a, row, compact, col, acc);
+            store_row<O, V>(a, row, compact, piece, acc);
         }
         compact += !open;
         open = false;
@@ -483,7 +460,7 @@ __global__ __launch_bounds__(256) void sum_runs_kernel(GradArgs a, int side) {
             const uint32_t j = min(i + u, end - 1);
             key[u] = keys[j];
             w[u] = weights[j];
-            x[u] = load_pack<E, V>(g + (uint64_t)bags[j] * a.grad_stride);
+            x[u] = load_piece<E, V>(g + (uint64_t)bags[j] * a.grad_stride, piece, a.dim);
         }
 #pragma unroll
         for (int u = 0; u < U; ++u) {
@@ -545,7 +522,7 @@ __global__ __launch_bounds__(256) void join_runs_kernel(GradArgs a, int side) {
     if (wave || chunk >= a.chunks) return;
 #pragma unroll
     for (int v = 0; v < V; ++v) acc[v] = part[0][v][lane] + part[1][v][lane] + part[2][v][lane] + part[3][v][lane];
-    store_row<O, V>(a, row, compact, chunk * V, acc);
+    store_row<O, V>(a, row, compact, Piece<V>(chunk, a.dim), acc);
 }
 
 // A wave takes `span` neighbouring positions (64 at most: a lane looks up the row and the bag of each), four at a time:
@@ -583,17 +560,21 @@ __global__ __launch_bounds__(256) void weight_grads_kernel(WeightArgs a) {
             g[u] = (uint32_t)__builtin_amdgcn_readlane((int)bag, (int)min(i + u, 63u));
         }
         for (uint32_t c = lane; c < a.chunks; c += 64) {
+            const Piece<V> piece(c, a.t.dim);
             Pack<E, V> x[U];
             Pack<G, V> y[U];
 #pragma unroll
             for (int u = 0; u < U; ++u) {  // (a position without a row reads row 0 and bag 0, and is not used)
-                x[u] = load_pack<E, V>(rows + (uint64_t)(r[u] == NONE ? 0 : r[u]) * a.t.stride + c * V);
-                y[u] = load_pack<G, V>(grads + (uint64_t)(r[u] == NONE ? 0 : g[u]) * a.grad_stride + c * V);
+                x[u] = load_piece<E, V>(rows + (uint64_t)(r[u] == NONE ? 0 : r[u]) * a.t.stride, piece, a.t.dim);
+                y[u] = load_piece<G, V>(grads + (uint64_t)(r[u] == NONE ? 0 : g[u]) * a.grad_stride, piece, a.t.dim);
             }
 #pragma unroll
             for (int u = 0; u < U; ++u)
 #pragma unroll
-                for (int v = 0; v < V; ++v) sum[u] = __builtin_fmaf(to_f32(x[u].e[v]), to_f32(y[u].e[v]), sum[u]);
+                for (int v = 0; v < V; ++v) {
+                    const float s = __builtin_fmaf(to_f32(x[u].e[v]), to_f32(y[u].e[v]), sum[u]);
+                    sum[u] = v >= (int)piece.skip ? s : sum[u];
+                }
         }
 #pragma unroll
         for (int u = 0; u < U; ++u) {
@@ -606,8 +587,7 @@ __global__ __launch_bounds__(256) void weight_grads_kernel(WeightArgs a) {
 
 template <typename E, typename O, int V>
 hipError_t run_lookup_grad(GradArgs a, hipStream_t stream) {
-    a.chunks = a.dim / V;
-    a.wide = aligned_rows<O, V>(a.out.rows, a.out.stride);
+    a.chunks = (a.dim + V - 1) / V;
     const uint32_t col_blocks = (a.chunks + 63) / 64;
     if (a.n <= SMALL) {
         a.heads = nullptr;
@@ -671,8 +651,7 @@ hipError_t launch_lookup_grad(const void* grad_out, int32_t dtype, uint64_t grad
         using E = decltype(e);
         using O = decltype(o);
         constexpr int V = 16 / sizeof(E);
-        return aligned_rows<E, V>(grad_out, grad_stride) && dim % V == 0 ? run_lookup_grad<E, O, V>(a, stream)
-                                                                         : run_lookup_grad<E, O, 1>(a, stream);
+        return run_lookup_grad<E, O, V>(a, stream);
     };
     if (dtype == VS_F32) return out.dtype == VS_F32 ? pick(float{}, float{}) : pick(float{}, bf16{});
     return out.dtype == VS_F32 ? pick(bf16{}, float{}) : pick(bf16{}, bf16{});
@@ -693,13 +672,8 @@ hipError_t launch_lookup_grad_weights(const Table& t, const Bags& b, const void*
         using E = decltype(e);
         using G = decltype(g);
         constexpr int V = 16 / sizeof(E);
-        if (aligned_rows<E, V>(t.rows, t.stride) && aligned_rows<G, V>(grad_out, grad_stride) && t.dim % V == 0) {
-            a.chunks = t.dim / V;
-            weight_grads_kernel<E, G, V><<<grid, 256, 0, stream>>>(a);
-        } else {
-            a.chunks = t.dim;
-            weight_grads_kernel<E, G, 1><<<grid, 256, 0, stream>>>(a);
-        }
+        a.chunks = (t.dim + V - 1) / V;
+        weight_grads_kernel<E, G, V><<<grid, 256, 0, stream>>>(a);
         return hipGetLastError();
     };
     if (t.dtype == VS_F32) return grad_dtype == VS_F32 ? pick(float{}, float{}) : pick(float{}, bf16{});

@@ -202,25 +202,21 @@ __global__ __launch_bounds__(256) void pack_queries_kernel(XentArgs a, const Q* 
 }
 
 // A piece of the candidates as planes: eight elements a thread, zeros from `dim` on.
-template <typename E, int P, bool WIDE>
+template <typename E, int P>
 __global__ __launch_bounds__(256) void pack_rows_kernel(XentArgs a, const E* table, uint64_t stride, char* out) {
     const uint32_t end = min(candidates(a), a.piece_begin + a.piece_rows);
     const uint64_t total = end > a.piece_begin ? (uint64_t)(end - a.piece_begin) * a.rows.chunks : 0;
     for (uint64_t i = (uint64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (uint64_t)gridDim.x * 256) {
         const uint32_t r = (uint32_t)(i / a.rows.chunks), d = (uint32_t)(i - (uint64_t)r * a.rows.chunks) * 8;
         const E* from = table + row_at(a, a.piece_begin + r) * stride + d;
+        constexpr int V = 16 / sizeof(E);
         float x[8];
-        if (WIDE && d + 8 <= a.dim) {
-            constexpr int V = 16 / sizeof(E);
 #pragma unroll
-            for (int h = 0; h < 8 / V; ++h) {
-                const Pack<E, V> v = load_pack<E, V>(from + h * V);
+        for (int h = 0; h < 8 / V; ++h) {
+            const uint32_t at = d + h * V;
+            const Pack<E, V> v = load_any<E, V>(from + h * V, at < a.dim ? a.dim - at : 0);
 #pragma unroll
-                for (int j = 0; j < V; ++j) x[h * V + j] = to_f32(v.e[j]);
-            }
-        } else {
-#pragma unroll
-            for (int j = 0; j < 8; ++j) x[j] = d + j < a.dim ? to_f32(from[j]) : 0.0f;
+            for (int j = 0; j < V; ++j) x[h * V + j] = to_f32(v.e[j]);
         }
         Pack<uint16_t, 8> plane[3];
 #pragma unroll
@@ -247,6 +243,7 @@ struct Scores {
     static constexpr int WAVES_R = 8 / WAVES_Q;
     static constexpr int WQ = BQ / WAVES_Q / 16, WR = TILE / WAVES_R / 16;  // fragments of a wave
     static constexpr int TM = LANES_ARE_QUERIES ? WR : WQ, TN = LANES_ARE_QUERIES ? WQ : WR;
+    static constexpr int T = TILE, Q_TILE = BQ;
     using R = Rows<TILE, LISTED>;
     using Q = Rows<BQ>;
     static constexpr int LDS = 2 * (R::BYTES + Q::BYTES);
@@ -335,16 +332,88 @@ struct Scores {
     }
 };
 
+// f32 tables with up to 128 queries: tiles of 64 queries by 128 candidates, all planes a step.
+template <bool LANES_ARE_QUERIES>
+struct SplitScores {
+    static constexpr int T = 128, Q_TILE = 64;
+    static constexpr int WAVES_Q = 2, WAVES_R = 4, WQ = 2, WR = 2, TM = 2, TN = 2;
+    using R = Rows<T>;
+    using Q = Rows<Q_TILE>;
+    static constexpr int LDS = 2 * 3 * (R::BYTES + Q::BYTES);
+
+    __device__ __forceinline__ static uint32_t wave_q() { return uniform_u32(threadIdx.x >> 6) % WAVES_Q; }
+    __device__ __forceinline__ static uint32_t wave_r() { return uniform_u32(threadIdx.x >> 6) / WAVES_Q; }
+
+    // As in Scores.
+    template <int STORES, typename F>
+    __device__ __forceinline__ static void run(const XentArgs& a, uint32_t end, uint32_t q0, uint32_t along, char* lds, F&& done) {
+        Planes rows = a.rows;
+        rows.rows = end - a.place0;
+        R r;
+        Q q;
+        r.init();
+        q.init();
+        q.aim(q0);
+        const uint32_t tiles = (end - a.piece_begin + T - 1) / T;
+        if (along >= tiles) return;
+        const uint32_t steps = (a.rows.chunks + 7) / 8, base = a.piece_begin - a.place0;
+        auto half_r = [&](uint32_t i) { return lds + i * 3 * (R::BYTES + Q::BYTES); };
+        auto half_q = [&](uint32_t i) { return lds + i * 3 * (R::BYTES + Q::BYTES) + 3 * R::BYTES; };
+        Cursor next{0, 0, along};  // of both operands' loads
+        r.aim(base + along * T);
+        auto load = [&](uint32_t to) {
+            if (next.tile >= tiles) return;
+#pragma unroll
+            for (int p = 0; p < 3; ++p) {
+#pragma unroll
+                for (int i = 0; i < R::LOADS; ++i) r.load(i, rows, next.k, p, a.zeros, half_r(to) + p * R::BYTES);
+                q.load(0, a.q, next.k, p, a.zeros, half_q(to) + p * Q::BYTES);
+            }
+            if (next.advance(1, steps, a.splits)) r.aim(base + next.tile * T);
+        };
+        load(0);
+        step_barrier();
+        using E = SplitEngine<std::conditional_t<LANES_ARE_QUERIES, R, Q>, std::conditional_t<LANES_ARE_QUERIES, Q, R>, TM, TN>;
+        E e;
+        e.m0 = LANES_ARE_QUERIES ? wave_r() * WR : wave_q() * WQ;
+        e.n0 = LANES_ARE_QUERIES ? wave_q() * WQ : wave_r() * WR;
+        e.ask(LANES_ARE_QUERIES ? half_r(0) : half_q(0), LANES_ARE_QUERIES ? half_q(0) : half_r(0), 0);
+        load(1);
+        uint32_t at = 0, stored = 0;
+#pragma nounroll
+        for (uint32_t tile = along; tile < tiles; tile += a.splits) {
+            f32x4 acc[TM][TN] = {}, small[TM][TN] = {};
+#pragma nounroll
+            for (uint32_t s = 0; s < steps; ++s) {
+                const uint32_t other = at ^ 1;
+                char *ar = half_r(at), *aq = half_q(at), *br = half_r(other), *bq = half_q(other);
+                // (the step after next goes into this one's half, behind the barrier: ahead of any stores of the tile's end)
+                e.template step<STORES>(LANES_ARE_QUERIES ? ar : aq, LANES_ARE_QUERIES ? aq : ar, LANES_ARE_QUERIES ? br : bq,
+                                        LANES_ARE_QUERIES ? bq : br, acc, small, stored, [&](int kk) {
+                    if (kk) load(at);
+                });
+                stored = afresh_uniform(0);
+                at = other;
+            }
+#pragma unroll
+            for (int m = 0; m < TM; ++m)
+#pragma unroll
+                for (int n = 0; n < TN; ++n) acc[m][n] += small[m][n];
+            stored = afresh_uniform(done(acc, a.piece_begin + tile * T));
+        }
+    }
+};
+
 __device__ __forceinline__ float finite_or_zero(float m) { return m == -__builtin_inff() ? 0.0f : m; }
 
 // Per query the largest logit of a share of the candidates and the sum of the exponentials over it, the clicked row kept
 // out. Everything is in base 2 (logits times log2 e): an exponential is one instruction. A lane keeps the running largest
 // and sum of its own candidates, in registers, for each of its queries; lanes, waves and shares are joined at the end.
-template <int BQ, bool NORMS, bool LISTED>
+template <typename S, bool NORMS>
 __global__ __launch_bounds__(THREADS, 2) void loss_kernel(XentArgs a) {
-    using S = Scores<BQ, true, LISTED>;
+    constexpr int BQ = S::Q_TILE;
     extern __shared__ __attribute__((aligned(128))) char lds[];
-    __shared__ float inverse[TILE], sm[S::WAVES_R][BQ], sl[S::WAVES_R][BQ];
+    __shared__ float inverse[S::T], sm[S::WAVES_R][BQ], sl[S::WAVES_R][BQ];
     const uint32_t lane = threadIdx.x & 63, group = lane >> 4;
     uint32_t tile_q, along;
     place_of_workgroup(a.across, a.splits, &tile_q, &along);
@@ -363,7 +432,7 @@ __global__ __launch_bounds__(THREADS, 2) void loss_kernel(XentArgs a) {
     if (end > a.piece_begin)
         S::template run<0>(a, end, tile_q * BQ, along, lds, [&](f32x4 (&acc)[S::TM][S::TN], uint32_t first) {
             if constexpr (NORMS) {
-                if (threadIdx.x < TILE) {
+                if (threadIdx.x < S::T) {
                     const float x = first + threadIdx.x < end ? a.norms[row_at(a, first + threadIdx.x)] : 0.0f;
                     inverse[threadIdx.x] = x > 0 ? 1.0f / x : 0.0f;
                 }
@@ -379,15 +448,15 @@ __global__ __launch_bounds__(THREADS, 2) void loss_kernel(XentArgs a) {
                 }
                 __syncthreads();  // (the next tile writes them)
             }
-            bool special = end - first < TILE;
+            bool special = end - first < S::T;
 #pragma unroll
-            for (int n = 0; n < S::TN; ++n) special |= click[n] - first < TILE;
+            for (int n = 0; n < S::TN; ++n) special |= click[n] - first < S::T;
             if (__any(special)) {
                 // a tile with a clicked row, or the last one: what does not belong to the sum is taken out of it
 #pragma unroll
                 for (int n = 0; n < S::TN; ++n) {
                     const uint32_t at = click[n] - first - local;
-                    const int left = (int)min(end - first, (uint32_t)TILE) - (int)local;
+                    const int left = (int)min(end - first, (uint32_t)S::T) - (int)local;
                     float clicked = 0;
 #pragma unroll
                     for (int t = 0; t < S::TM; ++t)
@@ -460,14 +529,16 @@ __global__ __launch_bounds__(256) void loss_few_kernel(XentArgs a, Few f) {
     __shared__ float sm[4][64], sl[4][64], sums[4];
     float* const query = reinterpret_cast<float*>(lds);  // [NQ][padded], as they are multiplied
     const uint32_t lane = threadIdx.x & 63, wave = uniform_u32(threadIdx.x >> 6);
-    const uint32_t chunks = (a.dim + V - 1) / V, padded = chunks * V;
+    const uint32_t chunks = (a.dim + V - 1) / V, padded = chunks * V;  // (a last, broken piece: see Piece)
     const Q* queries = static_cast<const Q*>(f.queries);
     float factor = 0;  // of the lane's query, base 2
     const uint32_t mine = lane % NQ;
     for (int q = 0; q < NQ; ++q) {
         float sq = 0;
         for (uint32_t d = threadIdx.x; d < padded; d += 256) {
-            float x = d < a.dim ? to_f32(queries[q * f.query_stride + d]) : 0.0f;
+            const Piece<V> piece(d / V, a.dim);
+            const uint32_t from = piece.col + d % V;
+            float x = d % V >= piece.skip && from < a.dim ? to_f32(queries[q * f.query_stride + from]) : 0.0f;
             if (sizeof(E) == 2) x = __builtin_bit_cast(float, bf16_bits(x) << 16);
             query[q * padded + d] = x;
             sq = __builtin_fmaf(x, x, sq);
@@ -506,7 +577,7 @@ __global__ __launch_bounds__(256) void loss_few_kernel(XentArgs a, Few f) {
             for (uint32_t c = lane; c < chunks; c += 64) {
                 Pack<E, V> x[U];
 #pragma unroll
-                for (int u = 0; u < U; ++u) x[u] = load_pack<E, V>(table + (uint64_t)row[u] * f.stride + c * V);
+                for (int u = 0; u < U; ++u) x[u] = load_piece<E, V>(table + (uint64_t)row[u] * f.stride, Piece<V>(c, a.dim), a.dim);
 #pragma unroll
                 for (int q = 0; q < NQ; ++q) {
                     const Pack<float, V> y = load_pack<float, V>(query + q * padded + c * V);
@@ -559,23 +630,30 @@ __global__ __launch_bounds__(256) void loss_few_kernel(XentArgs a, Few f) {
     a.part_l[(uint64_t)blockIdx.x * NQ + threadIdx.x] = sum;
 }
 
-// A query's shares joined, in 64 bits (one thread's worth of work per query); a wave per query.
+// A query's shares joined, in 64 bits (one thread's worth of work per query); a workgroup per query.
 __global__ __launch_bounds__(256) void join_loss_kernel(XentArgs a, Few f, float* loss, float* lse) {
-    const uint32_t q = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
-    if (q >= a.n_q) return;
+    __shared__ float tops[4];
+    __shared__ double sums[4];
+    const uint32_t q = blockIdx.x, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     float top = -__builtin_inff();
-    for (uint32_t s = lane; s < a.splits; s += 64) top = __builtin_fmaxf(top, a.part_m[(uint64_t)s * a.n_q + q]);
+    for (uint32_t s = threadIdx.x; s < a.splits; s += 256) top = __builtin_fmaxf(top, a.part_m[(uint64_t)s * a.n_q + q]);
 #pragma unroll
     for (int d = 32; d; d /= 2) top = __builtin_fmaxf(top, __shfl_xor(top, d));
+    if (!lane) tops[wave] = top;
+    __syncthreads();
+    top = __builtin_fmaxf(__builtin_fmaxf(tops[0], tops[1]), __builtin_fmaxf(tops[2], tops[3]));
     const float ref = finite_or_zero(top);
     double sum = 0;
-    for (uint32_t s = lane; s < a.splits; s += 64) {
+    for (uint32_t s = threadIdx.x; s < a.splits; s += 256) {
         const uint64_t at = (uint64_t)s * a.n_q + q;
         sum += (double)a.part_l[at] * (double)__builtin_amdgcn_exp2f(a.part_m[at] - ref);
     }
 #pragma unroll
     for (int d = 32; d; d /= 2) sum += __shfl_xor(sum, d);
-    if (lane) return;
+    if (!lane) sums[wave] = sum;
+    __syncthreads();
+    if (threadIdx.x) return;
+    sum = (sums[0] + sums[1]) + (sums[2] + sums[3]);
     constexpr double LN2 = 0.693147180559945309417;
     const double rest = ref * LN2 + log(sum);  // -inf: no other candidate
     bool clicked;
@@ -599,9 +677,12 @@ __global__ __launch_bounds__(256) void join_loss_kernel(XentArgs a, Few f, float
 
 // The weights G of a piece, [candidate][query], rounded to bf16 (PG = 1), or kept to 16 bits (2) or all 24 (3) by as many
 // planes. A lane holds four neighbouring queries of a candidate: eight bytes a store.
-template <int BQ, bool NORMS, bool LISTED, int PG>
+template <typename S>  // fragments that go through LDS at a time: up to 64 queries of 16 candidates
+using weights_turn = Turn<8, (S::TM < 4 ? S::TM : 4)>;
+
+template <typename S, bool NORMS, int PG>
 __global__ __launch_bounds__(THREADS, 2) void weights_kernel(XentArgs a) {
-    using S = Scores<BQ, false, LISTED>;
+    constexpr int BQ = S::Q_TILE;
     extern __shared__ __attribute__((aligned(128))) char lds[];
     __shared__ __attribute__((aligned(16))) float s2[BQ], lse2[BQ], factor[BQ], at_click[BQ];
     __shared__ __attribute__((aligned(16))) uint32_t click[BQ];
@@ -623,8 +704,8 @@ __global__ __launch_bounds__(THREADS, 2) void weights_kernel(XentArgs a) {
     // (the first barrier of the loop below orders these before they are read)
     // Every lane stores every time (so that the number of stores is known to the next step's barrier): rows of G are whole
     // tiles of queries, and G is whole tiles of candidates.
-    constexpr int UNIT = S::TM < 4 ? S::TM : 4;  // fragments that go through LDS at a time: 64 queries of 16 candidates
-    using T = Turn<8, UNIT>;
+    constexpr int UNIT = S::TM < 4 ? S::TM : 4;
+    using T = weights_turn<S>;
     char* const wave_lds = lds + S::LDS + uniform_u32(threadIdx.x >> 6) * T::BYTES;
     S::template run<S::TN * (S::TM / UNIT) * T::STORES * PG>(a, end, q0, along, lds, [&](f32x4 (&acc)[S::TM][S::TN], uint32_t first) {
         const uint32_t l = afresh(threadIdx.x) & 63, row0 = S::wave_r() * S::WR * 16, i0 = S::wave_q() * S::WQ * 16 + (l >> 4) * 4;
@@ -681,9 +762,9 @@ __global__ __launch_bounds__(THREADS, 2) void weights_kernel(XentArgs a) {
 }
 
 // drows of a piece: transposed queries (BD columns of the rows) by G. A lane holds four neighbouring columns of a row.
-// WIDE: rows take 16 bytes at a time; as in weights_kernel every lane stores every time, to its own 16 bytes of a.spill
-// where it has no row or column.
-template <int BD, typename E, bool WIDE>
+// As in weights_kernel every lane stores every time, to its own 16 bytes of a.spill where it has no row or no whole
+// 16 bytes of columns; the columns of a last, broken 16 bytes are stored one by one besides.
+template <int BD, typename E>
 __global__ __launch_bounds__(THREADS, 2) void row_grads_kernel(XentArgs a) {
     using A = Rows<BD>;
     using B = Rows<TILE>;
@@ -736,7 +817,7 @@ __global__ __launch_bounds__(THREADS, 2) void row_grads_kernel(XentArgs a) {
 #pragma nounroll
         for (uint32_t s = 0; s < steps; ++s) {
             const uint32_t other = at ^ 1;
-            e.template step<WIDE ? TN * (TM / UNIT) * T::STORES : 0>(half_q(at), half_g(at), half_q(other), half_g(other), acc, stored, [&](int phase) {
+            e.template step<TN * (TM / UNIT) * T::STORES>(half_q(at), half_g(at), half_q(other), half_g(other), acc, stored, [&](int phase) {
                 if (phase < En::PHASES - 1) {
                     constexpr int EACH = (A::LOADS + En::PHASES - 2) / (En::PHASES - 1);
                     if (early || cq.tile >= tiles) return;
@@ -746,7 +827,7 @@ __global__ __launch_bounds__(THREADS, 2) void row_grads_kernel(XentArgs a) {
                 }
                 load_weights(at);
                 if (!early && cq.tile < tiles) cq.advance(planes, blocks, a.splits);
-                early = afresh_uniform(WIDE && s + 1 == steps && cq.tile < tiles);
+                early = afresh_uniform(s + 1 == steps && cq.tile < tiles);
                 if (!early) return;
 #pragma unroll
                 for (int i = 0; i < A::LOADS; ++i) load_queries(i, at);
@@ -756,41 +837,35 @@ __global__ __launch_bounds__(THREADS, 2) void row_grads_kernel(XentArgs a) {
             at = other;
         }
         const uint32_t l = afresh(threadIdx.x) & 63, d0 = tile_d * BD + wd * TM * 16, place0 = a.piece_begin + tile * TILE + wr * TN * 16;
-        if constexpr (WIDE) {
-            char* const spill = a.spill + (blockIdx.x * THREADS + threadIdx.x) * 16ull;
+        constexpr uint32_t V = 16 / sizeof(E);
+        char* const spill = a.spill + (blockIdx.x * THREADS + threadIdx.x) * 16ull;
+        const bool broken = a.dim % V;
 #pragma unroll
-            for (int n = 0; n < TN; ++n)
+        for (int n = 0; n < TN; ++n)
 #pragma unroll
-                for (int u = 0; u < TM / UNIT; ++u) {
+            for (int u = 0; u < TM / UNIT; ++u) {
 #pragma unroll
-                    for (int t = 0; t < UNIT; ++t) {
-                        Pack<E, 4> p;
+                for (int t = 0; t < UNIT; ++t) {
+                    Pack<E, 4> p;
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) p.e[i] = from_f32<E>(acc[u * UNIT + t][n][i]);
-                        T::put(wave_lds, l, t, p);
-                    }
-#pragma unroll
-                    for (int j = 0; j < T::STORES; ++j) {
-                        const uint32_t place = place0 + n * 16 + T::row(l, j), d = d0 + u * UNIT * 16 + T::chunk(l) * (16 / sizeof(E));
-                        E* out = static_cast<E*>(a.grad_rows) + row_at(a, min(place, end - 1)) * a.grad_row_stride + d;
-                        *reinterpret_cast<u32x4*>(place < end && d < a.dim ? (char*)out : spill) = T::get(wave_lds, l, j);
-                    }
-                    __builtin_amdgcn_sched_barrier(0);
+                    for (int i = 0; i < 4; ++i) p.e[i] = from_f32<E>(acc[u * UNIT + t][n][i]);
+                    T::put(wave_lds, l, t, p);
                 }
-        } else {
 #pragma unroll
-            for (int n = 0; n < TN; ++n) {
-                const uint32_t place = place0 + n * 16 + (l & 15);
-                E* out = static_cast<E*>(a.grad_rows) + row_at(a, min(place, end - 1)) * a.grad_row_stride;
+                for (int j = 0; j < T::STORES; ++j) {
+                    const uint32_t place = place0 + n * 16 + T::row(l, j), d = d0 + u * UNIT * 16 + T::chunk(l) * V;
+                    E* const out = static_cast<E*>(a.grad_rows) + row_at(a, min(place, end - 1)) * a.grad_row_stride + d;
+                    const u32x4 x = T::get(wave_lds, l, j);
+                    *reinterpret_cast<typename Words<sizeof(E)>::four*>(place < end && d + V <= a.dim ? (char*)out : spill) = x;
+                    if (broken && place < end && d < a.dim && d + V > a.dim) {
+                        const Pack<E, V> e = __builtin_bit_cast(Pack<E, V>, x);
 #pragma unroll
-                for (int m = 0; m < TM; ++m)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const uint32_t d = d0 + m * 16 + (l >> 4) * 4 + i;
-                        if (place < end && d < a.dim) out[d] = from_f32<E>(acc[m][n][i]);
+                        for (uint32_t i = 0; i < V - 1; ++i)
+                            if (d + i < a.dim) out[i] = e.e[i];
                     }
+                }
+                __builtin_amdgcn_sched_barrier(0);
             }
-        }
         stored = afresh_uniform(early);
     }
 }
@@ -949,7 +1024,7 @@ constexpr Steps ONE{1, 0, 0}, TWO{2, 0u | 1u << 2, 0};
 bool few_queries(uint32_t n_q, uint32_t dim) { return n_q <= 4 && n_q * (uint64_t)dim <= 12288; }
 
 struct Plan {
-    uint32_t planes, g_planes, kp, gq, loss_bq, bq, bd, q_tiles, loss_q_tiles, d_tiles;
+    uint32_t planes, g_planes, kp, gq, loss_bq, score_bq, bq, bd, q_tiles, loss_q_tiles, score_q_tiles, d_tiles;
     uint32_t loss_splits, weight_splits, row_splits, grad_splits;
     uint64_t piece_rows, packed_rows;
 };
@@ -971,10 +1046,12 @@ Plan plan_for(uint32_t n_q, uint64_t n_rows, uint32_t dim, int32_t dtype) {
     p.g_planes = dtype == VS_F32 ? 3 : n_q <= 64 ? 2 : 1;
     p.kp = (uint32_t)round_up(dim, 64);
     p.gq = (uint32_t)round_up(n_q, 64);
-    p.loss_bq = n_q <= 16 ? 16 : n_q <= 64 ? 64 : n_q <= 128 ? 128 : 256;
     p.bq = n_q <= 64 ? 64 : n_q <= 128 ? 128 : 256;
+    p.score_bq = dtype == VS_F32 && n_q <= 128 ? 64 : p.bq;
+    p.loss_bq = dtype == VS_F32 || n_q > 16 ? p.score_bq : 16;
     p.bd = (dim + 127) / 128 % 2 ? 128 : 256;
     p.loss_q_tiles = (n_q + p.loss_bq - 1) / p.loss_bq;
+    p.score_q_tiles = (n_q + p.score_bq - 1) / p.score_bq;
     p.q_tiles = (n_q + p.bq - 1) / p.bq;
     p.d_tiles = (dim + p.bd - 1) / p.bd;
     const uint64_t rows = round_up(n_rows, TILE), per = TILE * (uint64_t)WORKGROUPS;
@@ -986,8 +1063,9 @@ Plan plan_for(uint32_t n_q, uint64_t n_rows, uint32_t dim, int32_t dtype) {
     p.piece_rows = piece((uint64_t)p.q_tiles * p.bq * 2 * p.g_planes);
     p.packed_rows = std::min(p.piece_rows, piece((uint64_t)p.kp * 2 * p.planes));
     const uint64_t tiles = rows / TILE;
-    p.loss_splits = splits_for(p.loss_q_tiles, tiles);
-    p.weight_splits = splits_for(p.q_tiles, tiles);
+    const uint64_t score_tiles = dtype == VS_F32 && n_q <= 128 ? rows / SplitScores<true>::T : tiles;
+    p.loss_splits = splits_for(p.loss_q_tiles, score_tiles);
+    p.weight_splits = splits_for(p.score_q_tiles, score_tiles);
     p.row_splits = splits_for(p.d_tiles, tiles);
     p.grad_splits = splits_for(p.q_tiles * p.d_tiles, tiles * (TILE / STEP));
     return p;
@@ -1093,14 +1171,10 @@ struct Call {
     void pack_rows() {
         const uint64_t threads = (uint64_t)a.piece_rows * a.rows.chunks;
         const uint32_t grid = (uint32_t)std::min<uint64_t>((threads + 255) / 256, 1u << 16);
-        auto go = [&](auto wide, auto kernel, auto* t) { kernel<<<grid, 256, 0, stream>>>(a, t, x.t.stride, b.packed); };
-        if (x.t.dtype == VS_F32) {
-            const float* t = (const float*)x.t.rows;
-            aligned_rows<float, 4>(t, x.t.stride) ? go(0, pack_rows_kernel<float, 3, true>, t) : go(0, pack_rows_kernel<float, 3, false>, t);
-        } else {
-            const bf16* t = (const bf16*)x.t.rows;
-            aligned_rows<bf16, 8>(t, x.t.stride) ? go(0, pack_rows_kernel<bf16, 1, true>, t) : go(0, pack_rows_kernel<bf16, 1, false>, t);
-        }
+        if (x.t.dtype == VS_F32)
+            pack_rows_kernel<float, 3><<<grid, 256, 0, stream>>>(a, (const float*)x.t.rows, x.t.stride, b.packed);
+        else
+            pack_rows_kernel<bf16, 1><<<grid, 256, 0, stream>>>(a, (const bf16*)x.t.rows, x.t.stride, b.packed);
     }
 
     // A product over the tiles of the piece.
@@ -1112,53 +1186,46 @@ struct Call {
         if (error == hipSuccess) kernel<<<across * splits, THREADS, lds, stream>>>(a);
     }
 
-    // Calls `f` with whether logits are cosines and whether rows are read through the list, as constants.
-    template <typename F>
-    void by_kind(F&& f) {
-        const bool listed = a.rows.list;
-        if (a.norms)
-            listed ? f(std::true_type{}, std::true_type{}) : f(std::true_type{}, std::false_type{});
-        else
-            listed ? f(std::false_type{}, std::true_type{}) : f(std::false_type{}, std::false_type{});
+    // Calls `f` with a Scores type for tiles of BQ queries and whether logits are cosines, as constants.
+    template <int BQ, bool LANES_ARE_QUERIES, typename F>
+    void with_scores(F&& f) {
+        auto by_norms = [&](auto scores) { a.norms ? f(scores, std::true_type{}) : f(scores, std::false_type{}); };
+        if (BQ == 64 && p.planes == 3) return by_norms(SplitScores<LANES_ARE_QUERIES>{});
+        if (a.rows.list) return by_norms(Scores<BQ, LANES_ARE_QUERIES, true>{});
+        by_norms(Scores<BQ, LANES_ARE_QUERIES, false>{});
     }
 
     template <int BQ>
     void loss() {
-        by_kind([&](auto norms, auto listed) {
-            product(loss_kernel<BQ, norms, listed>, Scores<BQ, true, listed>::LDS, p.loss_q_tiles, p.loss_splits);
+        with_scores<BQ, true>([&](auto scores, auto norms) {
+            using S = decltype(scores);
+            product(loss_kernel<S, norms>, S::LDS, p.loss_q_tiles, p.loss_splits);
         });
     }
 
     template <int BQ, int PG>
     void weights() {
-        by_kind([&](auto norms, auto listed) {
-            product(weights_kernel<BQ, norms, listed, PG>, Scores<BQ, false, listed>::LDS + 8 * 2048, p.q_tiles, p.weight_splits);
+        with_scores<BQ, false>([&](auto scores, auto norms) {
+            using S = decltype(scores);
+            // (f32 rows are never read through the list, and take all planes a step where BQ is 64; bf16 rows have one)
+            constexpr bool SPLIT = std::is_same_v<S, SplitScores<false>>, LISTED = std::is_same_v<S, Scores<BQ, false, true>>;
+            if constexpr (PG == 3 ? SPLIT || (BQ == 256 && !LISTED) : !SPLIT)
+                product(weights_kernel<S, norms, PG>, S::LDS + 8 * weights_turn<S>::BYTES, p.score_q_tiles, p.weight_splits);
         });
     }
     template <int BQ>
     void weights() {
-        if (p.planes == 3) return product_f32_weights<BQ>();
+        if (p.planes == 3) return weights<BQ, 3>();
         if constexpr (BQ == 64)
             weights<BQ, 2>();
         else
             weights<BQ, 1>();
     }
-    template <int BQ>
-    void product_f32_weights() {  // (always from planes, never through the list)
-        if (a.norms)
-            product(weights_kernel<BQ, true, false, 3>, Scores<BQ, false, false>::LDS + 8 * 2048, p.q_tiles, p.weight_splits);
-        else
-            product(weights_kernel<BQ, false, false, 3>, Scores<BQ, false, false>::LDS + 8 * 2048, p.q_tiles, p.weight_splits);
-    }
 
     template <int BD, typename E>
     void row_grads() {
-        constexpr int V = 16 / sizeof(E);
-        constexpr uint32_t LDS = 2 * (Rows<BD>::BYTES + Rows<TILE>::BYTES) + 8 * 4096;  // and a Turn's rows for every wave
-        if (aligned_rows<E, V>(a.grad_rows, a.grad_row_stride) && a.dim % V == 0)
-            product(row_grads_kernel<BD, E, true>, LDS, p.d_tiles, p.row_splits);
-        else
-            product(row_grads_kernel<BD, E, false>, LDS, p.d_tiles, p.row_splits);
+        // (and a Turn's rows for every wave)
+        product(row_grads_kernel<BD, E>, 2 * (Rows<BD>::BYTES + Rows<TILE>::BYTES) + 8 * 4096, p.d_tiles, p.row_splits);
     }
     template <typename E>
     void row_grads() {
@@ -1188,7 +1255,7 @@ hipError_t run_loss_few(const Xent& x, XentArgs a, const Few& f, float* loss, fl
         loss_few_kernel<E, Q, V, NQ, true><<<a.splits, 256, lds, stream>>>(a, f);
     else
         loss_few_kernel<E, Q, V, NQ, false><<<a.splits, 256, lds, stream>>>(a, f);
-    join_loss_kernel<<<1, 256, 0, stream>>>(a, f, loss, lse);
+    join_loss_kernel<<<x.n_q, 256, 0, stream>>>(a, f, loss, lse);
     return hipGetLastError();
 }
 template <typename E, typename Q, int V>
@@ -1199,13 +1266,6 @@ hipError_t pick_loss_few(const Xent& x, const XentArgs& a, const Few& f, float* 
         case 3: return run_loss_few<E, Q, V, 3>(x, a, f, loss, lse, stream);
         default: return run_loss_few<E, Q, V, 4>(x, a, f, loss, lse, stream);
     }
-}
-template <typename E, typename Q>
-hipError_t pick_loss_few(const Xent& x, const XentArgs& a, const Few& f, float* loss, float* lse, hipStream_t stream) {
-    constexpr int V = 16 / sizeof(E);
-    // (columns from dim on are read too where a slab has them, times zero: only if they are whole chunks of the row)
-    return aligned_rows<E, V>(x.t.rows, x.t.stride) && x.t.dim % V == 0 ? pick_loss_few<E, Q, V>(x, a, f, loss, lse, stream)
-                                                                        : pick_loss_few<E, Q, 1>(x, a, f, loss, lse, stream);
 }
 hipError_t launch_loss_few(const Xent& x, void* workspace, float* loss, float* lse, hipStream_t stream) {
     const Buffers b = carve(workspace, plan_for(x.n_q, x.t.n_rows, x.t.dim, x.t.dtype), x.n_q, x.t.n_rows, x.t.dim);
@@ -1220,8 +1280,8 @@ hipError_t launch_loss_few(const Xent& x, void* workspace, float* loss, float* l
     Few f{x.t.rows, x.queries, x.t.stride, x.query_stride, x.targets, x.mask, x.t.present, x.t.first_id, x.scale, 1};
     // small tables: parts of a word, down to eight rows, until there is one for every wave
     while (f.parts < 8 && (x.t.n_rows + 63) / 64 * f.parts * 2 <= FEW_WORKGROUPS * 4) f.parts *= 2;
-    if (x.t.dtype == VS_F32) return pick_loss_few<float, float>(x, a, f, loss, lse, stream);
-    return x.queries_f32 ? pick_loss_few<bf16, float>(x, a, f, loss, lse, stream) : pick_loss_few<bf16, bf16>(x, a, f, loss, lse, stream);
+    if (x.t.dtype == VS_F32) return pick_loss_few<float, float, 4>(x, a, f, loss, lse, stream);
+    return x.queries_f32 ? pick_loss_few<bf16, float, 8>(x, a, f, loss, lse, stream) : pick_loss_few<bf16, bf16, 8>(x, a, f, loss, lse, stream);
 }
 
 void clear_rows(const Xent& x, void* grad_rows, uint64_t stride, bool all, hipStream_t stream) {
@@ -1251,7 +1311,7 @@ hipError_t launch_xent(const Xent& x, void* workspace, float* loss, float* lse, 
     });
     c.a.splits = c.p.loss_splits;
     if (c.error != hipSuccess) return c.error;
-    join_loss_kernel<<<(x.n_q + 3) / 4, 256, 0, stream>>>(c.a, Few{}, loss, lse);
+    join_loss_kernel<<<x.n_q, 256, 0, stream>>>(c.a, Few{}, loss, lse);
     return hipGetLastError();
 }
 
@@ -1272,7 +1332,7 @@ hipError_t launch_xent_grad(const Xent& x, const float* loss, const float* lse, 
     const bool f32 = x.t.dtype == VS_F32;
     if (grad_rows && c.a.list) clear_rows(x, grad_rows, grad_row_stride, false, stream);
     c.for_pieces(c.packed ? c.p.packed_rows : c.p.piece_rows, [&] {
-        c.p.bq == 64 ? c.weights<64>() : c.p.bq == 128 ? c.weights<128>() : c.weights<256>();
+        c.p.score_bq == 64 ? c.weights<64>() : c.p.score_bq == 128 ? c.weights<128>() : c.weights<256>();
         if (grad_rows) f32 ? c.row_grads<float>() : c.row_grads<bf16>();
         if (!grad_queries) return;
         c.p.bq == 64 ? c.query_grads<64>() : c.p.bq == 128 ? c.query_grads<128>() : c.query_grads<256>();
