@@ -1,8 +1,9 @@
 // Products of tiles on the bf16 matrix cores: the loop that the cross entropy's four products share.
 //
 // A workgroup of eight waves makes a tile of M x N sums over k, 64 k at a time. Both operands' pieces of a step go from
-// memory straight into LDS (16 bytes a lane, no registers), into the half that the step before has left, while the matrix
-// cores work on the other half: one barrier a step. 64 KiB a step, twice, are 128 of the 160 KiB of a CU.
+// memory straight into LDS (16 bytes a lane, no registers), into a buffer that an earlier step has left, while the matrix
+// cores work on another: one barrier a step. 64 KiB a step (256 x 256), twice, are 128 of the 160 KiB of a CU; smaller
+// tiles, whose steps are over sooner than memory answers, have up to four buffers and load as many steps ahead.
 //
 // Operands come in two shapes:
 //   Rows<R>  [R rows][64 k], k contiguous: read as one ds_read_b128 a fragment;
@@ -48,12 +49,11 @@ __device__ __forceinline__ void load_to_lds(const char* from, const char* to) {
                  : "v"((global_void)from), "s"(uniform_u32((uint32_t)(uintptr_t)(lds_void)to))
                  : "memory", "m0");
 }
-// My loads have written LDS and my reads of it are done, and so are everybody's. STORES: so many stores of mine, at
-// least, were issued behind the last of those loads; they need not be done (the counter of loads and stores falls in the
-// order of their issue).
-template <int STORES = 0>
+// My loads have written LDS, but for the last BEHIND loads and stores that I issued (there have to be so many at least: the
+// counter of both falls in the order of their issue), and my reads of it are done, and so are everybody's.
+template <int BEHIND = 0>
 __device__ __forceinline__ void step_barrier() {
-    constexpr int N = STORES > 63 ? 63 : STORES;
+    constexpr int N = BEHIND > 63 ? 63 : BEHIND;
     asm volatile("" ::: "memory");
     __builtin_amdgcn_s_waitcnt(0x0070 | (N & 15) | (N >> 4) << 14);  // vmcnt(N) lgkmcnt(0)
     __builtin_amdgcn_s_barrier();
@@ -76,7 +76,7 @@ struct Rows {
 #pragma unroll
             for (int i = 0; i < LOADS; ++i) next[i] = p.list[min(at + i * 64 + (threadIdx.x >> 3), p.rows - 1)];
     }
-    __device__ __forceinline__ void aim(uint32_t at) {
+    __device__ __forceinline__ void aim(uint32_t at) {  // (at or behind the last row: zeros)
         first = at;
         if constexpr (LISTED)
 #pragma unroll
@@ -98,13 +98,13 @@ struct Rows {
 };
 
 // [64 k][C]: C * 2 bytes a k, chunk c of k at place c ^ turn(k).
-template <int C>
+template <int C, bool LISTED = false>
 struct Cols {
     static constexpr int BYTES = C * 128;
     static constexpr int CHUNKS = C / 8;
     static constexpr int LOADS = CHUNKS / 8;
     static constexpr int APART = 512 / CHUNKS;  // k between two loads of a thread
-    uint32_t index[LOADS];
+    uint32_t index[LISTED ? LOADS : 1];
     uint32_t k0, chunk;
     __device__ __forceinline__ static uint32_t turn(uint32_t k) {
         return CHUNKS >= 16 ? (2 * (k & 3)) ^ (8 * (k >> 3 & 1)) : 2 * (k & 3);
@@ -115,14 +115,14 @@ struct Cols {
     }
     // The memory rows of the step whose first k is row `first` of `end`: reads the list, ahead of its use.
     __device__ __forceinline__ void peek(const Planes& p, uint32_t first, uint32_t end) {
-        if (!p.list) return;
+        if constexpr (LISTED)
 #pragma unroll
-        for (int i = 0; i < LOADS; ++i) index[i] = p.list[min(first + k0 + i * APART, end - 1)];
+            for (int i = 0; i < LOADS; ++i) index[i] = p.list[min(first + k0 + i * APART, end - 1)];
     }
     __device__ __forceinline__ void load(int i, const Planes& p, uint32_t first, uint32_t end, uint32_t first_chunk, uint32_t plane,
                                          const char* zeros, char* lds) const {
         const uint32_t c = first_chunk + chunk, r = first + k0 + i * APART;
-        const char* from = p.base + (plane * p.plane + c * 16ull) + (uint64_t)(p.list ? index[i] : r) * p.stride;
+        const char* from = p.base + (plane * p.plane + c * 16ull) + (uint64_t)(LISTED ? index[i] : r) * p.stride;
         load_to_lds(r < end && c < p.chunks ? from : zeros, lds + uniform_u32(threadIdx.x >> 6) * 1024 + i * 8192);
     }
     __device__ __forceinline__ static bf16x8 read(char* lds, uint32_t tile, int kk) {
@@ -162,10 +162,10 @@ struct Engine {
             for (int n = 0; n < TN; ++n) fb[kk][n] = B::read(b, n0 + n, kk);
         __builtin_amdgcn_sched_barrier(0);
     }
-    // (a, b): this step's operands in LDS; (next_a, next_b): the next one's. `under_way(phase)` issues loads: in phases
-    // before the last into the next step's half, in the last into this step's. `stored`: the next step's loads were all
-    // issued before the STORES of a tile's end.
-    template <int STORES, typename F>
+    // (a, b): this step's operands in LDS; (next_a, next_b): the next one's. `under_way(phase)` issues loads, in the last
+    // phase into this step's buffer. BEHIND: loads of later steps that were issued after the last of the next one's;
+    // `stored`: and after those the STORES of a tile's end.
+    template <int BEHIND, int STORES, typename F>
     __device__ __forceinline__ void step(char* a, char* b, char* next_a, char* next_b, f32x4 (&acc)[TM][TN], uint32_t stored, F&& under_way) {
 #pragma unroll
         for (int p = 0; p < PHASES; ++p) {
@@ -174,9 +174,9 @@ struct Engine {
                 ask(a, b, p + 1);
             } else {
                 if (STORES && stored)
-                    step_barrier<STORES>();
+                    step_barrier<BEHIND + STORES>();
                 else
-                    step_barrier();
+                    step_barrier<BEHIND>();
                 ask(next_a, next_b, 0);
             }
             under_way(p);
@@ -262,6 +262,9 @@ struct Turn {
         return *reinterpret_cast<const u32x4*>(at(wave_lds, row(lane, j), chunk(lane)));
     }
 };
+
+// Buffers of a step's `bytes` that fit beside `others` in the LDS of a CU.
+constexpr int buffers_of(int bytes, int others) { return std::min((160 * 1024 - others) / bytes, 4); }
 
 // Which step of the products a side's loads have come to: plane pair c of 64 k block k of the workgroup's tile `tile`.
 struct Cursor {

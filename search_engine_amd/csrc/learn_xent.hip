@@ -29,6 +29,7 @@ namespace {
 constexpr uint32_t NONE = 0xFFFFFFFFu;
 constexpr float LOG2E = 1.44269504088896340736f;
 constexpr int TILE = 256;  // candidates of a tile
+constexpr uint32_t NO_ROW = 0xF0000000u;  // behind every row, and no sum with a tile's rows wraps
 
 struct XentArgs {
     Planes rows;            // of the candidates, or of the whole table with the list of candidates
@@ -246,7 +247,10 @@ struct Scores {
     static constexpr int T = TILE, Q_TILE = BQ;
     using R = Rows<TILE, LISTED>;
     using Q = Rows<BQ>;
-    static constexpr int LDS = 2 * (R::BYTES + Q::BYTES);
+    // Beside the buffers: results on their way out (16 KiB) and numbers of each query and candidate. With sixteen queries
+    // not every wave has a load of theirs, and the count of those behind would not be one number: two buffers.
+    static constexpr int BUFFERS = BQ < 64 ? 2 : buffers_of(R::BYTES + Q::BYTES, 16384 + 6144);
+    static constexpr int LDS = BUFFERS * (R::BYTES + Q::BYTES);
 
     __device__ __forceinline__ static uint32_t wave_q() { return uniform_u32(threadIdx.x >> 6) % WAVES_Q; }
     __device__ __forceinline__ static uint32_t wave_r() { return uniform_u32(threadIdx.x >> 6) / WAVES_Q; }
@@ -267,68 +271,71 @@ struct Scores {
         const uint32_t base = a.piece_begin - a.place0;
         auto half_r = [&](uint32_t i) { return lds + i * (R::BYTES + Q::BYTES); };
         auto half_q = [&](uint32_t i) { return lds + i * (R::BYTES + Q::BYTES) + R::BYTES; };
-        // The rows have furthest to come: theirs go first, a step earlier than the queries'. (Steps are counted as
-        // queries x rows; which of the two is A does not matter to six symmetric steps.)
+        // The rows have furthest to come: theirs go first, behind a step's barrier into the buffer that it has freed; the
+        // queries of that step follow in the next step's first phases. Loads go on behind the last tile, of zeros, so
+        // that their number stays what the barriers count on. (Steps are counted as queries x rows; which of the two is A
+        // does not matter to six symmetric steps.)
         Cursor cr{0, 0, along}, cq{0, 0, along};
-        bool rows_left = true;
         r.peek(rows, base + along * TILE);
         r.aim(base + along * TILE);
         r.peek(rows, base + (along + a.splits) * TILE);
         auto load_rows = [&](uint32_t to) {
-            if (!rows_left) return;
 #pragma unroll
             for (int i = 0; i < R::LOADS; ++i) r.load(i, rows, cr.k, a.score_steps.plane_b(cr.c), a.zeros, half_r(to));
             if (!cr.advance(planes, blocks, a.splits)) return;
-            rows_left = cr.tile < tiles;
-            r.aim(base + cr.tile * TILE);
-            r.peek(rows, base + (cr.tile + a.splits) * TILE);
+            r.aim(cr.tile < tiles ? base + cr.tile * TILE : NO_ROW);
+            r.peek(rows, cr.tile + a.splits < tiles ? base + (cr.tile + a.splits) * TILE : 0);
         };
         auto load_queries = [&](int i, uint32_t to) { q.load(i, a.q, cq.k, a.score_steps.plane_a(cq.c), a.zeros, half_q(to)); };
-        load_rows(0);
+        auto load_all_queries = [&](uint32_t to) {
 #pragma unroll
-        for (int i = 0; i < Q::LOADS; ++i) load_queries(i, 0);
-        cq.advance(planes, blocks, a.splits);
-        step_barrier();
+            for (int i = 0; i < Q::LOADS; ++i) load_queries(i, to);
+            cq.advance(planes, blocks, a.splits);
+        };
+        constexpr int BEHIND = (BUFFERS - 2) * (R::LOADS + Q::LOADS);
+#pragma unroll
+        for (int i = 0; i < BUFFERS - 1; ++i) {
+            load_rows(i);
+            load_all_queries(i);
+        }
+        step_barrier<BEHIND>();
         using E = Engine<std::conditional_t<LANES_ARE_QUERIES, R, Q>, std::conditional_t<LANES_ARE_QUERIES, Q, R>, TM, TN>;
         E e;
         e.m0 = LANES_ARE_QUERIES ? wave_r() * WR : wave_q() * WQ;
         e.n0 = LANES_ARE_QUERIES ? wave_q() * WQ : wave_r() * WR;
         e.ask(LANES_ARE_QUERIES ? half_r(0) : half_q(0), LANES_ARE_QUERIES ? half_q(0) : half_r(0), 0);
-        load_rows(1);
+        load_rows(BUFFERS - 1);
         uint32_t at = 0;
-        uint32_t early = 0, stored = 0;  // the next step's queries are under way already; stores are
+        uint32_t early = 0, stored = 0;  // the queries to be loaded in this step are under way already; stores are
 #pragma nounroll
         for (uint32_t tile = along; tile < tiles; tile += a.splits) {
             f32x4 acc[TM][TN] = {};
 #pragma nounroll
             for (uint32_t s = 0; s < steps; ++s) {
-                const uint32_t other = at ^ 1;
-                char *ar = half_r(at), *aq = half_q(at), *br = half_r(other), *bq = half_q(other);
-                e.template step<STORES>(LANES_ARE_QUERIES ? ar : aq, LANES_ARE_QUERIES ? aq : ar, LANES_ARE_QUERIES ? br : bq,
-                                        LANES_ARE_QUERIES ? bq : br, acc, stored, [&](int phase) {
+                const uint32_t next = at + 1 == BUFFERS ? 0 : at + 1, last = at ? at - 1 : BUFFERS - 1;
+                char *ar = half_r(at), *aq = half_q(at), *br = half_r(next), *bq = half_q(next);
+                e.template step<BEHIND, STORES>(LANES_ARE_QUERIES ? ar : aq, LANES_ARE_QUERIES ? aq : ar, LANES_ARE_QUERIES ? br : bq,
+                                                LANES_ARE_QUERIES ? bq : br, acc, stored, [&](int phase) {
                     if (phase < E::PHASES - 1) {
-                        // the queries of the next step, over the phases before the barrier
                         constexpr int EACH = (Q::LOADS + E::PHASES - 2) / (E::PHASES - 1);
-                        if (early || cq.tile >= tiles) return;
+                        if (BUFFERS == 2 && STORES && early) return;
 #pragma unroll
-                        for (int i = phase * EACH; i < min((phase + 1) * EACH, Q::LOADS); ++i) load_queries(i, other);
+                        for (int i = phase * EACH; i < min((phase + 1) * EACH, Q::LOADS); ++i) load_queries(i, last);
                         return;
                     }
+                    if (!(BUFFERS == 2 && STORES && early)) cq.advance(planes, blocks, a.splits);
                     load_rows(at);
-                    if (!early && cq.tile < tiles) cq.advance(planes, blocks, a.splits);
-                    early = afresh_uniform(STORES && s + 1 == steps && cq.tile < tiles);
-                    if (!early) return;
-                    // the end of a tile stores: what the step after next needs goes before that
-#pragma unroll
-                    for (int i = 0; i < Q::LOADS; ++i) load_queries(i, at);
-                    cq.advance(planes, blocks, a.splits);
+                    if (BUFFERS > 2 || !STORES) return;
+                    // two buffers, and the tile's end stores: what the step after next needs goes before that
+                    early = afresh_uniform(s + 1 == steps);
+                    if (early) load_all_queries(at);
                 });
                 stored = afresh_uniform(0);
-                at = other;
+                at = next;
             }
-            stored = afresh_uniform(done(acc, a.piece_begin + tile * TILE) && early);
+            stored = afresh_uniform(done(acc, a.piece_begin + tile * TILE));
         }
-        // (nothing is under way any more: the last step's barrier waited for all, and no load followed it)
+        __builtin_amdgcn_s_waitcnt(0x0F70);  // (the zeros have come: nothing writes LDS behind the workgroup's end)
     }
 };
 
@@ -764,6 +771,8 @@ __global__ __launch_bounds__(THREADS, 2) void weights_kernel(XentArgs a) {
 // drows of a piece: transposed queries (BD columns of the rows) by G. A lane holds four neighbouring columns of a row.
 // As in weights_kernel every lane stores every time, to its own 16 bytes of a.spill where it has no row or no whole
 // 16 bytes of columns; the columns of a last, broken 16 bytes are stored one by one besides.
+template <int BD>
+constexpr int row_grads_buffers = buffers_of(Rows<BD>::BYTES + Rows<TILE>::BYTES, 8 * 4096);
 template <int BD, typename E>
 __global__ __launch_bounds__(THREADS, 2) void row_grads_kernel(XentArgs a) {
     using A = Rows<BD>;
@@ -785,56 +794,61 @@ __global__ __launch_bounds__(THREADS, 2) void row_grads_kernel(XentArgs a) {
     q.aim(tile_d * BD);
     r.aim(along * TILE);
     const uint32_t planes = a.grad_steps.n, blocks = a.gq / 64, steps = planes * blocks;
+    constexpr int BUFFERS = row_grads_buffers<BD>, BEHIND = (BUFFERS - 2) * (A::LOADS + B::LOADS);
     auto half_q = [&](uint32_t i) { return lds + i * (A::BYTES + B::BYTES); };
     auto half_g = [&](uint32_t i) { return lds + i * (A::BYTES + B::BYTES) + A::BYTES; };
+    // (as in Scores::run: the weights are the operand that has further to come)
     Cursor cg{0, 0, along}, cq{0, 0, along};
     auto load_weights = [&](uint32_t to) {
-        if (cg.tile >= tiles) return;
 #pragma unroll
         for (int i = 0; i < B::LOADS; ++i) r.load(i, g, cg.k, a.grad_steps.plane_a(cg.c), a.zeros, half_g(to));
-        if (cg.advance(planes, blocks, a.splits)) r.aim(cg.tile * TILE);
+        if (cg.advance(planes, blocks, a.splits)) r.aim(cg.tile < tiles ? cg.tile * TILE : NO_ROW);
     };
     auto load_queries = [&](int i, uint32_t to) { q.load(i, a.qt, cq.k, a.grad_steps.plane_b(cq.c), a.zeros, half_q(to)); };
-    load_weights(0);
+    auto load_all_queries = [&](uint32_t to) {
 #pragma unroll
-    for (int i = 0; i < A::LOADS; ++i) load_queries(i, 0);
-    cq.advance(planes, blocks, a.splits);
-    step_barrier();
+        for (int i = 0; i < A::LOADS; ++i) load_queries(i, to);
+        cq.advance(planes, blocks, a.splits);
+    };
+#pragma unroll
+    for (int i = 0; i < BUFFERS - 1; ++i) {
+        load_weights(i);
+        load_all_queries(i);
+    }
+    step_barrier<BEHIND>();
     using En = Engine<A, B, TM, TN>;
     En e;
     e.m0 = wd * TM;
     e.n0 = wr * TN;
     e.ask(half_q(0), half_g(0), 0);
-    load_weights(1);
+    load_weights(BUFFERS - 1);
     uint32_t at = 0;
     constexpr int UNIT = sizeof(E) == 2 ? TM : 4;  // fragments that go through LDS at a time: 256 bytes of a row at most
     using T = Turn<4 * sizeof(E), UNIT>;
-    char* const wave_lds = lds + 2 * (A::BYTES + B::BYTES) + wave * T::BYTES;
+    char* const wave_lds = lds + BUFFERS * (A::BYTES + B::BYTES) + wave * T::BYTES;
     uint32_t early = 0, stored = 0;  // as in Scores::run
 #pragma nounroll
     for (uint32_t tile = along; tile < tiles; tile += a.splits) {
         f32x4 acc[TM][TN] = {};
 #pragma nounroll
         for (uint32_t s = 0; s < steps; ++s) {
-            const uint32_t other = at ^ 1;
-            e.template step<TN * (TM / UNIT) * T::STORES>(half_q(at), half_g(at), half_q(other), half_g(other), acc, stored, [&](int phase) {
+            const uint32_t next = at + 1 == BUFFERS ? 0 : at + 1, last = at ? at - 1 : BUFFERS - 1;
+            e.template step<BEHIND, TN * (TM / UNIT) * T::STORES>(half_q(at), half_g(at), half_q(next), half_g(next), acc, stored, [&](int phase) {
                 if (phase < En::PHASES - 1) {
                     constexpr int EACH = (A::LOADS + En::PHASES - 2) / (En::PHASES - 1);
-                    if (early || cq.tile >= tiles) return;
+                    if (BUFFERS == 2 && early) return;
 #pragma unroll
-                    for (int i = phase * EACH; i < min((phase + 1) * EACH, A::LOADS); ++i) load_queries(i, other);
+                    for (int i = phase * EACH; i < min((phase + 1) * EACH, A::LOADS); ++i) load_queries(i, last);
                     return;
                 }
+                if (!(BUFFERS == 2 && early)) cq.advance(planes, blocks, a.splits);
                 load_weights(at);
-                if (!early && cq.tile < tiles) cq.advance(planes, blocks, a.splits);
-                early = afresh_uniform(s + 1 == steps && cq.tile < tiles);
-                if (!early) return;
-#pragma unroll
-                for (int i = 0; i < A::LOADS; ++i) load_queries(i, at);
-                cq.advance(planes, blocks, a.splits);
+                if (BUFFERS > 2) return;
+                early = afresh_uniform(s + 1 == steps);
+                if (early) load_all_queries(at);
             });
             stored = afresh_uniform(0);
-            at = other;
+            at = next;
         }
         const uint32_t l = afresh(threadIdx.x) & 63, d0 = tile_d * BD + wd * TM * 16, place0 = a.piece_begin + tile * TILE + wr * TN * 16;
         constexpr uint32_t V = 16 / sizeof(E);
@@ -866,15 +880,20 @@ __global__ __launch_bounds__(THREADS, 2) void row_grads_kernel(XentArgs a) {
                 }
                 __builtin_amdgcn_sched_barrier(0);
             }
-        stored = afresh_uniform(early);
+        stored = afresh_uniform(1);
     }
+    __builtin_amdgcn_s_waitcnt(0x0F70);
 }
 
 // dqueries over one share of a piece's candidates: G by rows, the sum running over the candidates.
-template <int BQ, int BD>
+// (Through the list two buffers: its reads are waited for with the loads under way counted in, so that only those that
+// the barrier has waited for already may be.)
+template <int BQ, int BD, bool LISTED>
+constexpr int query_grads_buffers = LISTED ? 2 : buffers_of(Cols<BQ>::BYTES + Cols<BD>::BYTES, 0);
+template <int BQ, int BD, bool LISTED>
 __global__ __launch_bounds__(THREADS, 2) void query_grads_kernel(XentArgs a) {
     using A = Cols<BQ>;
-    using B = Cols<BD>;
+    using B = Cols<BD, LISTED>;
     constexpr int WAVES_Q = BQ >= 128 ? 2 : 1, WAVES_D = 8 / WAVES_Q;
     constexpr int TM = BQ / WAVES_Q / 16, TN = BD / WAVES_D / 16;
     extern __shared__ __attribute__((aligned(128))) char lds[];
@@ -899,47 +918,53 @@ __global__ __launch_bounds__(THREADS, 2) void query_grads_kernel(XentArgs a) {
         B r;
         w.init();
         r.init();
+        constexpr int BUFFERS = query_grads_buffers<BQ, BD, LISTED>, BEHIND = (BUFFERS - 2) * (A::LOADS + B::LOADS);
         auto half_g = [&](uint32_t i) { return lds + i * (A::BYTES + B::BYTES); };
         auto half_r = [&](uint32_t i) { return lds + i * (A::BYTES + B::BYTES) + A::BYTES; };
         Cursor cr{0, 0, 0}, cg{0, 0, 0};
         const uint32_t planes = a.grad_steps.n;
         auto load_rows = [&](uint32_t to) {
-            if (cr.tile) return;
             const uint32_t from = begin + cr.k * STEP;
 #pragma unroll
             for (int i = 0; i < B::LOADS; ++i)
                 r.load(i, rows, base + from, base + stop, tile_d * (BD / 8), a.grad_steps.plane_b(cr.c), a.zeros, half_r(to));
-            if (!cr.advance(planes, blocks, 1) && !cr.c) r.peek(rows, base + from + STEP, base + stop);  // while this step multiplies
+            cr.advance(planes, blocks + BUFFERS, 1);  // (behind the last block: zeros)
+            if (!cr.c) r.peek(rows, base + from + STEP, base + stop);  // while this step multiplies
         };
         auto load_weights = [&](int i, uint32_t to) {
             w.load(i, g, begin + cg.k * STEP, stop, tile_q * (BQ / 8), a.grad_steps.plane_a(cg.c), a.zeros, half_g(to));
         };
         r.peek(rows, base + begin, base + stop);
-        load_rows(0);
 #pragma unroll
-        for (int i = 0; i < A::LOADS; ++i) load_weights(i, 0);
-        cg.advance(planes, blocks, 1);
-        step_barrier();
+        for (int i = 0; i < BUFFERS - 1; ++i) {
+            load_rows(i);
+#pragma unroll
+            for (int j = 0; j < A::LOADS; ++j) load_weights(j, i);
+            cg.advance(planes, blocks + BUFFERS, 1);
+        }
+        step_barrier<BEHIND>();
         using En = Engine<A, B, TM, TN>;
         En e;
         e.m0 = wq * TM;
         e.n0 = wd * TN;
         e.ask(half_g(0), half_r(0), 0);
-        load_rows(1);
+        load_rows(BUFFERS - 1);
         uint32_t at = 0;
 #pragma nounroll
         for (uint32_t s = 0; s < steps; ++s) {
-            const uint32_t other = at ^ 1;
-            e.template step<0>(half_g(at), half_r(at), half_g(other), half_r(other), acc, false, [&](int phase) {
-                if (phase == En::PHASES - 1) return load_rows(at);
+            const uint32_t next = at + 1 == BUFFERS ? 0 : at + 1, last = at ? at - 1 : BUFFERS - 1;
+            e.template step<BEHIND, 0>(half_g(at), half_r(at), half_g(next), half_r(next), acc, 0, [&](int phase) {
+                if (phase == En::PHASES - 1) {
+                    cg.advance(planes, blocks + BUFFERS, 1);
+                    return load_rows(at);
+                }
                 constexpr int EACH = (A::LOADS + En::PHASES - 2) / (En::PHASES - 1);
-                if (cg.tile) return;
 #pragma unroll
-                for (int i = phase * EACH; i < min((phase + 1) * EACH, A::LOADS); ++i) load_weights(i, other);
+                for (int i = phase * EACH; i < min((phase + 1) * EACH, A::LOADS); ++i) load_weights(i, last);
             });
-            if (!cg.tile) cg.advance(planes, blocks, 1);
-            at = other;
+            at = next;
         }
+        __builtin_amdgcn_s_waitcnt(0x0F70);
     }
 #pragma unroll
     for (int m = 0; m < TM; ++m)
@@ -1225,18 +1250,24 @@ struct Call {
     template <int BD, typename E>
     void row_grads() {
         // (and a Turn's rows for every wave)
-        product(row_grads_kernel<BD, E>, 2 * (Rows<BD>::BYTES + Rows<TILE>::BYTES) + 8 * 4096, p.d_tiles, p.row_splits);
+        product(row_grads_kernel<BD, E>, row_grads_buffers<BD> * (Rows<BD>::BYTES + Rows<TILE>::BYTES) + 8 * 4096, p.d_tiles, p.row_splits);
     }
     template <typename E>
     void row_grads() {
         p.bd == 256 ? row_grads<256, E>() : row_grads<128, E>();
     }
 
+    template <int BQ, int BD, bool LISTED>
+    void query_grads() {
+        product(query_grads_kernel<BQ, BD, LISTED>, query_grads_buffers<BQ, BD, LISTED> * (Cols<BQ>::BYTES + Cols<BD>::BYTES),
+                p.q_tiles * p.d_tiles, p.grad_splits);
+    }
     template <int BQ>
     void query_grads() {
-        const uint32_t across = p.q_tiles * p.d_tiles;
-        p.bd == 256 ? product(query_grads_kernel<BQ, 256>, 2 * (Cols<BQ>::BYTES + Cols<256>::BYTES), across, p.grad_splits)
-                    : product(query_grads_kernel<BQ, 128>, 2 * (Cols<BQ>::BYTES + Cols<128>::BYTES), across, p.grad_splits);
+        if (a.rows.list)
+            p.bd == 256 ? query_grads<BQ, 256, true>() : query_grads<BQ, 128, true>();
+        else
+            p.bd == 256 ? query_grads<BQ, 256, false>() : query_grads<BQ, 128, false>();
     }
 
     template <typename Q, typename O>
