@@ -132,6 +132,14 @@ __device__ __forceinline__ Pack<E, V> load_piece(const E* row, const Piece<V>& p
     if (dim >= V) return load_any<E, V>(row + piece.col, V);
     return load_any<E, V>(row, dim);
 }
+// The same for rows that a call reads once (they are not kept in the caches for what others would read again).
+template <typename E, int V>
+__device__ __forceinline__ Pack<E, V> load_piece_once(const E* row, const Piece<V>& piece, uint32_t dim) {
+    if (dim < V) return load_any<E, V>(row, dim);
+    static_assert(V * sizeof(E) == 16);
+    using four = typename Words<sizeof(E)>::four;
+    return __builtin_bit_cast(Pack<E, V>, __builtin_nontemporal_load(reinterpret_cast<const four*>(row + piece.col)));
+}
 // Stores a piece; the columns in common with the one before are left to that one if ONCE (an addition), or else get the
 // same value twice.
 template <typename E, int V>

@@ -509,7 +509,7 @@ __global__ __launch_bounds__(256) void join_runs_kernel(GradArgs a, int side) {
 #pragma unroll
             for (int v = 0; v < V; ++v) acc[v] = p[v];
         }
-#pragma unroll 4
+#pragma unroll 8
         for (uint32_t r = run + 1 + wave; r <= last; r += 4) {
             const float* p = a.partial + ((uint64_t)r * 2 * a.chunks + chunk) * V;
 #pragma unroll

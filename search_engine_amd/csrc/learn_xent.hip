@@ -56,7 +56,7 @@ struct XentArgs {
     const float *lse, *loss, *grad_loss;
     char* g;                  // [planes][piece][whole tiles of queries] bf16
     uint64_t g_plane;
-    uint32_t g_stride;
+    uint32_t g_stride, g_planes;
     char* spill;              // 16 bytes of every thread of a product, for what it has no place for
     void* grad_rows;
     uint64_t grad_row_stride;
@@ -584,7 +584,7 @@ __global__ __launch_bounds__(256) void loss_few_kernel(XentArgs a, Few f) {
             for (uint32_t c = lane; c < chunks; c += 64) {
                 Pack<E, V> x[U];
 #pragma unroll
-                for (int u = 0; u < U; ++u) x[u] = load_piece<E, V>(table + (uint64_t)row[u] * f.stride, Piece<V>(c, a.dim), a.dim);
+                for (int u = 0; u < U; ++u) x[u] = load_piece_once<E, V>(table + (uint64_t)row[u] * f.stride, Piece<V>(c, a.dim), a.dim);
 #pragma unroll
                 for (int q = 0; q < NQ; ++q) {
                     const Pack<float, V> y = load_pack<float, V>(query + q * padded + c * V);
@@ -682,6 +682,33 @@ __global__ __launch_bounds__(256) void join_loss_kernel(XentArgs a, Few f, float
 
 // ---- gradients ----------------------------------------------------------------------------
 
+// What a query's weights have in common: zero without a click.
+__device__ __forceinline__ float query_factor(const XentArgs& a, uint32_t q) {
+    return a.click[q] != NONE ? (a.grad_loss ? a.grad_loss[q] : 1.0f) * a.qscale[q] * a.sign : 0.0f;
+}
+
+// The weights of the clicked rows of a piece, after weights_kernel, which takes every row alike (to look for them there
+// costs two instructions in eight of each element).
+__global__ __launch_bounds__(256) void click_weights_kernel(XentArgs a) {
+    const uint32_t q = blockIdx.x * 256 + threadIdx.x;
+    if (q >= a.n_q) return;
+    const uint32_t place = a.click[q];
+    if (place == NONE || place < a.piece_begin || place - a.piece_begin >= a.piece_rows) return;
+    float g = query_factor(a, q) * expm1f(-a.loss[q]);
+    if (a.norms) {
+        const float x = a.norms[row_at(a, place)];
+        g = x > 0 ? g / x : 0.0f;
+    }
+    char* out = a.g + (uint64_t)(place - a.piece_begin) * a.g_stride + q * 2;
+    if (a.g_planes == 1) {
+        *reinterpret_cast<uint16_t*>(out) = (uint16_t)bf16_bits(g);
+        return;
+    }
+    const Split s = split(g);
+    const uint16_t part[3] = {s.h, s.m, s.l};
+    for (uint32_t p = 0; p < a.g_planes; ++p) *reinterpret_cast<uint16_t*>(out + p * a.g_plane) = part[p];
+}
+
 // The weights G of a piece, [candidate][query], rounded to bf16 (PG = 1), or kept to 16 bits (2) or all 24 (3) by as many
 // planes. A lane holds four neighbouring queries of a candidate: eight bytes a store.
 template <typename S>  // fragments that go through LDS at a time: up to 64 queries of 16 candidates
@@ -691,8 +718,7 @@ template <typename S, bool NORMS, int PG>
 __global__ __launch_bounds__(THREADS, 2) void weights_kernel(XentArgs a) {
     constexpr int BQ = S::Q_TILE;
     extern __shared__ __attribute__((aligned(128))) char lds[];
-    __shared__ __attribute__((aligned(16))) float s2[BQ], lse2[BQ], factor[BQ], at_click[BQ];
-    __shared__ __attribute__((aligned(16))) uint32_t click[BQ];
+    __shared__ __attribute__((aligned(16))) float s2[BQ], lse2[BQ], factor[BQ];
     uint32_t tile_q, along;
     place_of_workgroup(a.across, a.splits, &tile_q, &along);
     const uint32_t q0 = tile_q * BQ;
@@ -701,12 +727,9 @@ __global__ __launch_bounds__(THREADS, 2) void weights_kernel(XentArgs a) {
     if (threadIdx.x < BQ) {
         const uint32_t q = q0 + threadIdx.x;
         const bool in = q < a.n_q;
-        click[threadIdx.x] = in ? a.click[q] : NONE;
         s2[threadIdx.x] = in ? a.qscale[q] * LOG2E : 0.0f;
         lse2[threadIdx.x] = in ? a.lse[q] * LOG2E : 0.0f;
-        const float f = in && a.click[q] != NONE ? (a.grad_loss ? a.grad_loss[q] : 1.0f) * a.qscale[q] * a.sign : 0.0f;
-        factor[threadIdx.x] = f;
-        at_click[threadIdx.x] = in ? f * expm1f(-a.loss[q]) : 0.0f;
+        factor[threadIdx.x] = in ? query_factor(a, q) : 0.0f;
     }
     // (the first barrier of the loop below orders these before they are read)
     // Every lane stores every time (so that the number of stores is known to the next step's barrier): rows of G are whole
@@ -728,20 +751,18 @@ __global__ __launch_bounds__(THREADS, 2) void weights_kernel(XentArgs a) {
         for (int u = 0; u < S::TM / UNIT; ++u)
 #pragma unroll
             for (int n = 0; n < S::TN; ++n) {
-                const uint32_t place = first + row0 + (l & 15) + n * 16;
                 Pack<uint16_t, 4> p[UNIT][3];
 #pragma unroll
                 for (int t = 0; t < UNIT; ++t) {
                     const uint32_t i = i0 + (u * UNIT + t) * 16;
                     const f32x4 vs = *reinterpret_cast<const f32x4*>(s2 + i), vl = *reinterpret_cast<const f32x4*>(lse2 + i);
-                    const f32x4 vf = *reinterpret_cast<const f32x4*>(factor + i), vc = *reinterpret_cast<const f32x4*>(at_click + i);
-                    const u32x4 vp = *reinterpret_cast<const u32x4*>(click + i);
+                    const f32x4 vf = *reinterpret_cast<const f32x4*>(factor + i);
 #pragma unroll
                     for (int r = 0; r < 4; ++r) {
                         float z = acc[u * UNIT + t][n][r];
                         if constexpr (NORMS) z *= inverse[n];
                         // (a query without a click has factor 0 and a finite lse if there is any candidate)
-                        float g = vp[r] == place ? vc[r] : vf[r] * __builtin_amdgcn_exp2f(__builtin_fmaf(z, vs[r], -vl[r]));
+                        float g = vf[r] * __builtin_amdgcn_exp2f(__builtin_fmaf(z, vs[r], -vl[r]));
                         if constexpr (NORMS) g *= inverse[n];
                         if constexpr (PG == 1) {
                             p[t][0].e[r] = (uint16_t)bf16_bits(g);
@@ -1035,8 +1056,8 @@ __global__ __launch_bounds__(256) void clear_rows_kernel(const uint64_t* mask, c
 
 // ---- host side ----------------------------------------------------------------------------
 
-constexpr uint64_t PIECE_BYTES = 512u << 20;  // of weights, and of planes, that are held at a time (half of it, a piece that
-                                              // the memory-side cache holds, costs more in launches than it saves)
+constexpr uint64_t PIECE_BYTES = 1u << 30;  // of weights, and of planes, that are held at a time (a quarter of it, a piece that the
+                                            // memory-side cache holds, costs more in launches than it saves)
 constexpr uint32_t WORKGROUPS = 256;          // of a product: one per CU (the LDS of a tile fills one)
 constexpr uint32_t FEW_WORKGROUPS = 2048;     // of the loss of a few queries: eight per CU
 
@@ -1157,6 +1178,7 @@ struct Call {
         a.click_z = b.click_z;
         a.g = b.g;
         a.g_stride = p.q_tiles * p.bq * 2;
+        a.g_planes = p.g_planes;
         a.g_plane = p.piece_rows * a.g_stride;
         a.spill = b.spill;
         a.part_q = b.part_q;
@@ -1364,6 +1386,7 @@ hipError_t launch_xent_grad(const Xent& x, const float* loss, const float* lse, 
     if (grad_rows && c.a.list) clear_rows(x, grad_rows, grad_row_stride, false, stream);
     c.for_pieces(c.packed ? c.p.packed_rows : c.p.piece_rows, [&] {
         c.p.score_bq == 64 ? c.weights<64>() : c.p.score_bq == 128 ? c.weights<128>() : c.weights<256>();
+        if (c.error == hipSuccess) click_weights_kernel<<<(x.n_q + 255) / 256, 256, 0, stream>>>(c.a);
         if (grad_rows) f32 ? c.row_grads<float>() : c.row_grads<bf16>();
         if (!grad_queries) return;
         c.p.bq == 64 ? c.query_grads<64>() : c.p.bq == 128 ? c.query_grads<128>() : c.query_grads<256>();
