@@ -155,12 +155,6 @@ __device__ __forceinline__ void store_piece(E* row, const Piece<V>& piece, uint3
     }
 }
 
-// Whether every row of a table starts where a Pack<E, V> may.
-template <typename E, int V>
-inline bool aligned_rows(const void* base, uint64_t stride) {
-    return (uintptr_t)base % alignof(Pack<E, V>) == 0 && stride * sizeof(E) % alignof(Pack<E, V>) == 0;
-}
-
 // A value that the compiler takes for a new one: what is computed from it is not kept in registers across a loop.
 __device__ __forceinline__ uint32_t afresh(uint32_t x) {
     asm volatile("" : "+v"(x));

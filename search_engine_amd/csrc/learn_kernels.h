@@ -15,7 +15,6 @@ struct Table {
     uint64_t stride;
     uint64_t n_rows;
     uint32_t dim;
-    uint32_t dim_read;  // columns of a row that may be read (zero from `dim` on): dim, or a slab's padded length
     int32_t dtype;      // VS_F32 or VS_BF16
     const uint64_t* present;  // rows that exist, bit r & 63 of word r >> 6; null = all
     uint32_t first_id;  // the id of row 0
@@ -61,9 +60,10 @@ struct Xent {
 };
 uint64_t xent_workspace_bytes(uint32_t n_q, uint64_t n_rows, uint32_t dim, int32_t dtype);
 hipError_t launch_xent(const Xent& x, void* workspace, float* loss, float* lse, hipStream_t stream);
+// (gradients are of the queries' and the rows' types)
 hipError_t launch_xent_grad(const Xent& x, const float* loss, const float* lse, const float* grad_loss, void* workspace,
-                            void* grad_queries, bool grad_queries_f32, uint64_t grad_query_stride, void* grad_rows,
-                            uint64_t grad_row_stride, hipStream_t stream);
+                            void* grad_queries, uint64_t grad_query_stride, void* grad_rows, uint64_t grad_row_stride,
+                            hipStream_t stream);
 
 }  // namespace learn
 }  // namespace vs

@@ -57,14 +57,14 @@ int32_t check_queries(uint32_t n_q) {
 
 int32_t make_table(const void* rows, int32_t dtype, uint64_t n_rows, uint64_t stride, uint32_t dim, learn::Table* t) {
     if (int32_t rc = check_table(rows, dtype, n_rows, stride, dim)) return rc;
-    *t = learn::Table{rows, stride, n_rows, dim, dim, dtype, nullptr, 0};
+    *t = learn::Table{rows, stride, n_rows, dim, dtype, nullptr, 0};
     return VS_OK;
 }
 
 // The sealed rows of a store, as registered in a snapshot.
 learn::Table table_of(const vs::SlabView& v) {
     const uint64_t padded = (uint64_t)v.row_vecs * 16 / size_of(v.dtype);  // columns from `dim` on are zero
-    return learn::Table{v.rows, padded, v.n_slots, v.dim, (uint32_t)padded, v.dtype, v.present, v.docid_base};
+    return learn::Table{v.rows, padded, v.n_slots, v.dim, v.dtype, v.present, v.docid_base};
 }
 
 int32_t check_sealed(vs_store* s) {
@@ -252,7 +252,7 @@ extern "C" int32_t vs_xent_grad_device(vs_ctx* ctx, const void* d_queries, uint3
     for (const void* p : {(const void*)d_grad_queries, (const void*)d_grad_rows})
         if ((uintptr_t)p % size_of(dtype)) return fail(VS_E_INVALID_ARG, "gradients: address is not aligned to its elements");
     if (int32_t rc = use_ctx(ctx)) return rc;
-    return status(learn::launch_xent_grad(x, d_loss, d_lse, d_grad_loss, d_workspace, d_grad_queries, x.queries_f32, query_stride,
+    return status(learn::launch_xent_grad(x, d_loss, d_lse, d_grad_loss, d_workspace, d_grad_queries, query_stride,
                                           d_grad_rows, row_stride, stream_of(hip_stream)), "cross entropy gradient");
 }
 
@@ -293,6 +293,6 @@ extern "C" int32_t vs_store_xent_grad_device(vs_store* s, const float* d_queries
                                          "vs_store_xent_workspace_bytes"))
             return rc;
         return status(learn::launch_xent_grad(xent_of(v, d_queries, n_q, d_targets, d_mask_words, scale), d_loss, d_lse, d_grad_loss,
-                                              d_workspace, d_grad_queries, true, v.dim, nullptr, 0, stream), "cross entropy gradient");
+                                              d_workspace, d_grad_queries, v.dim, nullptr, 0, stream), "cross entropy gradient");
     });
 }

@@ -27,7 +27,7 @@ namespace learn {
 namespace {
 
 constexpr uint32_t NONE = 0xFFFFFFFFu;
-constexpr float LOG2E = 1.44269504088896340736f;
+constexpr float LOG2E = 1.44269504088896340736f, LOG2E_REST = (float)(1.44269504088896340736 - (double)LOG2E);
 constexpr int TILE = 256;  // candidates of a tile
 constexpr uint32_t NO_ROW = 0xF0000000u;  // behind every row, and no sum with a tile's rows wraps
 
@@ -49,9 +49,7 @@ struct XentArgs {
     uint32_t piece_begin, piece_rows;
     bool first_piece;
     uint32_t across, splits;  // workgroups side by side (query or column tiles), and along the rows
-    // loss, base 2
-    float *part_m, *part_l;   // [splits][n_q]
-    float* click_z;           // [n_q]
+    float *part_m, *part_l;   // [splits][n_q] of the loss, base 2
     // gradients
     const float *lse, *loss, *grad_loss;
     char* g;                  // [planes][piece][whole tiles of queries] bf16
@@ -63,7 +61,7 @@ struct XentArgs {
     float* part_q;            // [splits][n_q][dim]
 };
 
-// What the loss of a few queries reads as the caller has it.
+// What is read as the caller has it: by the loss of a few queries all of it, else the clicks.
 struct Few {
     const void *rows, *queries;
     uint64_t stride, query_stride;
@@ -102,16 +100,37 @@ __device__ __forceinline__ uint64_t word_at(const uint64_t* mask, const uint64_t
     return left < 64 ? w & ((1ull << left) - 1) : w;
 }
 
+__device__ __forceinline__ bool clicked_candidate(const Few& f, uint32_t q, uint64_t n_rows) {
+    const uint32_t id = f.targets[q], row = id - f.first_id;
+    return id >= f.first_id && row < n_rows && word_at(f.mask, f.present, row >> 6, n_rows) >> (row & 63) & 1;
+}
+
+// An element of a query as it is multiplied with rows of type E.
+template <typename E, typename Q>
+__device__ __forceinline__ float query_element(Q x) {
+    return sizeof(E) == 2 ? __builtin_bit_cast(float, bf16_bits(to_f32(x)) << 16) : to_f32(x);
+}
+
 // The candidate rows in ascending order: 256 words of the masks per workgroup, which counts the words before its own by
-// itself (at ten million rows the last one reads 1.2 MB for that). A wave writes a word's rows together, lane l the l-th
+// itself, or (`sums` given) adds up the counts that count_words_kernel has left for each 256 words. A wave writes a word's rows together, lane l the l-th
 // bit's: a lane writing its own word's rows would touch a line of its own with each.
 constexpr uint32_t LIST_WORDS = 256;
+__global__ __launch_bounds__(256) void count_words_kernel(const uint64_t* mask, const uint64_t* present, uint64_t n_rows, uint32_t* sums) {
+    __shared__ uint32_t wave_sum[4];
+    const uint64_t i = (uint64_t)blockIdx.x * LIST_WORDS + threadIdx.x;
+    uint32_t total;
+    block_exclusive(i < (n_rows + 63) / 64 ? __popcll(word_at(mask, present, i, n_rows)) : 0, wave_sum, &total);
+    if (!threadIdx.x) sums[blockIdx.x] = total;
+}
 __global__ __launch_bounds__(256) void list_candidates_kernel(const uint64_t* mask, const uint64_t* present, uint64_t n_rows,
-                                                              uint32_t* list, uint32_t* count) {
+                                                              const uint32_t* sums, uint32_t* list, uint32_t* count) {
     __shared__ uint32_t wave_sum[4];
     const uint64_t n_words = (n_rows + 63) / 64, first = (uint64_t)blockIdx.x * LIST_WORDS;
     uint32_t n = 0, before, total;
-    for (uint64_t i = threadIdx.x; i < first; i += 256) n += __popcll(word_at(mask, present, i, n_rows));
+    if (sums)
+        for (uint32_t i = threadIdx.x; i < blockIdx.x; i += 256) n += sums[i];
+    else
+        for (uint64_t i = threadIdx.x; i < first; i += 256) n += __popcll(word_at(mask, present, i, n_rows));
     block_exclusive(n, wave_sum, &before);
     const uint64_t i = first + threadIdx.x;
     const uint64_t word = i < n_words ? word_at(mask, present, i, n_rows) : 0;
@@ -126,13 +145,16 @@ __global__ __launch_bounds__(256) void list_candidates_kernel(const uint64_t* ma
     if (blockIdx.x == gridDim.x - 1 && !threadIdx.x) *count = before + total;
 }
 
-// Queries as planes, [n_q][k] and transposed [dim][gq], by tiles of 64 x 64; the workgroups behind the tiles take four
-// queries each: length, factor, and the place of the click.
+// Queries as planes, [n_q][k] and, for gradients, transposed [dim][gq], by tiles of 64 x 64; the workgroups behind the
+// tiles take four queries each: length, factor, and the place of the click. For gradients a query whose click is no
+// candidate is zeros, whatever it holds (padding of a batch may hold anything): its weights are zero, and zero times what
+// is no number would be none in every row's gradient.
 template <typename Q, int P>
-__global__ __launch_bounds__(256) void pack_queries_kernel(XentArgs a, const Q* queries, uint64_t stride, const uint32_t* targets,
-                                                           uint32_t first_id, uint64_t n_rows, float scale, uint32_t* click,
-                                                           float* qscale, uint32_t* zeros, bool transposed) {
+__global__ __launch_bounds__(256) void pack_queries_kernel(XentArgs a, Few f, uint32_t* click, float* qscale, uint32_t* zeros,
+                                                           bool gradients) {
     __shared__ uint16_t t[P][64][72];  // [column][query], eight queries more than there are: rows stay 16-byte aligned
+    const Q* const queries = static_cast<const Q*>(f.queries);
+    const uint64_t stride = f.query_stride;
     const uint32_t n_tiles = a.gq / 64 * (a.q.chunks / 8);
     if (!blockIdx.x && threadIdx.x < 64) zeros[threadIdx.x] = 0;
     if (blockIdx.x < n_tiles) {
@@ -140,10 +162,11 @@ __global__ __launch_bounds__(256) void pack_queries_kernel(XentArgs a, const Q* 
 #pragma unroll
         for (uint32_t k = 0; k < 512; k += 256) {
             const uint32_t i = k + threadIdx.x, q = q0 + i / 8, d = d0 + i % 8 * 8;
+            const bool in = q < a.n_q && (!gradients || clicked_candidate(f, q, a.n_rows));
             Pack<uint16_t, 8> part[3];
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-                const Split s = split(q < a.n_q && d + j < a.dim ? to_f32(queries[q * stride + d + j]) : 0.0f);
+                const Split s = split(in && d + j < a.dim ? to_f32(queries[q * stride + d + j]) : 0.0f);
                 part[0].e[j] = s.h;
                 part[1].e[j] = s.m;
                 part[2].e[j] = s.l;
@@ -159,7 +182,7 @@ __global__ __launch_bounds__(256) void pack_queries_kernel(XentArgs a, const Q* 
                     store_pack<uint16_t, 8>(reinterpret_cast<uint16_t*>(const_cast<char*>(a.q.base) + p * a.q.plane + q * (uint64_t)a.q.stride) + d, part[p]);
             }
         }
-        if (!transposed) return;
+        if (!gradients) return;
         __syncthreads();
 #pragma unroll
         for (uint32_t k = 0; k < 512; k += 256) {
@@ -177,19 +200,18 @@ __global__ __launch_bounds__(256) void pack_queries_kernel(XentArgs a, const Q* 
     float sq = 0;
     if (a.norms) {
         for (uint32_t d = lane; d < a.dim; d += 64) {
-            float x = to_f32(queries[q * stride + d]);
-            if (P == 1) x = __builtin_bit_cast(float, bf16_bits(x) << 16);  // as it is multiplied
+            const float x = query_element<std::conditional_t<P == 1, bf16, float>>(queries[q * stride + d]);
             sq = __builtin_fmaf(x, x, sq);
         }
         sq = wave_sum(sq);
     }
     if (lane) return;
-    const float norm = __builtin_sqrtf(sq), size = __builtin_fabsf(scale);
+    const float norm = __builtin_sqrtf(sq), size = __builtin_fabsf(f.scale);
     qscale[q] = !a.norms ? size : norm > 0 ? size / norm : 0.0f;
-    const uint32_t id = targets[q], row = id - first_id;
-    uint32_t place = id >= first_id && row < n_rows ? row : NONE;
+    const uint32_t row = f.targets[q] - f.first_id;
+    uint32_t place = clicked_candidate(f, q, a.n_rows) ? row : NONE;
     if (a.list && place != NONE) {
-        uint32_t lo = 0, hi = *a.count;  // the first candidate that is not before the row
+        uint32_t lo = 0, hi = *a.count;  // where the row stands in the list
         while (lo < hi) {
             const uint32_t mid = (lo + hi) / 2;
             if (a.list[mid] < row)
@@ -197,7 +219,7 @@ __global__ __launch_bounds__(256) void pack_queries_kernel(XentArgs a, const Q* 
             else
                 hi = mid;
         }
-        place = lo < *a.count && a.list[lo] == row ? lo : NONE;
+        place = lo;
     }
     click[q] = place;
 }
@@ -464,18 +486,13 @@ __global__ __launch_bounds__(THREADS, 2) void loss_kernel(XentArgs a) {
                 for (int n = 0; n < S::TN; ++n) {
                     const uint32_t at = click[n] - first - local;
                     const int left = (int)min(end - first, (uint32_t)S::T) - (int)local;
-                    float clicked = 0;
 #pragma unroll
                     for (int t = 0; t < S::TM; ++t)
 #pragma unroll
                         for (int r = 0; r < 4; ++r) {
                             const uint32_t i = t * 16 + r;
-                            clicked = at == i ? acc[t][n][r] : clicked;
                             acc[t][n][r] = at == i || left <= (int)i ? -__builtin_inff() : acc[t][n][r];
                         }
-                    // (the clicked row is one of the lane's if it is 0 .. 3 rows into one of its fragments)
-                    if (click[n] != NONE && at < S::TM * 16 && at % 16 < 4)
-                        a.click_z[tile_q * BQ + (S::wave_q() * S::WQ + n) * 16 + (lane & 15)] = clicked * s2[n];
                 }
             }
 #pragma unroll
@@ -545,8 +562,7 @@ __global__ __launch_bounds__(256) void loss_few_kernel(XentArgs a, Few f) {
         for (uint32_t d = threadIdx.x; d < padded; d += 256) {
             const Piece<V> piece(d / V, a.dim);
             const uint32_t from = piece.col + d % V;
-            float x = d % V >= piece.skip && from < a.dim ? to_f32(queries[q * f.query_stride + from]) : 0.0f;
-            if (sizeof(E) == 2) x = __builtin_bit_cast(float, bf16_bits(x) << 16);
+            const float x = d % V >= piece.skip && from < a.dim ? query_element<E>(queries[q * f.query_stride + from]) : 0.0f;
             query[q * padded + d] = x;
             sq = __builtin_fmaf(x, x, sq);
         }
@@ -613,9 +629,7 @@ __global__ __launch_bounds__(256) void loss_few_kernel(XentArgs a, Few f) {
                     const float x = a.norms[r];
                     z = x > 0 ? z / x : 0.0f;
                 }
-                if (r == click) {
-                    a.click_z[mine] = z;
-                } else {
+                if (r != click) {
                     const float top = __builtin_fmaxf(m, z), ref = finite_or_zero(top);
                     l = l * __builtin_amdgcn_exp2f(m - ref) + __builtin_amdgcn_exp2f(z - ref);
                     m = top;
@@ -637,11 +651,26 @@ __global__ __launch_bounds__(256) void loss_few_kernel(XentArgs a, Few f) {
     a.part_l[(uint64_t)blockIdx.x * NQ + threadIdx.x] = sum;
 }
 
-// A query's shares joined, in 64 bits (one thread's worth of work per query); a workgroup per query.
+// A query's shares joined, in 64 bits; a workgroup per query. The clicked row's logit is made here, in 64 bits: its error
+// is that of a loss near zero, while those of the others' mostly cancel in their sum.
+template <typename E, typename Q>
 __global__ __launch_bounds__(256) void join_loss_kernel(XentArgs a, Few f, float* loss, float* lse) {
     __shared__ float tops[4];
-    __shared__ double sums[4];
+    __shared__ double sums[4][3];
     const uint32_t q = blockIdx.x, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const bool clicked = clicked_candidate(f, q, a.n_rows);
+    const uint32_t click = clicked ? f.targets[q] - f.first_id : 0;
+    double dot = 0, sq = 0;
+    if (clicked) {
+        const E* const row = static_cast<const E*>(f.rows) + click * f.stride;
+        const Q* const query = static_cast<const Q*>(f.queries) + q * f.query_stride;
+#pragma unroll 4
+        for (uint32_t d = threadIdx.x; d < a.dim; d += 256) {
+            const double x = query_element<E>(query[d]);
+            dot += x * to_f32(row[d]);
+            sq += x * x;
+        }
+    }
     float top = -__builtin_inff();
     for (uint32_t s = threadIdx.x; s < a.splits; s += 256) top = __builtin_fmaxf(top, a.part_m[(uint64_t)s * a.n_q + q]);
 #pragma unroll
@@ -656,35 +685,43 @@ __global__ __launch_bounds__(256) void join_loss_kernel(XentArgs a, Few f, float
         sum += (double)a.part_l[at] * (double)__builtin_amdgcn_exp2f(a.part_m[at] - ref);
     }
 #pragma unroll
-    for (int d = 32; d; d /= 2) sum += __shfl_xor(sum, d);
-    if (!lane) sums[wave] = sum;
+    for (int d = 32; d; d /= 2) {
+        sum += __shfl_xor(sum, d);
+        dot += __shfl_xor(dot, d);
+        sq += __shfl_xor(sq, d);
+    }
+    if (!lane) {
+        sums[wave][0] = sum;
+        sums[wave][1] = dot;
+        sums[wave][2] = sq;
+    }
     __syncthreads();
     if (threadIdx.x) return;
-    sum = (sums[0] + sums[1]) + (sums[2] + sums[3]);
+    sum = (sums[0][0] + sums[1][0]) + (sums[2][0] + sums[3][0]);
+    dot = (sums[0][1] + sums[1][1]) + (sums[2][1] + sums[3][1]);
+    sq = (sums[0][2] + sums[1][2]) + (sums[2][2] + sums[3][2]);
     constexpr double LN2 = 0.693147180559945309417;
     const double rest = ref * LN2 + log(sum);  // -inf: no other candidate
-    bool clicked;
-    if (a.click) {
-        clicked = a.click[q] != NONE;
-    } else {  // (few queries: whether the click is a candidate stands in the masks)
-        const uint32_t id = f.targets[q], row = id - f.first_id;
-        clicked = id >= f.first_id && row < a.n_rows && word_at(f.mask, f.present, row >> 6, a.n_rows) >> (row & 63) & 1;
-    }
     if (!clicked) {
         loss[q] = 0.0f;
         lse[q] = (float)rest;
         return;
     }
-    const double z = a.click_z[q] * LN2, d = rest - z;
+    double z = f.scale * dot;
+    if (a.norms) {
+        const float x = a.norms[click];
+        z = x > 0 && sq != 0 ? z / (x * sqrt(sq)) : 0.0;
+    }
+    const double d = rest - z;
     loss[q] = (float)(d > 0 ? d + log1p(exp(-d)) : log1p(exp(d)));
     lse[q] = (float)(d > 0 ? rest + log1p(exp(-d)) : z + log1p(exp(d)));
 }
 
 // ---- gradients ----------------------------------------------------------------------------
 
-// What a query's weights have in common: zero without a click.
+// What the weights of a query with a click have in common.
 __device__ __forceinline__ float query_factor(const XentArgs& a, uint32_t q) {
-    return a.click[q] != NONE ? (a.grad_loss ? a.grad_loss[q] : 1.0f) * a.qscale[q] * a.sign : 0.0f;
+    return (a.grad_loss ? a.grad_loss[q] : 1.0f) * a.qscale[q] * a.sign;
 }
 
 // The weights of the clicked rows of a piece, after weights_kernel, which takes every row alike (to look for them there
@@ -709,11 +746,11 @@ __global__ __launch_bounds__(256) void click_weights_kernel(XentArgs a) {
     for (uint32_t p = 0; p < a.g_planes; ++p) *reinterpret_cast<uint16_t*>(out + p * a.g_plane) = part[p];
 }
 
-// The weights G of a piece, [candidate][query], rounded to bf16 (PG = 1), or kept to 16 bits (2) or all 24 (3) by as many
-// planes. A lane holds four neighbouring queries of a candidate: eight bytes a store.
 template <typename S>  // fragments that go through LDS at a time: up to 64 queries of 16 candidates
 using weights_turn = Turn<8, (S::TM < 4 ? S::TM : 4)>;
 
+// The weights G of a piece, [candidate][query], rounded to bf16 (PG = 1), or kept to 16 bits (2) or all 24 (3) by as many
+// planes. A lane holds four neighbouring queries of a candidate: eight bytes a store.
 template <typename S, bool NORMS, int PG>
 __global__ __launch_bounds__(THREADS, 2) void weights_kernel(XentArgs a) {
     constexpr int BQ = S::Q_TILE;
@@ -726,10 +763,14 @@ __global__ __launch_bounds__(THREADS, 2) void weights_kernel(XentArgs a) {
     if (end <= a.piece_begin) return;
     if (threadIdx.x < BQ) {
         const uint32_t q = q0 + threadIdx.x;
-        const bool in = q < a.n_q;
+        // lse in base 2 has a rounding of its own, half a step of a number near 20: as a relative error of all of a
+        // query's weights it would be ten times the roundings of the products. What is behind it goes into the factor.
+        const bool in = q < a.n_q && a.click[q] != NONE;
+        const float lse = in ? a.lse[q] : 0.0f, high = lse * LOG2E;
+        const float low = __builtin_fmaf(lse, LOG2E, -high) + lse * LOG2E_REST;
         s2[threadIdx.x] = in ? a.qscale[q] * LOG2E : 0.0f;
-        lse2[threadIdx.x] = in ? a.lse[q] * LOG2E : 0.0f;
-        factor[threadIdx.x] = in ? query_factor(a, q) : 0.0f;
+        lse2[threadIdx.x] = high;
+        factor[threadIdx.x] = in ? query_factor(a, q) * (low == low ? __builtin_amdgcn_exp2f(-low) : 1.0f) : 0.0f;
     }
     // (the first barrier of the loop below orders these before they are read)
     // Every lane stores every time (so that the number of stores is known to the next step's barrier): rows of G are whole
@@ -761,7 +802,6 @@ __global__ __launch_bounds__(THREADS, 2) void weights_kernel(XentArgs a) {
                     for (int r = 0; r < 4; ++r) {
                         float z = acc[u * UNIT + t][n][r];
                         if constexpr (NORMS) z *= inverse[n];
-                        // (a query without a click has factor 0 and a finite lse if there is any candidate)
                         float g = vf[r] * __builtin_amdgcn_exp2f(__builtin_fmaf(z, vs[r], -vl[r]));
                         if constexpr (NORMS) g *= inverse[n];
                         if constexpr (PG == 1) {
@@ -798,7 +838,7 @@ template <int BD, typename E>
 __global__ __launch_bounds__(THREADS, 2) void row_grads_kernel(XentArgs a) {
     using A = Rows<BD>;
     using B = Rows<TILE>;
-    constexpr int WAVES_D = BD >= 256 ? 2 : 2, WAVES_R = 8 / WAVES_D;
+    constexpr int WAVES_D = 2, WAVES_R = 8 / WAVES_D;
     constexpr int TM = BD / WAVES_D / 16, TN = TILE / WAVES_R / 16;
     extern __shared__ __attribute__((aligned(128))) char lds[];
     const uint32_t wave = uniform_u32(threadIdx.x >> 6), wd = wave % WAVES_D, wr = wave / WAVES_D;
@@ -1005,11 +1045,15 @@ __global__ __launch_bounds__(THREADS, 2) void query_grads_kernel(XentArgs a) {
 
 // The shares of a query's gradient joined, and taken through the query's length where logits are cosines; one
 // workgroup per (query, 256 columns), or per query where its length is needed.
-template <typename Q, typename O>
-__global__ __launch_bounds__(256) void join_query_grads_kernel(XentArgs a, const Q* queries, uint64_t stride, bool round, O* out,
+template <typename E, typename Q, typename O>
+__global__ __launch_bounds__(256) void join_query_grads_kernel(XentArgs a, const Q* queries, uint64_t stride, O* out,
                                                                uint64_t out_stride) {
     __shared__ float sums[8];
     const uint32_t q = blockIdx.x;
+    if (a.click[q] == NONE) {
+        for (uint32_t d = blockIdx.y * 256 + threadIdx.x; d < a.dim; d += gridDim.y * 256) out[q * out_stride + d] = from_f32<O>(0.0f);
+        return;
+    }
     float* sum0 = a.part_q + (uint64_t)q * a.dim;
     float dot = 0, sq = 0;
     for (uint32_t d = blockIdx.y * 256 + threadIdx.x; d < a.dim; d += gridDim.y * 256) {
@@ -1020,8 +1064,7 @@ __global__ __launch_bounds__(256) void join_query_grads_kernel(XentArgs a, const
             out[q * out_stride + d] = from_f32<O>(sum);
             continue;
         }
-        float x = to_f32(queries[q * stride + d]);
-        if (round) x = __builtin_bit_cast(float, bf16_bits(x) << 16);
+        const float x = query_element<E>(queries[q * stride + d]);
         dot = __builtin_fmaf(sum, x, dot);
         sq = __builtin_fmaf(x, x, sq);
         sum0[d] = sum;
@@ -1038,8 +1081,7 @@ __global__ __launch_bounds__(256) void join_query_grads_kernel(XentArgs a, const
     sq = sums[4] + sums[5] + sums[6] + sums[7];
     const float along = sq > 0 ? dot / sq : 0.0f;
     for (uint32_t d = threadIdx.x; d < a.dim; d += 256) {
-        float x = to_f32(queries[q * stride + d]);
-        if (round) x = __builtin_bit_cast(float, bf16_bits(x) << 16);
+        const float x = query_element<E>(queries[q * stride + d]);
         out[q * out_stride + d] = from_f32<O>(sum0[d] - along * x);
     }
 }
@@ -1117,9 +1159,14 @@ Plan plan_for(uint32_t n_q, uint64_t n_rows, uint32_t dim, int32_t dtype) {
     return p;
 }
 
+// Workgroups of the list of candidates. Up to LIST_ALONE of them each counts the words before its own: a launch less (31
+// of them, 500 thousand rows: 13.7 us so, 9.5 with counts made first; 977, 16 million rows: 395 and 19).
+uint32_t list_blocks(uint64_t n_rows) { return (uint32_t)(((n_rows + 63) / 64 + LIST_WORDS - 1) / LIST_WORDS); }
+constexpr uint32_t LIST_ALONE = 8;
+
 struct Buffers {
-    uint32_t *zeros, *list, *count, *click;
-    float *qscale, *part_m, *part_l, *click_z, *part_q;
+    uint32_t *zeros, *list, *count, *sums, *click;
+    float *qscale, *part_m, *part_l, *part_q;
     char *q, *qt, *g, *packed, *spill;
     uint64_t bytes;
 };
@@ -1129,9 +1176,9 @@ Buffers carve(void* workspace, const Plan& p, uint32_t n_q, uint64_t n_rows, uin
     b.zeros = w.take<uint32_t>(64);
     b.list = w.take<uint32_t>(n_rows);
     b.count = w.take<uint32_t>(1);
+    b.sums = w.take<uint32_t>(list_blocks(n_rows));
     b.click = w.take<uint32_t>(n_q);
     b.qscale = w.take<float>(n_q);
-    b.click_z = w.take<float>(n_q);
     b.q = w.take<char>((uint64_t)n_q * p.kp * 2 * p.planes);
     b.qt = w.take<char>((uint64_t)dim * p.gq * 2 * p.planes);
     const uint64_t parts = n_q * (uint64_t)(few_queries(n_q, dim) ? FEW_WORKGROUPS : p.loss_splits);
@@ -1143,6 +1190,10 @@ Buffers carve(void* workspace, const Plan& p, uint32_t n_q, uint64_t n_rows, uin
     b.packed = w.take<char>(p.packed_rows * p.kp * 2 * p.planes);
     b.bytes = w.at() - (char*)workspace;
     return b;
+}
+
+Few few_of(const Xent& x) {
+    return Few{x.t.rows, x.queries, x.t.stride, x.query_stride, x.targets, x.mask, x.t.present, x.t.first_id, x.scale, 1};
 }
 
 // A call's plan, buffers and arguments.
@@ -1175,7 +1226,6 @@ struct Call {
         a.zeros = (const char*)b.zeros;
         a.part_m = b.part_m;
         a.part_l = b.part_l;
-        a.click_z = b.click_z;
         a.g = b.g;
         a.g_stride = p.q_tiles * p.bq * 2;
         a.g_planes = p.g_planes;
@@ -1185,21 +1235,20 @@ struct Call {
         if (x.mask || x.t.present) {
             a.list = b.list;
             a.count = b.count;
-            const uint64_t n_words = (x.t.n_rows + 63) / 64;
-            list_candidates_kernel<<<(uint32_t)((n_words + LIST_WORDS - 1) / LIST_WORDS), 256, 0, stream>>>(x.mask, x.t.present, x.t.n_rows, b.list, b.count);
+            const uint32_t blocks = list_blocks(x.t.n_rows), *sums = blocks > LIST_ALONE ? b.sums : nullptr;
+            if (sums) count_words_kernel<<<blocks, 256, 0, stream>>>(x.mask, x.t.present, x.t.n_rows, b.sums);
+            list_candidates_kernel<<<blocks, 256, 0, stream>>>(x.mask, x.t.present, x.t.n_rows, sums, b.list, b.count);
         }
         a.rows = packed ? Planes{b.packed, p.packed_rows * p.kp * 2, p.kp * 2, nullptr, 0, p.kp / 8}
                         : Planes{(const char*)x.t.rows, 0, (uint32_t)x.t.stride * 2, a.list, 0, dim / 8};
         const uint32_t grid = p.gq / 64 * (p.kp / 64) + (x.n_q + 3) / 4;
-        auto pack = [&](auto kernel, auto* q) {
-            kernel<<<grid, 256, 0, stream>>>(a, q, x.query_stride, x.targets, x.t.first_id, x.t.n_rows, x.scale, b.click, b.qscale, b.zeros, gradients);
-        };
+        auto pack = [&](auto kernel) { kernel<<<grid, 256, 0, stream>>>(a, few_of(x), b.click, b.qscale, b.zeros, gradients); };
         if (x.t.dtype == VS_F32)
-            pack(pack_queries_kernel<float, 3>, (const float*)x.queries);
+            pack(pack_queries_kernel<float, 3>);
         else if (x.queries_f32)
-            pack(pack_queries_kernel<float, 1>, (const float*)x.queries);
+            pack(pack_queries_kernel<float, 1>);
         else
-            pack(pack_queries_kernel<bf16, 1>, (const bf16*)x.queries);
+            pack(pack_queries_kernel<bf16, 1>);
     }
 
     // `body` for every piece of the candidates, of at most `rows`, its planes ready.
@@ -1292,11 +1341,11 @@ struct Call {
             p.bd == 256 ? query_grads<BQ, 256, false>() : query_grads<BQ, 128, false>();
     }
 
-    template <typename Q, typename O>
+    template <typename E, typename Q, typename O>
     void join_query_grads(void* out, uint64_t out_stride) {
         a.splits = p.grad_splits;
         const dim3 grid(x.n_q, a.norms ? 1 : (a.dim + 255) / 256);
-        join_query_grads_kernel<Q, O><<<grid, 256, 0, stream>>>(a, (const Q*)x.queries, x.query_stride, x.t.dtype == VS_BF16, (O*)out, out_stride);
+        join_query_grads_kernel<E, Q, O><<<grid, 256, 0, stream>>>(a, (const Q*)x.queries, x.query_stride, (O*)out, out_stride);
     }
 };
 
@@ -1308,7 +1357,7 @@ hipError_t run_loss_few(const Xent& x, XentArgs a, const Few& f, float* loss, fl
         loss_few_kernel<E, Q, V, NQ, true><<<a.splits, 256, lds, stream>>>(a, f);
     else
         loss_few_kernel<E, Q, V, NQ, false><<<a.splits, 256, lds, stream>>>(a, f);
-    join_loss_kernel<<<x.n_q, 256, 0, stream>>>(a, f, loss, lse);
+    join_loss_kernel<E, Q><<<x.n_q, 256, 0, stream>>>(a, f, loss, lse);
     return hipGetLastError();
 }
 template <typename E, typename Q, int V>
@@ -1329,8 +1378,7 @@ hipError_t launch_loss_few(const Xent& x, void* workspace, float* loss, float* l
     a.norms = x.norms;
     a.part_m = b.part_m;
     a.part_l = b.part_l;
-    a.click_z = b.click_z;
-    Few f{x.t.rows, x.queries, x.t.stride, x.query_stride, x.targets, x.mask, x.t.present, x.t.first_id, x.scale, 1};
+    Few f = few_of(x);
     // small tables: parts of a word, down to eight rows, until there is one for every wave
     while (f.parts < 8 && (x.t.n_rows + 63) / 64 * f.parts * 2 <= FEW_WORKGROUPS * 4) f.parts *= 2;
     if (x.t.dtype == VS_F32) return pick_loss_few<float, float, 4>(x, a, f, loss, lse, stream);
@@ -1364,13 +1412,19 @@ hipError_t launch_xent(const Xent& x, void* workspace, float* loss, float* lse, 
     });
     c.a.splits = c.p.loss_splits;
     if (c.error != hipSuccess) return c.error;
-    join_loss_kernel<<<x.n_q, 256, 0, stream>>>(c.a, Few{}, loss, lse);
+    auto join = [&](auto kernel) { kernel<<<x.n_q, 256, 0, stream>>>(c.a, few_of(x), loss, lse); };
+    if (x.t.dtype == VS_F32)
+        join(join_loss_kernel<float, float>);
+    else if (x.queries_f32)
+        join(join_loss_kernel<bf16, float>);
+    else
+        join(join_loss_kernel<bf16, bf16>);
     return hipGetLastError();
 }
 
 hipError_t launch_xent_grad(const Xent& x, const float* loss, const float* lse, const float* grad_loss, void* workspace,
-                            void* grad_queries, bool grad_queries_f32, uint64_t grad_query_stride, void* grad_rows,
-                            uint64_t grad_row_stride, hipStream_t stream) {
+                            void* grad_queries, uint64_t grad_query_stride, void* grad_rows, uint64_t grad_row_stride,
+                            hipStream_t stream) {
     if (!x.n_q) {
         if (grad_rows) clear_rows(x, grad_rows, grad_row_stride, true, stream);
         return hipGetLastError();
@@ -1394,11 +1448,11 @@ hipError_t launch_xent_grad(const Xent& x, const float* loss, const float* lse, 
     if (c.error != hipSuccess) return c.error;
     if (grad_queries) {
         if (f32)
-            c.join_query_grads<float, float>(grad_queries, grad_query_stride);
-        else if (grad_queries_f32)
-            c.join_query_grads<float, float>(grad_queries, grad_query_stride);
+            c.join_query_grads<float, float, float>(grad_queries, grad_query_stride);
+        else if (x.queries_f32)
+            c.join_query_grads<bf16, float, float>(grad_queries, grad_query_stride);
         else
-            c.join_query_grads<bf16, bf16>(grad_queries, grad_query_stride);
+            c.join_query_grads<bf16, bf16, bf16>(grad_queries, grad_query_stride);
     }
     return hipGetLastError();
 }
