@@ -26,6 +26,10 @@ typedef __attribute__((address_space(3))) void* lds_void;
 typedef __attribute__((address_space(1))) const void* global_void;
 typedef __attribute__((address_space(3))) s16x4* lds_s16x4;
 
+struct f32x8 {
+    f32x4 half[2];
+};
+
 constexpr uint32_t THREADS = 512;
 constexpr uint32_t STEP = 64;  // k of a step
 
@@ -95,6 +99,15 @@ struct Rows {
         const uint32_t l = threadIdx.x & 63;
         return *reinterpret_cast<const bf16x8*>(lds + (tile * 16 + (l & 15)) * 128 + (((kk * 4 + (l >> 4)) ^ (l & 7)) * 16));
     }
+    // The same of f32 elements, 32 of which are a row of LDS: a half of the step is a tile of its own.
+    __device__ __forceinline__ static f32x8 read_f32(const char* lds, uint32_t tile, int kk) {
+        const uint32_t l = threadIdx.x & 63;
+        const char* row = lds + kk * BYTES + (tile * 16 + (l & 15)) * 128;
+        f32x8 x;
+        x.half[0] = *reinterpret_cast<const f32x4*>(row + (((l >> 4) * 2) ^ (l & 7)) * 16);
+        x.half[1] = *reinterpret_cast<const f32x4*>(row + (((l >> 4) * 2 + 1) ^ (l & 7)) * 16);
+        return x;
+    }
 };
 
 // [64 k][C]: C * 2 bytes a k, chunk c of k at place c ^ turn(k).
@@ -137,6 +150,105 @@ struct Cols {
         return x.all;
     }
 };
+
+// [64 k][C] of f32: C * 4 bytes a k, chunk c of k at place c ^ turn(k): the four groups of 16 lanes that read 16 columns
+// of k, k + 8, k + 16 and k + 24 fall on different banks.
+template <int C, bool LISTED = false>
+struct FloatCols {
+    static constexpr int BYTES = C * 256;
+    static constexpr int CHUNKS = C / 4;
+    static constexpr int LOADS = CHUNKS / 8;
+    static constexpr int APART = 512 / CHUNKS;  // k between two loads of a thread
+    static_assert(APART == 16 && CHUNKS >= 16);
+    uint32_t index[LISTED ? LOADS : 1];
+    uint32_t k0, chunk;
+    __device__ __forceinline__ static uint32_t turn(uint32_t k) { return 4 * (k >> 3 & 3); }
+    __device__ __forceinline__ void init() {
+        k0 = threadIdx.x / CHUNKS;
+        chunk = (threadIdx.x % CHUNKS) ^ turn(k0);
+    }
+    __device__ __forceinline__ void peek(const Planes& p, uint32_t first, uint32_t end) {
+        if constexpr (LISTED)
+#pragma unroll
+            for (int i = 0; i < LOADS; ++i) index[i] = p.list[min(first + k0 + i * APART, end - 1)];
+    }
+    __device__ __forceinline__ void load(int i, const Planes& p, uint32_t first, uint32_t end, uint32_t first_chunk, const char* zeros,
+                                         char* lds) const {
+        const uint32_t c = first_chunk + (chunk ^ turn(i * APART)), r = first + k0 + i * APART;
+        const char* from = p.base + c * 16ull + (uint64_t)(LISTED ? index[i] : r) * p.stride;
+        load_to_lds(r < end && c < p.chunks ? from : zeros, lds + uniform_u32(threadIdx.x >> 6) * 1024 + i * 8192);
+    }
+    __device__ __forceinline__ static f32x8 read_f32(const char* lds, uint32_t tile, int kk) {
+        const uint32_t l = threadIdx.x & 63, c = tile * 16 + (l & 15);
+        const char* at = lds + (kk * 32 + (l >> 4) * 8) * (C * 4) + ((c / 4) ^ turn((l >> 4) * 8)) * 16 + c % 4 * 4;
+        f32x8 x;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x.half[i / 4][i % 4] = *reinterpret_cast<const float*>(at + i * (C * 4));
+        return x;
+    }
+};
+
+// x = planes[0] + .. exactly, three bf16.
+struct Split {
+    uint16_t h, m, l;
+};
+__device__ __forceinline__ Split split(float x) {
+    Split s;
+    s.h = (uint16_t)bf16_bits(x);
+    const float hv = __builtin_bit_cast(float, (uint32_t)s.h << 16);
+    // beyond bf16's largest number the rounding gives an infinity; of an infinity, or a NaN, nothing is left to split
+    const bool whole = !(__builtin_fabsf(hv) < __builtin_inff());
+    if (whole && __builtin_fabsf(x) < __builtin_inff()) s.h = (uint16_t)(__builtin_bit_cast(uint32_t, x) >> 16);
+    const float r = whole && !(__builtin_fabsf(x) < __builtin_inff()) ? 0.0f : x - __builtin_bit_cast(float, (uint32_t)s.h << 16);
+    s.m = (uint16_t)bf16_bits(r);
+    s.l = (uint16_t)bf16_bits(r - __builtin_bit_cast(float, (uint32_t)s.m << 16));
+    return s;
+}
+
+
+// The planes of eight elements each, with packed conversions: five and a half instructions an element. `top`: the largest
+// magnitude. Beyond the largest number of bf16 (an infinity, or near f32's largest) it takes split_all instead.
+constexpr float SPLIT_TOP = 3.38953139e38f;
+template <int N>
+__device__ __forceinline__ void split_fast(const f32x8 (&x)[N], bf16x8 (&planes)[3][N], float* top) {
+    typedef float f32x2 __attribute__((ext_vector_type(2)));
+    typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+    *top = 0;
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+        u32x4 part[3];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            float a = x[n].half[i / 2][i % 2 * 2], b = x[n].half[i / 2][i % 2 * 2 + 1];
+            *top = __builtin_fmaxf(__builtin_fmaxf(*top, __builtin_fabsf(a)), __builtin_fabsf(b));
+#pragma unroll
+            for (int p = 0; p < 3; ++p) {
+                const uint32_t both = __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2{a, b}), bf16x2));
+                part[p][i] = both;
+                a -= __builtin_bit_cast(float, both << 16);
+                b -= __builtin_bit_cast(float, both & 0xFFFF0000);
+            }
+        }
+#pragma unroll
+        for (int p = 0; p < 3; ++p) planes[p][n] = __builtin_bit_cast(bf16x8, part[p]);
+    }
+}
+template <int N>
+__device__ __forceinline__ void split_all(const f32x8 (&x)[N], bf16x8 (&planes)[3][N]) {
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+        Pack<uint16_t, 8> part[3];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const Split s = split(x[n].half[i / 4][i % 4]);
+            part[0].e[i] = s.h;
+            part[1].e[i] = s.m;
+            part[2].e[i] = s.l;
+        }
+#pragma unroll
+        for (int p = 0; p < 3; ++p) planes[p][n] = __builtin_bit_cast(bf16x8, part[p]);
+    }
+}
 
 // The products of a step: TM x TN fragments of 16 x 16 per wave, which start at fragments m0 and n0. Lane l holds rows
 // (of A) 4 (l >> 4) + 0..3 and column (of B) l & 15 of each.
@@ -190,53 +302,66 @@ struct Engine {
     }
 };
 
-// The same with all three planes of both operands in a step: six products a barrier. For few queries, whose steps are over
-// before the next one's loads have come (a step of one pair of planes takes 1.3 us then, its products 0.25): a sixth of
-// the steps, and every plane is loaded once and not twice. The largest product has a sum of its own, so that its f32
+// f32 products with all six steps of planes at once: of the one operand, which many tiles share, the planes P (P::BYTES
+// apart) are in LDS, of the other the f32 elements themselves, X, which the wave splits as it reads them. TP x TX
+// fragments; P_FIRST: P's rows are the rows of the result. The largest product has a sum of its own, so that its f32
 // roundings are not taken again with each of the smaller ones.
-template <typename A, typename B, int TM, int TN>
+template <typename P, typename X, int TP, int TX, bool P_FIRST>
 struct SplitEngine {
-    static constexpr int PHASES = 2;
-    bf16x8 fa[2][3][TM], fb[2][3][TN];
-    uint32_t m0, n0;
+    static constexpr int TM = P_FIRST ? TP : TX, TN = P_FIRST ? TX : TP;
+    bf16x8 fp[2][3][TP], planes[2][3][TX];
+    f32x8 fx[TX];
+    uint32_t p0, x0;
 
-    __device__ __forceinline__ void ask(char* a, char* b, int kk) {
+    // The fragments of the k that come next: half `kk` of P's step, and of X's the half `xk`.
+    __device__ __forceinline__ void ask(char* p, int kk, char* x, int xk) {
 #pragma unroll
-        for (int p = 0; p < 3; ++p) {
+        for (int t = 0; t < TX; ++t) fx[t] = X::read_f32(x, x0 + t, xk);
 #pragma unroll
-            for (int m = 0; m < TM; ++m) fa[kk][p][m] = A::read(a + p * A::BYTES, m0 + m, kk);
+        for (int i = 0; i < 3; ++i)
 #pragma unroll
-            for (int n = 0; n < TN; ++n) fb[kk][p][n] = B::read(b + p * B::BYTES, n0 + n, kk);
-        }
+            for (int t = 0; t < TP; ++t) fp[kk][i][t] = P::read(p + i * P::BYTES, p0 + t, kk);
         __builtin_amdgcn_sched_barrier(0);
     }
-    template <int STORES, typename F>
-    __device__ __forceinline__ void step(char* a, char* b, char* next_a, char* next_b, f32x4 (&large)[TM][TN], f32x4 (&small)[TM][TN],
-                                         uint32_t stored, F&& under_way) {
-        constexpr int PA[6] = {2, 0, 1, 1, 0, 0}, PB[6] = {0, 2, 1, 0, 1, 0};
+    // Before the first half step.
+    __device__ __forceinline__ void start(char* p, char* x) {
+        ask(p, 0, x, 0);
+        split_all(fx, planes[0]);
+    }
+    // The products of half KK of a step. `wait` lets everybody's loads of the next half have come; (p, x, xk) are that
+    // one's; `under_way` issues loads. While the matrix cores multiply, the wave splits the next half.
+    template <int KK, typename W, typename F>
+    __device__ __forceinline__ void half(W&& wait, char* p, char* x, int xk, f32x4 (&large)[TM][TN], f32x4 (&small)[TM][TN], F&& under_way) {
+        constexpr int PP[6] = {2, 0, 1, 1, 0, 0}, PX[6] = {0, 2, 1, 0, 1, 0};
+        wait();
+        ask(p, KK ^ 1, x, xk);
+        under_way();
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-        for (int kk = 0; kk < 2; ++kk) {
-            if (kk == 0) {
-                ask(a, b, 1);
-            } else {
-                if (STORES && stored)
-                    step_barrier<STORES>();
-                else
-                    step_barrier();
-                ask(next_a, next_b, 0);
-            }
-            under_way(kk);
+        for (int c = 0; c < 6; ++c)
 #pragma unroll
-            for (int c = 0; c < 6; ++c)
+            for (int i = 0; i < TP; ++i)
 #pragma unroll
-                for (int m = 0; m < TM; ++m)
+                for (int j = 0; j < TX; ++j) {
+                    const int m = P_FIRST ? i : j, n = P_FIRST ? j : i;
+                    f32x4& sum = c == 5 ? large[m][n] : small[m][n];
+                    sum = P_FIRST ? __builtin_amdgcn_mfma_f32_16x16x32_bf16(fp[KK][PP[c]][i], planes[KK][PX[c]][j], sum, 0, 0, 0)
+                                  : __builtin_amdgcn_mfma_f32_16x16x32_bf16(planes[KK][PX[c]][j], fp[KK][PP[c]][i], sum, 0, 0, 0);
+                }
+        float top;
+        split_fast(fx, planes[KK ^ 1], &top);
 #pragma unroll
-                    for (int n = 0; n < TN; ++n) {
-                        f32x4& sum = c == 5 ? large[m][n] : small[m][n];
-                        sum = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fa[kk][PA[c]][m], fb[kk][PB[c]][n], sum, 0, 0, 0);
-                    }
-            __builtin_amdgcn_sched_barrier(0);
+        for (int i = 0; i < 3; ++i)
+#pragma unroll
+            for (int t = 0; t < TX; ++t) asm("" : "+v"(planes[KK ^ 1][i][t]));  // (here, and not behind the branch below)
+        __builtin_amdgcn_sched_group_barrier(8, 4, 0);
+#pragma unroll
+        for (int i = 4; i < 6 * TP * TX; ++i) {
+            __builtin_amdgcn_sched_group_barrier(8, 1, 0);  // a matrix instruction (16 cycles, four of them to issue),
+            __builtin_amdgcn_sched_group_barrier(2, 3, 0);  // and three others meanwhile
         }
+        __builtin_amdgcn_sched_barrier(0);
+        if (__any(top > SPLIT_TOP)) split_all(fx, planes[KK ^ 1]);
     }
 };
 
@@ -287,23 +412,6 @@ struct Steps {
     __device__ __forceinline__ uint32_t plane_a(uint32_t c) const { return a >> (2 * c) & 3; }
     __device__ __forceinline__ uint32_t plane_b(uint32_t c) const { return b >> (2 * c) & 3; }
 };
-
-// x = planes[0] + .. exactly, three bf16.
-struct Split {
-    uint16_t h, m, l;
-};
-__device__ __forceinline__ Split split(float x) {
-    Split s;
-    s.h = (uint16_t)bf16_bits(x);
-    const float hv = __builtin_bit_cast(float, (uint32_t)s.h << 16);
-    // beyond bf16's largest number the rounding gives an infinity; of an infinity, or a NaN, nothing is left to split
-    const bool whole = !(__builtin_fabsf(hv) < __builtin_inff());
-    if (whole && __builtin_fabsf(x) < __builtin_inff()) s.h = (uint16_t)(__builtin_bit_cast(uint32_t, x) >> 16);
-    const float r = whole && !(__builtin_fabsf(x) < __builtin_inff()) ? 0.0f : x - __builtin_bit_cast(float, (uint32_t)s.h << 16);
-    s.m = (uint16_t)bf16_bits(r);
-    s.l = (uint16_t)bf16_bits(r - __builtin_bit_cast(float, (uint32_t)s.m << 16));
-    return s;
-}
 
 }  // namespace learn
 }  // namespace vs

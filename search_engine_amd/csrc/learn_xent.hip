@@ -14,8 +14,8 @@
 //
 // Four products on the bf16 matrix cores (learn_mma.h) carry it: rows x queries for the loss, the same again for the
 // weights G, and G with the queries and with the rows for the gradients. G is made for a piece of the rows at a time and
-// read twice before the next piece takes its place. f32 tables, and bf16 ones whose rows are not 16-byte aligned, are
-// copied piece by piece into planes first.
+// read twice before the next piece takes its place. Rows that are not whole 16-byte chunks at multiples of 16 bytes are
+// copied to such, piece by piece, first.
 #include "../../include/vs_abi.h"
 #include "learn_kernels.h"
 #include "learn_mma.h"
@@ -44,7 +44,7 @@ struct XentArgs {
     const uint32_t* click;  // [n_q] place of the clicked row among the candidates, or NONE
     const float* qscale;    // [n_q] factor of a query's products, without its sign
     float sign;
-    Steps score_steps, grad_steps;
+    Steps grad_steps;
     const char* zeros;
     uint32_t piece_begin, piece_rows;
     bool first_piece;
@@ -224,34 +224,16 @@ __global__ __launch_bounds__(256) void pack_queries_kernel(XentArgs a, Few f, ui
     click[q] = place;
 }
 
-// A piece of the candidates as planes: eight elements a thread, zeros from `dim` on.
-template <typename E, int P>
+// A piece of the candidates as rows that start at multiples of 16 bytes, zeros from `dim` on: 16 bytes a thread.
+template <typename E>
 __global__ __launch_bounds__(256) void pack_rows_kernel(XentArgs a, const E* table, uint64_t stride, char* out) {
+    constexpr int V = 16 / sizeof(E);
     const uint32_t end = min(candidates(a), a.piece_begin + a.piece_rows);
     const uint64_t total = end > a.piece_begin ? (uint64_t)(end - a.piece_begin) * a.rows.chunks : 0;
     for (uint64_t i = (uint64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (uint64_t)gridDim.x * 256) {
-        const uint32_t r = (uint32_t)(i / a.rows.chunks), d = (uint32_t)(i - (uint64_t)r * a.rows.chunks) * 8;
+        const uint32_t r = (uint32_t)(i / a.rows.chunks), d = (uint32_t)(i - (uint64_t)r * a.rows.chunks) * V;
         const E* from = table + row_at(a, a.piece_begin + r) * stride + d;
-        constexpr int V = 16 / sizeof(E);
-        float x[8];
-#pragma unroll
-        for (int h = 0; h < 8 / V; ++h) {
-            const uint32_t at = d + h * V;
-            const Pack<E, V> v = load_any<E, V>(from + h * V, at < a.dim ? a.dim - at : 0);
-#pragma unroll
-            for (int j = 0; j < V; ++j) x[h * V + j] = to_f32(v.e[j]);
-        }
-        Pack<uint16_t, 8> plane[3];
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            const Split s = split(x[j]);
-            plane[0].e[j] = s.h;
-            plane[1].e[j] = s.m;
-            plane[2].e[j] = s.l;
-        }
-#pragma unroll
-        for (int p = 0; p < P; ++p)
-            store_pack<uint16_t, 8>(reinterpret_cast<uint16_t*>(out + p * a.rows.plane + r * (uint64_t)a.rows.stride) + d, plane[p]);
+        store_pack<E, V>(reinterpret_cast<E*>(out + r * (uint64_t)a.rows.stride) + d, load_any<E, V>(from, d < a.dim ? a.dim - d : 0));
     }
 }
 
@@ -266,7 +248,8 @@ struct Scores {
     static constexpr int WAVES_R = 8 / WAVES_Q;
     static constexpr int WQ = BQ / WAVES_Q / 16, WR = TILE / WAVES_R / 16;  // fragments of a wave
     static constexpr int TM = LANES_ARE_QUERIES ? WR : WQ, TN = LANES_ARE_QUERIES ? WQ : WR;
-    static constexpr int T = TILE, Q_TILE = BQ;
+    static constexpr int T = TILE, Q_TILE = BQ, UNIT = TM < 4 ? TM : 4;  // (fragments of weights that go through LDS at a time)
+    static constexpr bool SPLIT = false;
     using R = Rows<TILE, LISTED>;
     using Q = Rows<BQ>;
     // Beside the buffers: results on their way out (16 KiB) and numbers of each query and candidate. With sixteen queries
@@ -289,30 +272,32 @@ struct Scores {
         q.aim(q0);
         const uint32_t tiles = (end - a.piece_begin + TILE - 1) / TILE;
         if (along >= tiles) return;
-        const uint32_t planes = a.score_steps.n, blocks = (a.rows.chunks + 7) / 8, steps = planes * blocks;
+        const uint32_t steps = (a.rows.chunks + 7) / 8;
+        // (the pairs of planes of a step. Where rows come through the list and results through LDS, a compiler that knows it
+        // to be one keeps addresses in registers that the sums need, and spills in the loop: 1.6 times the time)
+        const uint32_t planes = LISTED && !LANES_ARE_QUERIES ? afresh_uniform(1) : 1;
         const uint32_t base = a.piece_begin - a.place0;
         auto half_r = [&](uint32_t i) { return lds + i * (R::BYTES + Q::BYTES); };
         auto half_q = [&](uint32_t i) { return lds + i * (R::BYTES + Q::BYTES) + R::BYTES; };
         // The rows have furthest to come: theirs go first, behind a step's barrier into the buffer that it has freed; the
         // queries of that step follow in the next step's first phases. Loads go on behind the last tile, of zeros, so
-        // that their number stays what the barriers count on. (Steps are counted as queries x rows; which of the two is A
-        // does not matter to six symmetric steps.)
+        // that their number stays what the barriers count on.
         Cursor cr{0, 0, along}, cq{0, 0, along};
         r.peek(rows, base + along * TILE);
         r.aim(base + along * TILE);
         r.peek(rows, base + (along + a.splits) * TILE);
         auto load_rows = [&](uint32_t to) {
 #pragma unroll
-            for (int i = 0; i < R::LOADS; ++i) r.load(i, rows, cr.k, a.score_steps.plane_b(cr.c), a.zeros, half_r(to));
-            if (!cr.advance(planes, blocks, a.splits)) return;
+            for (int i = 0; i < R::LOADS; ++i) r.load(i, rows, cr.k, 0, a.zeros, half_r(to));
+            if (!cr.advance(planes, steps, a.splits)) return;
             r.aim(cr.tile < tiles ? base + cr.tile * TILE : NO_ROW);
             r.peek(rows, cr.tile + a.splits < tiles ? base + (cr.tile + a.splits) * TILE : 0);
         };
-        auto load_queries = [&](int i, uint32_t to) { q.load(i, a.q, cq.k, a.score_steps.plane_a(cq.c), a.zeros, half_q(to)); };
+        auto load_queries = [&](int i, uint32_t to) { q.load(i, a.q, cq.k, 0, a.zeros, half_q(to)); };
         auto load_all_queries = [&](uint32_t to) {
 #pragma unroll
             for (int i = 0; i < Q::LOADS; ++i) load_queries(i, to);
-            cq.advance(planes, blocks, a.splits);
+            cq.advance(planes, steps, a.splits);
         };
         constexpr int BEHIND = (BUFFERS - 2) * (R::LOADS + Q::LOADS);
 #pragma unroll
@@ -345,7 +330,7 @@ struct Scores {
                         for (int i = phase * EACH; i < min((phase + 1) * EACH, Q::LOADS); ++i) load_queries(i, last);
                         return;
                     }
-                    if (!(BUFFERS == 2 && STORES && early)) cq.advance(planes, blocks, a.splits);
+                    if (!(BUFFERS == 2 && STORES && early)) cq.advance(planes, steps, a.splits);
                     load_rows(at);
                     if (BUFFERS > 2 || !STORES) return;
                     // two buffers, and the tile's end stores: what the step after next needs goes before that
@@ -361,14 +346,17 @@ struct Scores {
     }
 };
 
-// f32 tables with up to 128 queries: tiles of 64 queries by 128 candidates, all planes a step.
-template <bool LANES_ARE_QUERIES>
+// f32 tables: tiles of 64 queries, as planes, by T candidates as they are in the table. Rows go by 32 k at a time (half a
+// step) through three buffers, queries by 64 through two.
+template <bool LANES_ARE_QUERIES, bool LISTED, int ROWS>
 struct SplitScores {
-    static constexpr int T = 128, Q_TILE = 64;
-    static constexpr int WAVES_Q = 2, WAVES_R = 4, WQ = 2, WR = 2, TM = 2, TN = 2;
-    using R = Rows<T>;
+    static constexpr int T = ROWS, Q_TILE = 64, UNIT = T == 256 ? 2 : 4;
+    static constexpr bool SPLIT = true;
+    static constexpr int WAVES_Q = 1, WAVES_R = 8, WQ = 4, WR = T / 128;
+    static constexpr int TM = LANES_ARE_QUERIES ? WR : WQ, TN = LANES_ARE_QUERIES ? WQ : WR;
+    using R = Rows<T, LISTED>;
     using Q = Rows<Q_TILE>;
-    static constexpr int LDS = 2 * 3 * (R::BYTES + Q::BYTES);
+    static constexpr int LDS = 3 * R::BYTES + 2 * 3 * Q::BYTES;
 
     __device__ __forceinline__ static uint32_t wave_q() { return uniform_u32(threadIdx.x >> 6) % WAVES_Q; }
     __device__ __forceinline__ static uint32_t wave_r() { return uniform_u32(threadIdx.x >> 6) / WAVES_Q; }
@@ -385,44 +373,59 @@ struct SplitScores {
         q.aim(q0);
         const uint32_t tiles = (end - a.piece_begin + T - 1) / T;
         if (along >= tiles) return;
-        const uint32_t steps = (a.rows.chunks + 7) / 8, base = a.piece_begin - a.place0;
-        auto half_r = [&](uint32_t i) { return lds + i * 3 * (R::BYTES + Q::BYTES); };
-        auto half_q = [&](uint32_t i) { return lds + i * 3 * (R::BYTES + Q::BYTES) + 3 * R::BYTES; };
-        Cursor next{0, 0, along};  // of both operands' loads
+        const uint32_t steps = (a.rows.chunks + 15) / 16, base = a.piece_begin - a.place0;
+        auto half_r = [&](uint32_t i) { return lds + i * R::BYTES; };
+        auto half_q = [&](uint32_t i) { return lds + 3 * R::BYTES + i * 3 * Q::BYTES; };
+        Cursor cr{0, 0, along}, cq{0, 0, along};
+        r.peek(rows, base + along * T);
         r.aim(base + along * T);
-        auto load = [&](uint32_t to) {
-            if (next.tile >= tiles) return;
+        r.peek(rows, base + (along + a.splits) * T);
+        auto load_rows = [&](uint32_t to) {
 #pragma unroll
-            for (int p = 0; p < 3; ++p) {
-#pragma unroll
-                for (int i = 0; i < R::LOADS; ++i) r.load(i, rows, next.k, p, a.zeros, half_r(to) + p * R::BYTES);
-                q.load(0, a.q, next.k, p, a.zeros, half_q(to) + p * Q::BYTES);
-            }
-            if (next.advance(1, steps, a.splits)) r.aim(base + next.tile * T);
+            for (int i = 0; i < R::LOADS; ++i) r.load(i, rows, cr.k, 0, a.zeros, half_r(to));
+            if (!cr.advance(1, 2 * steps, a.splits)) return;
+            r.aim(cr.tile < tiles ? base + cr.tile * T : NO_ROW);
+            r.peek(rows, cr.tile + a.splits < tiles ? base + (cr.tile + a.splits) * T : 0);
         };
-        load(0);
-        step_barrier();
-        using E = SplitEngine<std::conditional_t<LANES_ARE_QUERIES, R, Q>, std::conditional_t<LANES_ARE_QUERIES, Q, R>, TM, TN>;
-        E e;
-        e.m0 = LANES_ARE_QUERIES ? wave_r() * WR : wave_q() * WQ;
-        e.n0 = LANES_ARE_QUERIES ? wave_q() * WQ : wave_r() * WR;
-        e.ask(LANES_ARE_QUERIES ? half_r(0) : half_q(0), LANES_ARE_QUERIES ? half_q(0) : half_r(0), 0);
-        load(1);
-        uint32_t at = 0, stored = 0;
+        auto load_queries = [&](uint32_t to) {
+#pragma unroll
+            for (int p = 0; p < 3; ++p) q.load(0, a.q, cq.k, p, a.zeros, half_q(to) + p * Q::BYTES);
+            cq.advance(1, steps, a.splits);
+        };
+        // What a barrier waits for are the next half's rows, and behind a step's second half the next step's queries; what
+        // was issued after those may be under way: the rows of the half after it, and before a second half the queries.
+        load_queries(0);
+        load_rows(0);
+        load_rows(1);
+        load_queries(1);
+        load_rows(2);
+        step_barrier<3 + 2 * R::LOADS>();
+        SplitEngine<Q, R, WQ, WR, !LANES_ARE_QUERIES> e;
+        e.p0 = wave_q() * WQ;
+        e.x0 = wave_r() * WR;
+        e.start(half_q(0), half_r(0));
+        uint32_t at = 0, at_q = 0, stored = 0;
+        auto wait = [&](auto behind) {
+            if (STORES && stored)
+                step_barrier<behind + STORES>();
+            else
+                step_barrier<behind>();
+        };
 #pragma nounroll
         for (uint32_t tile = along; tile < tiles; tile += a.splits) {
             f32x4 acc[TM][TN] = {}, small[TM][TN] = {};
 #pragma nounroll
             for (uint32_t s = 0; s < steps; ++s) {
-                const uint32_t other = at ^ 1;
-                char *ar = half_r(at), *aq = half_q(at), *br = half_r(other), *bq = half_q(other);
-                // (the step after next goes into this one's half, behind the barrier: ahead of any stores of the tile's end)
-                e.template step<STORES>(LANES_ARE_QUERIES ? ar : aq, LANES_ARE_QUERIES ? aq : ar, LANES_ARE_QUERIES ? br : bq,
-                                        LANES_ARE_QUERIES ? bq : br, acc, small, stored, [&](int kk) {
-                    if (kk) load(at);
+                const uint32_t second = at == 2 ? 0 : at + 1, third = second == 2 ? 0 : second + 1, next_q = at_q ^ 1;
+                e.template half<0>([&] { wait(std::integral_constant<int, R::LOADS + 3>{}); }, half_q(at_q), half_r(second), 0, acc, small,
+                                   [&] { load_rows(at); });
+                e.template half<1>([&] { wait(std::integral_constant<int, R::LOADS>{}); }, half_q(next_q), half_r(third), 0, acc, small, [&] {
+                    load_queries(at_q);
+                    load_rows(second);
                 });
                 stored = afresh_uniform(0);
-                at = other;
+                at = third;
+                at_q = next_q;
             }
 #pragma unroll
             for (int m = 0; m < TM; ++m)
@@ -430,6 +433,7 @@ struct SplitScores {
                 for (int n = 0; n < TN; ++n) acc[m][n] += small[m][n];
             stored = afresh_uniform(done(acc, a.piece_begin + tile * T));
         }
+        __builtin_amdgcn_s_waitcnt(0x0F70);  // (as in Scores)
     }
 };
 
@@ -461,22 +465,20 @@ __global__ __launch_bounds__(THREADS, 2) void loss_kernel(XentArgs a) {
     if (end > a.piece_begin)
         S::template run<0>(a, end, tile_q * BQ, along, lds, [&](f32x4 (&acc)[S::TM][S::TN], uint32_t first) {
             if constexpr (NORMS) {
+                // (the barriers of the steps before the next tile's end let everybody have read them. Of a row of zeros the
+                // factor is not zero, which would make a number of -inf as well)
                 if (threadIdx.x < S::T) {
                     const float x = first + threadIdx.x < end ? a.norms[row_at(a, first + threadIdx.x)] : 0.0f;
-                    inverse[threadIdx.x] = x > 0 ? 1.0f / x : 0.0f;
+                    inverse[threadIdx.x] = x > 0 ? 1.0f / x : 1e-37f;
                 }
                 __syncthreads();
             }
             const uint32_t local = S::wave_r() * S::WR * 16 + group * 4;  // of the lane's candidates t * 16 + r
-            if constexpr (NORMS) {
-#pragma unroll
-                for (int t = 0; t < S::TM; ++t) {
-                    const f32x4 inv = *reinterpret_cast<const f32x4*>(inverse + local + t * 16);
-#pragma unroll
-                    for (int n = 0; n < S::TN; ++n) acc[t][n] *= inv;
-                }
-                __syncthreads();  // (the next tile writes them)
-            }
+            // (multiplied where they are used: the products themselves stay in the matrix cores' registers)
+            auto length = [&](int t) {
+                if constexpr (NORMS) return *reinterpret_cast<const f32x4*>(inverse + local + t * 16);
+                return f32x4{1, 1, 1, 1};
+            };
             bool special = end - first < S::T;
 #pragma unroll
             for (int n = 0; n < S::TN; ++n) special |= click[n] - first < S::T;
@@ -497,18 +499,22 @@ __global__ __launch_bounds__(THREADS, 2) void loss_kernel(XentArgs a) {
             }
 #pragma unroll
             for (int n = 0; n < S::TN; ++n) {
-                float x = acc[0][n][0];
+                float x = -__builtin_inff();
 #pragma unroll
-                for (int t = 0; t < S::TM; ++t)
+                for (int t = 0; t < S::TM; ++t) {
+                    const f32x4 z = NORMS ? acc[t][n] * length(t) : acc[t][n];
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) x = __builtin_fmaxf(x, acc[t][n][r]);
+                    for (int r = 0; r < 4; ++r) x = __builtin_fmaxf(x, z[r]);
+                }
                 const float top = __builtin_fmaxf(m[n], x * s2[n]);  // (the factor is not negative)
                 const float ref = finite_or_zero(top);
                 float sum[4] = {l[n] * __builtin_amdgcn_exp2f(m[n] - ref), 0, 0, 0};
 #pragma unroll
-                for (int t = 0; t < S::TM; ++t)
+                for (int t = 0; t < S::TM; ++t) {
+                    const f32x4 z = NORMS ? acc[t][n] * length(t) : acc[t][n];
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) sum[r] += __builtin_amdgcn_exp2f(__builtin_fmaf(acc[t][n][r], s2[n], -ref));
+                    for (int r = 0; r < 4; ++r) sum[r] += __builtin_amdgcn_exp2f(__builtin_fmaf(z[r], s2[n], -ref));
+                }
                 l[n] = (sum[0] + sum[1]) + (sum[2] + sum[3]);
                 m[n] = top;
             }
@@ -746,8 +752,8 @@ __global__ __launch_bounds__(256) void click_weights_kernel(XentArgs a) {
     for (uint32_t p = 0; p < a.g_planes; ++p) *reinterpret_cast<uint16_t*>(out + p * a.g_plane) = part[p];
 }
 
-template <typename S>  // fragments that go through LDS at a time: up to 64 queries of 16 candidates
-using weights_turn = Turn<8, (S::TM < 4 ? S::TM : 4)>;
+template <typename S>
+using weights_turn = Turn<8, S::UNIT>;
 
 // The weights G of a piece, [candidate][query], rounded to bf16 (PG = 1), or kept to 16 bits (2) or all 24 (3) by as many
 // planes. A lane holds four neighbouring queries of a candidate: eight bytes a store.
@@ -775,7 +781,7 @@ __global__ __launch_bounds__(THREADS, 2) void weights_kernel(XentArgs a) {
     // (the first barrier of the loop below orders these before they are read)
     // Every lane stores every time (so that the number of stores is known to the next step's barrier): rows of G are whole
     // tiles of queries, and G is whole tiles of candidates.
-    constexpr int UNIT = S::TM < 4 ? S::TM : 4;
+    constexpr int UNIT = S::UNIT;
     using T = weights_turn<S>;
     char* const wave_lds = lds + S::LDS + uniform_u32(threadIdx.x >> 6) * T::BYTES;
     S::template run<S::TN * (S::TM / UNIT) * T::STORES * PG>(a, end, q0, along, lds, [&](f32x4 (&acc)[S::TM][S::TN], uint32_t first) {
@@ -1043,6 +1049,97 @@ __global__ __launch_bounds__(THREADS, 2) void query_grads_kernel(XentArgs a) {
         }
 }
 
+// The same of an f32 table: G's planes by the rows as they are.
+constexpr int FLOAT_BD = 128;
+template <int BQ, bool LISTED>
+constexpr int float_grads_row_buffers = LISTED || BQ > 64 ? 2 : 3;
+template <int BQ, bool LISTED>
+__global__ __launch_bounds__(THREADS, 2) void float_query_grads_kernel(XentArgs a) {
+    using A = Cols<BQ>;
+    using B = FloatCols<FLOAT_BD, LISTED>;
+    constexpr int WAVES_Q = 2, WAVES_D = 8 / WAVES_Q;
+    constexpr int TM = BQ / WAVES_Q / 16, TN = FLOAT_BD / WAVES_D / 16;
+    constexpr int ROW_BUFFERS = float_grads_row_buffers<BQ, LISTED>;
+    extern __shared__ __attribute__((aligned(128))) char lds[];
+    const uint32_t lane = threadIdx.x & 63, wave = uniform_u32(threadIdx.x >> 6), wq = wave % WAVES_Q, wd = wave / WAVES_Q;
+    const uint32_t d_tiles = (a.dim + FLOAT_BD - 1) / FLOAT_BD;
+    uint32_t tile, share;
+    place_of_workgroup(a.across, a.splits, &tile, &share);
+    const uint32_t tile_d = tile % d_tiles, tile_q = tile / d_tiles;
+    const uint32_t end = min(candidates(a), a.piece_begin + a.piece_rows);
+    const uint32_t n = end > a.piece_begin ? end - a.piece_begin : 0;
+    const uint32_t per = ((n + STEP - 1) / STEP + a.splits - 1) / a.splits * STEP;
+    const uint32_t begin = (uint32_t)min((uint64_t)share * per, (uint64_t)n), stop = min(begin + per, n);
+    f32x4 acc[TM][TN] = {}, small[TM][TN] = {};
+    const uint32_t steps = (stop - begin + STEP - 1) / STEP;
+    if (steps) {
+        const Planes g{a.g, a.g_plane, a.g_stride, nullptr, n, a.gq / 8};
+        Planes rows = a.rows;
+        rows.rows = end - a.place0;
+        const uint32_t base = a.piece_begin - a.place0;
+        A w;
+        B r;
+        w.init();
+        r.init();
+        auto half_r = [&](uint32_t i) { return lds + i * B::BYTES; };
+        auto half_g = [&](uint32_t i) { return lds + ROW_BUFFERS * B::BYTES + i * 3 * A::BYTES; };
+        uint32_t kr = begin, kg = begin;
+        auto load_rows = [&](uint32_t to) {
+#pragma unroll
+            for (int i = 0; i < B::LOADS; ++i) r.load(i, rows, base + kr, base + stop, tile_d * (FLOAT_BD / 4), a.zeros, half_r(to));
+            kr += STEP;
+            r.peek(rows, base + kr, base + stop);  // while this step multiplies
+        };
+        auto load_weights = [&](uint32_t to) {
+#pragma unroll
+            for (int p = 0; p < 3; ++p)
+#pragma unroll
+                for (int i = 0; i < A::LOADS; ++i) w.load(i, g, kg, stop, tile_q * (BQ / 8), p, a.zeros, half_g(to) + p * A::BYTES);
+            kg += STEP;
+        };
+        constexpr int BEHIND = (ROW_BUFFERS - 2) * B::LOADS;
+        r.peek(rows, base + begin, base + stop);
+        load_weights(0);
+        load_rows(0);
+        load_weights(1);
+        load_rows(1);
+        step_barrier<3 * A::LOADS + B::LOADS>();
+        SplitEngine<A, B, TM, TN, true> e;
+        e.p0 = wq * TM;
+        e.x0 = wd * TN;
+        e.start(half_g(0), half_r(0));
+        if (ROW_BUFFERS > 2) load_rows(2);
+        uint32_t at_r = 0, at_g = 0;
+#pragma nounroll
+        for (uint32_t s = 0; s < steps; ++s) {
+            const uint32_t next_r = at_r + 1 == ROW_BUFFERS ? 0 : at_r + 1, next_g = at_g ^ 1;
+            e.template half<0>([] {}, half_g(at_g), half_r(at_r), 1, acc, small, [] {});
+            e.template half<1>([] { step_barrier<BEHIND>(); }, half_g(next_g), half_r(next_r), 0, acc, small, [&] {
+                load_weights(at_g);
+                load_rows(at_r);
+            });
+            at_r = next_r;
+            at_g = next_g;
+        }
+        __builtin_amdgcn_s_waitcnt(0x0F70);
+    }
+#pragma unroll
+    for (int m = 0; m < TM; ++m)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const uint32_t q = tile_q * BQ + (wq * TM + m) * 16 + (lane >> 4) * 4 + i;
+            if (q >= a.n_q) continue;
+#pragma unroll
+            for (int t = 0; t < TN; ++t) {
+                const uint32_t d = tile_d * FLOAT_BD + (wd * TN + t) * 16 + (lane & 15);
+                if (d >= a.dim) continue;
+                float* p = a.part_q + ((uint64_t)share * a.n_q + q) * a.dim + d;
+                const float sum = acc[m][t][i] + small[m][t][i];
+                *p = a.first_piece ? sum : *p + sum;
+            }
+        }
+}
+
 // The shares of a query's gradient joined, and taken through the query's length where logits are cosines; one
 // workgroup per (query, 256 columns), or per query where its length is needed.
 template <typename E, typename Q, typename O>
@@ -1112,7 +1209,7 @@ constexpr Steps ONE{1, 0, 0}, TWO{2, 0u | 1u << 2, 0};
 bool few_queries(uint32_t n_q, uint32_t dim) { return n_q <= 4 && n_q * (uint64_t)dim <= 12288; }
 
 struct Plan {
-    uint32_t planes, g_planes, kp, gq, loss_bq, score_bq, bq, bd, q_tiles, loss_q_tiles, score_q_tiles, d_tiles;
+    uint32_t planes, g_planes, kp, gq, loss_bq, score_bq, score_rows, bq, bd, q_tiles, loss_q_tiles, score_q_tiles, d_tiles, grad_d_tiles;
     uint32_t loss_splits, weight_splits, row_splits, grad_splits;
     uint64_t piece_rows, packed_rows;
 };
@@ -1134,14 +1231,15 @@ Plan plan_for(uint32_t n_q, uint64_t n_rows, uint32_t dim, int32_t dtype) {
     p.g_planes = dtype == VS_F32 ? 3 : n_q <= 64 ? 2 : 1;
     p.kp = (uint32_t)round_up(dim, 64);
     p.gq = (uint32_t)round_up(n_q, 64);
-    p.bq = n_q <= 64 ? 64 : n_q <= 128 ? 128 : 256;
-    p.score_bq = dtype == VS_F32 && n_q <= 128 ? 64 : p.bq;
+    p.bq = n_q <= 64 ? 64 : n_q <= 128 || dtype == VS_F32 ? 128 : 256;
+    p.score_bq = dtype == VS_F32 ? 64 : p.bq;
     p.loss_bq = dtype == VS_F32 || n_q > 16 ? p.score_bq : 16;
     p.bd = (dim + 127) / 128 % 2 ? 128 : 256;
     p.loss_q_tiles = (n_q + p.loss_bq - 1) / p.loss_bq;
     p.score_q_tiles = (n_q + p.score_bq - 1) / p.score_bq;
     p.q_tiles = (n_q + p.bq - 1) / p.bq;
     p.d_tiles = (dim + p.bd - 1) / p.bd;
+    p.grad_d_tiles = dtype == VS_F32 ? (dim + FLOAT_BD - 1) / FLOAT_BD : p.d_tiles;
     const uint64_t rows = round_up(n_rows, TILE), per = TILE * (uint64_t)WORKGROUPS;
     auto piece = [&](uint64_t row_bytes) {
         uint64_t r = std::max<uint64_t>(PIECE_BYTES / row_bytes / TILE * TILE, TILE);
@@ -1149,13 +1247,14 @@ Plan plan_for(uint32_t n_q, uint64_t n_rows, uint32_t dim, int32_t dtype) {
         return std::min(r, rows);
     };
     p.piece_rows = piece((uint64_t)p.q_tiles * p.bq * 2 * p.g_planes);
-    p.packed_rows = std::min(p.piece_rows, piece((uint64_t)p.kp * 2 * p.planes));
+    p.packed_rows = std::min(p.piece_rows, piece((uint64_t)p.kp * (dtype == VS_F32 ? 4 : 2)));
     const uint64_t tiles = rows / TILE;
-    const uint64_t score_tiles = dtype == VS_F32 && n_q <= 128 ? rows / SplitScores<true>::T : tiles;
+    p.score_rows = dtype == VS_F32 && p.score_q_tiles * tiles < 2 * WORKGROUPS ? 128 : TILE;
+    const uint64_t score_tiles = rows / p.score_rows;
     p.loss_splits = splits_for(p.loss_q_tiles, score_tiles);
     p.weight_splits = splits_for(p.score_q_tiles, score_tiles);
     p.row_splits = splits_for(p.d_tiles, tiles);
-    p.grad_splits = splits_for(p.q_tiles * p.d_tiles, tiles * (TILE / STEP));
+    p.grad_splits = splits_for(p.q_tiles * p.grad_d_tiles, tiles * (TILE / STEP));
     return p;
 }
 
@@ -1187,7 +1286,7 @@ Buffers carve(void* workspace, const Plan& p, uint32_t n_q, uint64_t n_rows, uin
     b.g = w.take<char>(p.piece_rows * p.q_tiles * p.bq * 2 * p.g_planes);
     b.spill = w.take<char>(16ull * THREADS * WORKGROUPS);
     b.part_q = w.take<float>((uint64_t)p.grad_splits * n_q * dim);
-    b.packed = w.take<char>(p.packed_rows * p.kp * 2 * p.planes);
+    b.packed = w.take<char>(p.packed_rows * p.kp * (p.planes == 3 ? 4 : 2));
     b.bytes = w.at() - (char*)workspace;
     return b;
 }
@@ -1210,7 +1309,8 @@ struct Call {
         : x(x_), p(plan_for(x.n_q, x.t.n_rows, x.t.dim, x.t.dtype)), b(carve(workspace, p, x.n_q, x.t.n_rows, x.t.dim)), stream(stream_) {
         const uint32_t dim = x.t.dim;
         // straight from the table where a row is whole 16-byte chunks at multiples of 16 bytes
-        packed = x.t.dtype == VS_F32 || (uintptr_t)x.t.rows % 16 || x.t.stride % 8 || x.t.stride * 2 > 0xFFFFFFFFu || dim % 8;
+        const uint32_t size = x.t.dtype == VS_F32 ? 4 : 2, chunk = 16 / size;
+        packed = (uintptr_t)x.t.rows % 16 || x.t.stride % chunk || x.t.stride * size > 0xFFFFFFFFu || dim % chunk;
         a.n_rows = x.t.n_rows;
         a.norms = x.norms;
         a.q = Planes{b.q, (uint64_t)x.n_q * p.kp * 2, p.kp * 2, nullptr, x.n_q, p.kp / 8};
@@ -1221,7 +1321,6 @@ struct Call {
         a.click = b.click;
         a.qscale = b.qscale;
         a.sign = x.scale < 0 ? -1.0f : 1.0f;
-        a.score_steps = p.planes == 3 ? SIX : ONE;
         a.grad_steps = p.planes == 3 ? SIX : p.g_planes == 2 ? TWO : ONE;
         a.zeros = (const char*)b.zeros;
         a.part_m = b.part_m;
@@ -1239,8 +1338,8 @@ struct Call {
             if (sums) count_words_kernel<<<blocks, 256, 0, stream>>>(x.mask, x.t.present, x.t.n_rows, b.sums);
             list_candidates_kernel<<<blocks, 256, 0, stream>>>(x.mask, x.t.present, x.t.n_rows, sums, b.list, b.count);
         }
-        a.rows = packed ? Planes{b.packed, p.packed_rows * p.kp * 2, p.kp * 2, nullptr, 0, p.kp / 8}
-                        : Planes{(const char*)x.t.rows, 0, (uint32_t)x.t.stride * 2, a.list, 0, dim / 8};
+        a.rows = packed ? Planes{b.packed, 0, p.kp * size, nullptr, 0, p.kp / chunk}
+                        : Planes{(const char*)x.t.rows, 0, (uint32_t)x.t.stride * size, a.list, 0, dim / chunk};
         const uint32_t grid = p.gq / 64 * (p.kp / 64) + (x.n_q + 3) / 4;
         auto pack = [&](auto kernel) { kernel<<<grid, 256, 0, stream>>>(a, few_of(x), b.click, b.qscale, b.zeros, gradients); };
         if (x.t.dtype == VS_F32)
@@ -1268,9 +1367,9 @@ struct Call {
         const uint64_t threads = (uint64_t)a.piece_rows * a.rows.chunks;
         const uint32_t grid = (uint32_t)std::min<uint64_t>((threads + 255) / 256, 1u << 16);
         if (x.t.dtype == VS_F32)
-            pack_rows_kernel<float, 3><<<grid, 256, 0, stream>>>(a, (const float*)x.t.rows, x.t.stride, b.packed);
+            pack_rows_kernel<float><<<grid, 256, 0, stream>>>(a, (const float*)x.t.rows, x.t.stride, b.packed);
         else
-            pack_rows_kernel<bf16, 1><<<grid, 256, 0, stream>>>(a, (const bf16*)x.t.rows, x.t.stride, b.packed);
+            pack_rows_kernel<bf16><<<grid, 256, 0, stream>>>(a, (const bf16*)x.t.rows, x.t.stride, b.packed);
     }
 
     // A product over the tiles of the piece.
@@ -1286,7 +1385,15 @@ struct Call {
     template <int BQ, bool LANES_ARE_QUERIES, typename F>
     void with_scores(F&& f) {
         auto by_norms = [&](auto scores) { a.norms ? f(scores, std::true_type{}) : f(scores, std::false_type{}); };
-        if (BQ == 64 && p.planes == 3) return by_norms(SplitScores<LANES_ARE_QUERIES>{});
+        if constexpr (BQ == 64)
+            if (p.planes == 3) {
+                if (p.score_rows == 256) {
+                    if (a.rows.list) return by_norms(SplitScores<LANES_ARE_QUERIES, true, 256>{});
+                    return by_norms(SplitScores<LANES_ARE_QUERIES, false, 256>{});
+                }
+                if (a.rows.list) return by_norms(SplitScores<LANES_ARE_QUERIES, true, 128>{});
+                return by_norms(SplitScores<LANES_ARE_QUERIES, false, 128>{});
+            }
         if (a.rows.list) return by_norms(Scores<BQ, LANES_ARE_QUERIES, true>{});
         by_norms(Scores<BQ, LANES_ARE_QUERIES, false>{});
     }
@@ -1303,17 +1410,15 @@ struct Call {
     void weights() {
         with_scores<BQ, false>([&](auto scores, auto norms) {
             using S = decltype(scores);
-            // (f32 rows are never read through the list, and take all planes a step where BQ is 64; bf16 rows have one)
-            constexpr bool SPLIT = std::is_same_v<S, SplitScores<false>>, LISTED = std::is_same_v<S, Scores<BQ, false, true>>;
-            if constexpr (PG == 3 ? SPLIT || (BQ == 256 && !LISTED) : !SPLIT)
+            // (three planes of weights are an f32 table's)
+            if constexpr ((PG == 3) == S::SPLIT)
                 product(weights_kernel<S, norms, PG>, S::LDS + 8 * weights_turn<S>::BYTES, p.score_q_tiles, p.weight_splits);
         });
     }
     template <int BQ>
     void weights() {
-        if (p.planes == 3) return weights<BQ, 3>();
         if constexpr (BQ == 64)
-            weights<BQ, 2>();
+            p.planes == 3 ? weights<BQ, 3>() : weights<BQ, 2>();
         else
             weights<BQ, 1>();
     }
@@ -1339,6 +1444,16 @@ struct Call {
             p.bd == 256 ? query_grads<BQ, 256, true>() : query_grads<BQ, 128, true>();
         else
             p.bd == 256 ? query_grads<BQ, 256, false>() : query_grads<BQ, 128, false>();
+    }
+    template <int BQ>
+    void float_query_grads() {
+        auto run = [&](auto kernel, int row_buffers) {
+            product(kernel, 2 * 3 * Cols<BQ>::BYTES + row_buffers * FloatCols<FLOAT_BD>::BYTES, p.q_tiles * p.grad_d_tiles, p.grad_splits);
+        };
+        if (a.rows.list)
+            run(float_query_grads_kernel<BQ, true>, float_grads_row_buffers<BQ, true>);
+        else
+            run(float_query_grads_kernel<BQ, false>, float_grads_row_buffers<BQ, false>);
     }
 
     template <typename E, typename Q, typename O>
@@ -1443,6 +1558,7 @@ hipError_t launch_xent_grad(const Xent& x, const float* loss, const float* lse, 
         if (c.error == hipSuccess) click_weights_kernel<<<(x.n_q + 255) / 256, 256, 0, stream>>>(c.a);
         if (grad_rows) f32 ? c.row_grads<float>() : c.row_grads<bf16>();
         if (!grad_queries) return;
+        if (f32) return c.p.bq == 64 ? c.float_query_grads<64>() : c.float_query_grads<128>();
         c.p.bq == 64 ? c.query_grads<64>() : c.p.bq == 128 ? c.query_grads<128>() : c.query_grads<256>();
     });
     if (c.error != hipSuccess) return c.error;
