@@ -466,8 +466,10 @@ int32_t vs_search_sharded_device(vs_group* g, vs_store* s, const void* d_queries
  *     says, private to the call until the stream has passed it (two graphs that may
  *     run at once need one each); VS_E_CAPACITY if workspace_bytes is less;
  *   - types are VS_F32 or VS_BF16; a stride counts elements from one row to the
- *     next, at least `dim`; rows of 16-byte aligned length and address run fastest,
- *     any other length and alignment (of one element) is served;
+ *     next, at least `dim`; rows whose address, stride and length are multiples of 16
+ *     bytes run fastest, any other length and alignment (of one element) is served;
+ *   - outputs share no memory with inputs, with each other or with the workspace
+ *     (but for rows that vs_lookup_grad_device adds to);
  *   - an id that names no row (VS_ROW_NONE, any id from n_rows on, in a store any
  *     document that is not in it) adds nothing and gets no gradient;
  *   - sums are f32 or wider, in an order that depends on the sizes alone: a call
@@ -531,11 +533,14 @@ int32_t vs_lookup_grad_weights_device(vs_ctx* ctx, const void* d_rows, int32_t d
  * zero keeps its relative precision.
  *   d_queries:    n_q <= VS_XENT_MAX_QUERIES rows of `dtype`
  *   d_targets:    the clicked row of each query. A query whose click is no candidate
- *                 (VS_ROW_NONE; outside the filter) has loss 0 and gradients 0; its
- *                 lse is that of the candidates (-inf if there are none)
+ *                 (VS_ROW_NONE; outside the filter) has loss 0 and gradients 0,
+ *                 whatever it holds (padding of a batch); its lse is that of the
+ *                 candidates (-inf if there are none)
  *   d_mask_words: candidate words as in the searches, bit r & 63 of word r >> 6,
  *                 ceil(n_rows / 64) words; NULL = every row. Rows that are no
- *                 candidates are not read. */
+ *                 candidates are not read
+ * A candidate row, or a query with a click, that holds an infinity or a NaN gives no
+ * number in what it takes part in. */
 int32_t vs_xent_workspace_bytes(vs_ctx* ctx, uint32_t n_q, uint64_t n_rows, uint32_t dim,
                                 int32_t dtype, uint64_t* bytes);
 int32_t vs_xent_device(vs_ctx* ctx, const void* d_queries, uint32_t n_q, uint64_t query_stride,
@@ -548,9 +553,10 @@ int32_t vs_xent_device(vs_ctx* ctx, const void* d_queries, uint32_t n_q, uint64_
  *   d_grad_queries: laid out as d_queries (same type and stride), or NULL
  *   d_grad_rows:    laid out as d_rows, every row written (zeros for a row that is no
  *                   candidate; between rows nothing is written), or NULL
- * The products are recomputed, a piece of the rows at a time. With VS_BF16 the
- * weights exp(z - lse) are rounded to bf16 before they multiply queries and rows, as
- * those are; sums stay f32 and each gradient is rounded once. */
+ * The products are recomputed, a piece of the rows at a time. With VS_BF16 and more
+ * than 64 queries the weights exp(z - lse) are rounded to bf16 before they multiply
+ * queries and rows, as those are (with up to 64 they keep 16 bits); sums stay f32 and
+ * each gradient is rounded once. */
 int32_t vs_xent_grad_device(vs_ctx* ctx, const void* d_queries, uint32_t n_q, uint64_t query_stride,
                             const void* d_rows, uint64_t n_rows, uint64_t row_stride, int32_t dtype,
                             uint32_t dim, const uint32_t* d_targets, const uint64_t* d_mask_words,

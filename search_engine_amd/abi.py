@@ -19,7 +19,7 @@ VS_MAX_K = 1024
 VS_GROUP_ID_BYTES = 128
 VS_SHARDED_SHARE_PASSES, VS_SHARDED_ALWAYS_GATHER = 1, 2
 VS_ROW_NONE = 0xFFFFFFFF
-VS_LEARN_MAX_DIM, VS_XENT_MAX_QUERIES, VS_LOOKUP_MAX_IDS = 8192, 65536, 1 << 24
+VS_LEARN_MAX_DIM, VS_LEARN_MAX_ROWS, VS_XENT_MAX_QUERIES, VS_LOOKUP_MAX_IDS = 8192, 1 << 31, 65536, 1 << 24
 
 # VS_AMD_LIB names another build of the same library (measurement variants of the tools)
 LIB_PATH = os.environ.get("VS_AMD_LIB") or os.path.join(os.path.dirname(os.path.abspath(__file__)), "libvs_amd.so")

@@ -81,7 +81,8 @@ __device__ __forceinline__ void store_out(const LookupArgs& a, uint64_t bag, con
 }
 
 // One thread per (bag, V columns): a wave reads 64 neighbouring pieces of a row (1 KiB of 16-byte pieces), and no lane
-// idles whatever the row's length.
+// idles whatever the row's length. 16384 bags of 0 to 40 of 1M x 768 bf16: 100 us, 5.0 TB/s of rows (popular ones come from
+// cache); one bag of three: 3.5 us, two trips to memory.
 template <typename E, typename O, int V>
 __global__ __launch_bounds__(256) void lookup_kernel(LookupArgs a) {
     const uint64_t total = a.b.n_bags * a.chunks;
@@ -132,7 +133,8 @@ hipError_t run_lookup(LookupArgs a, hipStream_t stream) {
     const uint64_t threads = a.b.n_bags * a.chunks;
     const uint64_t blocks = (a.chunks + 63) / 64;
     // With one thread per piece a bag of n ids takes n / 4 trips to memory; fewer threads than an eighth of what the
-    // card holds (512 K) leave most of it idle meanwhile. Splitting pays once a bag has more ids than the 16 waves.
+    // card holds (512 K) leave most of it idle meanwhile. Splitting pays once a bag has more ids than the 16 waves (4 bags of
+    // up to 500, 768 f32: 13 us, 130 without; 64 of up to 40, 768 bf16: 5.4 and 14).
     if (threads < 65536 && a.b.n_ids > 16 * a.b.n_bags && a.b.n_bags * blocks < (1u << 20))
         lookup_split_kernel<E, O, V><<<(uint32_t)(a.b.n_bags * blocks), 1024, 0, stream>>>(a);
     else
@@ -204,7 +206,8 @@ __device__ __forceinline__ uint32_t key_of(const GradArgs& a, uint32_t p) {
 
 // Up to SMALL ids: entry p's place is the number of entries that sort before it, counted against all of them in LDS,
 // four threads an entry and four comparisons a read. One launch, where the passes below are nine. The offsets are
-// searched in LDS too: from memory, each step of a search would wait for the one before it.
+// searched in LDS too: from memory, each step of a search would wait for the one before it. 160 ids: 5 us and the sums 5,
+// by the passes 72 in all; 2000 ids: 24 and 13, by the passes 105.
 __global__ __launch_bounds__(256) void rank_sort_kernel(GradArgs a) {
     __shared__ __align__(16) uint32_t keys[SMALL];
     __shared__ uint32_t offsets[SMALL + 1];
@@ -233,7 +236,7 @@ __global__ __launch_bounds__(256) void rank_sort_kernel(GradArgs a) {
     reinterpret_cast<float*>(a.keys[1])[place] = a.b.weights ? a.b.weights[p] : 1.0f;
 }
 
-// A stable pass by 8 bits: counts of each digit in each tile ...
+// A stable pass by 8 bits (328 thousand ids: 19 us, of launches mostly): counts of each digit in each tile ...
 __global__ __launch_bounds__(256) void sort_count_kernel(GradArgs a, int pass, uint32_t n_tiles) {
     __shared__ uint32_t hist[256];
     hist[threadIdx.x] = 0;
@@ -404,7 +407,8 @@ __global__ __launch_bounds__(256) void sum_small_kernel(GradArgs a) {
 // Many ids: one thread per (RUN sorted entries, V columns) walks its entries in order, eight gradients in flight. A
 // row's run that lies within them is stored; what belongs to a run that began before or goes on behind is handed over
 // in `partial`: [0] the run that was open at the first entry, [1] the one that is still open at the last (a run
-// through all of them: [0] alone).
+// through all of them: [0] alone). 328 thousand gradients of 768 bf16, summed to 190 thousand f32 rows: 214 us, 5.1 TB/s of
+// what is read (from cache) and written; entries are walked in order, so a thread waits for the eight it has asked for.
 template <typename E, typename O, int V>
 __global__ __launch_bounds__(256) void sum_runs_kernel(GradArgs a, int side) {
     constexpr int U = 8;
@@ -480,8 +484,8 @@ __global__ __launch_bounds__(256) void sum_runs_kernel(GradArgs a, int side) {
     hand_over(end < a.n && keys[end] == row);
 }
 
-// The runs that were handed over: a workgroup per (piece where one began, 64 pieces of columns); four waves take every
-// fourth part each.
+// The runs that were handed over (of 328 thousand ids: 32 us): a workgroup per (piece where one began, 64 pieces of
+// columns); four waves take every fourth part each.
 template <typename O, int V>
 __global__ __launch_bounds__(256) void join_runs_kernel(GradArgs a, int side) {
     __shared__ float part[4][V][64];
@@ -526,7 +530,8 @@ __global__ __launch_bounds__(256) void join_runs_kernel(GradArgs a, int side) {
 }
 
 // A wave takes `span` neighbouring positions (64 at most: a lane looks up the row and the bag of each), four at a time:
-// the products of each one's row with its bag's gradient, in pieces of V columns, joined over the lanes.
+// the products of each one's row with its bag's gradient, in pieces of V columns, joined over the lanes. 328 thousand of 768
+// bf16: 133 us, 3.8 TB/s of rows and as much of gradients, which come from cache.
 struct WeightArgs {
     Table t;
     Bags b;

@@ -5,11 +5,12 @@
 // cores work on another: one barrier a step. 64 KiB a step (256 x 256), twice, are 128 of the 160 KiB of a CU; smaller
 // tiles, whose steps are over sooner than memory answers, have up to four buffers and load as many steps ahead.
 //
-// Operands come in two shapes:
+// Operands come in three shapes:
 //   Rows<R>  [R rows][64 k], k contiguous: read as one ds_read_b128 a fragment;
 //   Cols<C>  [64 k][C columns], columns contiguous (the sum runs over memory rows): read with the transposing
-//            ds_read_b64_tr_b16, four k x 16 columns per 16 lanes.
-// Both keep their 16-byte chunks rotated by XOR with the row, so that the lanes of a read fall on different banks.
+//            ds_read_b64_tr_b16, four k x 16 columns per 16 lanes;
+//   FloatCols<C>  the same of f32 elements, read one by one.
+// All keep their 16-byte chunks rotated by XOR with the row, so that the lanes of a read fall on different banks.
 //
 // f32 operands are three bf16 planes: x = h + m + l exactly (8 + 8 + 8 bits), and a product takes the six steps hh, hm, mh,
 // mm, hl, lh; what is left out (ml, lm, ll) is below 2^-23 of hh. Six steps on the bf16 cores are 2.7 times as fast as the
@@ -69,7 +70,7 @@ __device__ __forceinline__ void step_barrier() {
 template <int R, bool LISTED = false>
 struct Rows {
     static constexpr int BYTES = R * 128;
-    static constexpr int LOADS = R >= 64 ? R / 64 : 1;
+    static constexpr int LOADS = R / 64;
     uint32_t index[LISTED ? LOADS : 1], next[LISTED ? LOADS : 1];  // rows in memory, of this tile and (as listed) the next
     uint32_t first, chunk;
     __device__ __forceinline__ void init() { chunk = (threadIdx.x & 7) ^ (threadIdx.x >> 3 & 7); }
@@ -88,7 +89,6 @@ struct Rows {
     }
     // Piece i of the step's loads.
     __device__ __forceinline__ void load(int i, const Planes& p, uint32_t kstep, uint32_t plane, const char* zeros, char* lds) const {
-        if (R < 64 && threadIdx.x >= R * 8) return;
         const uint32_t r = first + i * 64 + (threadIdx.x >> 3);
         const bool in = kstep * 8 + chunk < p.chunks && r < p.rows;
         const char* from = p.base + ((uint64_t)kstep * 128 + plane * p.plane) + ((uint64_t)(LISTED ? index[i] : r) * p.stride + chunk * 16);

@@ -145,7 +145,7 @@ __global__ __launch_bounds__(256) void list_candidates_kernel(const uint64_t* ma
     if (blockIdx.x == gridDim.x - 1 && !threadIdx.x) *count = before + total;
 }
 
-// Queries as planes, [n_q][k] and, for gradients, transposed [dim][gq], by tiles of 64 x 64; the workgroups behind the
+// Queries as planes (5 - 9 us: latency), [n_q][k] and, for gradients, transposed [dim][gq], by tiles of 64 x 64; the workgroups behind the
 // tiles take four queries each: length, factor, and the place of the click. For gradients a query whose click is no
 // candidate is zeros, whatever it holds (padding of a batch may hold anything): its weights are zero, and zero times what
 // is no number would be none in every row's gradient.
@@ -224,7 +224,8 @@ __global__ __launch_bounds__(256) void pack_queries_kernel(XentArgs a, Few f, ui
     click[q] = place;
 }
 
-// A piece of the candidates as rows that start at multiples of 16 bytes, zeros from `dim` on: 16 bytes a thread.
+// A piece of the candidates as rows that start at multiples of 16 bytes, zeros from `dim` on: 16 bytes a thread (45 thousand
+// x 383 f32: 23 us, 6.0 TB/s).
 template <typename E>
 __global__ __launch_bounds__(256) void pack_rows_kernel(XentArgs a, const E* table, uint64_t stride, char* out) {
     constexpr int V = 16 / sizeof(E);
@@ -252,9 +253,8 @@ struct Scores {
     static constexpr bool SPLIT = false;
     using R = Rows<TILE, LISTED>;
     using Q = Rows<BQ>;
-    // Beside the buffers: results on their way out (16 KiB) and numbers of each query and candidate. With sixteen queries
-    // not every wave has a load of theirs, and the count of those behind would not be one number: two buffers.
-    static constexpr int BUFFERS = BQ < 64 ? 2 : buffers_of(R::BYTES + Q::BYTES, 16384 + 6144);
+    // Beside the buffers: results on their way out (16 KiB) and numbers of each query and candidate.
+    static constexpr int BUFFERS = buffers_of(R::BYTES + Q::BYTES, 16384 + 6144);
     static constexpr int LDS = BUFFERS * (R::BYTES + Q::BYTES);
 
     __device__ __forceinline__ static uint32_t wave_q() { return uniform_u32(threadIdx.x >> 6) % WAVES_Q; }
@@ -440,7 +440,10 @@ struct SplitScores {
 __device__ __forceinline__ float finite_or_zero(float m) { return m == -__builtin_inff() ? 0.0f : m; }
 
 // Per query the largest logit of a share of the candidates and the sum of the exponentials over it, the clicked row kept
-// out. Everything is in base 2 (logits times log2 e): an exponential is one instruction. A lane keeps the running largest
+// out. Bound by the products from 64 queries (bf16) or so on, by the rows' bytes below: 256 queries over 1M x 768 bf16 take
+// 420 - 510 us (0.8 - 0.95 PFLOP/s; a large library product reaches 1.5), 10 take 255 (6.0 TB/s); over 250 thousand x 768
+// f32 256 take 660 (149 TFLOP/s in f32 products, 0.9 PFLOP/s of the six bf16 ones: the wave's splitting and the matrix
+// cores take 45 % of the cycles each). Everything is in base 2 (logits times log2 e): an exponential is one instruction. A lane keeps the running largest
 // and sum of its own candidates, in registers, for each of its queries; lanes, waves and shares are joined at the end.
 template <typename S, bool NORMS>
 __global__ __launch_bounds__(THREADS, 2) void loss_kernel(XentArgs a) {
@@ -548,7 +551,7 @@ __global__ __launch_bounds__(THREADS, 2) void loss_kernel(XentArgs a) {
     a.part_l[to] = sum;
 }
 
-// Up to four queries: bound by the rows' bytes, so plain f32 products, straight from the table and under the masks
+// Up to four queries: bound by the rows' bytes (one over 1M x 768 bf16: 237 us, 6.5 TB/s), so plain f32 products, straight from the table and under the masks
 // themselves, with nothing laid out before. A wave takes the words of the masks in turn, and of each word's candidates U at
 // a time: their loads are in flight together, and the U x NQ sums over the lanes leave each (candidate, query) to a lane
 // of its own, which keeps the running largest and sum of its logits.
@@ -657,7 +660,7 @@ __global__ __launch_bounds__(256) void loss_few_kernel(XentArgs a, Few f) {
     a.part_l[(uint64_t)blockIdx.x * NQ + threadIdx.x] = sum;
 }
 
-// A query's shares joined, in 64 bits; a workgroup per query. The clicked row's logit is made here, in 64 bits: its error
+// A query's shares joined, in 64 bits; a workgroup per query: 5 - 10 us, two trips to memory one behind the other. The clicked row's logit is made here, in 64 bits: its error
 // is that of a loss near zero, while those of the others' mostly cancel in their sum.
 template <typename E, typename Q>
 __global__ __launch_bounds__(256) void join_loss_kernel(XentArgs a, Few f, float* loss, float* lse) {
@@ -756,7 +759,9 @@ template <typename S>
 using weights_turn = Turn<8, S::UNIT>;
 
 // The weights G of a piece, [candidate][query], rounded to bf16 (PG = 1), or kept to 16 bits (2) or all 24 (3) by as many
-// planes. A lane holds four neighbouring queries of a candidate: eight bytes a store.
+// planes. A lane holds four neighbouring queries of a candidate: eight bytes a store. Bound as the loss is, and by what
+// it writes: 256 queries over 1M x 768 bf16 505 us (0.78 PFLOP/s, of which 512 MB written take about 100), 256 over 250
+// thousand x 768 f32 715.
 template <typename S, bool NORMS, int PG>
 __global__ __launch_bounds__(THREADS, 2) void weights_kernel(XentArgs a) {
     constexpr int BQ = S::Q_TILE;
@@ -835,7 +840,9 @@ __global__ __launch_bounds__(THREADS, 2) void weights_kernel(XentArgs a) {
     });
 }
 
-// drows of a piece: transposed queries (BD columns of the rows) by G. A lane holds four neighbouring columns of a row.
+// drows of a piece: transposed queries (BD columns of the rows) by G. The sums are short (as many steps as 64 queries, or six
+// times as many in f32) and every one is written: 256 queries, 1M x 768 bf16: 698 us (0.56 PFLOP/s; 1.5 GB written and 0.5
+// read take 400 by themselves); 250 thousand x 768 f32: 677 us. A lane holds four neighbouring columns of a row.
 // As in weights_kernel every lane stores every time, to its own 16 bytes of a.spill where it has no row or no whole
 // 16 bytes of columns; the columns of a last, broken 16 bytes are stored one by one besides.
 template <int BD>
@@ -952,7 +959,8 @@ __global__ __launch_bounds__(THREADS, 2) void row_grads_kernel(XentArgs a) {
     __builtin_amdgcn_s_waitcnt(0x0F70);
 }
 
-// dqueries over one share of a piece's candidates: G by rows, the sum running over the candidates.
+// dqueries over one share of a piece's candidates: G by rows, the sum running over the candidates. 256 queries over 1M x
+// 768 bf16: 483 us (0.81 PFLOP/s); 1000 over 100 thousand of 200 thousand x 1536, through the list: 366 us (0.84).
 // (Through the list two buffers: its reads are waited for with the loads under way counted in, so that only those that
 // the barrier has waited for already may be.)
 template <int BQ, int BD, bool LISTED>
@@ -1049,7 +1057,8 @@ __global__ __launch_bounds__(THREADS, 2) void query_grads_kernel(XentArgs a) {
         }
 }
 
-// The same of an f32 table: G's planes by the rows as they are.
+// The same of an f32 table: G's planes by the rows as they are, split as in SplitScores. 128 queries a tile (256 over 250
+// thousand x 768: 610 us, 0.97 PFLOP/s of bf16; by 64 a tile 843), the LDS of two steps.
 constexpr int FLOAT_BD = 128;
 template <int BQ, bool LISTED>
 constexpr int float_grads_row_buffers = LISTED || BQ > 64 ? 2 : 3;
@@ -1183,7 +1192,8 @@ __global__ __launch_bounds__(256) void join_query_grads_kernel(XentArgs a, const
     }
 }
 
-// Rows that are no candidates have gradient zero (`all`: every row, where there is no query).
+// Rows that are no candidates have gradient zero (`all`: every row, where there is no query). A wave a row: 7 us for a tenth
+// of 50 thousand.
 template <typename E>
 __global__ __launch_bounds__(256) void clear_rows_kernel(const uint64_t* mask, const uint64_t* present, bool all, uint64_t n_rows,
                                                          uint32_t dim, E* out, uint64_t stride) {
@@ -1204,13 +1214,19 @@ constexpr uint32_t FEW_WORKGROUPS = 2048;     // of the loss of a few queries: e
 constexpr Steps SIX{6, 0u | 0u << 2 | 1u << 4 | 1u << 6 | 0u << 8 | 2u << 10, 0u | 1u << 2 | 0u << 4 | 1u << 6 | 2u << 8 | 0u << 10};
 constexpr Steps ONE{1, 0, 0}, TWO{2, 0u | 1u << 2, 0};
 
-// The matrix cores take sixteen queries at least, and rows through LDS; plain products of four queries or fewer take less
-// time than the rows' bytes do. (Queries of all lanes' columns have to fit LDS.)
-bool few_queries(uint32_t n_q, uint32_t dim) { return n_q <= 4 && n_q * (uint64_t)dim <= 12288; }
+// Up to four queries by plain products, which need no list of candidates and no planes of queries: rows of f32 always (200
+// thousand x 768, four queries: 115 us, on the matrix cores 164), rows of bf16 while their bytes still bound them (one
+// query over 1M x 768: 238 us and 260; two 260 and 261, three 276 and 260, four 320 and 261) or launches do (20 thousand x
+// 384, a fifth of them: four queries 16 us and 26). Queries of all lanes' columns have to fit LDS.
+bool few_queries(uint32_t n_q, uint64_t n_rows, uint32_t dim, int32_t dtype) {
+    const bool bound = dtype == VS_F32 || n_rows * dim * 2 <= 256u << 20;
+    return n_q <= (bound ? 4 : 2) && n_q * (uint64_t)dim <= 12288;
+}
 
 struct Plan {
-    uint32_t planes, g_planes, kp, gq, loss_bq, score_bq, score_rows, bq, bd, q_tiles, loss_q_tiles, score_q_tiles, d_tiles, grad_d_tiles;
-    uint32_t loss_splits, weight_splits, row_splits, grad_splits;
+    bool few;
+    uint32_t planes, g_planes, kp, gq, score_bq, score_rows, bq, bd, q_tiles, score_q_tiles, d_tiles, grad_d_tiles;
+    uint32_t score_splits, row_splits, grad_splits;
     uint64_t piece_rows, packed_rows;
 };
 
@@ -1225,17 +1241,19 @@ uint32_t splits_for(uint32_t across, uint64_t tiles) {
 
 Plan plan_for(uint32_t n_q, uint64_t n_rows, uint32_t dim, int32_t dtype) {
     Plan p;
+    p.few = few_queries(n_q, n_rows, dim, dtype);
     p.planes = dtype == VS_F32 ? 3 : 1;
-    // One rounding of a weight is of the size of the rounding of a gradient. Where few queries, or few large weights, make
-    // up a gradient it shows, and where queries are few the second plane costs nothing: the rows' bytes bound the products.
+    // One rounding of a weight (2^-8 at most) is of the size of the rounding of a gradient to bf16, and like it once in a
+    // value. Where few queries, or few large weights, make up a gradient it shows, and where queries are few the second plane
+    // costs nothing: the rows' bytes bound the products.
     p.g_planes = dtype == VS_F32 ? 3 : n_q <= 64 ? 2 : 1;
     p.kp = (uint32_t)round_up(dim, 64);
     p.gq = (uint32_t)round_up(n_q, 64);
     p.bq = n_q <= 64 ? 64 : n_q <= 128 || dtype == VS_F32 ? 128 : 256;
     p.score_bq = dtype == VS_F32 ? 64 : p.bq;
-    p.loss_bq = dtype == VS_F32 || n_q > 16 ? p.score_bq : 16;
+    // an odd number of 128 columns by 128 at a time: no half-empty tiles (200 thousand x 384, 128 queries: rows' gradients
+    // 49 us, 57 by 256; queries' 41 and 48)
     p.bd = (dim + 127) / 128 % 2 ? 128 : 256;
-    p.loss_q_tiles = (n_q + p.loss_bq - 1) / p.loss_bq;
     p.score_q_tiles = (n_q + p.score_bq - 1) / p.score_bq;
     p.q_tiles = (n_q + p.bq - 1) / p.bq;
     p.d_tiles = (dim + p.bd - 1) / p.bd;
@@ -1249,10 +1267,11 @@ Plan plan_for(uint32_t n_q, uint64_t n_rows, uint32_t dim, int32_t dtype) {
     p.piece_rows = piece((uint64_t)p.q_tiles * p.bq * 2 * p.g_planes);
     p.packed_rows = std::min(p.piece_rows, piece((uint64_t)p.kp * (dtype == VS_F32 ? 4 : 2)));
     const uint64_t tiles = rows / TILE;
+    // f32 rows by 256 a tile, or by 128 where that leaves CUs idle for most of a round (256 queries, 250 thousand rows: 664 us
+    // and 813; 100 queries, 50 thousand: 52 and 43)
     p.score_rows = dtype == VS_F32 && p.score_q_tiles * tiles < 2 * WORKGROUPS ? 128 : TILE;
     const uint64_t score_tiles = rows / p.score_rows;
-    p.loss_splits = splits_for(p.loss_q_tiles, score_tiles);
-    p.weight_splits = splits_for(p.score_q_tiles, score_tiles);
+    p.score_splits = splits_for(p.score_q_tiles, score_tiles);
     p.row_splits = splits_for(p.d_tiles, tiles);
     p.grad_splits = splits_for(p.q_tiles * p.grad_d_tiles, tiles * (TILE / STEP));
     return p;
@@ -1280,7 +1299,7 @@ Buffers carve(void* workspace, const Plan& p, uint32_t n_q, uint64_t n_rows, uin
     b.qscale = w.take<float>(n_q);
     b.q = w.take<char>((uint64_t)n_q * p.kp * 2 * p.planes);
     b.qt = w.take<char>((uint64_t)dim * p.gq * 2 * p.planes);
-    const uint64_t parts = n_q * (uint64_t)(few_queries(n_q, dim) ? FEW_WORKGROUPS : p.loss_splits);
+    const uint64_t parts = n_q * (uint64_t)(p.few ? FEW_WORKGROUPS : p.score_splits);
     b.part_m = w.take<float>(parts);
     b.part_l = w.take<float>(parts);
     b.g = w.take<char>(p.piece_rows * p.q_tiles * p.bq * 2 * p.g_planes);
@@ -1402,7 +1421,7 @@ struct Call {
     void loss() {
         with_scores<BQ, true>([&](auto scores, auto norms) {
             using S = decltype(scores);
-            product(loss_kernel<S, norms>, S::LDS, p.loss_q_tiles, p.loss_splits);
+            product(loss_kernel<S, norms>, S::LDS, p.score_q_tiles, p.score_splits);
         });
     }
 
@@ -1412,7 +1431,7 @@ struct Call {
             using S = decltype(scores);
             // (three planes of weights are an f32 table's)
             if constexpr ((PG == 3) == S::SPLIT)
-                product(weights_kernel<S, norms, PG>, S::LDS + 8 * weights_turn<S>::BYTES, p.score_q_tiles, p.weight_splits);
+                product(weights_kernel<S, norms, PG>, S::LDS + 8 * weights_turn<S>::BYTES, p.score_q_tiles, p.score_splits);
         });
     }
     template <int BQ>
@@ -1515,17 +1534,12 @@ uint64_t xent_workspace_bytes(uint32_t n_q, uint64_t n_rows, uint32_t dim, int32
 }
 
 hipError_t launch_xent(const Xent& x, void* workspace, float* loss, float* lse, hipStream_t stream) {
-    if (few_queries(x.n_q, x.t.dim)) return launch_loss_few(x, workspace, loss, lse, stream);
+    if (few_queries(x.n_q, x.t.n_rows, x.t.dim, x.t.dtype)) return launch_loss_few(x, workspace, loss, lse, stream);
     Call c(x, workspace, false, stream);
     c.for_pieces(c.packed ? c.p.packed_rows : x.t.n_rows, [&] {
-        switch (c.p.loss_bq) {
-            case 16: return c.loss<16>();
-            case 64: return c.loss<64>();
-            case 128: return c.loss<128>();
-            default: return c.loss<256>();
-        }
+        c.p.score_bq == 64 ? c.loss<64>() : c.p.score_bq == 128 ? c.loss<128>() : c.loss<256>();
     });
-    c.a.splits = c.p.loss_splits;
+    c.a.splits = c.p.score_splits;
     if (c.error != hipSuccess) return c.error;
     auto join = [&](auto kernel) { kernel<<<x.n_q, 256, 0, stream>>>(c.a, few_of(x), loss, lse); };
     if (x.t.dtype == VS_F32)

@@ -138,6 +138,50 @@ def test_the_list_of_candidates_of_a_large_corpus(gpu_ctx):
     whole(gpu_ctx, queries, table, targets, keep, 5.0, None)
 
 
+def test_numbers_beyond_the_largest_of_bf16(gpu_ctx):
+    """f32 rows with elements that bf16 would round to an infinity: where the queries are zero there, nothing of them is in
+    the loss, and all of them in the queries' gradient."""
+    rows, dim, scale = 600, 40, 4.0
+    for n_q in (3, 30, 150):
+        table, queries = matrix(rows, dim, F32, 50), matrix(n_q, dim, F32, 51)
+        queries[:, 3] = 0
+        table[5::7, 3] = torch.finfo(F32).max
+        table[6::7, 3] = -3.3961775e38
+        whole(gpu_ctx, queries, table, clicks(n_q, rows, None, 52), None, scale, torch.full((n_q,), 1e-3, device=DEV))
+
+
+@pytest.mark.parametrize("metric", [abi.VS_ANGULAR, abi.VS_DOT])
+@pytest.mark.parametrize("dim", [40, 41])
+def test_a_large_batch_over_an_f32_store(gpu_ctx, metric, dim):
+    """So many queries and rows that the tiles are the largest ones, aligned rows and others."""
+    rng = np.random.default_rng(53)
+    n, n_q = 40000, 256
+    rows = rng.standard_normal((n, dim), dtype=np.float32)
+    rows[100] = 0  # no direction
+    store = gpu_ctx.create_store(0x4500, dim, n, dtype=abi.VS_F32, metric=metric)
+    store.upload(np.arange(n, dtype=np.uint32), rows)
+    store.remove(np.array([7, 39999], np.uint32))
+    store.seal()
+    keep = torch.ones(n, dtype=torch.bool, device=DEV)
+    keep[[7, 39999]] = False
+    queries = torch.from_numpy(rng.standard_normal((n_q, dim), dtype=np.float32)).to(DEV)
+    targets = torch.arange(n_q, device=DEV).int() * 150
+    targets[0] = 7
+    ws = torch.empty(store.xent_workspace_bytes(n_q), dtype=torch.uint8, device=DEV)
+    loss, lse = torch.empty(2, n_q, device=DEV)
+    dq = torch.empty(n_q, dim, device=DEV)
+    scale = 8.0 if metric == abi.VS_ANGULAR else 0.4
+    st = torch.cuda.current_stream().cuda_stream
+    store.xent_device(ptr(queries), n_q, dim, ptr(targets), None, scale, ptr(ws), ws.numel(), ptr(loss), ptr(lse), st)
+    store.xent_grad_device(ptr(queries), n_q, dim, ptr(targets), None, scale, ptr(loss), ptr(lse), None, ptr(ws), ws.numel(), ptr(dq), st)
+    want = xent_reference(queries, torch.from_numpy(rows).to(DEV), targets, keep, scale, cosine=metric == abi.VS_ANGULAR)
+    check(loss, want["loss"], "loss")
+    check(lse, want["lse"], "lse")
+    check(dq, rounded(want["queries"], F32), "gradient of the queries")
+    torch.cuda.synchronize()
+    store.destroy()
+
+
 @pytest.mark.parametrize("dtype,rows", [(BF16, 300000), (F32, 140000)])
 def test_tables_beyond_4_gib(gpu_ctx, dtype, rows):
     """Rows whose byte offsets pass 32 bits (and, in bf16, element offsets 31): lookups, loss and gradients at the far end.
