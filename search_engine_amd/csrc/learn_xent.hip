@@ -78,17 +78,13 @@ __device__ __forceinline__ uint32_t candidates(const XentArgs& a) {
 }
 __device__ __forceinline__ uint64_t row_at(const XentArgs& a, uint32_t place) { return a.list ? a.list[place] : place; }
 
-// Workgroups that share a tile of rows get numbers eight apart: the dispatcher deals numbers out to the eight XCDs in
-// turn, so they land on one XCD and its L2 holds the tile for all of them.
-__device__ __forceinline__ void place_of_workgroup(uint32_t across, uint32_t splits, uint32_t* a, uint32_t* along) {
-    if (splits % 8) {  // (too few for that: see splits_for)
-        *a = blockIdx.x % across;
-        *along = blockIdx.x / across;
-        return;
-    }
-    const uint32_t local = blockIdx.x >> 3;
-    *a = local % across;
-    *along = local / across * 8 + (blockIdx.x & 7);
+// The dispatcher deals workgroups out to the eight XCDs in turn. Renumbered, an XCD's are neighbours: those that share a
+// tile of rows, `across` of them, are on one XCD (or two), and its L2 holds the tile for all of them (dealt out as they come,
+// the gradient of 256 queries from 250 thousand x 768 f32 fetched 3.8 GB, so 1.6).
+__device__ __forceinline__ void place_of_workgroup(uint32_t across, uint32_t* a, uint32_t* along) {
+    const uint32_t xcd = blockIdx.x & 7, n = xcd * (gridDim.x >> 3) + min(xcd, gridDim.x & 7) + (blockIdx.x >> 3);
+    *a = n % across;
+    *along = n / across;
 }
 
 // ---- candidates and queries ------------------------------------------------------------------
@@ -452,7 +448,7 @@ __global__ __launch_bounds__(THREADS, 2) void loss_kernel(XentArgs a) {
     __shared__ float inverse[S::T], sm[S::WAVES_R][BQ], sl[S::WAVES_R][BQ];
     const uint32_t lane = threadIdx.x & 63, group = lane >> 4;
     uint32_t tile_q, along;
-    place_of_workgroup(a.across, a.splits, &tile_q, &along);
+    place_of_workgroup(a.across, &tile_q, &along);
     const uint32_t end = min(candidates(a), a.piece_begin + a.piece_rows);
     uint32_t click[S::TN];
     float s2[S::TN], m[S::TN], l[S::TN];
@@ -768,7 +764,7 @@ __global__ __launch_bounds__(THREADS, 2) void weights_kernel(XentArgs a) {
     extern __shared__ __attribute__((aligned(128))) char lds[];
     __shared__ __attribute__((aligned(16))) float s2[BQ], lse2[BQ], factor[BQ];
     uint32_t tile_q, along;
-    place_of_workgroup(a.across, a.splits, &tile_q, &along);
+    place_of_workgroup(a.across, &tile_q, &along);
     const uint32_t q0 = tile_q * BQ;
     const uint32_t end = min(candidates(a), a.piece_begin + a.piece_rows);
     if (end <= a.piece_begin) return;
@@ -841,8 +837,8 @@ __global__ __launch_bounds__(THREADS, 2) void weights_kernel(XentArgs a) {
 }
 
 // drows of a piece: transposed queries (BD columns of the rows) by G. The sums are short (as many steps as 64 queries, or six
-// times as many in f32) and every one is written: 256 queries, 1M x 768 bf16: 698 us (0.56 PFLOP/s; 1.5 GB written and 0.5
-// read take 400 by themselves); 250 thousand x 768 f32: 677 us. A lane holds four neighbouring columns of a row.
+// times as many in f32) and every one is written: 256 queries, 1M x 768 bf16: 660 us (0.60 PFLOP/s; 1.5 GB written and 0.5
+// read take 400 by themselves); 250 thousand x 768 f32: 630 us. A lane holds four neighbouring columns of a row.
 // As in weights_kernel every lane stores every time, to its own 16 bytes of a.spill where it has no row or no whole
 // 16 bytes of columns; the columns of a last, broken 16 bytes are stored one by one besides.
 template <int BD>
@@ -856,7 +852,7 @@ __global__ __launch_bounds__(THREADS, 2) void row_grads_kernel(XentArgs a) {
     extern __shared__ __attribute__((aligned(128))) char lds[];
     const uint32_t wave = uniform_u32(threadIdx.x >> 6), wd = wave % WAVES_D, wr = wave / WAVES_D;
     uint32_t tile_d, along;
-    place_of_workgroup(a.across, a.splits, &tile_d, &along);
+    place_of_workgroup(a.across, &tile_d, &along);
     const uint32_t end = min(candidates(a), a.piece_begin + a.piece_rows);
     const uint32_t tiles = end > a.piece_begin ? (end - a.piece_begin + TILE - 1) / TILE : 0;
     if (along >= tiles) return;
@@ -960,7 +956,7 @@ __global__ __launch_bounds__(THREADS, 2) void row_grads_kernel(XentArgs a) {
 }
 
 // dqueries over one share of a piece's candidates: G by rows, the sum running over the candidates. 256 queries over 1M x
-// 768 bf16: 483 us (0.81 PFLOP/s); 1000 over 100 thousand of 200 thousand x 1536, through the list: 366 us (0.84).
+// 768 bf16: 471 us (0.83 PFLOP/s); 1000 over 100 thousand of 200 thousand x 1536, through the list: 340 us (0.90).
 // (Through the list two buffers: its reads are waited for with the loads under way counted in, so that only those that
 // the barrier has waited for already may be.)
 template <int BQ, int BD, bool LISTED>
@@ -975,7 +971,7 @@ __global__ __launch_bounds__(THREADS, 2) void query_grads_kernel(XentArgs a) {
     const uint32_t lane = threadIdx.x & 63, wave = uniform_u32(threadIdx.x >> 6), wq = wave % WAVES_Q, wd = wave / WAVES_Q;
     const uint32_t d_tiles = (a.dim + BD - 1) / BD;
     uint32_t tile, share;
-    place_of_workgroup(a.across, a.splits, &tile, &share);
+    place_of_workgroup(a.across, &tile, &share);
     const uint32_t tile_d = tile % d_tiles, tile_q = tile / d_tiles;
     const uint32_t end = min(candidates(a), a.piece_begin + a.piece_rows);
     const uint32_t n = end > a.piece_begin ? end - a.piece_begin : 0;
@@ -1073,7 +1069,7 @@ __global__ __launch_bounds__(THREADS, 2) void float_query_grads_kernel(XentArgs 
     const uint32_t lane = threadIdx.x & 63, wave = uniform_u32(threadIdx.x >> 6), wq = wave % WAVES_Q, wd = wave / WAVES_Q;
     const uint32_t d_tiles = (a.dim + FLOAT_BD - 1) / FLOAT_BD;
     uint32_t tile, share;
-    place_of_workgroup(a.across, a.splits, &tile, &share);
+    place_of_workgroup(a.across, &tile, &share);
     const uint32_t tile_d = tile % d_tiles, tile_q = tile / d_tiles;
     const uint32_t end = min(candidates(a), a.piece_begin + a.piece_rows);
     const uint32_t n = end > a.piece_begin ? end - a.piece_begin : 0;
@@ -1231,12 +1227,8 @@ struct Plan {
 };
 
 // Workgroups along the rows for `across` side by side: one round of the CUs (a workgroup more would take a second one).
-// A multiple of eight keeps those that share rows on one XCD, unless more than a tenth of the CUs would go idle for it.
 uint32_t splits_for(uint32_t across, uint64_t tiles) {
-    const uint64_t want = std::max<uint64_t>(WORKGROUPS / across, 1);
-    if (tiles <= want) return (uint32_t)tiles;
-    const uint64_t aligned = want / 8 * 8;
-    return (uint32_t)(aligned * across * 10 >= WORKGROUPS * 9 ? aligned : want);
+    return (uint32_t)std::min<uint64_t>(std::max<uint64_t>(WORKGROUPS / across, 1), tiles);
 }
 
 Plan plan_for(uint32_t n_q, uint64_t n_rows, uint32_t dim, int32_t dtype) {
