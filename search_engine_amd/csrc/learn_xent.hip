@@ -55,6 +55,7 @@ struct XentArgs {
     char* g;                  // [planes][piece][whole tiles of queries] bf16
     uint64_t g_plane;
     uint32_t g_stride, g_planes;
+    float* click_rest;        // [n_q] what the planes of the clicked row's weight leave of it
     char* spill;              // 16 bytes of every thread of a product, for what it has no place for
     void* grad_rows;
     uint64_t grad_row_stride;
@@ -730,7 +731,8 @@ __device__ __forceinline__ float query_factor(const XentArgs& a, uint32_t q) {
 }
 
 // The weights of the clicked rows of a piece, after weights_kernel, which takes every row alike (to look for them there
-// costs two instructions in eight of each element).
+// costs two instructions in eight of each element). A clicked row's weight is as large as all others of its query together:
+// what its rounding takes away is kept, and goes into the query's gradient at the end.
 __global__ __launch_bounds__(256) void click_weights_kernel(XentArgs a) {
     const uint32_t q = blockIdx.x * 256 + threadIdx.x;
     if (q >= a.n_q) return;
@@ -742,13 +744,12 @@ __global__ __launch_bounds__(256) void click_weights_kernel(XentArgs a) {
         g = x > 0 ? g / x : 0.0f;
     }
     char* out = a.g + (uint64_t)(place - a.piece_begin) * a.g_stride + q * 2;
-    if (a.g_planes == 1) {
-        *reinterpret_cast<uint16_t*>(out) = (uint16_t)bf16_bits(g);
-        return;
+    for (uint32_t p = 0; p < a.g_planes; ++p) {
+        const uint32_t bits = bf16_bits(g);
+        *reinterpret_cast<uint16_t*>(out + p * a.g_plane) = (uint16_t)bits;
+        g -= __builtin_bit_cast(float, bits << 16);
     }
-    const Split s = split(g);
-    const uint16_t part[3] = {s.h, s.m, s.l};
-    for (uint32_t p = 0; p < a.g_planes; ++p) *reinterpret_cast<uint16_t*>(out + p * a.g_plane) = part[p];
+    a.click_rest[q] = g;
 }
 
 template <typename S>
@@ -1148,25 +1149,27 @@ __global__ __launch_bounds__(THREADS, 2) void float_query_grads_kernel(XentArgs 
 // The shares of a query's gradient joined, and taken through the query's length where logits are cosines; one
 // workgroup per (query, 256 columns), or per query where its length is needed.
 template <typename E, typename Q, typename O>
-__global__ __launch_bounds__(256) void join_query_grads_kernel(XentArgs a, const Q* queries, uint64_t stride, O* out,
-                                                               uint64_t out_stride) {
+__global__ __launch_bounds__(256) void join_query_grads_kernel(XentArgs a, Few f, O* out, uint64_t out_stride) {
     __shared__ float sums[8];
     const uint32_t q = blockIdx.x;
     if (a.click[q] == NONE) {
         for (uint32_t d = blockIdx.y * 256 + threadIdx.x; d < a.dim; d += gridDim.y * 256) out[q * out_stride + d] = from_f32<O>(0.0f);
         return;
     }
+    const Q* const query = static_cast<const Q*>(f.queries) + q * f.query_stride;
+    const E* const clicked = static_cast<const E*>(f.rows) + (f.targets[q] - f.first_id) * f.stride;
+    const float rest = a.click_rest[q];
     float* sum0 = a.part_q + (uint64_t)q * a.dim;
     float dot = 0, sq = 0;
     for (uint32_t d = blockIdx.y * 256 + threadIdx.x; d < a.dim; d += gridDim.y * 256) {
-        float sum = 0;
+        float sum = sizeof(E) == 2 ? rest * to_f32(clicked[d]) : 0.0f;  // (of three planes nothing is left)
 #pragma unroll 8
         for (uint32_t s = 0; s < a.splits; ++s) sum += a.part_q[((uint64_t)s * a.n_q + q) * a.dim + d];
         if (!a.norms) {
             out[q * out_stride + d] = from_f32<O>(sum);
             continue;
         }
-        const float x = query_element<E>(queries[q * stride + d]);
+        const float x = query_element<E>(query[d]);
         dot = __builtin_fmaf(sum, x, dot);
         sq = __builtin_fmaf(x, x, sq);
         sum0[d] = sum;
@@ -1183,7 +1186,7 @@ __global__ __launch_bounds__(256) void join_query_grads_kernel(XentArgs a, const
     sq = sums[4] + sums[5] + sums[6] + sums[7];
     const float along = sq > 0 ? dot / sq : 0.0f;
     for (uint32_t d = threadIdx.x; d < a.dim; d += 256) {
-        const float x = query_element<E>(queries[q * stride + d]);
+        const float x = query_element<E>(query[d]);
         out[q * out_stride + d] = from_f32<O>(sum0[d] - along * x);
     }
 }
@@ -1276,7 +1279,7 @@ constexpr uint32_t LIST_ALONE = 8;
 
 struct Buffers {
     uint32_t *zeros, *list, *count, *sums, *click;
-    float *qscale, *part_m, *part_l, *part_q;
+    float *qscale, *click_rest, *part_m, *part_l, *part_q;
     char *q, *qt, *g, *packed, *spill;
     uint64_t bytes;
 };
@@ -1289,6 +1292,7 @@ Buffers carve(void* workspace, const Plan& p, uint32_t n_q, uint64_t n_rows, uin
     b.sums = w.take<uint32_t>(list_blocks(n_rows));
     b.click = w.take<uint32_t>(n_q);
     b.qscale = w.take<float>(n_q);
+    b.click_rest = w.take<float>(n_q);
     b.q = w.take<char>((uint64_t)n_q * p.kp * 2 * p.planes);
     b.qt = w.take<char>((uint64_t)dim * p.gq * 2 * p.planes);
     const uint64_t parts = n_q * (uint64_t)(p.few ? FEW_WORKGROUPS : p.score_splits);
@@ -1339,6 +1343,7 @@ struct Call {
         a.g = b.g;
         a.g_stride = p.q_tiles * p.bq * 2;
         a.g_planes = p.g_planes;
+        a.click_rest = b.click_rest;
         a.g_plane = p.piece_rows * a.g_stride;
         a.spill = b.spill;
         a.part_q = b.part_q;
@@ -1471,7 +1476,7 @@ struct Call {
     void join_query_grads(void* out, uint64_t out_stride) {
         a.splits = p.grad_splits;
         const dim3 grid(x.n_q, a.norms ? 1 : (a.dim + 255) / 256);
-        join_query_grads_kernel<E, Q, O><<<grid, 256, 0, stream>>>(a, (const Q*)x.queries, x.query_stride, (O*)out, out_stride);
+        join_query_grads_kernel<E, Q, O><<<grid, 256, 0, stream>>>(a, few_of(x), (O*)out, out_stride);
     }
 };
 
