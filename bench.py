@@ -520,8 +520,8 @@ def csrc_sha256():
     """Hash of what libvs_amd.so is built from -- search_engine_amd/csrc/vs_* and the Makefile's
     compiler, architecture, flags and source lists (the host mirror and the programs beside them are
     compiled into their own users, not into the library; the learn_* kernels are in it, and no search
-    uses them): names a build for the recorded-traffic check. (The tree travels to the GPU box without its .git, so a git tree hash cannot be asked for
-    there; this is the same information from the files themselves.)"""
+    uses them): names a build for the recorded-traffic check. (The tree may be run without its .git,
+    so a git tree hash cannot be asked for; this is the same information from the files themselves.)"""
     import hashlib
     h = hashlib.sha256()
     d = os.path.join(ROOT, "search_engine_amd", "csrc")

@@ -102,6 +102,11 @@ learn::Xent xent_of(const vs::SlabView& v, const float* queries, uint32_t n_q, c
 // Runs `body` (which returns a hipError_t) over the registered rows of a sealed store on the caller's stream.
 template <typename F>
 int32_t over_store(vs_store* s, hipStream_t stream, F&& body) {
+    // (the event that a later seal waits for would become part of the graph, and the store's buffers of today with it)
+    hipStreamCaptureStatus capture = hipStreamCaptureStatusNone;
+    HIP_TRY(hipStreamIsCapturing(stream, &capture));
+    if (capture != hipStreamCaptureStatusNone)
+        return fail(VS_E_INVALID_ARG, "store %u: the call may not be recorded into a graph", s->index);
     Snapshot snap;
     vsrt::snapshot_begin(s, &snap);
     const int32_t rc = body(snap.v);

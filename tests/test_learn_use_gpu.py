@@ -301,3 +301,35 @@ def test_two_graphs_beside_each_other(gpu_ctx):
             for a, b in zip(got, side.results()):
                 assert torch.equal(a, b)
     assert math.isfinite(float(sides[0].loss.sum()))
+
+
+def test_calls_on_a_store_are_refused_under_capture(gpu_ctx):
+    store = gpu_ctx.create_store(0x4600, 32, 100)
+    rows = np.random.default_rng(60).standard_normal((100, 32), dtype=np.float32)
+    store.upload(np.arange(100, dtype=np.uint32), rows)
+    store.seal()
+    ids = torch.arange(3, device=DEV).int()
+    out, queries = torch.zeros(3, 32, device=DEV), torch.ones(3, 32, device=DEV)
+    loss, lse = torch.zeros(2, 3, device=DEV)
+    ws = torch.empty(store.xent_workspace_bytes(3), dtype=torch.uint8, device=DEV)
+
+    def calls(st):
+        yield lambda: store.lookup_device(ptr(ids), 3, None, 3, None, 1.0, ptr(out), abi.VS_F32, 32, st)
+        yield lambda: store.xent_device(ptr(queries), 3, 32, ptr(ids), None, 1.0, ptr(ws), ws.numel(), ptr(loss), ptr(lse), st)
+        yield lambda: store.xent_grad_device(ptr(queries), 3, 32, ptr(ids), None, 1.0, ptr(loss), ptr(lse), None, ptr(ws), ws.numel(),
+                                             ptr(out), st)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        queries += 1  # (something to record)
+        for call in calls(torch.cuda.current_stream().cuda_stream):
+            with pytest.raises(abi.VsError) as e:
+                call()
+            assert e.value.code == abi.VS_E_INVALID_ARG
+    graph.replay()
+    torch.cuda.synchronize()
+    assert (queries == 2).all() and (out == 0).all()
+    for call in calls(torch.cuda.current_stream().cuda_stream):
+        call()
+    torch.cuda.synchronize()
+    assert torch.isfinite(out).all() and torch.isfinite(loss).all() and (loss != 0).any()
+    store.destroy()
