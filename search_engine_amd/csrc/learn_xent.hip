@@ -347,9 +347,9 @@ struct Scores {
 // step) through three buffers, queries by 64 through two.
 template <bool LANES_ARE_QUERIES, bool LISTED, int ROWS>
 struct SplitScores {
-    static constexpr int T = ROWS, Q_TILE = 64, UNIT = T == 256 ? 2 : 4;
+    static constexpr int T = ROWS, Q_TILE = 64, UNIT = T == 128 ? 4 : 2;
     static constexpr bool SPLIT = true;
-    static constexpr int WAVES_Q = 1, WAVES_R = 8, WQ = 4, WR = T / 128;
+    static constexpr int WAVES_Q = T == 64 ? 2 : 1, WAVES_R = 8 / WAVES_Q, WQ = 4 / WAVES_Q, WR = T / WAVES_R / 16;
     static constexpr int TM = LANES_ARE_QUERIES ? WR : WQ, TN = LANES_ARE_QUERIES ? WQ : WR;
     using R = Rows<T, LISTED>;
     using Q = Rows<Q_TILE>;
@@ -1263,8 +1263,10 @@ Plan plan_for(uint32_t n_q, uint64_t n_rows, uint32_t dim, int32_t dtype) {
     p.packed_rows = std::min(p.piece_rows, piece((uint64_t)p.kp * (dtype == VS_F32 ? 4 : 2)));
     const uint64_t tiles = rows / TILE;
     // f32 rows by 256 a tile, or by 128 where that leaves CUs idle for most of a round (256 queries, 250 thousand rows: 664 us
-    // and 813; 100 queries, 50 thousand: 52 and 43)
-    p.score_rows = dtype == VS_F32 && p.score_q_tiles * tiles < 2 * WORKGROUPS ? 128 : TILE;
+    // and 813; 100 queries, 50 thousand: 52 and 43), or by 64 where all tiles have a CU then (64 queries, 10 thousand x 384:
+    // 13 us and 17 by 128; 30, 20 thousand x 768, which take two rounds: 35 and 28)
+    const uint64_t score_tiles_256 = p.score_q_tiles * tiles;
+    p.score_rows = dtype != VS_F32 || score_tiles_256 >= 2 * WORKGROUPS ? TILE : score_tiles_256 * 4 > WORKGROUPS ? 128 : 64;
     const uint64_t score_tiles = rows / p.score_rows;
     p.score_splits = splits_for(p.score_q_tiles, score_tiles);
     p.row_splits = splits_for(p.d_tiles, tiles);
@@ -1403,12 +1405,13 @@ struct Call {
         auto by_norms = [&](auto scores) { a.norms ? f(scores, std::true_type{}) : f(scores, std::false_type{}); };
         if constexpr (BQ == 64)
             if (p.planes == 3) {
-                if (p.score_rows == 256) {
-                    if (a.rows.list) return by_norms(SplitScores<LANES_ARE_QUERIES, true, 256>{});
-                    return by_norms(SplitScores<LANES_ARE_QUERIES, false, 256>{});
-                }
-                if (a.rows.list) return by_norms(SplitScores<LANES_ARE_QUERIES, true, 128>{});
-                return by_norms(SplitScores<LANES_ARE_QUERIES, false, 128>{});
+                auto by_list = [&](auto rows) {
+                    if (a.rows.list) return by_norms(SplitScores<LANES_ARE_QUERIES, true, rows>{});
+                    by_norms(SplitScores<LANES_ARE_QUERIES, false, rows>{});
+                };
+                if (p.score_rows == 256) return by_list(std::integral_constant<int, 256>{});
+                if (p.score_rows == 128) return by_list(std::integral_constant<int, 128>{});
+                return by_list(std::integral_constant<int, 64>{});
             }
         if (a.rows.list) return by_norms(Scores<BQ, LANES_ARE_QUERIES, true>{});
         by_norms(Scores<BQ, LANES_ARE_QUERIES, false>{});
