@@ -44,7 +44,7 @@ struct XentArgs {
     const uint32_t* click;  // [n_q] place of the clicked row among the candidates, or NONE
     const float* qscale;    // [n_q] factor of a query's products, without its sign
     float sign;
-    Steps grad_steps;
+    Steps row_steps, query_steps;  // of the gradients' products
     const char* zeros;
     uint32_t piece_begin, piece_rows;
     bool first_piece;
@@ -55,7 +55,7 @@ struct XentArgs {
     char* g;                  // [planes][piece][whole tiles of queries] bf16
     uint64_t g_plane;
     uint32_t g_stride, g_planes;
-    float* click_rest;        // [n_q] what the planes of the clicked row's weight leave of it
+    float* click_rest;        // [n_q] what the queries' product does not see of the clicked row's weight
     char* spill;              // 16 bytes of every thread of a product, for what it has no place for
     void* grad_rows;
     uint64_t grad_row_stride;
@@ -748,15 +748,15 @@ __global__ __launch_bounds__(256) void click_weights_kernel(XentArgs a) {
         const uint32_t bits = bf16_bits(g);
         *reinterpret_cast<uint16_t*>(out + p * a.g_plane) = (uint16_t)bits;
         g -= __builtin_bit_cast(float, bits << 16);
+        if (p + 1 == min(a.query_steps.n, a.g_planes)) a.click_rest[q] = g;
     }
-    a.click_rest[q] = g;
 }
 
 template <typename S>
 using weights_turn = Turn<8, S::UNIT>;
 
 // The weights G of a piece, [candidate][query], rounded to bf16 (PG = 1), or kept to 16 bits (2) or all 24 (3) by as many
-// planes. A lane holds four neighbouring queries of a candidate: eight bytes a store. Bound as the loss is, and by what
+// planes (which: see two_for_queries). A lane holds four neighbouring queries of a candidate: eight bytes a store. Bound as the loss is, and by what
 // it writes: 256 queries over 1M x 768 bf16 505 us (0.78 PFLOP/s, of which 512 MB written take about 100), 256 over 250
 // thousand x 768 f32 715.
 template <typename S, bool NORMS, int PG>
@@ -864,7 +864,7 @@ __global__ __launch_bounds__(THREADS, 2) void row_grads_kernel(XentArgs a) {
     r.init();
     q.aim(tile_d * BD);
     r.aim(along * TILE);
-    const uint32_t planes = a.grad_steps.n, blocks = a.gq / 64, steps = planes * blocks;
+    const uint32_t planes = a.row_steps.n, blocks = a.gq / 64, steps = planes * blocks;
     constexpr int BUFFERS = row_grads_buffers<BD>, BEHIND = (BUFFERS - 2) * (A::LOADS + B::LOADS);
     auto half_q = [&](uint32_t i) { return lds + i * (A::BYTES + B::BYTES); };
     auto half_g = [&](uint32_t i) { return lds + i * (A::BYTES + B::BYTES) + A::BYTES; };
@@ -872,10 +872,10 @@ __global__ __launch_bounds__(THREADS, 2) void row_grads_kernel(XentArgs a) {
     Cursor cg{0, 0, along}, cq{0, 0, along};
     auto load_weights = [&](uint32_t to) {
 #pragma unroll
-        for (int i = 0; i < B::LOADS; ++i) r.load(i, g, cg.k, a.grad_steps.plane_a(cg.c), a.zeros, half_g(to));
+        for (int i = 0; i < B::LOADS; ++i) r.load(i, g, cg.k, a.row_steps.plane_a(cg.c), a.zeros, half_g(to));
         if (cg.advance(planes, blocks, a.splits)) r.aim(cg.tile < tiles ? cg.tile * TILE : NO_ROW);
     };
-    auto load_queries = [&](int i, uint32_t to) { q.load(i, a.qt, cq.k, a.grad_steps.plane_b(cq.c), a.zeros, half_q(to)); };
+    auto load_queries = [&](int i, uint32_t to) { q.load(i, a.qt, cq.k, a.row_steps.plane_b(cq.c), a.zeros, half_q(to)); };
     auto load_all_queries = [&](uint32_t to) {
 #pragma unroll
         for (int i = 0; i < A::LOADS; ++i) load_queries(i, to);
@@ -980,7 +980,7 @@ __global__ __launch_bounds__(THREADS, 2) void query_grads_kernel(XentArgs a) {
     const uint32_t per = ((n + STEP - 1) / STEP + a.splits - 1) / a.splits * STEP;
     const uint32_t begin = (uint32_t)min((uint64_t)share * per, (uint64_t)n), stop = min(begin + per, n);
     f32x4 acc[TM][TN] = {};
-    const uint32_t blocks = (stop - begin + STEP - 1) / STEP, steps = blocks * a.grad_steps.n;
+    const uint32_t blocks = (stop - begin + STEP - 1) / STEP, steps = blocks * a.query_steps.n;
     if (steps) {
         const Planes g{a.g, a.g_plane, a.g_stride, nullptr, n, a.gq / 8};
         Planes rows = a.rows;
@@ -994,17 +994,17 @@ __global__ __launch_bounds__(THREADS, 2) void query_grads_kernel(XentArgs a) {
         auto half_g = [&](uint32_t i) { return lds + i * (A::BYTES + B::BYTES); };
         auto half_r = [&](uint32_t i) { return lds + i * (A::BYTES + B::BYTES) + A::BYTES; };
         Cursor cr{0, 0, 0}, cg{0, 0, 0};
-        const uint32_t planes = a.grad_steps.n;
+        const uint32_t planes = a.query_steps.n;
         auto load_rows = [&](uint32_t to) {
             const uint32_t from = begin + cr.k * STEP;
 #pragma unroll
             for (int i = 0; i < B::LOADS; ++i)
-                r.load(i, rows, base + from, base + stop, tile_d * (BD / 8), a.grad_steps.plane_b(cr.c), a.zeros, half_r(to));
+                r.load(i, rows, base + from, base + stop, tile_d * (BD / 8), a.query_steps.plane_b(cr.c), a.zeros, half_r(to));
             cr.advance(planes, blocks + BUFFERS, 1);  // (behind the last block: zeros)
             if (!cr.c) r.peek(rows, base + from + STEP, base + stop);  // while this step multiplies
         };
         auto load_weights = [&](int i, uint32_t to) {
-            w.load(i, g, begin + cg.k * STEP, stop, tile_q * (BQ / 8), a.grad_steps.plane_a(cg.c), a.zeros, half_g(to));
+            w.load(i, g, begin + cg.k * STEP, stop, tile_q * (BQ / 8), a.query_steps.plane_a(cg.c), a.zeros, half_g(to));
         };
         r.peek(rows, base + begin, base + stop);
 #pragma unroll
@@ -1234,14 +1234,19 @@ uint32_t splits_for(uint32_t across, uint64_t tiles) {
     return (uint32_t)std::min<uint64_t>(std::max<uint64_t>(WORKGROUPS / across, 1), tiles);
 }
 
-Plan plan_for(uint32_t n_q, uint64_t n_rows, uint32_t dim, int32_t dtype) {
+// Planes of a bf16 table's weights. One rounding of a weight to bf16 (2^-8 of it at most) is as large as the rounding of a
+// gradient to bf16: a row's gradient, of few terms of like size, would be 1.4 times as far off as its type makes it, and an
+// f32 gradient 2^-8 and not 2^-24. So the weights have two planes (16 bits) wherever that shows. It does not in a bf16 gradient
+// of queries, a sum over all candidates whose largest term, the clicked row's, is exact (see click_rest); with up to 64
+// queries, where the rows' bytes bound the products, the second plane costs nothing.
+bool two_for_queries(const Xent& x) { return x.n_q <= 64 || x.queries_f32; }
+
+// `two`: whether a bf16 table's weights have two planes.
+Plan plan_for(uint32_t n_q, uint64_t n_rows, uint32_t dim, int32_t dtype, bool two) {
     Plan p;
     p.few = few_queries(n_q, n_rows, dim, dtype);
     p.planes = dtype == VS_F32 ? 3 : 1;
-    // One rounding of a weight (2^-8 at most) is of the size of the rounding of a gradient to bf16, and like it once in a
-    // value. Where few queries, or few large weights, make up a gradient it shows, and where queries are few the second plane
-    // costs nothing: the rows' bytes bound the products.
-    p.g_planes = dtype == VS_F32 ? 3 : n_q <= 64 ? 2 : 1;
+    p.g_planes = dtype == VS_F32 ? 3 : two || n_q <= 64 ? 2 : 1;
     p.kp = (uint32_t)round_up(dim, 64);
     p.gq = (uint32_t)round_up(n_q, 64);
     p.bq = n_q <= 64 ? 64 : n_q <= 128 || dtype == VS_F32 ? 128 : 256;
@@ -1322,8 +1327,9 @@ struct Call {
     hipStream_t stream;
     hipError_t error = hipSuccess;
 
-    Call(const Xent& x_, void* workspace, bool gradients, hipStream_t stream_)
-        : x(x_), p(plan_for(x.n_q, x.t.n_rows, x.t.dim, x.t.dtype)), b(carve(workspace, p, x.n_q, x.t.n_rows, x.t.dim)), stream(stream_) {
+    Call(const Xent& x_, void* workspace, bool gradients, bool rows_too, hipStream_t stream_)
+        : x(x_), p(plan_for(x.n_q, x.t.n_rows, x.t.dim, x.t.dtype, rows_too || two_for_queries(x))),
+          b(carve(workspace, p, x.n_q, x.t.n_rows, x.t.dim)), stream(stream_) {
         const uint32_t dim = x.t.dim;
         // straight from the table where a row is whole 16-byte chunks at multiples of 16 bytes
         const uint32_t size = x.t.dtype == VS_F32 ? 4 : 2, chunk = 16 / size;
@@ -1338,7 +1344,8 @@ struct Call {
         a.click = b.click;
         a.qscale = b.qscale;
         a.sign = x.scale < 0 ? -1.0f : 1.0f;
-        a.grad_steps = p.planes == 3 ? SIX : p.g_planes == 2 ? TWO : ONE;
+        a.row_steps = p.planes == 3 ? SIX : p.g_planes == 2 ? TWO : ONE;
+        a.query_steps = p.planes == 3 ? SIX : two_for_queries(x) ? TWO : ONE;
         a.zeros = (const char*)b.zeros;
         a.part_m = b.part_m;
         a.part_l = b.part_l;
@@ -1439,7 +1446,7 @@ struct Call {
         if constexpr (BQ == 64)
             p.planes == 3 ? weights<BQ, 3>() : weights<BQ, 2>();
         else
-            weights<BQ, 1>();
+            p.g_planes == 2 ? weights<BQ, 2>() : weights<BQ, 1>();
     }
 
     template <int BD, typename E>
@@ -1504,7 +1511,7 @@ hipError_t pick_loss_few(const Xent& x, const XentArgs& a, const Few& f, float* 
     }
 }
 hipError_t launch_loss_few(const Xent& x, void* workspace, float* loss, float* lse, hipStream_t stream) {
-    const Buffers b = carve(workspace, plan_for(x.n_q, x.t.n_rows, x.t.dim, x.t.dtype), x.n_q, x.t.n_rows, x.t.dim);
+    const Buffers b = carve(workspace, plan_for(x.n_q, x.t.n_rows, x.t.dim, x.t.dtype, false), x.n_q, x.t.n_rows, x.t.dim);
     XentArgs a{};
     a.n_rows = x.t.n_rows;
     a.dim = x.t.dim;
@@ -1530,12 +1537,14 @@ void clear_rows(const Xent& x, void* grad_rows, uint64_t stride, bool all, hipSt
 }  // namespace
 
 uint64_t xent_workspace_bytes(uint32_t n_q, uint64_t n_rows, uint32_t dim, int32_t dtype) {
-    return carve(nullptr, plan_for(n_q, n_rows, dim, dtype), n_q, n_rows, dim).bytes + 256;
+    uint64_t bytes = 0;
+    for (bool two : {false, true}) bytes = std::max(bytes, carve(nullptr, plan_for(n_q, n_rows, dim, dtype, two), n_q, n_rows, dim).bytes);
+    return bytes + 256;
 }
 
 hipError_t launch_xent(const Xent& x, void* workspace, float* loss, float* lse, hipStream_t stream) {
     if (few_queries(x.n_q, x.t.n_rows, x.t.dim, x.t.dtype)) return launch_loss_few(x, workspace, loss, lse, stream);
-    Call c(x, workspace, false, stream);
+    Call c(x, workspace, false, false, stream);
     c.for_pieces(c.packed ? c.p.packed_rows : x.t.n_rows, [&] {
         c.p.score_bq == 64 ? c.loss<64>() : c.p.score_bq == 128 ? c.loss<128>() : c.loss<256>();
     });
@@ -1559,7 +1568,7 @@ hipError_t launch_xent_grad(const Xent& x, const float* loss, const float* lse, 
         return hipGetLastError();
     }
     if (!grad_queries && !grad_rows) return hipSuccess;
-    Call c(x, workspace, true, stream);
+    Call c(x, workspace, true, grad_rows != nullptr, stream);
     c.a.loss = loss;
     c.a.lse = lse;
     c.a.grad_loss = grad_loss;

@@ -1,0 +1,123 @@
+"""What the cross entropy over a corpus keeps of its numbers: weights, exponents and lengths, against tight bounds."""
+import math
+
+import numpy as np
+import pytest
+import torch
+
+from learn_bounds import bounds, weight_bits
+from learn_helpers import DEV, U32, call_xent, call_xent_grads, check, ptr, rounded, words_of
+from search_engine_amd import abi
+from test_learn_xent_gpu import clicks, like, matrix
+
+pytestmark = pytest.mark.gpu
+F32, BF16 = torch.float32, torch.bfloat16
+
+
+def steps(rows, dim, dtype, seed):
+    """Elements -1/4, -1/8, 0, 1/8, 1/4: whatever order a product is summed in, nothing of it is rounded."""
+    g = torch.Generator(device=DEV).manual_seed(seed)
+    return (torch.randint(-2, 3, (rows, dim), generator=g, device=DEV) / 8).to(dtype)
+
+
+@pytest.fixture
+def store_of(gpu_ctx):
+    """Makes stores of rows, sealed; they go when the test ends."""
+    made = []
+
+    def make(dtype, metric, rows):
+        store = gpu_ctx.create_store(0x4700 + len(made), rows.shape[1], rows.shape[0], dtype=dtype, metric=metric)
+        made.append(store)
+        store.upload(np.arange(rows.shape[0], dtype=np.uint32), rows)
+        store.seal()
+        return store
+    yield make
+    torch.cuda.synchronize()
+    for store in made:
+        store.destroy()
+
+
+def store_loss_and_grad(store, queries, targets, scale, words=None):
+    n_q, dim = queries.shape
+    ws = torch.empty(store.xent_workspace_bytes(n_q), dtype=torch.uint8, device=DEV)
+    loss, lse = torch.empty(2, n_q, device=DEV)
+    dq = torch.empty(n_q, dim, device=DEV)
+    st = torch.cuda.current_stream().cuda_stream
+    store.xent_device(ptr(queries), n_q, dim, ptr(targets), ptr(words), scale, ptr(ws), ws.numel(), ptr(loss), ptr(lse), st)
+    store.xent_grad_device(ptr(queries), n_q, dim, ptr(targets), ptr(words), scale, ptr(loss), ptr(lse), None, ptr(ws), ws.numel(), ptr(dq), st)
+    torch.cuda.synchronize()
+    return loss, lse, dq
+
+
+@pytest.mark.parametrize("filtered", [False, True])
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("n_q", [3, 40, 64, 65, 100, 300])
+def test_weights_keep_their_bits(gpu_ctx, dtype, n_q, filtered):
+    """A rounding of the weights to 8 bits (2^-8 of each) lies far outside of what a row's gradient may be off by, whatever the
+    size of the batch."""
+    rows, dim, scale = 700, 32, 8.0
+    table, queries = steps(rows, dim, dtype, 1), steps(n_q, dim, dtype, 2)
+    keep = torch.rand(rows, generator=torch.Generator(device=DEV).manual_seed(3), device=DEV) < 0.6 if filtered else None
+    words = None if keep is None else words_of(keep)
+    targets = clicks(n_q, rows, keep, 4)
+    c = torch.rand(n_q, generator=torch.Generator(device=DEV).manual_seed(5), device=DEV)
+    loss, lse = call_xent(gpu_ctx, queries, table, targets, words, scale)
+    dq, dr = like(queries), like(table)
+    call_xent_grads(gpu_ctx, queries, table, targets, words, scale, loss, lse, c, dq, dr)
+    g_queries, g_rows = weight_bits(dtype, n_q, dtype)
+    want = bounds(queries, table, targets, keep, scale, c, exact_products=True, g_queries=g_queries, g_rows=g_rows)
+    check(loss, want["loss"], "loss")
+    check(lse, want["lse"], "lse")
+    check(dr, rounded(want["rows"], dtype), "gradient of the rows")
+    check(dq, rounded(want["queries"], dtype), "gradient of the queries")
+
+
+@pytest.mark.parametrize("metric", [abi.VS_ANGULAR, abi.VS_DOT])
+@pytest.mark.parametrize("dtype,t", [(abi.VS_F32, F32), (abi.VS_BF16, BF16)])
+@pytest.mark.parametrize("n_q", [4, 64, 65, 300])
+def test_weights_keep_their_bits_over_a_store(store_of, dtype, t, metric, n_q):
+    """The gradient of a store's queries is f32, so nothing else rounds them."""
+    rows, dim = 700, 32
+    table, queries = steps(rows, dim, t, 6), steps(n_q, dim, F32, 7)
+    queries[0, 0] = table[:, 0] = 0.25  # (no vector of zeros)
+    scale = 10.0 if metric == abi.VS_ANGULAR else 8.0
+    store = store_of(dtype, metric, table.float().cpu().numpy())
+    targets = clicks(n_q, rows, None, 8)
+    loss, lse, dq = store_loss_and_grad(store, queries, targets, scale)
+    want = bounds(queries, table, targets, None, scale, cosine=metric == abi.VS_ANGULAR, exact_products=True,
+                  g_queries=weight_bits(t, n_q, F32)[0])
+    check(loss, want["loss"], "loss")
+    check(lse, want["lse"], "lse")
+    check(dq, rounded(want["queries"], F32), "gradient of the queries")
+
+
+@pytest.mark.parametrize("n_q", [5, 70, 300])
+def test_an_improbable_click(store_of, n_q):
+    """A clicked document far from its query: its weight, nearly one, is as large as all others together, and reaches the
+    queries' gradient in f32."""
+    rows, dim, scale = 640, 64, 16.0
+    table, queries = steps(rows, dim, BF16, 9), steps(n_q, dim, BF16, 10)
+    targets = (torch.arange(n_q, device=DEV) * 2).int()
+    table[targets.long()] = -queries
+    store = store_of(abi.VS_BF16, abi.VS_DOT, table.float().cpu().numpy())
+    loss, lse, dq = store_loss_and_grad(store, queries.float(), targets, scale)
+    want = bounds(queries, table, targets, None, scale, exact_products=True, g_queries=2.0**-16)
+    check(loss, want["loss"], "loss")
+    check(dq, rounded(want["queries"], F32), "gradient of the queries")
+
+
+@pytest.mark.parametrize("n_q", [1, 4, 5, 70])
+@pytest.mark.parametrize("dim", [1, 4, 8])
+def test_f32_products_keep_24_bits(gpu_ctx, n_q, dim):
+    """So few terms that a product of planes that is missing (2^-16 of it) shows."""
+    for rows in (6, 300):
+        table, queries = matrix(rows, dim, F32, 11, unit=False), matrix(n_q, dim, F32, 12, unit=False)
+        targets = torch.arange(n_q, device=DEV).int() % rows
+        loss, lse = call_xent(gpu_ctx, queries, table, targets, None, 6.0)
+        dq, dr = like(queries), like(table)
+        call_xent_grads(gpu_ctx, queries, table, targets, None, 6.0, loss, lse, None, dq, dr)
+        want = bounds(queries, table, targets, None, 6.0, chain=rows, share=rows)
+        check(loss, want["loss"], "loss")
+        check(lse, want["lse"], "lse")
+        check(dq, rounded(want["queries"], F32), "gradient of the queries")
+        check(dr, rounded(want["rows"], F32), "gradient of the rows")
