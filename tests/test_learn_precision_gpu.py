@@ -121,3 +121,31 @@ def test_f32_products_keep_24_bits(gpu_ctx, n_q, dim):
         check(lse, want["lse"], "lse")
         check(dq, rounded(want["queries"], F32), "gradient of the queries")
         check(dr, rounded(want["rows"], F32), "gradient of the rows")
+
+
+@pytest.mark.parametrize("filtered", [False, True])
+@pytest.mark.parametrize("n_q", [20, 100, 300])
+def test_the_clicked_rows_weight_is_not_rounded(gpu_ctx, n_q, filtered):
+    """bf16 gradients of queries in columns that the clicked documents have nearly to themselves: a weight that had been rounded
+    to bf16 before, as those of the other documents are, would make two roundings where the bound has one."""
+    rows, dim, scale = 700, 64, 8.0
+    table, queries = steps(rows, dim, BF16, 13), steps(n_q, dim, BF16, 14)
+    targets = (torch.arange(n_q, device=DEV) * 2).int()
+    table[:, :32] = 0
+    table[targets.long(), :32] = steps(n_q, 32, BF16, 15)
+    keep = torch.rand(rows, generator=torch.Generator(device=DEV).manual_seed(16), device=DEV) < 0.5 if filtered else None
+    if filtered:
+        keep[targets.long()[: n_q - 3]] = True
+    words = None if keep is None else words_of(keep)
+    c = torch.rand(n_q, generator=torch.Generator(device=DEV).manual_seed(17), device=DEV) + 0.5
+    loss, lse = call_xent(gpu_ctx, queries, table, targets, words, scale)
+    dq, dr = like(queries), like(table)
+    call_xent_grads(gpu_ctx, queries, table, targets, words, scale, loss, lse, c, dq, dr)
+    want = bounds(queries, table, targets, keep, scale, c, exact_products=True, g_queries=weight_bits(BF16, n_q, BF16)[0], g_rows=2.0**-16)
+    check(dq, rounded(want["queries"], BF16), "gradient of the queries")
+    # (with the mistake in the 64-bit value, the clicked weights rounded, the bound is left)
+    value, bound = want["queries"]
+    weight = torch.expm1(-want["loss"][0]) * c * scale
+    wrong = (value + (weight.bfloat16().double() - weight)[:, None] * table[targets.long()].double()).bfloat16().double()
+    assert ((wrong - value).abs() > rounded((value, bound), BF16)[1]).any()
+    check(dr, rounded(want["rows"], BF16), "gradient of the rows")
