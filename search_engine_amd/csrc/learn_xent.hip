@@ -630,14 +630,14 @@ __global__ __launch_bounds__(256) void loss_few_kernel(XentArgs a, Few f) {
                     }
                 }
             if (lane < n * NQ) {
-                z *= factor;
                 if constexpr (NORMS) {
                     const float x = a.norms[r];
                     z = x > 0 ? z / x : 0.0f;
                 }
                 if (r != click) {
-                    const float top = __builtin_fmaxf(m, z), ref = finite_or_zero(top);
-                    l = l * __builtin_amdgcn_exp2f(m - ref) + __builtin_amdgcn_exp2f(z - ref);
+                    // (an fma: of a logit of hundreds the rounding alone would show in the exponential)
+                    const float top = __builtin_fmaxf(m, z * factor), ref = finite_or_zero(top);
+                    l = l * __builtin_amdgcn_exp2f(m - ref) + __builtin_amdgcn_exp2f(__builtin_fmaf(z, factor, -ref));
                     m = top;
                 }
             }

@@ -5,7 +5,9 @@ U32 = 2^-24 is one rounding to f32. To first order:
   product   depth + 8 roundings of the sum of its magnitudes (the three smallest of nine products of planes, left out, are
             below 2^-22 of it and among the 8), none where every partial sum is a whole number of some power of two and
             below 2^24 of it (`exact_products`); a cosine's row length takes depth / 2 + 2 more and its quotients 4
-  exponent  the factor times log2 e 2 roundings and the product one, of |z|; its distance from the largest one more
+  exponent  the factor times log2 e 2 roundings and the product one, of |z|, or none where the factor is such that it is not
+            rounded (`exact_factor`: one fma takes the product and its distance from the largest); the distance two more, and
+            two where sums over it are brought together, each with the term's share of the sum
   sum       `chain` roundings: as many terms as one workgroup adds up, and 20 for the joins
   lse       all of these, and one rounding of itself
   weight    its own product and exponent, lse's error, 8 roundings; and `g_*`, where it is kept to fewer bits
@@ -29,7 +31,7 @@ def weight_bits(dtype, n_q, out):
     return 2.0**-16 if n_q <= 64 or out == torch.float32 else 2.0**-8, 2.0**-16
 
 
-def bounds(queries, table, targets, keep, scale, grad_loss=None, cosine=False, exact_products=False, chain=None, g_queries=0.0,
+def bounds(queries, table, targets, keep, scale, grad_loss=None, cosine=False, exact_products=False, exact_factor=False, chain=None, g_queries=0.0,
            g_rows=0.0, share=None):
     """{loss, lse, queries, rows: (value in 64 bits, bound)}, the gradients before the rounding to their type. share: the
     candidates that one running sum of a query's gradient takes."""
@@ -47,7 +49,7 @@ def bounds(queries, table, targets, keep, scale, grad_loss=None, cosine=False, e
         rs = torch.where(rn > 0, r / rn, 0.0)
         terms += depth / 2 + 6
     z = qs @ rs.T * scale
-    zb = terms * U32 * abs(scale) * (qs.abs() @ rs.abs().T) + 3 * U32 * z.abs()
+    zb = terms * U32 * abs(scale) * (qs.abs() @ rs.abs().T) + (0 if exact_factor else 3 * U32) * z.abs()
     column = torch.full((n_rows,), -1, dtype=torch.int64, device=DEV)
     column[at] = torch.arange(at.numel(), device=DEV)
     t = targets.long() & 0xFFFFFFFF
@@ -60,7 +62,7 @@ def bounds(queries, table, targets, keep, scale, grad_loss=None, cosine=False, e
     click, clickb = torch.zeros_like(lse), torch.zeros_like(lse)
     click[ok], clickb[ok] = z[row[ok], column[ok]], zb[row[ok], column[ok]]
     loss = torch.where(ok, torch.nn.functional.softplus(rest - click, threshold=1e9), 0.0).nan_to_num()
-    e = zb.amax(1) + (2 * (z.amax(1) - z.amin(1)) + chain + 20) * U32
+    e = zb.amax(1) + (4 * (torch.softmax(z, 1) * (z.amax(1, keepdim=True) - z)).sum(1) + chain + 20) * U32
     p_not = -torch.expm1(-loss)
     lossb = p_not * (e + clickb) + 2 * U32 * loss + 1e-37
     out = {"lse": (lse, e + U32 * lse.abs() + 1e-37), "loss": (loss, lossb)}

@@ -149,3 +149,25 @@ def test_the_clicked_rows_weight_is_not_rounded(gpu_ctx, n_q, filtered):
     wrong = (value + (weight.bfloat16().double() - weight)[:, None] * table[targets.long()].double()).bfloat16().double()
     assert ((wrong - value).abs() > rounded((value, bound), BF16)[1]).any()
     check(dr, rounded(want["rows"], BF16), "gradient of the rows")
+
+
+def exact_factor():
+    """A scale near 100 whose product with log2 e is nearly a number of f32."""
+    s = (64 + np.arange(1 << 16) / 1024).astype(np.float32)
+    product = s * np.float32(np.log2(np.e))
+    return float(s[np.argmin(np.abs(product.astype(np.float64) / (s.astype(np.float64) * np.log2(np.e)) - 1))])
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("n_q", [1, 2, 3, 4, 5, 70, 300])
+def test_large_logits_lose_nothing_to_their_size(gpu_ctx, dtype, n_q):
+    """Logits of hundreds, the clicked one and another equal and far above the rest: the loss is log 2, and a rounding of a
+    logit before the largest is taken off (2^-24 of hundreds) would show."""
+    dim, rows, scale = 8, 200, exact_factor()
+    table, queries = steps(rows + n_q, dim, dtype, 18) * 8, steps(n_q, dim, dtype, 19) * 8
+    targets = (rows + torch.arange(n_q, device=DEV)).int()
+    table[targets.long()] = table[(queries.double() @ table[:rows].double().T).argmax(1)]
+    loss, lse = call_xent(gpu_ctx, queries, table, targets, None, scale)
+    want = bounds(queries, table, targets, None, scale, exact_products=True, exact_factor=True)
+    check(loss, want["loss"], "loss")
+    check(lse, want["lse"], "lse")
