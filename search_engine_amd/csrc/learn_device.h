@@ -170,6 +170,11 @@ __device__ __forceinline__ uint32_t afresh_uniform(uint32_t x) {
 }
 
 __device__ __forceinline__ float wave_sum(float v) { return wave_sum_f32(v); }
+__device__ __forceinline__ double wave_sum(double v) {
+#pragma unroll
+    for (int d = 32; d; d /= 2) v += __shfl_xor(v, d);
+    return v;
+}
 
 // Sum of x over the threads before this one, and over all, in a workgroup of 256.
 __device__ __forceinline__ uint32_t block_exclusive(uint32_t x, uint32_t* wave_sums /* 4, LDS */, uint32_t* total) {

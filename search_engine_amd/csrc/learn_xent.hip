@@ -194,16 +194,16 @@ __global__ __launch_bounds__(256) void pack_queries_kernel(XentArgs a, Few f, ui
     }
     const uint32_t q = (blockIdx.x - n_tiles) * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
     if (q >= a.n_q) return;
-    float sq = 0;
+    double sq = 0;  // (64 bits: f32 holds no square of a vector longer than 2^64, or shorter than 2^-75)
     if (a.norms) {
         for (uint32_t d = lane; d < a.dim; d += 64) {
-            const float x = query_element<std::conditional_t<P == 1, bf16, float>>(queries[q * stride + d]);
-            sq = __builtin_fmaf(x, x, sq);
+            const double x = query_element<std::conditional_t<P == 1, bf16, float>>(queries[q * stride + d]);
+            sq += x * x;
         }
         sq = wave_sum(sq);
     }
     if (lane) return;
-    const float norm = __builtin_sqrtf(sq), size = __builtin_fabsf(f.scale);
+    const float norm = (float)sqrt(sq), size = __builtin_fabsf(f.scale);
     qscale[q] = !a.norms ? size : norm > 0 ? size / norm : 0.0f;
     const uint32_t row = f.targets[q] - f.first_id;
     uint32_t place = clicked_candidate(f, q, a.n_rows) ? row : NONE;
@@ -556,7 +556,8 @@ template <typename E, typename Q, int V, int NQ, bool NORMS>
 __global__ __launch_bounds__(256) void loss_few_kernel(XentArgs a, Few f) {
     constexpr int U = NQ == 1 ? 8 : 4;
     extern __shared__ __attribute__((aligned(128))) char lds[];
-    __shared__ float sm[4][64], sl[4][64], sums[4];
+    __shared__ float sm[4][64], sl[4][64];
+    __shared__ double sums[4];
     float* const query = reinterpret_cast<float*>(lds);  // [NQ][padded], as they are multiplied
     const uint32_t lane = threadIdx.x & 63, wave = uniform_u32(threadIdx.x >> 6);
     const uint32_t chunks = (a.dim + V - 1) / V, padded = chunks * V;  // (a last, broken piece: see Piece)
@@ -564,13 +565,13 @@ __global__ __launch_bounds__(256) void loss_few_kernel(XentArgs a, Few f) {
     float factor = 0;  // of the lane's query, base 2
     const uint32_t mine = lane % NQ;
     for (int q = 0; q < NQ; ++q) {
-        float sq = 0;
+        double sq = 0;  // (as in pack_queries_kernel)
         for (uint32_t d = threadIdx.x; d < padded; d += 256) {
             const Piece<V> piece(d / V, a.dim);
             const uint32_t from = piece.col + d % V;
             const float x = d % V >= piece.skip && from < a.dim ? query_element<E>(queries[q * f.query_stride + from]) : 0.0f;
             query[q * padded + d] = x;
-            sq = __builtin_fmaf(x, x, sq);
+            if constexpr (NORMS) sq += (double)x * x;
         }
         float scale = f.scale * LOG2E;
         if constexpr (NORMS) {
@@ -578,7 +579,7 @@ __global__ __launch_bounds__(256) void loss_few_kernel(XentArgs a, Few f) {
             __syncthreads();
             if (!lane) sums[wave] = sq;
             __syncthreads();
-            const float norm = __builtin_sqrtf(sums[0] + sums[1] + sums[2] + sums[3]);
+            const float norm = (float)sqrt(sums[0] + sums[1] + sums[2] + sums[3]);
             scale = norm > 0 ? scale / norm : 0.0f;
         }
         if (mine == (uint32_t)q) factor = scale;
@@ -690,12 +691,9 @@ __global__ __launch_bounds__(256) void join_loss_kernel(XentArgs a, Few f, float
         const uint64_t at = (uint64_t)s * a.n_q + q;
         sum += (double)a.part_l[at] * (double)__builtin_amdgcn_exp2f(a.part_m[at] - ref);
     }
-#pragma unroll
-    for (int d = 32; d; d /= 2) {
-        sum += __shfl_xor(sum, d);
-        dot += __shfl_xor(dot, d);
-        sq += __shfl_xor(sq, d);
-    }
+    sum = wave_sum(sum);
+    dot = wave_sum(dot);
+    sq = wave_sum(sq);
     if (!lane) {
         sums[wave][0] = sum;
         sums[wave][1] = dot;
@@ -1150,7 +1148,7 @@ __global__ __launch_bounds__(THREADS, 2) void float_query_grads_kernel(XentArgs 
 // workgroup per (query, 256 columns), or per query where its length is needed.
 template <typename E, typename Q, typename O>
 __global__ __launch_bounds__(256) void join_query_grads_kernel(XentArgs a, Few f, O* out, uint64_t out_stride) {
-    __shared__ float sums[8];
+    __shared__ double sums[8];
     const uint32_t q = blockIdx.x;
     if (a.click[q] == NONE) {
         for (uint32_t d = blockIdx.y * 256 + threadIdx.x; d < a.dim; d += gridDim.y * 256) out[q * out_stride + d] = from_f32<O>(0.0f);
@@ -1160,7 +1158,7 @@ __global__ __launch_bounds__(256) void join_query_grads_kernel(XentArgs a, Few f
     const E* const clicked = static_cast<const E*>(f.rows) + (f.targets[q] - f.first_id) * f.stride;
     const float rest = a.click_rest[q];
     float* sum0 = a.part_q + (uint64_t)q * a.dim;
-    float dot = 0, sq = 0;
+    double dot = 0, sq = 0;  // (as in pack_queries_kernel)
     for (uint32_t d = blockIdx.y * 256 + threadIdx.x; d < a.dim; d += gridDim.y * 256) {
         float sum = sizeof(E) == 2 ? rest * to_f32(clicked[d]) : 0.0f;  // (of three planes nothing is left)
 #pragma unroll 8
@@ -1169,9 +1167,9 @@ __global__ __launch_bounds__(256) void join_query_grads_kernel(XentArgs a, Few f
             out[q * out_stride + d] = from_f32<O>(sum);
             continue;
         }
-        const float x = query_element<E>(query[d]);
-        dot = __builtin_fmaf(sum, x, dot);
-        sq = __builtin_fmaf(x, x, sq);
+        const double x = query_element<E>(query[d]);
+        dot += sum * x;
+        sq += x * x;
         sum0[d] = sum;
     }
     if (!a.norms) return;
@@ -1184,10 +1182,10 @@ __global__ __launch_bounds__(256) void join_query_grads_kernel(XentArgs a, Few f
     __syncthreads();
     dot = sums[0] + sums[1] + sums[2] + sums[3];
     sq = sums[4] + sums[5] + sums[6] + sums[7];
-    const float along = sq > 0 ? dot / sq : 0.0f;
+    const double along = sq > 0 ? dot / sq : 0.0;
     for (uint32_t d = threadIdx.x; d < a.dim; d += 256) {
-        const float x = query_element<E>(query[d]);
-        out[q * out_stride + d] = from_f32<O>(sum0[d] - along * x);
+        const double x = query_element<E>(query[d]);
+        out[q * out_stride + d] = from_f32<O>((float)(sum0[d] - along * x));
     }
 }
 

@@ -171,3 +171,19 @@ def test_large_logits_lose_nothing_to_their_size(gpu_ctx, dtype, n_q):
     want = bounds(queries, table, targets, None, scale, exact_products=True, exact_factor=True)
     check(loss, want["loss"], "loss")
     check(lse, want["lse"], "lse")
+
+
+@pytest.mark.parametrize("dtype,t", [(abi.VS_F32, F32), (abi.VS_BF16, BF16)])
+@pytest.mark.parametrize("n_q", [3, 70])
+@pytest.mark.parametrize("size", [1e25, 1e-25])
+def test_cosines_of_long_and_short_queries(store_of, dtype, t, n_q, size):
+    """Queries whose squares f32 does not hold: a cosine knows no length."""
+    rows, dim, scale = 300, 40, 12.0
+    table, queries = matrix(rows, dim, t, 20), (matrix(n_q, dim, F32, 21) * size).to(t).float()
+    store = store_of(dtype, abi.VS_ANGULAR, table.float().cpu().numpy())
+    targets = torch.arange(n_q, device=DEV).int() * 4
+    loss, lse, dq = store_loss_and_grad(store, queries, targets, scale)
+    want = bounds(queries, table, targets, None, scale, cosine=True, g_queries=weight_bits(t, n_q, F32)[0])
+    check(loss, want["loss"], "loss")
+    check(lse, want["lse"], "lse")
+    check(dq, rounded(want["queries"], F32), "gradient of the queries")
