@@ -633,7 +633,7 @@ __global__ __launch_bounds__(256) void loss_few_kernel(XentArgs a, Few f) {
             if (lane < n * NQ) {
                 if constexpr (NORMS) {
                     const float x = a.norms[r];
-                    z = x > 0 ? z / x : 0.0f;
+                    z = x == 0 ? 0.0f : z / x;  // (a row that holds a NaN has no length, and no logit)
                 }
                 if (r != click) {
                     // (an fma: of a logit of hundreds the rounding alone would show in the exponential)
@@ -714,7 +714,7 @@ __global__ __launch_bounds__(256) void join_loss_kernel(XentArgs a, Few f, float
     double z = f.scale * dot;
     if (a.norms) {
         const float x = a.norms[click];
-        z = x > 0 && sq != 0 ? z / (x * sqrt(sq)) : 0.0;
+        z = x == 0 || sq == 0 ? 0.0 : z / (x * sqrt(sq));
     }
     const double d = rest - z;
     loss[q] = (float)(d > 0 ? d + log1p(exp(-d)) : log1p(exp(d)));
@@ -739,7 +739,7 @@ __global__ __launch_bounds__(256) void click_weights_kernel(XentArgs a) {
     float g = query_factor(a, q) * expm1f(-a.loss[q]);
     if (a.norms) {
         const float x = a.norms[row_at(a, place)];
-        g = x > 0 ? g / x : 0.0f;
+        g = x == 0 ? 0.0f : g / x;
     }
     char* out = a.g + (uint64_t)(place - a.piece_begin) * a.g_stride + q * 2;
     for (uint32_t p = 0; p < a.g_planes; ++p) {

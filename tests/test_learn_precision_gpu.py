@@ -187,3 +187,25 @@ def test_cosines_of_long_and_short_queries(store_of, dtype, t, n_q, size):
     check(loss, want["loss"], "loss")
     check(lse, want["lse"], "lse")
     check(dq, rounded(want["queries"], F32), "gradient of the queries")
+
+
+@pytest.mark.parametrize("dtype,t", [(abi.VS_F32, F32), (abi.VS_BF16, BF16)])
+@pytest.mark.parametrize("metric", [abi.VS_ANGULAR, abi.VS_DOT])
+@pytest.mark.parametrize("n_q", [1, 4, 70])
+def test_a_documents_nan_is_no_number_in_any_loss(store_of, dtype, t, metric, n_q):
+    """Whichever way a batch of this size goes, as a candidate and as the clicked document; filtered out it is in none."""
+    rows, dim = 300, 40
+    table = matrix(rows, dim, t, 22).float().cpu().numpy()
+    table[7, 3] = np.nan
+    store = store_of(dtype, metric, table)
+    queries = matrix(n_q, dim, F32, 23)
+    keep = torch.ones(rows, dtype=torch.bool, device=DEV)
+    keep[7] = False
+    for first in (7, 100):
+        targets = (first + torch.arange(n_q, device=DEV)).int()
+        loss, lse, dq = store_loss_and_grad(store, queries, targets, 5.0)
+        assert torch.isnan(loss).all() and torch.isnan(dq).all()
+        loss, lse, dq = store_loss_and_grad(store, queries, targets, 5.0, words_of(torch.nn.functional.pad(keep, (0, 20))))
+        assert torch.isfinite(lse).all() and torch.isfinite(loss).all() and torch.isfinite(dq).all()
+        assert (loss[targets != 7] > 0).all() and (loss[targets == 7] == 0).all()
+    assert torch.isnan(store_loss_and_grad(store, queries, torch.full((n_q,), -1, device=DEV).int(), 5.0)[1]).all()
