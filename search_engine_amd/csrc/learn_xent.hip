@@ -465,11 +465,11 @@ __global__ __launch_bounds__(THREADS, 2) void loss_kernel(XentArgs a) {
     if (end > a.piece_begin)
         S::template run<0>(a, end, tile_q * BQ, along, lds, [&](f32x4 (&acc)[S::TM][S::TN], uint32_t first) {
             if constexpr (NORMS) {
-                // (the barriers of the steps before the next tile's end let everybody have read them. Of a row of zeros the
-                // factor is not zero, which would make a number of -inf as well)
+                // (the barriers of the steps before the next tile's end let everybody have read them. Where it would be zero,
+                // of a length of zero or infinity, the factor is not: it would make a NaN of the -inf of what is left out)
                 if (threadIdx.x < S::T) {
-                    const float x = first + threadIdx.x < end ? a.norms[row_at(a, first + threadIdx.x)] : 0.0f;
-                    inverse[threadIdx.x] = x > 0 ? 1.0f / x : 1e-37f;
+                    const float x = first + threadIdx.x < end ? a.norms[row_at(a, first + threadIdx.x)] : 0.0f, over = 1.0f / x;
+                    inverse[threadIdx.x] = x > 0 && over > 0 ? over : 1.4e-45f;
                 }
                 __syncthreads();
             }

@@ -209,3 +209,25 @@ def test_a_documents_nan_is_no_number_in_any_loss(store_of, dtype, t, metric, n_
         assert torch.isfinite(lse).all() and torch.isfinite(loss).all() and torch.isfinite(dq).all()
         assert (loss[targets != 7] > 0).all() and (loss[targets == 7] == 0).all()
     assert torch.isnan(store_loss_and_grad(store, queries, torch.full((n_q,), -1, device=DEV).int(), 5.0)[1]).all()
+
+
+@pytest.mark.parametrize("dtype,t", [(abi.VS_F32, F32), (abi.VS_BF16, BF16)])
+@pytest.mark.parametrize("n_q", [1, 4, 5, 70])
+def test_a_clicked_document_without_a_length(store_of, dtype, t, n_q):
+    """Documents whose length a store keeps as infinity (its square passes f32) or as zero have cosine zero with everything, as
+    in the searches' quotient; a click on one counts like any other."""
+    rows, dim, scale = 300, 40, 7.0
+    table, queries = matrix(rows, dim, t, 24), matrix(n_q, dim, F32, 25).to(t).float()
+    as_stored = table.float().clone()
+    for i in range(0, 2 * n_q + 8, 4):
+        as_stored[i] *= 1e36 if i % 8 else 1e25
+        as_stored[i + 1] = 0
+        table[i : i + 2] = 0
+    store = store_of(dtype, abi.VS_ANGULAR, as_stored.cpu().numpy())
+    targets = (torch.arange(n_q, device=DEV) * 2).int()
+    targets[1::2] -= 1
+    loss, lse, dq = store_loss_and_grad(store, queries, targets, scale)
+    want = bounds(queries, table, targets, None, scale, cosine=True, g_queries=weight_bits(t, n_q, F32)[0])
+    check(loss, want["loss"], "loss")
+    check(lse, want["lse"], "lse")
+    check(dq, rounded(want["queries"], F32), "gradient of the queries")
