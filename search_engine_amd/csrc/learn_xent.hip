@@ -457,8 +457,9 @@ __global__ __launch_bounds__(THREADS, 2) void loss_kernel(XentArgs a) {
     for (int n = 0; n < S::TN; ++n) {
         const uint32_t q = tile_q * BQ + (S::wave_q() * S::WQ + n) * 16 + (lane & 15);
         click[n] = q < a.n_q ? a.click[q] : NONE;
-        // (a factor of zero would make a number of the -inf that stands for what is left out: this one's logits are zero too)
-        s2[n] = __builtin_fmaxf(q < a.n_q ? a.qscale[q] * LOG2E : 0.0f, 1e-37f);
+        // (a factor of zero would make a NaN of the -inf that stands for what is left out: this one's logits are zero too)
+        s2[n] = q < a.n_q ? a.qscale[q] * LOG2E : 0.0f;
+        s2[n] = s2[n] == 0 ? 1.4e-45f : s2[n];
         m[n] = -__builtin_inff();
         l[n] = 0;
     }

@@ -231,3 +231,26 @@ def test_a_clicked_document_without_a_length(store_of, dtype, t, n_q):
     check(loss, want["loss"], "loss")
     check(lse, want["lse"], "lse")
     check(dq, rounded(want["queries"], F32), "gradient of the queries")
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("n_q", [4, 5, 70])
+def test_a_scale_that_is_no_number(gpu_ctx, dtype, n_q):
+    table, queries = matrix(300, 40, dtype, 26), matrix(n_q, 40, dtype, 27)
+    loss, lse = call_xent(gpu_ctx, queries, table, clicks(n_q, 300, None, 28), None, float("nan"))
+    assert torch.isnan(lse).all() and torch.isnan(loss[0])
+
+
+@pytest.mark.parametrize("n_q", [3, 5, 70])
+def test_long_queries_under_a_small_scale(store_of, n_q):
+    """The factor of a query's products, scale over length, is below the smallest normal f32."""
+    rows, dim, scale = 300, 40, 0.01
+    table, queries = matrix(rows, dim, F32, 29), matrix(n_q, dim, F32, 30) * 1e37
+    store = store_of(abi.VS_F32, abi.VS_ANGULAR, table.cpu().numpy())
+    targets = torch.arange(n_q, device=DEV).int() * 4
+    loss, lse, _ = store_loss_and_grad(store, queries, targets, scale)
+    want = bounds(queries, table, targets, None, scale, cosine=True)
+    # (in base 2 a factor near 1e-39 is a multiple of 2^-149: off by 2^-150 times products of up to 2^123 each)
+    for got, name in ((loss, "loss"), (lse, "lse")):
+        value, bound = want[name]
+        check(got, (value, bound + 2 * 2.0**-27), name)
