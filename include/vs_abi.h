@@ -463,7 +463,7 @@ int32_t vs_search_sharded_device(vs_group* g, vs_store* s, const void* d_queries
  *     nothing is kept between calls, so a call may be recorded into a graph (the
  *     vs_store_* calls may not: they record an event for the snapshot rule);
  *   - d_workspace: at least the bytes that the matching *_workspace_bytes call
- *     says, private to the call until the stream has passed it (two graphs that may
+ *     says (or *_call_workspace_bytes, of one call), private to the call until the stream has passed it (two graphs that may
  *     run at once need one each); VS_E_CAPACITY if workspace_bytes is less;
  *   - types are VS_F32 or VS_BF16; a stride counts elements from one row to the
  *     next, at least `dim`; rows whose address, stride and length are multiples of 16
@@ -543,6 +543,15 @@ int32_t vs_lookup_grad_weights_device(vs_ctx* ctx, const void* d_rows, int32_t d
  * number in what it takes part in. */
 int32_t vs_xent_workspace_bytes(vs_ctx* ctx, uint32_t n_q, uint64_t n_rows, uint32_t dim,
                                 int32_t dtype, uint64_t* bytes);
+/* What ONE call on these rows needs (gradients 0: vs_xent_device, else
+ * vs_xent_grad_device), and all that it is refused for. vs_xent_workspace_bytes is
+ * enough for either call on rows of any alignment, and so as much as 2 GiB and more:
+ * the weights of a gradient (1 GiB at a time) and the copies of rows that are not
+ * whole 16 bytes (1 GiB at a time). A loss needs neither weights nor, of aligned rows,
+ * copies: of up to four queries 16 KiB each. The rows are not read. */
+int32_t vs_xent_call_workspace_bytes(vs_ctx* ctx, uint32_t n_q, const void* d_rows,
+                                     uint64_t n_rows, uint64_t row_stride, int32_t dtype,
+                                     uint32_t dim, int32_t gradients, uint64_t* bytes);
 int32_t vs_xent_device(vs_ctx* ctx, const void* d_queries, uint32_t n_q, uint64_t query_stride,
                        const void* d_rows, uint64_t n_rows, uint64_t row_stride, int32_t dtype,
                        uint32_t dim, const uint32_t* d_targets, const uint64_t* d_mask_words,
@@ -572,6 +581,8 @@ int32_t vs_xent_grad_device(vs_ctx* ctx, const void* d_queries, uint32_t n_q, ui
  * d_mask_words as in vs_search_device (aligned to the store). The two calls of a step
  * see the same rows if no seal comes between them. */
 int32_t vs_store_xent_workspace_bytes(vs_store* s, uint32_t n_q, uint64_t* bytes);
+int32_t vs_store_xent_call_workspace_bytes(vs_store* s, uint32_t n_q, int32_t gradients,
+                                           uint64_t* bytes);
 int32_t vs_store_xent_device(vs_store* s, const float* d_queries, uint32_t n_q, uint32_t dim,
                              const uint32_t* d_targets, const uint64_t* d_mask_words, float scale,
                              void* d_workspace, uint64_t workspace_bytes, float* d_loss,

@@ -90,10 +90,12 @@ SIGNATURES = {
     "vs_lookup_grad_weights_device": [_vp, _vp, _i32, _u64, _u64, _u32, _vp, _u64, _vp, _u64, _f32, _vp, _i32, _u64,
                                       _vp, _vp],
     "vs_xent_workspace_bytes": [_vp, _u32, _u64, _u32, _i32, _u64p],
+    "vs_xent_call_workspace_bytes": [_vp, _u32, _vp, _u64, _u64, _i32, _u32, _i32, _u64p],
     "vs_xent_device": [_vp, _vp, _u32, _u64, _vp, _u64, _u64, _i32, _u32, _vp, _vp, _f32, _vp, _u64, _vp, _vp, _vp],
     "vs_xent_grad_device": [_vp, _vp, _u32, _u64, _vp, _u64, _u64, _i32, _u32, _vp, _vp, _f32, _vp, _vp, _vp, _vp, _u64,
                             _vp, _vp, _vp],
     "vs_store_xent_workspace_bytes": [_vp, _u32, _u64p],
+    "vs_store_xent_call_workspace_bytes": [_vp, _u32, _i32, _u64p],
     "vs_store_xent_device": [_vp, _vp, _u32, _u32, _vp, _vp, _f32, _vp, _u64, _vp, _vp, _vp],
     "vs_store_xent_grad_device": [_vp, _vp, _u32, _u32, _vp, _vp, _f32, _vp, _vp, _vp, _vp, _u64, _vp, _vp],
     "vs_roaring_to_mask": [_u8p, _sz, _u64p, _u64, _u64p],
@@ -275,6 +277,13 @@ class Context:
     def xent_workspace_bytes(self, n_q, n_rows, dim, dtype):
         b = ctypes.c_uint64(0)
         _check(lib.vs_xent_workspace_bytes(self.handle, n_q, n_rows, dim, dtype, ctypes.byref(b)), self.handle)
+        return b.value
+
+    def xent_call_workspace_bytes(self, n_q, d_rows, n_rows, row_stride, dtype, dim, gradients):
+        """What one xent_device (gradients False) or xent_grad_device on these rows needs."""
+        b = ctypes.c_uint64(0)
+        _check(lib.vs_xent_call_workspace_bytes(self.handle, n_q, d_rows, n_rows, row_stride, dtype, dim, int(gradients),
+                                                ctypes.byref(b)), self.handle)
         return b.value
 
     def xent_device(self, d_queries, n_q, query_stride, d_rows, n_rows, row_stride, dtype, dim, d_targets, d_mask, scale,
@@ -520,6 +529,12 @@ class Store:
     def xent_workspace_bytes(self, n_q):
         b = ctypes.c_uint64(0)
         self._ck(lib.vs_store_xent_workspace_bytes(self.handle, n_q, ctypes.byref(b)))
+        return b.value
+
+    def xent_call_workspace_bytes(self, n_q, gradients):
+        """What one xent_device (gradients False) or xent_grad_device needs."""
+        b = ctypes.c_uint64(0)
+        self._ck(lib.vs_store_xent_call_workspace_bytes(self.handle, n_q, int(gradients), ctypes.byref(b)))
         return b.value
 
     def xent_device(self, d_queries, n_q, dim, d_targets, d_mask, scale, d_workspace, workspace_bytes, d_loss, d_lse,

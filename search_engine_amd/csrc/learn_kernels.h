@@ -58,7 +58,11 @@ struct Xent {
     const float* norms;       // not null: the rows' lengths; logits are scale * cosine
     float scale;
 };
-uint64_t xent_workspace_bytes(uint32_t n_q, uint64_t n_rows, uint32_t dim, int32_t dtype);
+// What a call needs: the loss, or the gradients, of n_q queries over rows of this layout (`aligned`: read straight from the
+// table, see rows_are_aligned).
+uint64_t xent_workspace_bytes(uint32_t n_q, uint64_t n_rows, uint32_t dim, int32_t dtype, bool aligned, bool gradients);
+// Whether rows are whole 16-byte chunks at multiples of 16 bytes; others are copied to such, in the workspace.
+bool rows_are_aligned(const Table& t);
 hipError_t launch_xent(const Xent& x, void* workspace, float* loss, float* lse, hipStream_t stream);
 // (gradients are of the queries' and the rows' types)
 hipError_t launch_xent_grad(const Xent& x, const float* loss, const float* lse, const float* grad_loss, void* workspace,

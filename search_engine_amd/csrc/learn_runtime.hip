@@ -1,5 +1,7 @@
 // The entry points that learn from clicks (declared in include/vs_abi.h): argument checks, the snapshot of a store,
 // and the launches of learn_lookup.hip and learn_xent.hip. No computation happens here.
+#include <algorithm>
+
 #include "learn_kernels.h"
 #include "vs_internal.h"
 
@@ -120,17 +122,26 @@ int32_t status(hipError_t e, const char* what) {
 
 hipStream_t stream_of(void* s) { return static_cast<hipStream_t>(s); }
 
+// Enough for the loss and the gradients both.
+uint64_t xent_bytes(uint32_t n_q, uint64_t n_rows, uint32_t dim, int32_t dtype, bool aligned) {
+    if (!n_q) return 0;
+    return std::max(learn::xent_workspace_bytes(n_q, n_rows, dim, dtype, aligned, false),
+                    learn::xent_workspace_bytes(n_q, n_rows, dim, dtype, aligned, true));
+}
+uint64_t xent_bytes(const learn::Table& t, uint32_t n_q, bool gradients) {
+    return n_q ? learn::xent_workspace_bytes(n_q, t.n_rows, t.dim, t.dtype, learn::rows_are_aligned(t), gradients) : 0;
+}
+
 // vs_xent_device and vs_xent_grad_device share their arguments.
 int32_t make_xent(const void* queries, uint32_t n_q, uint64_t query_stride, const void* rows, uint64_t n_rows,
                   uint64_t row_stride, int32_t dtype, uint32_t dim, const uint32_t* targets, const uint64_t* mask, float scale,
-                  const void* workspace, uint64_t workspace_bytes, learn::Xent* x) {
+                  const void* workspace, uint64_t workspace_bytes, bool gradients, learn::Xent* x) {
     *x = learn::Xent{};
     if (int32_t rc = make_table(rows, dtype, n_rows, row_stride, dim, &x->t)) return rc;
     if (int32_t rc = check_queries(n_q)) return rc;
     if (int32_t rc = check_matrix("queries", queries, dtype, n_q, query_stride, dim)) return rc;
     if (n_q && !targets) return fail(VS_E_INVALID_ARG, "targets: null device buffer");
-    if (int32_t rc = check_workspace(workspace, workspace_bytes, n_q ? learn::xent_workspace_bytes(n_q, n_rows, dim, dtype) : 0,
-                                     "vs_xent_workspace_bytes"))
+    if (int32_t rc = check_workspace(workspace, workspace_bytes, xent_bytes(x->t, n_q, gradients), "vs_xent_workspace_bytes"))
         return rc;
     x->queries = queries;
     x->queries_f32 = dtype == VS_F32;
@@ -226,7 +237,18 @@ extern "C" int32_t vs_xent_workspace_bytes(vs_ctx* ctx, uint32_t n_q, uint64_t n
     if (dim == 0 || dim > VS_LEARN_MAX_DIM) return fail(VS_E_INVALID_ARG, "dimension %u out of range", dim);
     if (!is_float(dtype)) return fail(VS_E_INVALID_ARG, "element type %d is not VS_F32 or VS_BF16", dtype);
     if (!ctx) return fail(VS_E_INVALID_ARG, "null context");
-    *bytes = n_q ? learn::xent_workspace_bytes(n_q, n_rows, dim, dtype) : 0;
+    *bytes = xent_bytes(n_q, n_rows, dim, dtype, false);
+    return VS_OK;
+}
+
+extern "C" int32_t vs_xent_call_workspace_bytes(vs_ctx* ctx, uint32_t n_q, const void* d_rows, uint64_t n_rows, uint64_t row_stride,
+                                                int32_t dtype, uint32_t dim, int32_t gradients, uint64_t* bytes) {
+    if (!bytes) return fail(VS_E_INVALID_ARG, "null argument");
+    learn::Table t;
+    if (int32_t rc = check_queries(n_q)) return rc;
+    if (int32_t rc = make_table(d_rows, dtype, n_rows, row_stride, dim, &t)) return rc;
+    if (!ctx) return fail(VS_E_INVALID_ARG, "null context");
+    *bytes = xent_bytes(t, n_q, gradients != 0);
     return VS_OK;
 }
 
@@ -236,7 +258,7 @@ extern "C" int32_t vs_xent_device(vs_ctx* ctx, const void* d_queries, uint32_t n
                                   float* d_loss, float* d_lse, void* hip_stream) {
     learn::Xent x;
     if (int32_t rc = make_xent(d_queries, n_q, query_stride, d_rows, n_rows, row_stride, dtype, dim, d_targets, d_mask_words,
-                               scale, d_workspace, workspace_bytes, &x))
+                               scale, d_workspace, workspace_bytes, false, &x))
         return rc;
     if (n_q && (!d_loss || !d_lse)) return fail(VS_E_INVALID_ARG, "loss or lse: null device buffer");
     if (int32_t rc = use_ctx(ctx)) return rc;
@@ -251,7 +273,7 @@ extern "C" int32_t vs_xent_grad_device(vs_ctx* ctx, const void* d_queries, uint3
                                        void* d_grad_rows, void* hip_stream) {
     learn::Xent x;
     if (int32_t rc = make_xent(d_queries, n_q, query_stride, d_rows, n_rows, row_stride, dtype, dim, d_targets, d_mask_words,
-                               scale, d_workspace, workspace_bytes, &x))
+                               scale, d_workspace, workspace_bytes, true, &x))
         return rc;
     if (n_q && (!d_loss || !d_lse)) return fail(VS_E_INVALID_ARG, "loss or lse: null device buffer");
     for (const void* p : {(const void*)d_grad_queries, (const void*)d_grad_rows})
@@ -265,7 +287,16 @@ extern "C" int32_t vs_store_xent_workspace_bytes(vs_store* s, uint32_t n_q, uint
     if (!s || !bytes) return fail(VS_E_INVALID_ARG, "null argument");
     if (!is_float(s->dtype)) return fail(VS_E_INVALID_ARG, "store %u holds no f32 or bf16 rows", s->index);
     if (int32_t rc = check_queries(n_q)) return rc;
-    *bytes = n_q ? learn::xent_workspace_bytes(n_q, s->view(0).n_slots, s->dim, s->dtype) : 0;
+    const learn::Table t = table_of(s->view(0));
+    *bytes = std::max(xent_bytes(t, n_q, false), xent_bytes(t, n_q, true));
+    return VS_OK;
+}
+
+extern "C" int32_t vs_store_xent_call_workspace_bytes(vs_store* s, uint32_t n_q, int32_t gradients, uint64_t* bytes) {
+    if (!s || !bytes) return fail(VS_E_INVALID_ARG, "null argument");
+    if (!is_float(s->dtype)) return fail(VS_E_INVALID_ARG, "store %u holds no f32 or bf16 rows", s->index);
+    if (int32_t rc = check_queries(n_q)) return rc;
+    *bytes = xent_bytes(table_of(s->view(0)), n_q, gradients != 0);
     return VS_OK;
 }
 
@@ -277,8 +308,7 @@ extern "C" int32_t vs_store_xent_device(vs_store* s, const float* d_queries, uin
     if (!d_loss || !d_lse) return fail(VS_E_INVALID_ARG, "loss or lse: null device buffer");
     hipStream_t stream = stream_of(hip_stream);
     return over_store(s, stream, [&](const vs::SlabView& v) {
-        if (int32_t rc = check_workspace(d_workspace, workspace_bytes, learn::xent_workspace_bytes(n_q, v.n_slots, v.dim, v.dtype),
-                                         "vs_store_xent_workspace_bytes"))
+        if (int32_t rc = check_workspace(d_workspace, workspace_bytes, xent_bytes(table_of(v), n_q, false), "vs_store_xent_workspace_bytes"))
             return rc;
         return status(learn::launch_xent(xent_of(v, d_queries, n_q, d_targets, d_mask_words, scale), d_workspace, d_loss, d_lse, stream),
                       "cross entropy");
@@ -294,8 +324,7 @@ extern "C" int32_t vs_store_xent_grad_device(vs_store* s, const float* d_queries
     if (!d_loss || !d_lse || !d_grad_queries) return fail(VS_E_INVALID_ARG, "loss, lse or grad_queries: null device buffer");
     hipStream_t stream = stream_of(hip_stream);
     return over_store(s, stream, [&](const vs::SlabView& v) {
-        if (int32_t rc = check_workspace(d_workspace, workspace_bytes, learn::xent_workspace_bytes(n_q, v.n_slots, v.dim, v.dtype),
-                                         "vs_store_xent_workspace_bytes"))
+        if (int32_t rc = check_workspace(d_workspace, workspace_bytes, xent_bytes(table_of(v), n_q, true), "vs_store_xent_workspace_bytes"))
             return rc;
         return status(learn::launch_xent_grad(xent_of(v, d_queries, n_q, d_targets, d_mask_words, scale), d_loss, d_lse, d_grad_loss,
                                               d_workspace, d_grad_queries, v.dim, nullptr, 0, stream), "cross entropy gradient");

@@ -1289,25 +1289,35 @@ struct Buffers {
     char *q, *qt, *g, *packed, *spill;
     uint64_t bytes;
 };
-Buffers carve(void* workspace, const Plan& p, uint32_t n_q, uint64_t n_rows, uint32_t dim) {
+// What a call does not use is not there: of the loss of few queries all but its shares, of other losses what belongs to the
+// gradients, of rows that are aligned their copies.
+Buffers carve(void* workspace, const Plan& p, uint32_t n_q, uint64_t n_rows, uint32_t dim, bool aligned, bool gradients) {
     Carver w(workspace);
-    Buffers b;
+    Buffers b{};
+    if (!gradients) {
+        const uint64_t parts = n_q * (uint64_t)(p.few ? FEW_WORKGROUPS : p.score_splits);
+        b.part_m = w.take<float>(parts);
+        b.part_l = w.take<float>(parts);
+        if (p.few) {
+            b.bytes = w.at() - (char*)workspace;
+            return b;
+        }
+    }
     b.zeros = w.take<uint32_t>(64);
     b.list = w.take<uint32_t>(n_rows);
     b.count = w.take<uint32_t>(1);
     b.sums = w.take<uint32_t>(list_blocks(n_rows));
     b.click = w.take<uint32_t>(n_q);
     b.qscale = w.take<float>(n_q);
-    b.click_rest = w.take<float>(n_q);
     b.q = w.take<char>((uint64_t)n_q * p.kp * 2 * p.planes);
-    b.qt = w.take<char>((uint64_t)dim * p.gq * 2 * p.planes);
-    const uint64_t parts = n_q * (uint64_t)(p.few ? FEW_WORKGROUPS : p.score_splits);
-    b.part_m = w.take<float>(parts);
-    b.part_l = w.take<float>(parts);
-    b.g = w.take<char>(p.piece_rows * p.q_tiles * p.bq * 2 * p.g_planes);
-    b.spill = w.take<char>(16ull * THREADS * WORKGROUPS);
-    b.part_q = w.take<float>((uint64_t)p.grad_splits * n_q * dim);
-    b.packed = w.take<char>(p.packed_rows * p.kp * (p.planes == 3 ? 4 : 2));
+    if (gradients) {
+        b.click_rest = w.take<float>(n_q);
+        b.qt = w.take<char>((uint64_t)dim * p.gq * 2 * p.planes);
+        b.g = w.take<char>(p.piece_rows * p.q_tiles * p.bq * 2 * p.g_planes);
+        b.spill = w.take<char>(16ull * THREADS * WORKGROUPS);
+        b.part_q = w.take<float>((uint64_t)p.grad_splits * n_q * dim);
+    }
+    if (!aligned) b.packed = w.take<char>(p.packed_rows * p.kp * (p.planes == 3 ? 4 : 2));
     b.bytes = w.at() - (char*)workspace;
     return b;
 }
@@ -1328,11 +1338,10 @@ struct Call {
 
     Call(const Xent& x_, void* workspace, bool gradients, bool rows_too, hipStream_t stream_)
         : x(x_), p(plan_for(x.n_q, x.t.n_rows, x.t.dim, x.t.dtype, rows_too || two_for_queries(x))),
-          b(carve(workspace, p, x.n_q, x.t.n_rows, x.t.dim)), stream(stream_) {
+          b(carve(workspace, p, x.n_q, x.t.n_rows, x.t.dim, rows_are_aligned(x.t), gradients)), stream(stream_) {
         const uint32_t dim = x.t.dim;
-        // straight from the table where a row is whole 16-byte chunks at multiples of 16 bytes
         const uint32_t size = x.t.dtype == VS_F32 ? 4 : 2, chunk = 16 / size;
-        packed = (uintptr_t)x.t.rows % 16 || x.t.stride % chunk || x.t.stride * size > 0xFFFFFFFFu || dim % chunk;
+        packed = !rows_are_aligned(x.t);
         a.n_rows = x.t.n_rows;
         a.norms = x.norms;
         a.q = Planes{b.q, (uint64_t)x.n_q * p.kp * 2, p.kp * 2, nullptr, x.n_q, p.kp / 8};
@@ -1510,7 +1519,7 @@ hipError_t pick_loss_few(const Xent& x, const XentArgs& a, const Few& f, float* 
     }
 }
 hipError_t launch_loss_few(const Xent& x, void* workspace, float* loss, float* lse, hipStream_t stream) {
-    const Buffers b = carve(workspace, plan_for(x.n_q, x.t.n_rows, x.t.dim, x.t.dtype, false), x.n_q, x.t.n_rows, x.t.dim);
+    const Buffers b = carve(workspace, plan_for(x.n_q, x.t.n_rows, x.t.dim, x.t.dtype, false), x.n_q, x.t.n_rows, x.t.dim, true, false);
     XentArgs a{};
     a.n_rows = x.t.n_rows;
     a.dim = x.t.dim;
@@ -1535,9 +1544,15 @@ void clear_rows(const Xent& x, void* grad_rows, uint64_t stride, bool all, hipSt
 
 }  // namespace
 
-uint64_t xent_workspace_bytes(uint32_t n_q, uint64_t n_rows, uint32_t dim, int32_t dtype) {
+bool rows_are_aligned(const Table& t) {
+    const uint32_t size = t.dtype == VS_F32 ? 4 : 2, chunk = 16 / size;
+    return (uintptr_t)t.rows % 16 == 0 && t.stride % chunk == 0 && t.stride * size <= 0xFFFFFFFFu && t.dim % chunk == 0;
+}
+
+uint64_t xent_workspace_bytes(uint32_t n_q, uint64_t n_rows, uint32_t dim, int32_t dtype, bool aligned, bool gradients) {
     uint64_t bytes = 0;
-    for (bool two : {false, true}) bytes = std::max(bytes, carve(nullptr, plan_for(n_q, n_rows, dim, dtype, two), n_q, n_rows, dim).bytes);
+    for (bool two : {false, true})
+        bytes = std::max(bytes, carve(nullptr, plan_for(n_q, n_rows, dim, dtype, two), n_q, n_rows, dim, aligned, gradients).bytes);
     return bytes + 256;
 }
 
