@@ -549,45 +549,98 @@ __global__ __launch_bounds__(THREADS, 2) void loss_kernel(XentArgs a) {
     a.part_l[to] = sum;
 }
 
-// Up to four queries: bound by the rows' bytes (one over 1M x 768 bf16: 237 us, 6.5 TB/s), so plain f32 products, straight from the table and under the masks
-// themselves, with nothing laid out before. A wave takes the words of the masks in turn, and of each word's candidates U at
-// a time: their loads are in flight together, and the U x NQ sums over the lanes leave each (candidate, query) to a lane
-// of its own, which keeps the running largest and sum of its logits.
+// Up to four queries: bound by the rows' bytes (one over 1M x 768 bf16: 237 us, 6.5 TB/s), so plain f32 products, straight from
+// the table. The loss and the weights of the gradients share them, bit for bit: of a document that has nearly all of the
+// probability, what its logit is off by is in lse and in its weight, and cancels only if it is the same.
+template <typename E, typename Q, int V, int NQ, bool NORMS>
+struct FewScores {
+    static constexpr int U = NQ == 1 ? 8 : 4;  // candidates that a wave takes at a time, their loads in flight together
+    uint32_t chunks, padded;                   // (a last, broken piece: see Piece)
+    float* query;                              // [NQ][padded], as they are multiplied
+    float factor;                              // of the lane's query, lane % NQ, base 2
+
+    // By the whole workgroup of 256.
+    __device__ __forceinline__ void init(const XentArgs& a, const Few& f, char* lds, double* sums /* 4, LDS */) {
+        const uint32_t lane = threadIdx.x & 63, wave = uniform_u32(threadIdx.x >> 6);
+        chunks = (a.dim + V - 1) / V;
+        padded = chunks * V;
+        query = reinterpret_cast<float*>(lds);
+        factor = 0;
+        const Q* queries = static_cast<const Q*>(f.queries);
+        for (int q = 0; q < NQ; ++q) {
+            double sq = 0;  // (as in pack_queries_kernel)
+            for (uint32_t d = threadIdx.x; d < padded; d += 256) {
+                const Piece<V> piece(d / V, a.dim);
+                const uint32_t from = piece.col + d % V;
+                const float x = d % V >= piece.skip && from < a.dim ? query_element<E>(queries[q * f.query_stride + from]) : 0.0f;
+                query[q * padded + d] = x;
+                if constexpr (NORMS) sq += (double)x * x;
+            }
+            float scale = f.scale * LOG2E;
+            if constexpr (NORMS) {
+                sq = wave_sum(sq);
+                __syncthreads();
+                if (!lane) sums[wave] = sq;
+                __syncthreads();
+                const float norm = (float)sqrt(sums[0] + sums[1] + sums[2] + sums[3]);
+                scale = norm > 0 ? scale / norm : 0.0f;
+            }
+            if (lane % NQ == (uint32_t)q) factor = scale;
+        }
+        __syncthreads();
+    }
+    // Lane u NQ + q gets candidate u's product with query q, and its row (cosines: over the row's length, and that).
+    __device__ __forceinline__ float products(const XentArgs& a, const Few& f, const uint32_t (&row)[U], uint32_t* its_row, float* length) const {
+        const uint32_t lane = threadIdx.x & 63;
+        const E* const table = static_cast<const E*>(f.rows);
+        float acc[U][NQ] = {};
+        for (uint32_t c = lane; c < chunks; c += 64) {
+            Pack<E, V> x[U];
+#pragma unroll
+            for (int u = 0; u < U; ++u) x[u] = load_piece_once<E, V>(table + (uint64_t)row[u] * f.stride, Piece<V>(c, a.dim), a.dim);
+#pragma unroll
+            for (int q = 0; q < NQ; ++q) {
+                const Pack<float, V> y = load_pack<float, V>(query + q * padded + c * V);
+#pragma unroll
+                for (int u = 0; u < U; ++u)
+#pragma unroll
+                    for (int v = 0; v < V; ++v) acc[u][q] = __builtin_fmaf(to_f32(x[u].e[v]), y.e[v], acc[u][q]);
+            }
+        }
+        float z = 0;
+        uint32_t r = row[0];
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+            for (int q = 0; q < NQ; ++q) {
+                const float sum = wave_sum(acc[u][q]);
+                if (lane == (uint32_t)(u * NQ + q)) {
+                    z = sum;
+                    r = row[u];
+                }
+            }
+        *its_row = r;
+        if constexpr (NORMS) {
+            *length = a.norms[r];
+            z = *length == 0 ? 0.0f : z / *length;  // (a row that holds a NaN has no length, and no logit)
+        }
+        return z;
+    }
+};
+
+// The loss, under the masks themselves, with nothing laid out before. A wave takes the words of the masks in turn, and of each
+// word's candidates U at a time; the lane of each (candidate, query) keeps the running largest and sum of its logits.
 template <typename E, typename Q, int V, int NQ, bool NORMS>
 __global__ __launch_bounds__(256) void loss_few_kernel(XentArgs a, Few f) {
-    constexpr int U = NQ == 1 ? 8 : 4;
+    using S = FewScores<E, Q, V, NQ, NORMS>;
+    constexpr int U = S::U;
     extern __shared__ __attribute__((aligned(128))) char lds[];
     __shared__ float sm[4][64], sl[4][64];
     __shared__ double sums[4];
-    float* const query = reinterpret_cast<float*>(lds);  // [NQ][padded], as they are multiplied
-    const uint32_t lane = threadIdx.x & 63, wave = uniform_u32(threadIdx.x >> 6);
-    const uint32_t chunks = (a.dim + V - 1) / V, padded = chunks * V;  // (a last, broken piece: see Piece)
-    const Q* queries = static_cast<const Q*>(f.queries);
-    float factor = 0;  // of the lane's query, base 2
-    const uint32_t mine = lane % NQ;
-    for (int q = 0; q < NQ; ++q) {
-        double sq = 0;  // (as in pack_queries_kernel)
-        for (uint32_t d = threadIdx.x; d < padded; d += 256) {
-            const Piece<V> piece(d / V, a.dim);
-            const uint32_t from = piece.col + d % V;
-            const float x = d % V >= piece.skip && from < a.dim ? query_element<E>(queries[q * f.query_stride + from]) : 0.0f;
-            query[q * padded + d] = x;
-            if constexpr (NORMS) sq += (double)x * x;
-        }
-        float scale = f.scale * LOG2E;
-        if constexpr (NORMS) {
-            sq = wave_sum(sq);
-            __syncthreads();
-            if (!lane) sums[wave] = sq;
-            __syncthreads();
-            const float norm = (float)sqrt(sums[0] + sums[1] + sums[2] + sums[3]);
-            scale = norm > 0 ? scale / norm : 0.0f;
-        }
-        if (mine == (uint32_t)q) factor = scale;
-    }
-    __syncthreads();
+    const uint32_t lane = threadIdx.x & 63, wave = uniform_u32(threadIdx.x >> 6), mine = lane % NQ;
+    S scores;
+    scores.init(a, f, lds, sums);
     const uint32_t click = f.targets[mine] < f.first_id ? NONE : f.targets[mine] - f.first_id;
-    const E* const table = static_cast<const E*>(f.rows);
     float m = -__builtin_inff(), l = 0;
     const uint32_t n_units = (uint32_t)((a.n_rows + 63) / 64) * f.parts, size = 64 / f.parts;
     for (uint32_t i = blockIdx.x * 4 + wave; i < n_units; i += gridDim.x * 4) {
@@ -604,44 +657,14 @@ __global__ __launch_bounds__(256) void loss_few_kernel(XentArgs a, Few f) {
                 n += bits != 0;
                 bits &= bits - 1;
             }
-            float acc[U][NQ] = {};
-            for (uint32_t c = lane; c < chunks; c += 64) {
-                Pack<E, V> x[U];
-#pragma unroll
-                for (int u = 0; u < U; ++u) x[u] = load_piece_once<E, V>(table + (uint64_t)row[u] * f.stride, Piece<V>(c, a.dim), a.dim);
-#pragma unroll
-                for (int q = 0; q < NQ; ++q) {
-                    const Pack<float, V> y = load_pack<float, V>(query + q * padded + c * V);
-#pragma unroll
-                    for (int u = 0; u < U; ++u)
-#pragma unroll
-                        for (int v = 0; v < V; ++v) acc[u][q] = __builtin_fmaf(to_f32(x[u].e[v]), y.e[v], acc[u][q]);
-                }
-            }
-            // lane u NQ + q takes candidate u's product with query q
-            float z = 0;
-            uint32_t r = 0;
-#pragma unroll
-            for (int u = 0; u < U; ++u)
-#pragma unroll
-                for (int q = 0; q < NQ; ++q) {
-                    const float sum = wave_sum(acc[u][q]);
-                    if (lane == (uint32_t)(u * NQ + q)) {
-                        z = sum;
-                        r = row[u];
-                    }
-                }
-            if (lane < n * NQ) {
-                if constexpr (NORMS) {
-                    const float x = a.norms[r];
-                    z = x == 0 ? 0.0f : z / x;  // (a row that holds a NaN has no length, and no logit)
-                }
-                if (r != click) {
-                    // (an fma: of a logit of hundreds the rounding alone would show in the exponential)
-                    const float top = __builtin_fmaxf(m, z * factor), ref = finite_or_zero(top);
-                    l = l * __builtin_amdgcn_exp2f(m - ref) + __builtin_amdgcn_exp2f(__builtin_fmaf(z, factor, -ref));
-                    m = top;
-                }
+            uint32_t r;
+            float length;
+            const float z = scores.products(a, f, row, &r, &length);
+            if (lane < n * NQ && r != click) {
+                // (an fma: of a logit of hundreds the rounding alone would show in the exponential)
+                const float top = __builtin_fmaxf(m, z * scores.factor), ref = finite_or_zero(top);
+                l = l * __builtin_amdgcn_exp2f(m - ref) + __builtin_amdgcn_exp2f(__builtin_fmaf(z, scores.factor, -ref));
+                m = top;
             }
         }
     }
@@ -729,6 +752,17 @@ __device__ __forceinline__ float query_factor(const XentArgs& a, uint32_t q) {
     return (a.grad_loss ? a.grad_loss[q] : 1.0f) * a.qscale[q] * a.sign;
 }
 
+// lse in base 2 has a rounding of its own, half a step of a number near 20: as a relative error of all of a query's weights
+// it would be ten times the roundings of the products. What is behind it goes into the factor.
+struct Base2 {
+    float high, rest;
+    __device__ __forceinline__ explicit Base2(float lse) {
+        high = lse * LOG2E;
+        const float low = __builtin_fmaf(lse, LOG2E, -high) + lse * LOG2E_REST;
+        rest = low == low ? __builtin_amdgcn_exp2f(-low) : 1.0f;
+    }
+};
+
 // The weights of the clicked rows of a piece, after weights_kernel, which takes every row alike (to look for them there
 // costs two instructions in eight of each element). A clicked row's weight is as large as all others of its query together:
 // what its rounding takes away is kept, and goes into the query's gradient at the end.
@@ -770,14 +804,11 @@ __global__ __launch_bounds__(THREADS, 2) void weights_kernel(XentArgs a) {
     if (end <= a.piece_begin) return;
     if (threadIdx.x < BQ) {
         const uint32_t q = q0 + threadIdx.x;
-        // lse in base 2 has a rounding of its own, half a step of a number near 20: as a relative error of all of a
-        // query's weights it would be ten times the roundings of the products. What is behind it goes into the factor.
         const bool in = q < a.n_q && a.click[q] != NONE;
-        const float lse = in ? a.lse[q] : 0.0f, high = lse * LOG2E;
-        const float low = __builtin_fmaf(lse, LOG2E, -high) + lse * LOG2E_REST;
+        const Base2 lse(in ? a.lse[q] : 0.0f);
         s2[threadIdx.x] = in ? a.qscale[q] * LOG2E : 0.0f;
-        lse2[threadIdx.x] = high;
-        factor[threadIdx.x] = in ? query_factor(a, q) * (low == low ? __builtin_amdgcn_exp2f(-low) : 1.0f) : 0.0f;
+        lse2[threadIdx.x] = lse.high;
+        factor[threadIdx.x] = in ? query_factor(a, q) * lse.rest : 0.0f;
     }
     // (the first barrier of the loop below orders these before they are read)
     // Every lane stores every time (so that the number of stores is known to the next step's barrier): rows of G are whole
@@ -834,6 +865,47 @@ __global__ __launch_bounds__(THREADS, 2) void weights_kernel(XentArgs a) {
             }
         return true;
     });
+}
+
+// The same of up to four queries, from the products that their loss was made of: a wave takes U neighbouring places at a time.
+// Rows of G are those of 64 queries, zeros from NQ on.
+template <typename E, typename Q, int V, int NQ, bool NORMS>
+__global__ __launch_bounds__(256) void weights_few_kernel(XentArgs a, Few f) {
+    using S = FewScores<E, Q, V, NQ, NORMS>;
+    constexpr int U = S::U, PG = sizeof(E) == 4 ? 3 : 2;
+    extern __shared__ __attribute__((aligned(128))) char lds[];
+    __shared__ double sums[4];
+    const uint32_t lane = threadIdx.x & 63, wave = uniform_u32(threadIdx.x >> 6), mine = lane % NQ;
+    S scores;
+    scores.init(a, f, lds, sums);
+    const uint32_t end = min(candidates(a), a.piece_begin + a.piece_rows);
+    const bool in = a.click[mine] != NONE;
+    const Base2 lse(in ? a.lse[mine] : 0.0f);
+    const float factor = in ? query_factor(a, mine) * lse.rest : 0.0f;
+    for (uint32_t place = a.piece_begin + (blockIdx.x * 4 + wave) * U; place < end; place += gridDim.x * 4 * U) {
+        uint32_t row[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) row[u] = uniform_u32((uint32_t)row_at(a, min(place + u, end - 1)));
+        uint32_t r;
+        float length;
+        const float z = scores.products(a, f, row, &r, &length);
+        float g = factor * __builtin_amdgcn_exp2f(__builtin_fmaf(z, scores.factor, -lse.high));
+        if constexpr (NORMS) g = length == 0 ? 0.0f : g / length;
+        const Split x = split(in ? g : 0.0f);
+        const uint32_t planes[3] = {x.h, x.m, x.l};
+        const uint32_t u = lane / 8, chunk = lane % 8;  // the 16 bytes of a row that the lane stores
+#pragma unroll
+        for (int k = 0; k < PG; ++k) {
+            Pack<uint16_t, 8> p = {};
+#pragma unroll
+            for (int q = 0; q < NQ; ++q) {
+                const uint32_t w = __shfl(planes[k], u * NQ + q);
+                p.e[q] = chunk ? 0 : (uint16_t)w;
+            }
+            if (u < U && place + u < end)
+                store_pack<uint16_t, 8>(reinterpret_cast<uint16_t*>(a.g + k * a.g_plane + (uint64_t)(place + u - a.piece_begin) * a.g_stride) + chunk * 8, p);
+        }
+    }
 }
 
 // drows of a piece: transposed queries (BD columns of the rows) by G. The sums are short (as many steps as 64 queries, or six
@@ -1498,25 +1570,32 @@ struct Call {
     }
 };
 
-template <typename E, typename Q, int V, int NQ>
+// Calls `f` with FewScores for a few queries of this call, as a type.
+template <typename E, typename Q, int V, typename F>
+void with_few_scores(uint32_t n_q, bool norms, F&& f) {
+    auto by_norms = [&](auto nq) {
+        if (norms)
+            f(FewScores<E, Q, V, nq, true>{}, nq, std::true_type{});
+        else
+            f(FewScores<E, Q, V, nq, false>{}, nq, std::false_type{});
+    };
+    switch (n_q) {
+        case 1: return by_norms(std::integral_constant<int, 1>{});
+        case 2: return by_norms(std::integral_constant<int, 2>{});
+        case 3: return by_norms(std::integral_constant<int, 3>{});
+        default: return by_norms(std::integral_constant<int, 4>{});
+    }
+}
+uint32_t few_lds(uint32_t n_q, uint32_t dim, uint32_t v) { return n_q * (uint32_t)round_up(dim, v) * 4; }
+
+template <typename E, typename Q, int V>
 hipError_t run_loss_few(const Xent& x, XentArgs a, const Few& f, float* loss, float* lse, hipStream_t stream) {
     a.splits = (uint32_t)std::min<uint64_t>(((x.t.n_rows + 63) / 64 * f.parts + 3) / 4, FEW_WORKGROUPS);
-    const uint32_t lds = NQ * (uint32_t)round_up(a.dim, V) * 4;
-    if (a.norms)
-        loss_few_kernel<E, Q, V, NQ, true><<<a.splits, 256, lds, stream>>>(a, f);
-    else
-        loss_few_kernel<E, Q, V, NQ, false><<<a.splits, 256, lds, stream>>>(a, f);
+    with_few_scores<E, Q, V>(x.n_q, a.norms, [&](auto, auto nq, auto norms) {
+        loss_few_kernel<E, Q, V, nq, norms><<<a.splits, 256, few_lds(x.n_q, a.dim, V), stream>>>(a, f);
+    });
     join_loss_kernel<E, Q><<<x.n_q, 256, 0, stream>>>(a, f, loss, lse);
     return hipGetLastError();
-}
-template <typename E, typename Q, int V>
-hipError_t pick_loss_few(const Xent& x, const XentArgs& a, const Few& f, float* loss, float* lse, hipStream_t stream) {
-    switch (x.n_q) {
-        case 1: return run_loss_few<E, Q, V, 1>(x, a, f, loss, lse, stream);
-        case 2: return run_loss_few<E, Q, V, 2>(x, a, f, loss, lse, stream);
-        case 3: return run_loss_few<E, Q, V, 3>(x, a, f, loss, lse, stream);
-        default: return run_loss_few<E, Q, V, 4>(x, a, f, loss, lse, stream);
-    }
 }
 hipError_t launch_loss_few(const Xent& x, void* workspace, float* loss, float* lse, hipStream_t stream) {
     const Buffers b = carve(workspace, plan_for(x.n_q, x.t.n_rows, x.t.dim, x.t.dtype, false), x.n_q, x.t.n_rows, x.t.dim, true, false);
@@ -1530,8 +1609,25 @@ hipError_t launch_loss_few(const Xent& x, void* workspace, float* loss, float* l
     Few f = few_of(x);
     // small tables: parts of a word, down to eight rows, until there is one for every wave
     while (f.parts < 8 && (x.t.n_rows + 63) / 64 * f.parts * 2 <= FEW_WORKGROUPS * 4) f.parts *= 2;
-    if (x.t.dtype == VS_F32) return pick_loss_few<float, float, 4>(x, a, f, loss, lse, stream);
-    return x.queries_f32 ? pick_loss_few<bf16, float, 8>(x, a, f, loss, lse, stream) : pick_loss_few<bf16, bf16, 8>(x, a, f, loss, lse, stream);
+    if (x.t.dtype == VS_F32) return run_loss_few<float, float, 4>(x, a, f, loss, lse, stream);
+    return x.queries_f32 ? run_loss_few<bf16, float, 8>(x, a, f, loss, lse, stream) : run_loss_few<bf16, bf16, 8>(x, a, f, loss, lse, stream);
+}
+
+template <typename E, typename Q, int V>
+void run_weights_few(const Xent& x, const XentArgs& a, hipStream_t stream) {
+    with_few_scores<E, Q, V>(x.n_q, a.norms, [&](auto scores, auto nq, auto norms) {
+        constexpr uint32_t each = 4 * decltype(scores)::U;
+        weights_few_kernel<E, Q, V, nq, norms>
+            <<<std::min((a.piece_rows + each - 1) / each, FEW_WORKGROUPS), 256, few_lds(x.n_q, a.dim, V), stream>>>(a, few_of(x));
+    });
+}
+void weights_few(const Xent& x, const XentArgs& a, hipStream_t stream) {
+    if (x.t.dtype == VS_F32)
+        run_weights_few<float, float, 4>(x, a, stream);
+    else if (x.queries_f32)
+        run_weights_few<bf16, float, 8>(x, a, stream);
+    else
+        run_weights_few<bf16, bf16, 8>(x, a, stream);
 }
 
 void clear_rows(const Xent& x, void* grad_rows, uint64_t stride, bool all, hipStream_t stream) {
@@ -1591,7 +1687,10 @@ hipError_t launch_xent_grad(const Xent& x, const float* loss, const float* lse, 
     const bool f32 = x.t.dtype == VS_F32;
     if (grad_rows && c.a.list) clear_rows(x, grad_rows, grad_row_stride, false, stream);
     c.for_pieces(c.packed ? c.p.packed_rows : c.p.piece_rows, [&] {
-        c.p.score_bq == 64 ? c.weights<64>() : c.p.score_bq == 128 ? c.weights<128>() : c.weights<256>();
+        if (c.p.few)
+            weights_few(x, c.a, stream);
+        else
+            c.p.score_bq == 64 ? c.weights<64>() : c.p.score_bq == 128 ? c.weights<128>() : c.weights<256>();
         if (c.error == hipSuccess) click_weights_kernel<<<(x.n_q + 255) / 256, 256, 0, stream>>>(c.a);
         if (grad_rows) f32 ? c.row_grads<float>() : c.row_grads<bf16>();
         if (!grad_queries) return;

@@ -32,9 +32,9 @@ def weight_bits(dtype, n_q, out):
 
 
 def bounds(queries, table, targets, keep, scale, grad_loss=None, cosine=False, exact_products=False, exact_factor=False, chain=None, g_queries=0.0,
-           g_rows=0.0, share=None):
+           g_rows=0.0, share=None, joins=256):
     """{loss, lse, queries, rows: (value in 64 bits, bound)}, the gradients before the rounding to their type. share: the
-    candidates that one running sum of a query's gradient takes."""
+    candidates that one running sum of a query's gradient takes; joins: how many of those are brought together, at most."""
     n_q, depth = queries.shape
     q, n_rows = queries.double(), table.shape[0]
     keep = torch.ones(n_rows, dtype=torch.bool, device=DEV) if keep is None else keep
@@ -82,12 +82,12 @@ def bounds(queries, table, targets, keep, scale, grad_loss=None, cosine=False, e
     if cosine:
         over = torch.where(qn > 0, 1 / qn, 0.0)
         d = (g * over) @ rs
-        db = (gb_queries * over) @ rs.abs() + (share + 256 + depth + 20) * U32 * ((g * over).abs() @ rs.abs())
+        db = (gb_queries * over) @ rs.abs() + (share + joins + depth + 20) * U32 * ((g * over).abs() @ rs.abs())
         along = (d * q).sum(1, keepdim=True) * over.square()
         alongb = ((db * q.abs()).sum(1, keepdim=True) + (depth + 8) * U32 * (d * q).abs().sum(1, keepdim=True)) * over.square()
         out["queries"] = d - along * q, db + alongb * q.abs() + 4 * U32 * (d.abs() + (along * q).abs()) + 1e-37
         return out
-    out["queries"] = g @ r, gb_queries @ r.abs() + (share + 256 + 8) * U32 * (g.abs() @ r.abs()) + 1e-37
+    out["queries"] = g @ r, gb_queries @ r.abs() + (share + joins + 8) * U32 * (g.abs() @ r.abs()) + 1e-37
     dr, drb = torch.zeros(2, n_rows, depth, dtype=torch.float64, device=DEV)
     dr[at] = g.T @ q
     drb[at] = gb_rows.T @ q.abs() + (n_q + 8) * U32 * (g.abs().T @ q.abs()) + 1e-37

@@ -254,3 +254,42 @@ def test_long_queries_under_a_small_scale(store_of, n_q):
     for got, name in ((loss, "loss"), (lse, "lse")):
         value, bound = want[name]
         check(got, (value, bound + 2 * 2.0**-27), name)
+
+
+def certain(rows, n_q, dim, dtype, seed):
+    """Queries with nearly all of their probability on one document, which was not clicked."""
+    table, near = matrix(rows, dim, dtype, seed), torch.arange(n_q, device=DEV)
+    queries = (table[near].float() * 6 + matrix(n_q, dim, F32, seed + 1) / 8).to(dtype)
+    return table, queries, near, (rows - 1 - near % 90).int()
+
+
+# The certain document's logit, a sum of thousands of roundings, is in lse with the weight of one and in its own weight again: what
+# the roundings make of it has to be the same both times, and cancel, whichever way the loss went. So the bounds count none of
+# them; nor those of the sums, of which the others are a millionth.
+ALONE = dict(exact_products=True, exact_factor=True, chain=2, share=2, joins=2)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("n_q,dim", [(1, 1024), (1, 8192), (2, 6000), (3, 4096), (4, 3071), (5, 8192), (70, 8192), (130, 4096), (300, 4100)])
+def test_a_certain_other_document(gpu_ctx, dtype, n_q, dim):
+    rows, scale = 400, 4.0
+    table, queries, near, targets = certain(rows, n_q, dim, dtype, 31)
+    loss, lse = call_xent(gpu_ctx, queries, table, targets, None, scale)
+    dq, dr = like(queries), like(table)
+    call_xent_grads(gpu_ctx, queries, table, targets, None, scale, loss, lse, None, dq, dr)
+    g_queries, g_rows = weight_bits(dtype, n_q, dtype)
+    want = bounds(queries, table, targets, None, scale, g_queries=g_queries, g_rows=g_rows, **ALONE)
+    assert float(want["loss"][0].min()) > 15
+    check(dq, rounded(want["queries"], dtype), "gradient of the queries")
+    value, bound = rounded(want["rows"], dtype)
+    check(dr[near], (value[near], bound[near]), "gradient of the certain rows")
+
+
+@pytest.mark.parametrize("dtype,t", [(abi.VS_F32, F32), (abi.VS_BF16, BF16)])
+@pytest.mark.parametrize("n_q,dim", [(1, 4096), (2, 4000), (3, 4000), (4, 3001), (5, 4096), (130, 4000)])
+def test_a_certain_other_document_of_a_store(store_of, dtype, t, n_q, dim):
+    table, queries, near, targets = certain(400, n_q, dim, t, 33)
+    store = store_of(dtype, abi.VS_DOT, table.float().cpu().numpy())
+    loss, lse, dq = store_loss_and_grad(store, queries.float(), targets, 4.0)
+    want = bounds(queries, table, targets, None, 4.0, g_queries=weight_bits(t, n_q, F32)[0], **ALONE)
+    check(dq, rounded(want["queries"], F32), "gradient of the queries")
