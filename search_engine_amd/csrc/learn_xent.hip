@@ -27,7 +27,7 @@ namespace learn {
 namespace {
 
 constexpr uint32_t NONE = 0xFFFFFFFFu;
-constexpr float LOG2E = 1.44269504088896340736f, LOG2E_REST = (float)(1.44269504088896340736 - (double)LOG2E);
+constexpr float LOG2E = 1.44269504088896340736f;
 constexpr int TILE = 256;  // candidates of a tile
 constexpr uint32_t NO_ROW = 0xF0000000u;  // behind every row, and no sum with a tile's rows wraps
 
@@ -435,13 +435,19 @@ struct SplitScores {
 };
 
 __device__ __forceinline__ float finite_or_zero(float m) { return m == -__builtin_inff() ? 0.0f : m; }
+// What products are multiplied with in base 2. (A factor of zero would make a NaN of the -inf that stands for what is left out:
+// this one's logits are zero too.)
+__device__ __forceinline__ float base2(float scale) {
+    const float s2 = scale * LOG2E;
+    return s2 == 0 ? 1.4e-45f : s2;
+}
 
 // Per query the largest logit of a share of the candidates and the sum of the exponentials over it, the clicked row kept
 // out. Bound by the products from 64 queries (bf16) or so on, by the rows' bytes below: 256 queries over 1M x 768 bf16 take
 // 420 - 510 us (0.8 - 0.95 PFLOP/s; a large library product reaches 1.5), 10 take 255 (6.0 TB/s); over 250 thousand x 768
 // f32 256 take 660 (149 TFLOP/s in f32 products, 0.9 PFLOP/s of the six bf16 ones: the wave's splitting and the matrix
 // cores take 45 % of the cycles each). Everything is in base 2 (logits times log2 e): an exponential is one instruction. A lane keeps the running largest
-// and sum of its own candidates, in registers, for each of its queries; lanes, waves and shares are joined at the end.
+// product and the sum of its own candidates, in registers, for each of its queries; lanes, waves and shares are joined at the end.
 template <typename S, bool NORMS>
 __global__ __launch_bounds__(THREADS, 2) void loss_kernel(XentArgs a) {
     constexpr int BQ = S::Q_TILE;
@@ -457,9 +463,7 @@ __global__ __launch_bounds__(THREADS, 2) void loss_kernel(XentArgs a) {
     for (int n = 0; n < S::TN; ++n) {
         const uint32_t q = tile_q * BQ + (S::wave_q() * S::WQ + n) * 16 + (lane & 15);
         click[n] = q < a.n_q ? a.click[q] : NONE;
-        // (a factor of zero would make a NaN of the -inf that stands for what is left out: this one's logits are zero too)
-        s2[n] = q < a.n_q ? a.qscale[q] * LOG2E : 0.0f;
-        s2[n] = s2[n] == 0 ? 1.4e-45f : s2[n];
+        s2[n] = base2(q < a.n_q ? a.qscale[q] : 0.0f);
         m[n] = -__builtin_inff();
         l[n] = 0;
     }
@@ -507,9 +511,9 @@ __global__ __launch_bounds__(THREADS, 2) void loss_kernel(XentArgs a) {
 #pragma unroll
                     for (int r = 0; r < 4; ++r) x = __builtin_fmaxf(x, z[r]);
                 }
-                const float top = __builtin_fmaxf(m[n], x * s2[n]);  // (the factor is not negative)
-                const float ref = finite_or_zero(top);
-                float sum[4] = {l[n] * __builtin_amdgcn_exp2f(m[n] - ref), 0, 0, 0};
+                const float top = __builtin_fmaxf(m[n], x);  // (the factor is not negative)
+                const float ref = finite_or_zero(top * s2[n]);
+                float sum[4] = {l[n] * __builtin_amdgcn_exp2f(m[n] * s2[n] - ref), 0, 0, 0};
 #pragma unroll
                 for (int t = 0; t < S::TM; ++t) {
                     const f32x4 z = NORMS ? acc[t][n] * length(t) : acc[t][n];
@@ -526,8 +530,8 @@ __global__ __launch_bounds__(THREADS, 2) void loss_kernel(XentArgs a) {
     for (int n = 0; n < S::TN; ++n) {
 #pragma unroll
         for (int d = 16; d < 64; d *= 2) {
-            const float om = __shfl_xor(m[n], d), ol = __shfl_xor(l[n], d), top = __builtin_fmaxf(m[n], om), ref = finite_or_zero(top);
-            l[n] = l[n] * __builtin_amdgcn_exp2f(m[n] - ref) + ol * __builtin_amdgcn_exp2f(om - ref);
+            const float om = __shfl_xor(m[n], d), ol = __shfl_xor(l[n], d), top = __builtin_fmaxf(m[n], om), ref = finite_or_zero(top * s2[n]);
+            l[n] = l[n] * __builtin_amdgcn_exp2f(m[n] * s2[n] - ref) + ol * __builtin_amdgcn_exp2f(om * s2[n] - ref);
             m[n] = top;
         }
         if (lane < 16) {
@@ -540,11 +544,11 @@ __global__ __launch_bounds__(THREADS, 2) void loss_kernel(XentArgs a) {
     if (threadIdx.x >= BQ || q >= a.n_q) return;
     const uint64_t to = (uint64_t)along * a.n_q + q;
     float top = a.first_piece ? -__builtin_inff() : a.part_m[to], sum = a.first_piece ? 0.0f : a.part_l[to];
-    const float before = top;
+    const float before = top, factor = base2(a.qscale[q]);
     for (int w = 0; w < S::WAVES_R; ++w) top = __builtin_fmaxf(top, sm[w][threadIdx.x]);
-    const float ref = finite_or_zero(top);
-    sum *= __builtin_amdgcn_exp2f(before - ref);
-    for (int w = 0; w < S::WAVES_R; ++w) sum += sl[w][threadIdx.x] * __builtin_amdgcn_exp2f(sm[w][threadIdx.x] - ref);
+    const float ref = finite_or_zero(top * factor);
+    sum *= __builtin_amdgcn_exp2f(before * factor - ref);
+    for (int w = 0; w < S::WAVES_R; ++w) sum += sl[w][threadIdx.x] * __builtin_amdgcn_exp2f(sm[w][threadIdx.x] * factor - ref);
     a.part_m[to] = top;
     a.part_l[to] = sum;
 }
@@ -556,8 +560,8 @@ template <typename E, typename Q, int V, int NQ, bool NORMS>
 struct FewScores {
     static constexpr int U = NQ == 1 ? 8 : 4;  // candidates that a wave takes at a time, their loads in flight together
     uint32_t chunks, padded;                   // (a last, broken piece: see Piece)
-    float* query;                              // [NQ][padded], as they are multiplied
-    float factor;                              // of the lane's query, lane % NQ, base 2
+    float* query;                              // [NQ][padded], as they are multiplied, with the sign of the scale
+    float scale;                               // of the lane's query, lane % NQ: the logit of a product
 
     // By the whole workgroup of 256.
     __device__ __forceinline__ void init(const XentArgs& a, const Few& f, char* lds, double* sums /* 4, LDS */) {
@@ -565,7 +569,7 @@ struct FewScores {
         chunks = (a.dim + V - 1) / V;
         padded = chunks * V;
         query = reinterpret_cast<float*>(lds);
-        factor = 0;
+        scale = 0;
         const Q* queries = static_cast<const Q*>(f.queries);
         for (int q = 0; q < NQ; ++q) {
             double sq = 0;  // (as in pack_queries_kernel)
@@ -573,19 +577,19 @@ struct FewScores {
                 const Piece<V> piece(d / V, a.dim);
                 const uint32_t from = piece.col + d % V;
                 const float x = d % V >= piece.skip && from < a.dim ? query_element<E>(queries[q * f.query_stride + from]) : 0.0f;
-                query[q * padded + d] = x;
+                query[q * padded + d] = f.scale < 0 ? -x : x;
                 if constexpr (NORMS) sq += (double)x * x;
             }
-            float scale = f.scale * LOG2E;
+            float its_scale = __builtin_fabsf(f.scale);
             if constexpr (NORMS) {
                 sq = wave_sum(sq);
                 __syncthreads();
                 if (!lane) sums[wave] = sq;
                 __syncthreads();
                 const float norm = (float)sqrt(sums[0] + sums[1] + sums[2] + sums[3]);
-                scale = norm > 0 ? scale / norm : 0.0f;
+                its_scale = norm > 0 ? its_scale / norm : 0.0f;
             }
-            if (lane % NQ == (uint32_t)q) factor = scale;
+            if (lane % NQ == (uint32_t)q) scale = its_scale;
         }
         __syncthreads();
     }
@@ -631,7 +635,7 @@ struct FewScores {
 // The loss, under the masks themselves, with nothing laid out before. A wave takes the words of the masks in turn, and of each
 // word's candidates U at a time; the lane of each (candidate, query) keeps the running largest and sum of its logits.
 template <typename E, typename Q, int V, int NQ, bool NORMS>
-__global__ __launch_bounds__(256) void loss_few_kernel(XentArgs a, Few f) {
+__global__ __launch_bounds__(256) void loss_few_kernel(XentArgs a, Few f, float* qscale) {
     using S = FewScores<E, Q, V, NQ, NORMS>;
     constexpr int U = S::U;
     extern __shared__ __attribute__((aligned(128))) char lds[];
@@ -640,6 +644,8 @@ __global__ __launch_bounds__(256) void loss_few_kernel(XentArgs a, Few f) {
     const uint32_t lane = threadIdx.x & 63, wave = uniform_u32(threadIdx.x >> 6), mine = lane % NQ;
     S scores;
     scores.init(a, f, lds, sums);
+    const float factor = base2(scores.scale);
+    if (!blockIdx.x && threadIdx.x < NQ) qscale[threadIdx.x] = scores.scale;
     const uint32_t click = f.targets[mine] < f.first_id ? NONE : f.targets[mine] - f.first_id;
     float m = -__builtin_inff(), l = 0;
     const uint32_t n_units = (uint32_t)((a.n_rows + 63) / 64) * f.parts, size = 64 / f.parts;
@@ -662,8 +668,8 @@ __global__ __launch_bounds__(256) void loss_few_kernel(XentArgs a, Few f) {
             const float z = scores.products(a, f, row, &r, &length);
             if (lane < n * NQ && r != click) {
                 // (an fma: of a logit of hundreds the rounding alone would show in the exponential)
-                const float top = __builtin_fmaxf(m, z * scores.factor), ref = finite_or_zero(top);
-                l = l * __builtin_amdgcn_exp2f(m - ref) + __builtin_amdgcn_exp2f(__builtin_fmaf(z, scores.factor, -ref));
+                const float top = __builtin_fmaxf(m, z), ref = finite_or_zero(top * factor);
+                l = l * __builtin_amdgcn_exp2f(m * factor - ref) + __builtin_amdgcn_exp2f(__builtin_fmaf(z, factor, -ref));
                 m = top;
             }
         }
@@ -675,9 +681,9 @@ __global__ __launch_bounds__(256) void loss_few_kernel(XentArgs a, Few f) {
     float top = -__builtin_inff(), sum = 0;
     for (int w = 0; w < 4; ++w)
         for (int u = 0; u < U; ++u) top = __builtin_fmaxf(top, sm[w][u * NQ + threadIdx.x]);
-    const float ref = finite_or_zero(top);
+    const float ref = finite_or_zero(top * factor);
     for (int w = 0; w < 4; ++w)
-        for (int u = 0; u < U; ++u) sum += sl[w][u * NQ + threadIdx.x] * __builtin_amdgcn_exp2f(sm[w][u * NQ + threadIdx.x] - ref);
+        for (int u = 0; u < U; ++u) sum += sl[w][u * NQ + threadIdx.x] * __builtin_amdgcn_exp2f(sm[w][u * NQ + threadIdx.x] * factor - ref);
     a.part_m[(uint64_t)blockIdx.x * NQ + threadIdx.x] = top;
     a.part_l[(uint64_t)blockIdx.x * NQ + threadIdx.x] = sum;
 }
@@ -709,11 +715,11 @@ __global__ __launch_bounds__(256) void join_loss_kernel(XentArgs a, Few f, float
     if (!lane) tops[wave] = top;
     __syncthreads();
     top = __builtin_fmaxf(__builtin_fmaxf(tops[0], tops[1]), __builtin_fmaxf(tops[2], tops[3]));
-    const float ref = finite_or_zero(top);
+    const float scale = a.qscale[q], factor = base2(scale), ref = finite_or_zero(top * factor);
     double sum = 0;
     for (uint32_t s = threadIdx.x; s < a.splits; s += 256) {
         const uint64_t at = (uint64_t)s * a.n_q + q;
-        sum += (double)a.part_l[at] * (double)__builtin_amdgcn_exp2f(a.part_m[at] - ref);
+        sum += (double)a.part_l[at] * (double)__builtin_amdgcn_exp2f(a.part_m[at] * factor - ref);
     }
     sum = wave_sum(sum);
     dot = wave_sum(dot);
@@ -728,11 +734,17 @@ __global__ __launch_bounds__(256) void join_loss_kernel(XentArgs a, Few f, float
     sum = (sums[0][0] + sums[1][0]) + (sums[2][0] + sums[3][0]);
     dot = (sums[0][1] + sums[1][1]) + (sums[2][1] + sums[3][1]);
     sq = (sums[0][2] + sums[1][2]) + (sums[2][2] + sums[3][2]);
+    // The sum is over the reference, a rounded product; taken back to the largest logit itself.
     constexpr double LN2 = 0.693147180559945309417;
-    const double rest = ref * LN2 + log(sum);  // -inf: no other candidate
+    const bool none = top == -__builtin_inff();  // no other candidate
+    const double over = none ? -__builtin_inf() : log(sum) - LN2 * __builtin_fmaf(top, factor, -ref);
+    const double rest = none ? over : (double)top * scale + over;
+    // lse is for the weights, which round every logit to f32: where one has nearly all of the probability it has to be that
+    // logit as it is rounded there, and not what a little more than it rounds to.
+    const double rest_of_weights = none ? over : (double)(top * scale) + over;
     if (!clicked) {
         loss[q] = 0.0f;
-        lse[q] = (float)rest;
+        lse[q] = (float)rest_of_weights;
         return;
     }
     double z = f.scale * dot;
@@ -742,7 +754,7 @@ __global__ __launch_bounds__(256) void join_loss_kernel(XentArgs a, Few f, float
     }
     const double d = rest - z;
     loss[q] = (float)(d > 0 ? d + log1p(exp(-d)) : log1p(exp(d)));
-    lse[q] = (float)(d > 0 ? rest + log1p(exp(-d)) : z + log1p(exp(d)));
+    lse[q] = (float)(d > 0 ? rest_of_weights + log1p(exp(-d)) : z + log1p(exp(d)));
 }
 
 // ---- gradients ----------------------------------------------------------------------------
@@ -752,15 +764,19 @@ __device__ __forceinline__ float query_factor(const XentArgs& a, uint32_t q) {
     return (a.grad_loss ? a.grad_loss[q] : 1.0f) * a.qscale[q] * a.sign;
 }
 
-// lse in base 2 has a rounding of its own, half a step of a number near 20: as a relative error of all of a query's weights
-// it would be ten times the roundings of the products. What is behind it goes into the factor.
+// exp(z - lse) of a logit z that has been rounded to f32: where one document has nearly all of the probability, lse is its logit as
+// it is rounded here (see join_loss_kernel), and the weight is one (of logits near 100, two that were rounded apart make an error of
+// 4e-6). Everything else goes by differences: z log2 e by an fma, and of lse log2 e, whose rounding would be an error of all of
+// a query's weights, what is behind it goes into the factor.
 struct Base2 {
     float high, rest;
     __device__ __forceinline__ explicit Base2(float lse) {
         high = lse * LOG2E;
-        const float low = __builtin_fmaf(lse, LOG2E, -high) + lse * LOG2E_REST;
+        const float low = __builtin_fmaf(lse, LOG2E, -high);
         rest = low == low ? __builtin_amdgcn_exp2f(-low) : 1.0f;
     }
+    // over `rest`
+    __device__ __forceinline__ static float weight(float z, float high) { return __builtin_amdgcn_exp2f(__builtin_fmaf(z, LOG2E, -high)); }
 };
 
 // The weights of the clicked rows of a piece, after weights_kernel, which takes every row alike (to look for them there
@@ -796,7 +812,7 @@ template <typename S, bool NORMS, int PG>
 __global__ __launch_bounds__(THREADS, 2) void weights_kernel(XentArgs a) {
     constexpr int BQ = S::Q_TILE;
     extern __shared__ __attribute__((aligned(128))) char lds[];
-    __shared__ __attribute__((aligned(16))) float s2[BQ], lse2[BQ], factor[BQ];
+    __shared__ __attribute__((aligned(16))) float scale[BQ], lse2[BQ], factor[BQ];
     uint32_t tile_q, along;
     place_of_workgroup(a.across, &tile_q, &along);
     const uint32_t q0 = tile_q * BQ;
@@ -806,7 +822,7 @@ __global__ __launch_bounds__(THREADS, 2) void weights_kernel(XentArgs a) {
         const uint32_t q = q0 + threadIdx.x;
         const bool in = q < a.n_q && a.click[q] != NONE;
         const Base2 lse(in ? a.lse[q] : 0.0f);
-        s2[threadIdx.x] = in ? a.qscale[q] * LOG2E : 0.0f;
+        scale[threadIdx.x] = in ? a.qscale[q] : 0.0f;
         lse2[threadIdx.x] = lse.high;
         factor[threadIdx.x] = in ? query_factor(a, q) * lse.rest : 0.0f;
     }
@@ -834,13 +850,13 @@ __global__ __launch_bounds__(THREADS, 2) void weights_kernel(XentArgs a) {
 #pragma unroll
                 for (int t = 0; t < UNIT; ++t) {
                     const uint32_t i = i0 + (u * UNIT + t) * 16;
-                    const f32x4 vs = *reinterpret_cast<const f32x4*>(s2 + i), vl = *reinterpret_cast<const f32x4*>(lse2 + i);
+                    const f32x4 vs = *reinterpret_cast<const f32x4*>(scale + i), vl = *reinterpret_cast<const f32x4*>(lse2 + i);
                     const f32x4 vf = *reinterpret_cast<const f32x4*>(factor + i);
 #pragma unroll
                     for (int r = 0; r < 4; ++r) {
                         float z = acc[u * UNIT + t][n][r];
                         if constexpr (NORMS) z *= inverse[n];
-                        float g = vf[r] * __builtin_amdgcn_exp2f(__builtin_fmaf(z, vs[r], -vl[r]));
+                        float g = vf[r] * Base2::weight(z * vs[r], vl[r]);
                         if constexpr (NORMS) g *= inverse[n];
                         if constexpr (PG == 1) {
                             p[t][0].e[r] = (uint16_t)bf16_bits(g);
@@ -889,7 +905,7 @@ __global__ __launch_bounds__(256) void weights_few_kernel(XentArgs a, Few f) {
         uint32_t r;
         float length;
         const float z = scores.products(a, f, row, &r, &length);
-        float g = factor * __builtin_amdgcn_exp2f(__builtin_fmaf(z, scores.factor, -lse.high));
+        float g = factor * Base2::weight(z * scores.scale, lse.high);
         if constexpr (NORMS) g = length == 0 ? 0.0f : g / length;
         const Split x = split(in ? g : 0.0f);
         const uint32_t planes[3] = {x.h, x.m, x.l};
@@ -1371,6 +1387,7 @@ Buffers carve(void* workspace, const Plan& p, uint32_t n_q, uint64_t n_rows, uin
         b.part_m = w.take<float>(parts);
         b.part_l = w.take<float>(parts);
         if (p.few) {
+            b.qscale = w.take<float>(n_q);
             b.bytes = w.at() - (char*)workspace;
             return b;
         }
@@ -1589,11 +1606,12 @@ void with_few_scores(uint32_t n_q, bool norms, F&& f) {
 uint32_t few_lds(uint32_t n_q, uint32_t dim, uint32_t v) { return n_q * (uint32_t)round_up(dim, v) * 4; }
 
 template <typename E, typename Q, int V>
-hipError_t run_loss_few(const Xent& x, XentArgs a, const Few& f, float* loss, float* lse, hipStream_t stream) {
+hipError_t run_loss_few(const Xent& x, XentArgs a, const Few& f, float* qscale, float* loss, float* lse, hipStream_t stream) {
     a.splits = (uint32_t)std::min<uint64_t>(((x.t.n_rows + 63) / 64 * f.parts + 3) / 4, FEW_WORKGROUPS);
     with_few_scores<E, Q, V>(x.n_q, a.norms, [&](auto, auto nq, auto norms) {
-        loss_few_kernel<E, Q, V, nq, norms><<<a.splits, 256, few_lds(x.n_q, a.dim, V), stream>>>(a, f);
+        loss_few_kernel<E, Q, V, nq, norms><<<a.splits, 256, few_lds(x.n_q, a.dim, V), stream>>>(a, f, qscale);
     });
+    a.qscale = qscale;
     join_loss_kernel<E, Q><<<x.n_q, 256, 0, stream>>>(a, f, loss, lse);
     return hipGetLastError();
 }
@@ -1609,8 +1627,8 @@ hipError_t launch_loss_few(const Xent& x, void* workspace, float* loss, float* l
     Few f = few_of(x);
     // small tables: parts of a word, down to eight rows, until there is one for every wave
     while (f.parts < 8 && (x.t.n_rows + 63) / 64 * f.parts * 2 <= FEW_WORKGROUPS * 4) f.parts *= 2;
-    if (x.t.dtype == VS_F32) return run_loss_few<float, float, 4>(x, a, f, loss, lse, stream);
-    return x.queries_f32 ? run_loss_few<bf16, float, 8>(x, a, f, loss, lse, stream) : run_loss_few<bf16, bf16, 8>(x, a, f, loss, lse, stream);
+    if (x.t.dtype == VS_F32) return run_loss_few<float, float, 4>(x, a, f, b.qscale, loss, lse, stream);
+    return x.queries_f32 ? run_loss_few<bf16, float, 8>(x, a, f, b.qscale, loss, lse, stream) : run_loss_few<bf16, bf16, 8>(x, a, f, b.qscale, loss, lse, stream);
 }
 
 template <typename E, typename Q, int V>

@@ -293,3 +293,35 @@ def test_a_certain_other_document_of_a_store(store_of, dtype, t, n_q, dim):
     loss, lse, dq = store_loss_and_grad(store, queries.float(), targets, 4.0)
     want = bounds(queries, table, targets, None, 4.0, g_queries=weight_bits(t, n_q, F32)[0], **ALONE)
     check(dq, rounded(want["queries"], F32), "gradient of the queries")
+
+
+@pytest.mark.parametrize("n_q", [1, 4, 5, 70, 300])
+@pytest.mark.parametrize("over_store", [False, True])
+def test_a_certain_other_document_with_a_large_logit(gpu_ctx, store_of, n_q, over_store):
+    """lse near 100 is the certain document's logit, rounded to f32 (2^-24 of 100). In its weight, nearly one, that rounding cancels
+    if the logit is rounded the same way there; products are exact here, so that it is known which way. (Left out: logits so near
+    to the middle between two numbers of f32 that the sum's own rounding may turn lse the other way.)"""
+    rows, dim, scale = 400, 64, 25.3
+    table, near = steps(rows, dim, F32, 35), torch.arange(n_q, device=DEV)
+    queries = table[near] * 2
+    targets = (rows - 1 - near % 90).int()
+    logit = (queries.double() * table[near].double()).sum(1) * float(np.float32(scale))
+    others = queries.double() @ table.double().T * scale
+    others[near, near] = -math.inf
+    other_way = (logit.float().double() - logit).abs() + 4 * U32 > (torch.nextafter(logit.float(), torch.full_like(logit, 1e9).float())
+                                                                    - logit.float()).double() / 2
+    sure = (logit - others.amax(1) > 25) & ~other_way & (targets.long() != near)
+    assert int(sure.sum()) > 0.6 * n_q and float(logit.min()) > 25 and float(logit.max()) > 90
+    if over_store:
+        store = store_of(abi.VS_F32, abi.VS_DOT, table.cpu().numpy())
+        loss, lse, dq = store_loss_and_grad(store, queries, targets, scale)
+    else:
+        loss, lse = call_xent(gpu_ctx, queries, table, targets, None, scale)
+        dq = like(queries)
+        call_xent_grads(gpu_ctx, queries, table, targets, None, scale, loss, lse, None, dq, None)
+    value = scale * (table[near].double() - table[targets.long()].double())
+    size = scale * (table[near].double().abs() + table[targets.long()].double().abs())
+    # the weight: 8 roundings; the product with the row and the sum: 4; the click's: 4; all others: exp(-25) each at most, of
+    # elements of 1/4 at most
+    bound = size * 16 * U32 + rows * math.exp(-25) * scale / 4
+    check(dq[sure], (value[sure], bound[sure]), "gradient of the queries")
