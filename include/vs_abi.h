@@ -562,11 +562,9 @@ int32_t vs_xent_device(vs_ctx* ctx, const void* d_queries, uint32_t n_q, uint64_
  *   d_grad_queries: laid out as d_queries (same type and stride), or NULL
  *   d_grad_rows:    laid out as d_rows, every row written (zeros for a row that is no
  *                   candidate; between rows nothing is written), or NULL
- * The products are recomputed, a piece of the rows at a time. With VS_BF16 the weights
- * exp(z - lse) keep 16 bits where they multiply queries (the rows' gradient), whatever
- * n_q, and where they multiply rows for f32 gradients (vs_store_xent_grad_device) or up
- * to 64 queries; for bf16 gradients of more queries they are rounded to bf16, like those,
- * but for the clicked row's. Sums stay f32 and each gradient is rounded once. */
+ * The products are recomputed, a piece of the rows at a time. The weights exp(z - lse)
+ * of VS_F32 keep all 24 bits, those of VS_BF16 16; sums stay f32 and each gradient is
+ * rounded once. */
 int32_t vs_xent_grad_device(vs_ctx* ctx, const void* d_queries, uint32_t n_q, uint64_t query_stride,
                             const void* d_rows, uint64_t n_rows, uint64_t row_stride, int32_t dtype,
                             uint32_t dim, const uint32_t* d_targets, const uint64_t* d_mask_words,

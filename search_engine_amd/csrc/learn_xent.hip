@@ -44,7 +44,7 @@ struct XentArgs {
     const uint32_t* click;  // [n_q] place of the clicked row among the candidates, or NONE
     const float* qscale;    // [n_q] factor of a query's products, without its sign
     float sign;
-    Steps row_steps, query_steps;  // of the gradients' products
+    Steps grad_steps;
     const char* zeros;
     uint32_t piece_begin, piece_rows;
     bool first_piece;
@@ -797,15 +797,14 @@ __global__ __launch_bounds__(256) void click_weights_kernel(XentArgs a) {
         const uint32_t bits = bf16_bits(g);
         *reinterpret_cast<uint16_t*>(out + p * a.g_plane) = (uint16_t)bits;
         g -= __builtin_bit_cast(float, bits << 16);
-        if (p + 1 == min(a.query_steps.n, a.g_planes)) a.click_rest[q] = g;
     }
+    a.click_rest[q] = g;
 }
 
 template <typename S>
 using weights_turn = Turn<8, S::UNIT>;
 
-// The weights G of a piece, [candidate][query], rounded to bf16 (PG = 1), or kept to 16 bits (2) or all 24 (3) by as many
-// planes (which: see two_for_queries). A lane holds four neighbouring queries of a candidate: eight bytes a store. Bound as the loss is, and by what
+// The weights G of a piece, [candidate][query], kept to 16 bits (PG = 2, of bf16 tables) or all 24 (3) by as many planes of bf16. A lane holds four neighbouring queries of a candidate: eight bytes a store. Bound as the loss is, and by what
 // it writes: 256 queries over 1M x 768 bf16 505 us (0.78 PFLOP/s, of which 512 MB written take about 100), 256 over 250
 // thousand x 768 f32 715.
 template <typename S, bool NORMS, int PG>
@@ -858,14 +857,10 @@ __global__ __launch_bounds__(THREADS, 2) void weights_kernel(XentArgs a) {
                         if constexpr (NORMS) z *= inverse[n];
                         float g = vf[r] * Base2::weight(z * vs[r], vl[r]);
                         if constexpr (NORMS) g *= inverse[n];
-                        if constexpr (PG == 1) {
-                            p[t][0].e[r] = (uint16_t)bf16_bits(g);
-                        } else {
-                            const Split x = split(g);
-                            p[t][0].e[r] = x.h;
-                            p[t][1].e[r] = x.m;
-                            p[t][2].e[r] = x.l;
-                        }
+                        const Split x = split(g);
+                        p[t][0].e[r] = x.h;
+                        p[t][1].e[r] = x.m;
+                        p[t][2].e[r] = x.l;
                     }
                 }
 #pragma unroll
@@ -951,7 +946,7 @@ __global__ __launch_bounds__(THREADS, 2) void row_grads_kernel(XentArgs a) {
     r.init();
     q.aim(tile_d * BD);
     r.aim(along * TILE);
-    const uint32_t planes = a.row_steps.n, blocks = a.gq / 64, steps = planes * blocks;
+    const uint32_t planes = a.grad_steps.n, blocks = a.gq / 64, steps = planes * blocks;
     constexpr int BUFFERS = row_grads_buffers<BD>, BEHIND = (BUFFERS - 2) * (A::LOADS + B::LOADS);
     auto half_q = [&](uint32_t i) { return lds + i * (A::BYTES + B::BYTES); };
     auto half_g = [&](uint32_t i) { return lds + i * (A::BYTES + B::BYTES) + A::BYTES; };
@@ -959,10 +954,10 @@ __global__ __launch_bounds__(THREADS, 2) void row_grads_kernel(XentArgs a) {
     Cursor cg{0, 0, along}, cq{0, 0, along};
     auto load_weights = [&](uint32_t to) {
 #pragma unroll
-        for (int i = 0; i < B::LOADS; ++i) r.load(i, g, cg.k, a.row_steps.plane_a(cg.c), a.zeros, half_g(to));
+        for (int i = 0; i < B::LOADS; ++i) r.load(i, g, cg.k, a.grad_steps.plane_a(cg.c), a.zeros, half_g(to));
         if (cg.advance(planes, blocks, a.splits)) r.aim(cg.tile < tiles ? cg.tile * TILE : NO_ROW);
     };
-    auto load_queries = [&](int i, uint32_t to) { q.load(i, a.qt, cq.k, a.row_steps.plane_b(cq.c), a.zeros, half_q(to)); };
+    auto load_queries = [&](int i, uint32_t to) { q.load(i, a.qt, cq.k, a.grad_steps.plane_b(cq.c), a.zeros, half_q(to)); };
     auto load_all_queries = [&](uint32_t to) {
 #pragma unroll
         for (int i = 0; i < A::LOADS; ++i) load_queries(i, to);
@@ -1067,7 +1062,7 @@ __global__ __launch_bounds__(THREADS, 2) void query_grads_kernel(XentArgs a) {
     const uint32_t per = ((n + STEP - 1) / STEP + a.splits - 1) / a.splits * STEP;
     const uint32_t begin = (uint32_t)min((uint64_t)share * per, (uint64_t)n), stop = min(begin + per, n);
     f32x4 acc[TM][TN] = {};
-    const uint32_t blocks = (stop - begin + STEP - 1) / STEP, steps = blocks * a.query_steps.n;
+    const uint32_t blocks = (stop - begin + STEP - 1) / STEP, steps = blocks * a.grad_steps.n;
     if (steps) {
         const Planes g{a.g, a.g_plane, a.g_stride, nullptr, n, a.gq / 8};
         Planes rows = a.rows;
@@ -1081,17 +1076,17 @@ __global__ __launch_bounds__(THREADS, 2) void query_grads_kernel(XentArgs a) {
         auto half_g = [&](uint32_t i) { return lds + i * (A::BYTES + B::BYTES); };
         auto half_r = [&](uint32_t i) { return lds + i * (A::BYTES + B::BYTES) + A::BYTES; };
         Cursor cr{0, 0, 0}, cg{0, 0, 0};
-        const uint32_t planes = a.query_steps.n;
+        const uint32_t planes = a.grad_steps.n;
         auto load_rows = [&](uint32_t to) {
             const uint32_t from = begin + cr.k * STEP;
 #pragma unroll
             for (int i = 0; i < B::LOADS; ++i)
-                r.load(i, rows, base + from, base + stop, tile_d * (BD / 8), a.query_steps.plane_b(cr.c), a.zeros, half_r(to));
+                r.load(i, rows, base + from, base + stop, tile_d * (BD / 8), a.grad_steps.plane_b(cr.c), a.zeros, half_r(to));
             cr.advance(planes, blocks + BUFFERS, 1);  // (behind the last block: zeros)
             if (!cr.c) r.peek(rows, base + from + STEP, base + stop);  // while this step multiplies
         };
         auto load_weights = [&](int i, uint32_t to) {
-            w.load(i, g, begin + cg.k * STEP, stop, tile_q * (BQ / 8), a.query_steps.plane_a(cg.c), a.zeros, half_g(to));
+            w.load(i, g, begin + cg.k * STEP, stop, tile_q * (BQ / 8), a.grad_steps.plane_a(cg.c), a.zeros, half_g(to));
         };
         r.peek(rows, base + begin, base + stop);
 #pragma unroll
@@ -1296,9 +1291,9 @@ constexpr uint64_t PIECE_BYTES = 1u << 30;  // of weights, and of planes, that a
 constexpr uint32_t WORKGROUPS = 256;          // of a product: one per CU (the LDS of a tile fills one)
 constexpr uint32_t FEW_WORKGROUPS = 2048;     // of the loss of a few queries: eight per CU
 
-// hh, hm, mh, mm, hl, lh | plane 0 alone | planes 0 and 1 of A
+// hh, hm, mh, mm, hl, lh | planes 0 and 1 of A
 constexpr Steps SIX{6, 0u | 0u << 2 | 1u << 4 | 1u << 6 | 0u << 8 | 2u << 10, 0u | 1u << 2 | 0u << 4 | 1u << 6 | 2u << 8 | 0u << 10};
-constexpr Steps ONE{1, 0, 0}, TWO{2, 0u | 1u << 2, 0};
+constexpr Steps TWO{2, 0u | 1u << 2, 0};
 
 // Up to four queries by plain products, which need no list of candidates and no planes of queries: rows of f32 always (200
 // thousand x 768, four queries: 115 us, on the matrix cores 164), rows of bf16 while their bytes still bound them (one
@@ -1321,19 +1316,15 @@ uint32_t splits_for(uint32_t across, uint64_t tiles) {
     return (uint32_t)std::min<uint64_t>(std::max<uint64_t>(WORKGROUPS / across, 1), tiles);
 }
 
-// Planes of a bf16 table's weights. One rounding of a weight to bf16 (2^-8 of it at most) is as large as the rounding of a
-// gradient to bf16: a row's gradient, of few terms of like size, would be 1.4 times as far off as its type makes it, and an
-// f32 gradient 2^-8 and not 2^-24. So the weights have two planes (16 bits) wherever that shows. It does not in a bf16 gradient
-// of queries, a sum over all candidates whose largest term, the clicked row's, is exact (see click_rest); with up to 64
-// queries, where the rows' bytes bound the products, the second plane costs nothing.
-bool two_for_queries(const Xent& x) { return x.n_q <= 64 || x.queries_f32; }
-
-// `two`: whether a bf16 table's weights have two planes.
-Plan plan_for(uint32_t n_q, uint64_t n_rows, uint32_t dim, int32_t dtype, bool two) {
+Plan plan_for(uint32_t n_q, uint64_t n_rows, uint32_t dim, int32_t dtype) {
     Plan p;
     p.few = few_queries(n_q, n_rows, dim, dtype);
     p.planes = dtype == VS_F32 ? 3 : 1;
-    p.g_planes = dtype == VS_F32 ? 3 : two || n_q <= 64 ? 2 : 1;
+    // Weights of a bf16 table have 16 bits. Rounded to bf16, 2^-8 of each at most, they would be as far off as a gradient's own
+    // rounding is, and further where a gradient is the difference of terms that nearly cancel, as those of a clicked document and
+    // a copy of it do. (The price: loss and gradients of 256 queries over 1M x 768 take 2.72 ms, 1.93 with bf16 weights; of 1000
+    // over half of 200 thousand x 1536, queries' alone, 1.25 and 0.94.)
+    p.g_planes = dtype == VS_F32 ? 3 : 2;
     p.kp = (uint32_t)round_up(dim, 64);
     p.gq = (uint32_t)round_up(n_q, 64);
     p.bq = n_q <= 64 ? 64 : n_q <= 128 || dtype == VS_F32 ? 128 : 256;
@@ -1425,8 +1416,8 @@ struct Call {
     hipStream_t stream;
     hipError_t error = hipSuccess;
 
-    Call(const Xent& x_, void* workspace, bool gradients, bool rows_too, hipStream_t stream_)
-        : x(x_), p(plan_for(x.n_q, x.t.n_rows, x.t.dim, x.t.dtype, rows_too || two_for_queries(x))),
+    Call(const Xent& x_, void* workspace, bool gradients, hipStream_t stream_)
+        : x(x_), p(plan_for(x.n_q, x.t.n_rows, x.t.dim, x.t.dtype)),
           b(carve(workspace, p, x.n_q, x.t.n_rows, x.t.dim, rows_are_aligned(x.t), gradients)), stream(stream_) {
         const uint32_t dim = x.t.dim;
         const uint32_t size = x.t.dtype == VS_F32 ? 4 : 2, chunk = 16 / size;
@@ -1441,8 +1432,7 @@ struct Call {
         a.click = b.click;
         a.qscale = b.qscale;
         a.sign = x.scale < 0 ? -1.0f : 1.0f;
-        a.row_steps = p.planes == 3 ? SIX : p.g_planes == 2 ? TWO : ONE;
-        a.query_steps = p.planes == 3 ? SIX : two_for_queries(x) ? TWO : ONE;
+        a.grad_steps = p.planes == 3 ? SIX : TWO;
         a.zeros = (const char*)b.zeros;
         a.part_m = b.part_m;
         a.part_l = b.part_l;
@@ -1543,7 +1533,7 @@ struct Call {
         if constexpr (BQ == 64)
             p.planes == 3 ? weights<BQ, 3>() : weights<BQ, 2>();
         else
-            p.g_planes == 2 ? weights<BQ, 2>() : weights<BQ, 1>();
+            weights<BQ, 2>();
     }
 
     template <int BD, typename E>
@@ -1616,7 +1606,7 @@ hipError_t run_loss_few(const Xent& x, XentArgs a, const Few& f, float* qscale, 
     return hipGetLastError();
 }
 hipError_t launch_loss_few(const Xent& x, void* workspace, float* loss, float* lse, hipStream_t stream) {
-    const Buffers b = carve(workspace, plan_for(x.n_q, x.t.n_rows, x.t.dim, x.t.dtype, false), x.n_q, x.t.n_rows, x.t.dim, true, false);
+    const Buffers b = carve(workspace, plan_for(x.n_q, x.t.n_rows, x.t.dim, x.t.dtype), x.n_q, x.t.n_rows, x.t.dim, true, false);
     XentArgs a{};
     a.n_rows = x.t.n_rows;
     a.dim = x.t.dim;
@@ -1664,15 +1654,12 @@ bool rows_are_aligned(const Table& t) {
 }
 
 uint64_t xent_workspace_bytes(uint32_t n_q, uint64_t n_rows, uint32_t dim, int32_t dtype, bool aligned, bool gradients) {
-    uint64_t bytes = 0;
-    for (bool two : {false, true})
-        bytes = std::max(bytes, carve(nullptr, plan_for(n_q, n_rows, dim, dtype, two), n_q, n_rows, dim, aligned, gradients).bytes);
-    return bytes + 256;
+    return carve(nullptr, plan_for(n_q, n_rows, dim, dtype), n_q, n_rows, dim, aligned, gradients).bytes + 256;
 }
 
 hipError_t launch_xent(const Xent& x, void* workspace, float* loss, float* lse, hipStream_t stream) {
     if (few_queries(x.n_q, x.t.n_rows, x.t.dim, x.t.dtype)) return launch_loss_few(x, workspace, loss, lse, stream);
-    Call c(x, workspace, false, false, stream);
+    Call c(x, workspace, false, stream);
     c.for_pieces(c.packed ? c.p.packed_rows : x.t.n_rows, [&] {
         c.p.score_bq == 64 ? c.loss<64>() : c.p.score_bq == 128 ? c.loss<128>() : c.loss<256>();
     });
@@ -1696,7 +1683,7 @@ hipError_t launch_xent_grad(const Xent& x, const float* loss, const float* lse, 
         return hipGetLastError();
     }
     if (!grad_queries && !grad_rows) return hipSuccess;
-    Call c(x, workspace, true, grad_rows != nullptr, stream);
+    Call c(x, workspace, true, stream);
     c.a.loss = loss;
     c.a.lse = lse;
     c.a.grad_loss = grad_loss;

@@ -10,7 +10,7 @@ U32 = 2^-24 is one rounding to f32. To first order:
             two where sums over it are brought together, each with the term's share of the sum
   sum       `chain` roundings: as many terms as one workgroup adds up, and 20 for the joins
   lse       all of these, and one rounding of itself
-  weight    its own product and exponent, lse's error, 8 roundings; and `g_*`, where it is kept to fewer bits
+  weight    its own product and exponent, lse's error, 8 roundings; and `kept`, where it is kept to fewer bits
 """
 import torch
 
@@ -23,16 +23,13 @@ def chain_of(n_rows, n_q):
     return n_rows * -(-n_q // 64) / 256 + 256
 
 
-def weight_bits(dtype, n_q, out):
-    """How far the unclicked weights of (queries' gradient, rows' gradient) may be from their f32 values: f32 tables keep 24
-    bits, bf16 tables 16, or 8 (one rounding) for queries' gradients that are bf16 themselves, of more than 64 queries."""
-    if dtype == torch.float32:
-        return 0.0, 0.0
-    return 2.0**-16 if n_q <= 64 or out == torch.float32 else 2.0**-8, 2.0**-16
+def weight_bits(dtype):
+    """How far the weights of the gradients may be from their f32 values: f32 tables keep 24 bits, bf16 tables 16."""
+    return 0.0 if dtype == torch.float32 else 2.0**-16
 
 
-def bounds(queries, table, targets, keep, scale, grad_loss=None, cosine=False, exact_products=False, exact_factor=False, chain=None, g_queries=0.0,
-           g_rows=0.0, share=None, joins=256):
+def bounds(queries, table, targets, keep, scale, grad_loss=None, cosine=False, exact_products=False, exact_factor=False, chain=None, kept=0.0,
+           share=None, joins=256):
     """{loss, lse, queries, rows: (value in 64 bits, bound)}, the gradients before the rounding to their type. share: the
     candidates that one running sum of a query's gradient takes; joins: how many of those are brought together, at most."""
     n_q, depth = queries.shape
@@ -71,12 +68,12 @@ def bounds(queries, table, targets, keep, scale, grad_loss=None, cosine=False, e
     rel = zb + 2 * U32 * (z - lse[:, None]).abs() + (e + U32 * lse.abs() + 8 * U32)[:, None]
     tiny = 2.0**-125 * (1 + w.abs())[:, None]
 
-    def sides(bits, click_bits):
-        b = g * (rel + bits)
-        b[row[ok], column[ok]] = (torch.exp(-loss) * lossb + p_not * (4 * U32 + click_bits))[ok]
+    def error_of(click_kept):
+        b = g * (rel + kept)
+        b[row[ok], column[ok]] = (torch.exp(-loss) * lossb + p_not * (4 * U32 + click_kept))[ok]
         return b * w.abs()[:, None] + tiny
-    # (a clicked row's weight leaves the queries' gradient nothing of its rounding)
-    gb_queries, gb_rows = sides(g_queries, 0.0), sides(g_rows, g_rows)
+    # (what a clicked row's weight is not kept to goes into the queries' gradient by itself)
+    gb_queries, gb_rows = error_of(0.0), error_of(kept)
     g[row[ok], column[ok]] = torch.expm1(-loss[ok])
     g = g * w[:, None]
     if cosine:

@@ -64,8 +64,7 @@ def test_weights_keep_their_bits(gpu_ctx, dtype, n_q, filtered):
     loss, lse = call_xent(gpu_ctx, queries, table, targets, words, scale)
     dq, dr = like(queries), like(table)
     call_xent_grads(gpu_ctx, queries, table, targets, words, scale, loss, lse, c, dq, dr)
-    g_queries, g_rows = weight_bits(dtype, n_q, dtype)
-    want = bounds(queries, table, targets, keep, scale, c, exact_products=True, g_queries=g_queries, g_rows=g_rows)
+    want = bounds(queries, table, targets, keep, scale, c, exact_products=True, kept=weight_bits(dtype))
     check(loss, want["loss"], "loss")
     check(lse, want["lse"], "lse")
     check(dr, rounded(want["rows"], dtype), "gradient of the rows")
@@ -85,7 +84,7 @@ def test_weights_keep_their_bits_over_a_store(store_of, dtype, t, metric, n_q):
     targets = clicks(n_q, rows, None, 8)
     loss, lse, dq = store_loss_and_grad(store, queries, targets, scale)
     want = bounds(queries, table, targets, None, scale, cosine=metric == abi.VS_ANGULAR, exact_products=True,
-                  g_queries=weight_bits(t, n_q, F32)[0])
+                  kept=weight_bits(t))
     check(loss, want["loss"], "loss")
     check(lse, want["lse"], "lse")
     check(dq, rounded(want["queries"], F32), "gradient of the queries")
@@ -101,7 +100,7 @@ def test_an_improbable_click(store_of, n_q):
     table[targets.long()] = -queries
     store = store_of(abi.VS_BF16, abi.VS_DOT, table.float().cpu().numpy())
     loss, lse, dq = store_loss_and_grad(store, queries.float(), targets, scale)
-    want = bounds(queries, table, targets, None, scale, exact_products=True, g_queries=2.0**-16)
+    want = bounds(queries, table, targets, None, scale, exact_products=True, kept=weight_bits(BF16))
     check(loss, want["loss"], "loss")
     check(dq, rounded(want["queries"], F32), "gradient of the queries")
 
@@ -141,7 +140,7 @@ def test_the_clicked_rows_weight_is_not_rounded(gpu_ctx, n_q, filtered):
     loss, lse = call_xent(gpu_ctx, queries, table, targets, words, scale)
     dq, dr = like(queries), like(table)
     call_xent_grads(gpu_ctx, queries, table, targets, words, scale, loss, lse, c, dq, dr)
-    want = bounds(queries, table, targets, keep, scale, c, exact_products=True, g_queries=weight_bits(BF16, n_q, BF16)[0], g_rows=2.0**-16)
+    want = bounds(queries, table, targets, keep, scale, c, exact_products=True, kept=weight_bits(BF16))
     check(dq, rounded(want["queries"], BF16), "gradient of the queries")
     # (with the mistake in the 64-bit value, the clicked weights rounded, the bound is left)
     value, bound = want["queries"]
@@ -183,7 +182,7 @@ def test_cosines_of_long_and_short_queries(store_of, dtype, t, n_q, size):
     store = store_of(dtype, abi.VS_ANGULAR, table.float().cpu().numpy())
     targets = torch.arange(n_q, device=DEV).int() * 4
     loss, lse, dq = store_loss_and_grad(store, queries, targets, scale)
-    want = bounds(queries, table, targets, None, scale, cosine=True, g_queries=weight_bits(t, n_q, F32)[0])
+    want = bounds(queries, table, targets, None, scale, cosine=True, kept=weight_bits(t))
     check(loss, want["loss"], "loss")
     check(lse, want["lse"], "lse")
     check(dq, rounded(want["queries"], F32), "gradient of the queries")
@@ -227,7 +226,7 @@ def test_a_clicked_document_without_a_length(store_of, dtype, t, n_q):
     targets = (torch.arange(n_q, device=DEV) * 2).int()
     targets[1::2] -= 1
     loss, lse, dq = store_loss_and_grad(store, queries, targets, scale)
-    want = bounds(queries, table, targets, None, scale, cosine=True, g_queries=weight_bits(t, n_q, F32)[0])
+    want = bounds(queries, table, targets, None, scale, cosine=True, kept=weight_bits(t))
     check(loss, want["loss"], "loss")
     check(lse, want["lse"], "lse")
     check(dq, rounded(want["queries"], F32), "gradient of the queries")
@@ -277,8 +276,7 @@ def test_a_certain_other_document(gpu_ctx, dtype, n_q, dim):
     loss, lse = call_xent(gpu_ctx, queries, table, targets, None, scale)
     dq, dr = like(queries), like(table)
     call_xent_grads(gpu_ctx, queries, table, targets, None, scale, loss, lse, None, dq, dr)
-    g_queries, g_rows = weight_bits(dtype, n_q, dtype)
-    want = bounds(queries, table, targets, None, scale, g_queries=g_queries, g_rows=g_rows, **ALONE)
+    want = bounds(queries, table, targets, None, scale, kept=weight_bits(dtype), **ALONE)
     assert float(want["loss"][0].min()) > 15
     check(dq, rounded(want["queries"], dtype), "gradient of the queries")
     value, bound = rounded(want["rows"], dtype)
@@ -291,7 +289,7 @@ def test_a_certain_other_document_of_a_store(store_of, dtype, t, n_q, dim):
     table, queries, near, targets = certain(400, n_q, dim, t, 33)
     store = store_of(dtype, abi.VS_DOT, table.float().cpu().numpy())
     loss, lse, dq = store_loss_and_grad(store, queries.float(), targets, 4.0)
-    want = bounds(queries, table, targets, None, 4.0, g_queries=weight_bits(t, n_q, F32)[0], **ALONE)
+    want = bounds(queries, table, targets, None, 4.0, kept=weight_bits(t), **ALONE)
     check(dq, rounded(want["queries"], F32), "gradient of the queries")
 
 
@@ -325,3 +323,43 @@ def test_a_certain_other_document_with_a_large_logit(gpu_ctx, store_of, n_q, ove
     # elements of 1/4 at most
     bound = size * 16 * U32 + rows * math.exp(-25) * scale / 4
     check(dq[sure], (value[sure], bound[sure]), "gradient of the queries")
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("n_q", [3, 64, 65, 300])
+@pytest.mark.parametrize("filtered", [False, True])
+def test_a_copy_of_the_clicked_document(gpu_ctx, dtype, n_q, filtered):
+    """The clicked document and one that differs from it in one column share the probability: the query's gradient is their
+    difference, and all that is left of the other columns is what the weights are off by (2^-8 of each, were they rounded to
+    bf16)."""
+    rows, dim, scale = 700, 64, 25.3
+    table, near = steps(rows, dim, dtype, 36), torch.arange(n_q, device=DEV)
+    queries = table[near] * 2
+    queries[:, 0] = 0
+    copies = rows - 1 - near
+    table[copies] = table[near]
+    table[copies, 0] = 0.25 - table[near, 0].abs()  # (another number than before)
+    logit = (queries.double() * table[near].double()).sum(1) * scale
+    others = queries.double() @ table.double().T * scale
+    others[near, near] = others[near, copies] = -math.inf
+    sure = logit - others.amax(1) > 25
+    assert int(sure.sum()) > 0.6 * n_q
+    words = None
+    if filtered:
+        keep = torch.ones(rows, dtype=torch.bool, device=DEV)
+        keep[n_q + 5 : n_q + 40] = False
+        words = words_of(keep)
+    c = torch.rand(n_q, generator=torch.Generator(device=DEV).manual_seed(37), device=DEV) + 0.5
+    loss, lse = call_xent(gpu_ctx, queries, table, near.int(), words, scale)
+    dq, dr = like(queries), like(table)
+    call_xent_grads(gpu_ctx, queries, table, near.int(), words, scale, loss, lse, c, dq, dr)
+    half = (c.double() * scale / 2)[:, None]
+    value = half * (table[copies].double() - table[near].double())
+    size = half * (table[copies].double().abs() + table[near].double().abs())
+    # the weights: lse's rounding and the logit's own (2^-24 of 100 and less), 8 roundings, the planes; all others exp(-25) each
+    off = 2 * U32 * logit[:, None] + 16 * U32 + (0 if dtype == F32 else 2.0**-16)
+    bound = size * off + rows * math.exp(-25) * c.double().max() * scale / 4
+    check(dq[sure], tuple(t[sure] for t in rounded((value, bound), dtype)), "gradient of the queries")
+    value, bound = half * queries.double(), half * queries.double().abs() * off + n_q * math.exp(-25) * c.double().max() * scale / 2
+    check(dr[copies[sure]], tuple(t[sure] for t in rounded((value, bound), dtype)), "gradient of the copies")
+    check(dr[near[sure]], tuple(t[sure] for t in rounded((-value, bound), dtype)), "gradient of the clicked rows")

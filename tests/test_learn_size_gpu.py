@@ -55,9 +55,8 @@ def test_every_tile_counts_once(gpu_ctx, dtype, n_q, rows, dim, filtered):
     loss, lse = call_xent(gpu_ctx, queries, table, targets, words, scale)
     dq, dr = like(queries), like(table)
     call_xent_grads(gpu_ctx, queries, table, targets, words, scale, loss, lse, c, dq, dr)
-    g_queries, g_rows = weight_bits(dtype, n_q, dtype)
     # (a share of a query's gradient: the workgroups side by side are tiles of 64 queries and of 128 columns, at least)
-    want = bounds(queries, table, targets, keep, scale, c, g_queries=g_queries, g_rows=g_rows,
+    want = bounds(queries, table, targets, keep, scale, c, kept=weight_bits(dtype),
                   share=chain_of(n, n_q) * -(-dim // 128))
     assert float((want["lse"][1]).max()) < 5e-3
     # (with the mistake in the 64-bit value, a border's word of 64 rows lost, the bound is left)
