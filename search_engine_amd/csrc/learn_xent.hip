@@ -1244,9 +1244,11 @@ __global__ __launch_bounds__(256) void join_query_grads_kernel(XentArgs a, Few f
     float* sum0 = a.part_q + (uint64_t)q * a.dim;
     double dot = 0, sq = 0;  // (as in pack_queries_kernel)
     for (uint32_t d = blockIdx.y * 256 + threadIdx.x; d < a.dim; d += gridDim.y * 256) {
-        float sum = sizeof(E) == 2 ? rest * to_f32(clicked[d]) : 0.0f;  // (of three planes nothing is left)
+        // (64 bits: the clicked row's share is as large as all others together, which would be added to it last bit by last bit)
+        double all = sizeof(E) == 2 ? rest * to_f32(clicked[d]) : 0.0f;  // (of three planes nothing is left)
 #pragma unroll 8
-        for (uint32_t s = 0; s < a.splits; ++s) sum += a.part_q[((uint64_t)s * a.n_q + q) * a.dim + d];
+        for (uint32_t s = 0; s < a.splits; ++s) all += a.part_q[((uint64_t)s * a.n_q + q) * a.dim + d];
+        const float sum = (float)all;
         if (!a.norms) {
             out[q * out_stride + d] = from_f32<O>(sum);
             continue;

@@ -363,3 +363,27 @@ def test_a_copy_of_the_clicked_document(gpu_ctx, dtype, n_q, filtered):
     value, bound = half * queries.double(), half * queries.double().abs() * off + n_q * math.exp(-25) * c.double().max() * scale / 2
     check(dr[copies[sure]], tuple(t[sure] for t in rounded((value, bound), dtype)), "gradient of the copies")
     check(dr[near[sure]], tuple(t[sure] for t in rounded((-value, bound), dtype)), "gradient of the clicked rows")
+
+
+@pytest.mark.parametrize("over_store", [False, True])
+@pytest.mark.parametrize("n_q", [1, 5, 100])
+def test_small_shares_are_not_lost_in_a_large_one(gpu_ctx, store_of, n_q, over_store):
+    """The clicked document's share of a query's gradient is nearly one, each other workgroup's 0.4 of its last bit: added to it
+    in f32 one after the other, all of them would be lost."""
+    rows, dim, scale = 16384, 64, 8.0
+    for dtype, t in ((abi.VS_F32, F32),) + (((abi.VS_BF16, BF16),) if over_store else ()):
+        table, queries = torch.zeros(rows, dim, dtype=t, device=DEV), torch.zeros(n_q, dim, dtype=t, device=DEV)
+        table[:, 0] = 0.4 * 256 * 2.0**-24  # (every logit is zero, each probability 1 / rows, and 64 rows or more a share)
+        table[0, 0] = 1
+        queries[:, 1] = 1
+        targets = torch.zeros(n_q, dtype=torch.int32, device=DEV)
+        if over_store:
+            store = store_of(dtype, abi.VS_DOT, table.float().cpu().numpy())
+            loss, lse, dq = store_loss_and_grad(store, queries.float(), targets, scale)
+        else:
+            loss, lse = call_xent(gpu_ctx, queries, table, targets, None, scale)
+            dq = like(queries)
+            call_xent_grads(gpu_ctx, queries, table, targets, None, scale, loss, lse, None, dq, None)
+        want = bounds(queries, table, targets, None, scale, exact_products=True, exact_factor=True, chain=64, kept=weight_bits(t),
+                      share=-(-rows * -(-n_q // 64) // 256), joins=0)
+        check(dq, rounded(want["queries"], F32), "gradient of the queries")
