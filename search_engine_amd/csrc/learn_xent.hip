@@ -857,10 +857,17 @@ __global__ __launch_bounds__(THREADS, 2) void weights_kernel(XentArgs a) {
                         if constexpr (NORMS) z *= inverse[n];
                         float g = vf[r] * Base2::weight(z * vs[r], vl[r]);
                         if constexpr (NORMS) g *= inverse[n];
-                        const Split x = split(g);
-                        p[t][0].e[r] = x.h;
-                        p[t][1].e[r] = x.m;
-                        p[t][2].e[r] = x.l;
+                        if constexpr (PG == 2) {
+                            // (beyond the largest number of bf16 no number; the general split costs twice the instructions)
+                            const uint32_t h = bf16_bits(g);
+                            p[t][0].e[r] = (uint16_t)h;
+                            p[t][1].e[r] = (uint16_t)bf16_bits(g - __builtin_bit_cast(float, h << 16));
+                        } else {
+                            const Split x = split(g);
+                            p[t][0].e[r] = x.h;
+                            p[t][1].e[r] = x.m;
+                            p[t][2].e[r] = x.l;
+                        }
                     }
                 }
 #pragma unroll
@@ -1324,8 +1331,8 @@ Plan plan_for(uint32_t n_q, uint64_t n_rows, uint32_t dim, int32_t dtype) {
     p.planes = dtype == VS_F32 ? 3 : 1;
     // Weights of a bf16 table have 16 bits. Rounded to bf16, 2^-8 of each at most, they would be as far off as a gradient's own
     // rounding is, and further where a gradient is the difference of terms that nearly cancel, as those of a clicked document and
-    // a copy of it do. (The price: loss and gradients of 256 queries over 1M x 768 take 2.72 ms, 1.93 with bf16 weights; of 1000
-    // over half of 200 thousand x 1536, queries' alone, 1.25 and 0.94.)
+    // a copy of it do. (The price: loss and gradients of 256 queries over 1M x 768 take 2.65 ms, 1.93 with bf16 weights; of 1000
+    // over half of 200 thousand x 1536, queries' alone, 1.24 and 0.94.)
     p.g_planes = dtype == VS_F32 ? 3 : 2;
     p.kp = (uint32_t)round_up(dim, 64);
     p.gq = (uint32_t)round_up(n_q, 64);
