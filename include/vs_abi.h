@@ -539,8 +539,9 @@ int32_t vs_lookup_grad_weights_device(vs_ctx* ctx, const void* d_rows, int32_t d
  *   d_mask_words: candidate words as in the searches, bit r & 63 of word r >> 6,
  *                 ceil(n_rows / 64) words; NULL = every row. Rows that are no
  *                 candidates are not read
- * A candidate row, or a query with a click, that holds an infinity or a NaN gives no
- * number in what it takes part in. */
+ * A NaN in a candidate row is in every loss, lse and gradient (but those of queries
+ * without a click); a NaN in a query with a click in its loss, its lse, its gradient
+ * and the rows'. What infinities, or logits beyond f32, give is not said. */
 int32_t vs_xent_workspace_bytes(vs_ctx* ctx, uint32_t n_q, uint64_t n_rows, uint32_t dim,
                                 int32_t dtype, uint64_t* bytes);
 /* What ONE call on these rows needs (gradients 0: vs_xent_device, else
@@ -563,8 +564,8 @@ int32_t vs_xent_device(vs_ctx* ctx, const void* d_queries, uint32_t n_q, uint64_
  *   d_grad_rows:    laid out as d_rows, every row written (zeros for a row that is no
  *                   candidate; between rows nothing is written), or NULL
  * The products are recomputed, a piece of the rows at a time. The weights exp(z - lse)
- * of VS_F32 keep all 24 bits, those of VS_BF16 16; sums stay f32 and each gradient is
- * rounded once. */
+ * of VS_F32 keep all 24 bits, those of VS_BF16 16, and those of one query share the
+ * rounding of its lse; sums stay f32 and each gradient is rounded once. */
 int32_t vs_xent_grad_device(vs_ctx* ctx, const void* d_queries, uint32_t n_q, uint64_t query_stride,
                             const void* d_rows, uint64_t n_rows, uint64_t row_stride, int32_t dtype,
                             uint32_t dim, const uint32_t* d_targets, const uint64_t* d_mask_words,
@@ -573,11 +574,13 @@ int32_t vs_xent_grad_device(vs_ctx* ctx, const void* d_queries, uint32_t n_q, ui
                             void* d_grad_queries, void* d_grad_rows, void* hip_stream);
 
 /* The same over a sealed store (VS_ANGULAR: logits are scale * cosine, VS_DOT: scale *
- * product; other metrics VS_E_INVALID_ARG), whose rows stay as they are: the loss and
- * the gradient of the queries, f32 [n_q][dim] in device memory as in
- * vs_search_batch_device (rounded to bf16 for a VS_BF16 store). Targets are docids;
- * d_mask_words as in vs_search_device (aligned to the store). The two calls of a step
- * see the same rows if no seal comes between them. */
+ * product; other metrics VS_E_INVALID_ARG), whose rows stay as they are. The cosine
+ * with a vector of zeros, or with a document whose length the store keeps as infinity
+ * (its square passes f32), is 0 here. The loss and the gradient of the queries, f32
+ * [n_q][dim] in device memory as in vs_search_batch_device (rounded to bf16 for a
+ * VS_BF16 store). Targets are docids; d_mask_words as in vs_search_device (aligned to
+ * the store). The two calls of a step see the same rows if no seal comes between
+ * them. */
 int32_t vs_store_xent_workspace_bytes(vs_store* s, uint32_t n_q, uint64_t* bytes);
 int32_t vs_store_xent_call_workspace_bytes(vs_store* s, uint32_t n_q, int32_t gradients,
                                            uint64_t* bytes);

@@ -13,7 +13,8 @@
 // never read (whatever it holds), and costs nothing.
 //
 // Four products on the bf16 matrix cores (learn_mma.h) carry it: rows x queries for the loss, the same again for the
-// weights G, and G with the queries and with the rows for the gradients. G is made for a piece of the rows at a time and
+// weights G, and G with the queries and with the rows for the gradients. Up to four queries make their logits by plain products,
+// both times. G is made for a piece of the rows at a time and
 // read twice before the next piece takes its place. Rows that are not whole 16-byte chunks at multiples of 16 bytes are
 // copied to such, piece by piece, first.
 #include "../../include/vs_abi.h"
@@ -444,10 +445,11 @@ __device__ __forceinline__ float base2(float scale) {
 
 // Per query the largest logit of a share of the candidates and the sum of the exponentials over it, the clicked row kept
 // out. Bound by the products from 64 queries (bf16) or so on, by the rows' bytes below: 256 queries over 1M x 768 bf16 take
-// 420 - 510 us (0.8 - 0.95 PFLOP/s; a large library product reaches 1.5), 10 take 255 (6.0 TB/s); over 250 thousand x 768
-// f32 256 take 660 (149 TFLOP/s in f32 products, 0.9 PFLOP/s of the six bf16 ones: the wave's splitting and the matrix
-// cores take 45 % of the cycles each). Everything is in base 2 (logits times log2 e): an exponential is one instruction. A lane keeps the running largest
-// product and the sum of its own candidates, in registers, for each of its queries; lanes, waves and shares are joined at the end.
+// 390 - 450 us (0.87 - 1.0 PFLOP/s, by the clock; a large library product reaches 1.5), 10 take 255 (6.0 TB/s); over 250
+// thousand x 768 f32 256 take 580 (168 TFLOP/s in f32 products, 1.0 PFLOP/s of the six bf16 ones: the wave's splitting and the
+// matrix cores take 45 % of the cycles each). Everything is in base 2 (logits times log2 e): an exponential is one
+// instruction. A lane keeps the running largest product and the sum of its own candidates, in registers, for each of its
+// queries; lanes, waves and shares are joined at the end.
 template <typename S, bool NORMS>
 __global__ __launch_bounds__(THREADS, 2) void loss_kernel(XentArgs a) {
     constexpr int BQ = S::Q_TILE;
@@ -553,7 +555,7 @@ __global__ __launch_bounds__(THREADS, 2) void loss_kernel(XentArgs a) {
     a.part_l[to] = sum;
 }
 
-// Up to four queries: bound by the rows' bytes (one over 1M x 768 bf16: 237 us, 6.5 TB/s), so plain f32 products, straight from
+// Up to four queries: bound by the rows' bytes (one over 1M x 768 bf16: 243 us, 6.3 TB/s), so plain f32 products, straight from
 // the table. The loss and the weights of the gradients share them, bit for bit: of a document that has nearly all of the
 // probability, what its logit is off by is in lse and in its weight, and cancels only if it is the same.
 template <typename E, typename Q, int V, int NQ, bool NORMS>
@@ -688,8 +690,9 @@ __global__ __launch_bounds__(256) void loss_few_kernel(XentArgs a, Few f, float*
     a.part_l[(uint64_t)blockIdx.x * NQ + threadIdx.x] = sum;
 }
 
-// A query's shares joined, in 64 bits; a workgroup per query: 5 - 10 us, two trips to memory one behind the other. The clicked row's logit is made here, in 64 bits: its error
-// is that of a loss near zero, while those of the others' mostly cancel in their sum.
+// A query's shares joined, in 64 bits; a workgroup per query: 5 - 10 us, two trips to memory one behind the other. The clicked
+// row's logit is made here, in 64 bits: its error is that of a loss near zero, while those of the others' mostly cancel in
+// their sum.
 template <typename E, typename Q>
 __global__ __launch_bounds__(256) void join_loss_kernel(XentArgs a, Few f, float* loss, float* lse) {
     __shared__ float tops[4];
@@ -804,9 +807,9 @@ __global__ __launch_bounds__(256) void click_weights_kernel(XentArgs a) {
 template <typename S>
 using weights_turn = Turn<8, S::UNIT>;
 
-// The weights G of a piece, [candidate][query], kept to 16 bits (PG = 2, of bf16 tables) or all 24 (3) by as many planes of bf16. A lane holds four neighbouring queries of a candidate: eight bytes a store. Bound as the loss is, and by what
-// it writes: 256 queries over 1M x 768 bf16 505 us (0.78 PFLOP/s, of which 512 MB written take about 100), 256 over 250
-// thousand x 768 f32 715.
+// The weights G of a piece, [candidate][query], kept to 16 bits (PG = 2, of bf16 tables) or all 24 (3) by as many planes of
+// bf16. A lane holds four neighbouring queries of a candidate: eight bytes a store. Bound as the loss is, and by what it writes:
+// 256 queries over 1M x 768 bf16 570 us (0.69 PFLOP/s; 1 GB written), 256 over 250 thousand x 768 f32 645.
 template <typename S, bool NORMS, int PG>
 __global__ __launch_bounds__(THREADS, 2) void weights_kernel(XentArgs a) {
     constexpr int BQ = S::Q_TILE;
@@ -926,9 +929,9 @@ __global__ __launch_bounds__(256) void weights_few_kernel(XentArgs a, Few f) {
     }
 }
 
-// drows of a piece: transposed queries (BD columns of the rows) by G. The sums are short (as many steps as 64 queries, or six
-// times as many in f32) and every one is written: 256 queries, 1M x 768 bf16: 660 us (0.60 PFLOP/s; 1.5 GB written and 0.5
-// read take 400 by themselves); 250 thousand x 768 f32: 630 us. A lane holds four neighbouring columns of a row.
+// drows of a piece: transposed queries (BD columns of the rows) by G. The sums are short (for each 64 queries two steps, or six in
+// f32) and every one is written: 256 queries, 1M x 768 bf16: 905 us (0.87 PFLOP/s of both planes; 1.5 GB written and 1 read take
+// 500 by themselves); 250 thousand x 768 f32: 585 us. A lane holds four neighbouring columns of a row.
 // As in weights_kernel every lane stores every time, to its own 16 bytes of a.spill where it has no row or no whole
 // 16 bytes of columns; the columns of a last, broken 16 bytes are stored one by one besides.
 template <int BD>
@@ -1046,7 +1049,7 @@ __global__ __launch_bounds__(THREADS, 2) void row_grads_kernel(XentArgs a) {
 }
 
 // dqueries over one share of a piece's candidates: G by rows, the sum running over the candidates. 256 queries over 1M x
-// 768 bf16: 471 us (0.83 PFLOP/s); 1000 over 100 thousand of 200 thousand x 1536, through the list: 340 us (0.90).
+// 768 bf16: 745 us (1.05 PFLOP/s of both planes); 1000 over 100 thousand of 200 thousand x 1536, through the list: 560 us (1.10).
 // (Through the list two buffers: its reads are waited for with the loads under way counted in, so that only those that
 // the barrier has waited for already may be.)
 template <int BQ, int BD, bool LISTED>
@@ -1144,7 +1147,7 @@ __global__ __launch_bounds__(THREADS, 2) void query_grads_kernel(XentArgs a) {
 }
 
 // The same of an f32 table: G's planes by the rows as they are, split as in SplitScores. 128 queries a tile (256 over 250
-// thousand x 768: 610 us, 0.97 PFLOP/s of bf16; by 64 a tile 843), the LDS of two steps.
+// thousand x 768: 570 us, 1.03 PFLOP/s of bf16; by 64 a tile a third more), the LDS of two steps.
 constexpr int FLOAT_BD = 128;
 template <int BQ, bool LISTED>
 constexpr int float_grads_row_buffers = LISTED || BQ > 64 ? 2 : 3;
@@ -1339,7 +1342,7 @@ Plan plan_for(uint32_t n_q, uint64_t n_rows, uint32_t dim, int32_t dtype) {
     p.bq = n_q <= 64 ? 64 : n_q <= 128 || dtype == VS_F32 ? 128 : 256;
     p.score_bq = dtype == VS_F32 ? 64 : p.bq;
     // an odd number of 128 columns by 128 at a time: no half-empty tiles (200 thousand x 384, 128 queries: rows' gradients
-    // 49 us, 57 by 256; queries' 41 and 48)
+    // 82 us, 89 by 256; queries' 61 and 65)
     p.bd = (dim + 127) / 128 % 2 ? 128 : 256;
     p.score_q_tiles = (n_q + p.score_bq - 1) / p.score_bq;
     p.q_tiles = (n_q + p.bq - 1) / p.bq;
