@@ -75,3 +75,33 @@ def test_every_tile_counts_once(gpu_ctx, dtype, n_q, rows, dim, filtered):
     dq2, dr2 = like(queries), like(table)
     call_xent_grads(gpu_ctx, queries, table, targets, words, scale, loss, lse, c, dq2, dr2)
     assert all(torch.equal(a, b) for a, b in ((loss, loss2), (lse, lse2), (dq, dq2), (dr, dr2)))
+
+
+@pytest.mark.parametrize("filtered", [False, True])
+@pytest.mark.parametrize("dtype,rows", [(BF16, 4300001), (F32, 2900003)])
+def test_a_few_queries_over_more_than_one_piece(gpu_ctx, dtype, rows, filtered):
+    """Weights of up to four queries, a piece of the rows at a time: documents at the pieces' borders have most of the probability."""
+    n_q, dim = 3, 8
+    table, queries = matrix(rows, dim, dtype, 6), matrix(n_q, dim, dtype, 7)
+    piece = (1 << 30) // (64 * 2 * (3 if dtype == F32 else 2)) // 65536 * 65536
+    places = torch.tensor([0, piece - 1, piece, rows - 1, piece + 7, 3, 63, 64, piece // 2], device=DEV)
+    queries *= 2
+    table[places] = queries[torch.arange(9, device=DEV) % n_q] * 2
+    keep = None
+    if filtered:
+        keep = torch.rand(rows, generator=torch.Generator(device=DEV).manual_seed(8), device=DEV) < 0.98
+        keep[places] = True
+        table[~keep] = float("nan")
+    targets = torch.tensor([5, piece + 1, rows - 2], device=DEV).int()
+    if keep is not None:
+        keep[targets.long()] = True
+        table[targets.long()] = 0.25
+    words = None if keep is None else words_of(keep)
+    loss, lse = call_xent(gpu_ctx, queries, table, targets, words, 2.0)
+    dq, dr = like(queries), like(table)
+    call_xent_grads(gpu_ctx, queries, table, targets, words, 2.0, loss, lse, None, dq, dr)
+    want = bounds(queries, table, targets, keep, 2.0, kept=weight_bits(dtype), share=chain_of(rows, n_q))
+    check(loss, want["loss"], "loss")
+    check(lse, want["lse"], "lse")
+    check(dq, rounded(want["queries"], dtype), "gradient of the queries")
+    check(dr, rounded(want["rows"], dtype), "gradient of the rows")

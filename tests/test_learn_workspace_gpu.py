@@ -104,3 +104,38 @@ def test_what_the_question_refuses():
         assert e.value.code == abi.VS_E_INVALID_ARG and part in e.value.message
     assert abi.lib.vs_xent_call_workspace_bytes(None, 1, p, 10, 8, abi.VS_F32, 8, 0, None) == abi.VS_E_INVALID_ARG
     assert abi.lib.vs_store_xent_call_workspace_bytes(None, 1, 0, ctypes.byref(n)) == abi.VS_E_INVALID_ARG
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("n_q", [1, 4])
+def test_a_few_queries_captured_with_what_they_need(gpu_ctx, dtype, n_q):
+    """Loss and gradients in a graph, each with one call's workspace; replayed with new queries and clicks, with eager calls
+    between, every replay gives the eager calls' bits."""
+    rows, dim, code = 5000, 60, TYPE[dtype]
+    table, queries, targets = matrix(rows, dim, dtype, 7), matrix(n_q, dim, dtype, 8), clicks(n_q, rows, None, 9)
+    ws = [torch.empty(gpu_ctx.xent_call_workspace_bytes(n_q, ptr(table), rows, dim, code, dim, g), dtype=torch.uint8, device=DEV)
+          for g in (False, True)]
+    loss, lse = torch.empty(2, n_q, device=DEV)
+    dq, dr = like(queries), like(table)
+
+    def run():
+        st = torch.cuda.current_stream().cuda_stream
+        args = (ptr(queries), n_q, dim, ptr(table), rows, dim, code, dim, ptr(targets), None, 7.0)
+        gpu_ctx.xent_device(*args, ptr(ws[0]), ws[0].numel(), ptr(loss), ptr(lse), st)
+        gpu_ctx.xent_grad_device(*args, ptr(loss), ptr(lse), None, ptr(ws[1]), ws[1].numel(), ptr(dq), ptr(dr), st)
+    run()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        run()
+    for seed in range(4):
+        queries.copy_(matrix(n_q, dim, dtype, 10 + seed))
+        targets.copy_(clicks(n_q, rows, None, 20 + seed))
+        graph.replay()
+        torch.cuda.synchronize()
+        first = [t.clone() for t in (loss, lse, dq, dr)]
+        run()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(first, (loss, lse, dq, dr)))
+    assert torch.isfinite(dr).all()
